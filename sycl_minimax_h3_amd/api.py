@@ -1,4 +1,4 @@
-"""Raw bindings to libh3hip.so: one ctypes function per declaration of include/h3hip.h.
+"""Raw bindings to libh3hip.so: one ctypes function per declaration of include/h3hip.h, and the table of include/h3lm.h.
 
 Mirrors engine/h3-sys/src/lib.rs (the Rust engine's loader of the reference library): the library is opened at run
 time, every function of the reference's header (kernels/h3sycl.h) is resolved by name, and a library missing any of
@@ -91,6 +91,35 @@ ADDITIONS = {
 }
 
 
+class KvCache(C.Structure):
+    """include/h3lm.h's h3_kv_cache."""
+
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("blocks", i64), ("heads", i64), ("dim", i64)]
+
+
+class KvBatch(C.Structure):
+    """include/h3lm.h's h3_kv_batch."""
+
+    _fields_ = [("table", vp), ("starts", vp), ("seqs", i64), ("width", i64), ("rows", i64), ("most", i64)]
+
+
+KV_BLOCK = 64
+_cache, _batch = C.POINTER(KvCache), C.POINTER(KvBatch)
+
+
+class LmApi(C.Structure):
+    """include/h3lm.h's h3_lm_api: the table of function pointers that the library exports as `h3lm`."""
+
+    _fields_ = [
+        ("size", i64),
+        ("kv_write", C.CFUNCTYPE(i32, vp, _cache, _batch, vp, vp, i64, vp, i64, i32)),
+        ("kv_read", C.CFUNCTYPE(i32, vp, _cache, _batch, vp, vp, i64, vp, i64, i32)),
+        ("kv_attention", C.CFUNCTYPE(i32, vp, _cache, _batch, vp, i64, vp, i64, i32, i64, f32, i64, vp, i64, vp, i32, vp, vp, u64)),
+        ("kv_attention_work", C.CFUNCTYPE(i64, vp, _cache, _batch, i64, i64, i64)),
+        ("linear4", C.CFUNCTYPE(i32, vp, vp, i32, i64, i64, vp, i64, vp, vp, i32, i64, vp, vp, i32)),
+    ]
+
+
 def candidates() -> list[str]:
     """Where the library is looked for: $H3SYCL_LIB, then beside this package (engine/h3-sys/src/lib.rs:181-193)."""
     out = []
@@ -114,6 +143,12 @@ class Api:
             fn.restype = res
             fn.argtypes = args
             setattr(self, name[len("h3s_"):], fn)
+        try:
+            self.lm = LmApi.in_dll(self.lib, "h3lm")
+        except ValueError:
+            raise OSError(f"h3lm is missing from the library ({path})") from None
+        if self.lm.size < C.sizeof(LmApi):
+            raise OSError(f"h3lm is an older library's ({path})")
 
     def error(self) -> str:
         """The library's last error on this thread."""

@@ -1,0 +1,105 @@
+// kv_attn.hip - kv_attention and kv_attention_work (h3lm.h) on the kernels of kv_attn_impl.h: the checks, the choice of the
+// kernel and of the parts that the cache is split into, and the workspace.
+#include <algorithm>
+#include <cmath>
+
+#include "kv_attn_impl.h"
+
+namespace h3 {
+
+// Rows: `most` tokens of a sequence times the heads that share a key/value head. Up to 64 rows the four wavefronts of a block
+// share 16 or 32 of them and the cache is read by all four (an answered token is bound by the cache's bytes); beyond, each has 32
+// rows of its own. Parts: as many as give each CU two blocks of threads, but at least four cache blocks each (one a
+// wavefront), because every part costs its sums, written and read, and the merge's launch.
+static KvPlan kv_plan(const KvArgs& P, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
+    KvPlan plan;
+    const int64_t rows = std::min<int64_t>(most, P.rows) * group;
+    plan.ks = rows <= 64 ? 4 : 1;
+    plan.nq = rows <= 16 ? 1 : 2;
+    plan.rt = 16 * plan.nq * (plan.ks == 1 ? 4 : 1);
+    plan.tiles = (rows + plan.rt - 1) / plan.rt;
+    plan.blocks = plan.tiles * P.seqs * P.heads;
+    int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
+    if (window > 0) keys = std::min(keys, window + most + 2 * kKvB);
+    const int64_t blocks = (keys + kKvB - 1) / kKvB;
+    const int64_t least = plan.ks == 4 ? 4 : 8;
+    int64_t ns = std::min(blocks / least, 2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1));
+    plan.nsplit = (int) std::max<int64_t>(1, std::min<int64_t>(ns, 1024));
+    return plan;
+}
+static int64_t kv_part_floats(const KvPlan& plan, int64_t W) { return plan.nsplit > 1 ? plan.blocks * plan.nsplit * plan.rt * (W + 2) : 0; }
+
+static int attn_checks(const char* fn, const KvArgs& P, int64_t max_len, int64_t q_heads, int64_t window) {
+    if (q_heads <= 0 || q_heads % P.heads != 0) return fail(std::string(fn) + ": the query heads must be a multiple of the key/value heads");
+    if (q_heads > 65535) return fail(std::string(fn) + ": too many heads");
+    if (max_len < 0 || window < 0) return fail(std::string(fn) + ": a negative length or window");
+    return 0;
+}
+
+int64_t kv_attention_work(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, int64_t max_len, int64_t q_heads, int64_t window) try {
+    const char* fn = "kv_attention_work";
+    KvArgs P;
+    if (kv_args(fn, cache, batch, P) || attn_checks(fn, P, max_len, q_heads, window)) return -1;
+    Ctx* c = ctx_of(ctx, fn);
+    if (!c) return -1;
+    if (P.seqs == 0 || P.rows == 0 || batch->most == 0) return 0;
+    return 4 * kv_part_floats(kv_plan(P, batch->most, q_heads / P.heads, max_len, window, c->cus), kv_width(P.dim));
+} catch (const std::exception& e) { return fail(e.what()); }
+
+int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* lengths, int64_t max_len, const void* q,
+                 int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window, const uint8_t* mask, int64_t mask_stride,
+                 void* out, int out_dt, float* lse, void* work, uint64_t work_bytes) try {
+    const char* fn = "kv_attention";
+    KvAttnArgs A;
+    if (kv_args(fn, cache, batch, A.kv) || attn_checks(fn, A.kv, max_len, q_heads, window)) return -1;
+    if (!dt_ok(dt) || !dt_ok(out_dt)) return fail(std::string(fn) + ": unknown element type");
+    if (!(scale >= 0.0f) || std::isinf(scale)) return fail(std::string(fn) + ": the scale must be a number above 0 (or 0: 1 / sqrt(dim))");
+    if (mask && mask_stride < 0) return fail(std::string(fn) + ": a negative mask stride");
+    if (A.kv.seqs == 0 || A.kv.rows == 0 || batch->most == 0) return 0;
+    const int64_t dim = A.kv.dim;
+    if (q_stride < q_heads * dim) return fail(std::string(fn) + ": the row stride is shorter than a row");
+    if (!lengths || !q || !out) return fail(std::string(fn) + ": lengths, q and out are required");
+    if (work && !aligned16(work)) return fail(std::string(fn) + ": the workspace must be 16-byte aligned");
+    const int64_t group = q_heads / A.kv.heads;
+    Ctx* c = ctx_of(ctx, fn);
+    if (!c) return -1;
+    if (A.kv.rows * group > INT32_MAX) return fail(std::string(fn) + ": too many rows");
+    const KvPlan plan = kv_plan(A.kv, batch->most, group, max_len, window, c->cus);
+    const int64_t W = kv_width(dim);
+    if (plan.blocks * plan.nsplit > 0x7fffffff || plan.blocks * plan.rt > 0x7fffffff) return fail(std::string(fn) + ": too many blocks of work");
+    const int64_t floats = kv_part_floats(plan, W);
+    A.po = nullptr;
+    if (floats) {
+        if (work) {
+            if (work_bytes < (uint64_t) (4 * floats)) return fail(std::string(fn) + ": the workspace is smaller than kv_attention_work() says");
+            A.po = (float*) work;
+        } else {
+            hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+            if (hipStreamIsCapturing(c->stream, &st) != hipSuccess) (void) hipGetLastError();
+            if (st != hipStreamCaptureStatusNone) return fail(std::string(fn) + ": a call recorded into a graph needs a workspace of its own");
+            A.po = c->scratch<float>(Ctx::KV_PART, (size_t) floats);
+            if (!A.po) return -1;
+        }
+    }
+    A.pml = A.po ? A.po + plan.blocks * plan.nsplit * plan.rt * W : nullptr;
+    A.lengths = lengths;
+    A.q = q; A.q_stride = q_stride; A.q_dt = dt; A.group = (int) group; A.q_heads = (int) q_heads;
+    A.scale = (float) ((scale > 0.0f ? (double) scale : 1.0 / std::sqrt((double) dim)) * 1.4426950408889634);
+    A.window = (int) std::min<int64_t>(window, INT32_MAX / 2);
+    A.mask = mask; A.mask_stride = mask_stride;
+    A.out = out; A.out_dt = out_dt; A.lse = lse;
+    A.tiles = (int) plan.tiles; A.nsplit = plan.nsplit;
+    A.q_vec = aligned16(q) && dim % 8 == 0 && (q_stride * elem_size(dt)) % 16 == 0;
+    A.out_vec = aligned16(out) && dim % 4 == 0;
+    A.mask_vec = mask && aligned16(mask) && mask_stride % 16 == 0;
+    const bool two = dt == H3S_F32;
+    switch (W / 64) {
+        case 1: kv_attn_64(c, A, plan, two); break;
+        case 2: kv_attn_128(c, A, plan, two); break;
+        case 3: kv_attn_192(c, A, plan, two); break;
+        default: kv_attn_256(c, A, plan, two); break;
+    }
+    return launched(fn);
+} catch (const std::exception& e) { return fail(e.what()); }
+
+}  // namespace h3

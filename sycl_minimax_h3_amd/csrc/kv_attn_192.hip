@@ -1,0 +1,6 @@
+// kv_attn_192.hip - kv_attn_impl.h's kernels for heads of up to 192 features
+#include "kv_attn_impl.h"
+
+namespace h3 {
+void kv_attn_192(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two) { kv_attn_width<3>(c, P, plan, two); }
+}  // namespace h3

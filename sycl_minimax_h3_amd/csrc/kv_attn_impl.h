@@ -1,0 +1,493 @@
+// kv_attn_impl.h - the attention over the 8-bit key/value cache (h3lm.h, kv_attention).
+//
+// Mathematics, for one query row with scores s_j = q . k_j * scale over the tokens j it sees: p_j = 2^(s_j log2(e) - m), m the
+// running maximum, l = sum p_j, o = sum p_j v_j / l, in one pass over the cache: where a block raises m, l and o are
+// multiplied by 2^(m_old - m). Keys are codes times a block's scale, so s = (q . codes) * (k_scale * scale * log2 e): one factor a
+// block. Values likewise: a block's sum of p_j codes_j is added to o with v_scale as the factor.
+//
+// Products on the matrix cores (16 x 16 x 32, half operands, float32 sums). The codes are whole numbers below 2^8, exact as
+// half. Query rows are scaled by a power of two that takes their largest value to 2^14 .. 2^15, so half holds 16-bit types
+// without loss down to 2^-29 of it; float32 rows are two halves (high and rest: 22 bits). Probabilities are 2^15 p, so that half keeps
+// them down to p = 2^-29 at full precision; for float32 queries they are two halves as well.
+//
+// Layout: S^T = K Q^T, with the keys as the first operand, leaves one query row a lane (lane % 16) and four keys a register
+// group; the row statistics are the lane's own but for two exchanges (lanes 16 and 32 apart). The rows of K are taken in the order
+// that makes those keys, as they stand, the second operand of O^T = V^T P^T: lane group g = lane / 16 holds the keys 16 g .. 16 g + 15
+// of a block, which is also the 16 bytes of a V row that it loads. Nothing goes through LDS on the way.
+//
+// Work: a block of threads takes one key/value head of one sequence, a tile of its rows (tokens x the heads that share the
+// key/value head) and a range of the cache blocks. KS = 4: its four wavefronts share 16 NQ rows and take every fourth cache block
+// (few rows: answered tokens; bound by the cache's bytes), joined through LDS. KS = 1: each has 16 NQ rows of its own (prompts).
+// Where that leaves the device idle, the cache blocks are split over several blocks of threads, whose sums kv_merge_kernel
+// joins in split order.
+#pragma once
+
+#include "kv.h"
+
+namespace h3 {
+
+typedef _Float16 v8h_kv __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h_kv __attribute__((ext_vector_type(2)));
+typedef float v4f_kv __attribute__((ext_vector_type(4)));
+
+// where m starts: below every score, and finite, so that m_old - m is never infinity minus infinity
+constexpr float kKvUnset = -3e38f;
+constexpr float kKvShift = 15.0f;                   // probabilities are held times 2^15
+
+struct KvAttnArgs {
+    KvArgs kv;
+    const int32_t* lengths;
+    const void* q;
+    int64_t q_stride, mask_stride;
+    int q_dt, group, q_heads;
+    float scale;                                    // times log2(e)
+    int window;                                     // 0: all
+    const uint8_t* mask;
+    void* out;
+    int out_dt;
+    float* lse;
+    int tiles, nsplit;                              // row tiles a sequence and head; parts of the cache blocks
+    float *po, *pml;                                // the parts' sums [item, part, rows, W] and (m, l) [item, part, rows, 2]
+    bool q_vec, out_vec, mask_vec;
+};
+
+// four codes as half: 2^10 + (code + 128) in the low bits of a half, less 2^10 + 128 (exact)
+__device__ __forceinline__ void kv_half4(uint32_t u, v2h_kv& a, v2h_kv& b) {
+    const uint32_t x = u ^ 0x80808080u;
+    const v2h_kv off = {(_Float16) -1152.0f, (_Float16) -1152.0f};
+    a = __builtin_bit_cast(v2h_kv, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) + off;
+    b = __builtin_bit_cast(v2h_kv, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + off;
+}
+__device__ __forceinline__ v8h_kv kv_half8(uint32_t u, uint32_t w) {
+    v2h_kv a, b, c, d;
+    kv_half4(u, a, b);
+    kv_half4(w, c, d);
+    return v8h_kv{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+__device__ __forceinline__ v4f_kv kv_mma(const v8h_kv& a, const v8h_kv& b, const v4f_kv& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// over the four lanes that share a query row (16 and 32 apart)
+__device__ __forceinline__ float kv_max4(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    x = fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+}
+__device__ __forceinline__ float kv_sum4(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    x = __int_as_float(r[0]) + __int_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+
+// four consecutive features of an output row
+__device__ __forceinline__ void kv_store4(const KvAttnArgs& P, int64_t at, int d, float a, float b, float c, float e) {
+    const int dim = P.kv.dim;
+    if (P.out_vec) {                                // dim a multiple of 4: all of them or none
+        if (d >= dim) return;
+        if (P.out_dt == H3S_F32) *reinterpret_cast<float4*>((float*) P.out + at + d) = make_float4(a, b, c, e);
+        else if (P.out_dt == H3S_BF16) *reinterpret_cast<uint2*>((uint16_t*) P.out + at + d) = make_uint2(pack_bf16(a, b), pack_bf16(c, e));
+        else *reinterpret_cast<uint2*>((uint16_t*) P.out + at + d) = make_uint2(pack_f16(a, b), pack_f16(c, e));
+    } else {
+        const float f[4] = {a, b, c, e};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < dim) store_any(P.out, P.out_dt, at + d + i, f[i]);
+    }
+}
+// the logarithm of the row's sum of exponentials from the maximum (base 2) and the sum times 2^15
+__device__ __forceinline__ float kv_lse(float m, float l) {
+    return l > 0.0f ? (m + (__builtin_log2f(l) - kKvShift)) * 0.69314718055994531f : l == 0.0f ? -__builtin_inff() : l;
+}
+
+template <int WC, int NQ, int KS, bool TWO>
+__global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
+    constexpr int W = 64 * WC, DT = 4 * WC, RT = 16 * NQ * (KS == 1 ? 4 : 1), PARTS = TWO ? 2 : 1;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
+    int64_t id = blockIdx.x;
+    const int h = (int) (id % P.kv.heads);
+    id /= P.kv.heads;
+    const int split = (int) (id % P.nsplit);
+    id /= P.nsplit;
+    const int b = (int) (id % P.kv.seqs), tile = P.tiles - 1 - (int) (id / P.kv.seqs);      // the longest rows first
+    int r0, n;
+    kv_rows_of(P.kv, b, r0, n);
+    const uint32_t R = (uint32_t) n * P.group, rt0 = (uint32_t) tile * RT;                    // (rows * group is below 2^31)
+    if (rt0 >= R) return;
+    const uint32_t rw = rt0 + (KS == 1 ? wave * 16 * NQ : 0), group = P.group;
+    if (KS == 1 && rw >= R) return;                                                          // (no barrier below for KS = 1)
+    const int len = min(max(P.lengths[b], 0), P.kv.width * kKvB);
+
+    // the query rows: lane % 16 of each of the NQ tiles
+    int pos[NQ];
+    int64_t tok[NQ];
+    int head[NQ];
+    float rowf[NQ];
+    v8h_kv qf[NQ][WC][2][PARTS];
+#pragma unroll
+    for (int e = 0; e < NQ; ++e) {
+        const bool valid = rw + 16 * e + l15 < R;
+        const uint32_t r = valid ? rw + 16 * e + l15 : 0;
+        const int j = (int) (r / group);
+        head[e] = (int) (h * group + r % group);
+        tok[e] = valid ? (int64_t) r0 + j : -1;
+        pos[e] = valid ? len - n + j : -1;
+        const int64_t row = ((int64_t) r0 + j) * P.q_stride + (int64_t) head[e] * P.kv.dim;
+        float f[WC * 2][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < WC; ++c)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int d = c * 64 + g * 16 + s * 8;
+                float* y = f[2 * c + s];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = 0.0f;
+                if (valid && P.q_vec) {
+                    if (d < P.kv.dim) {
+                        if (P.q_dt == H3S_F32) load_f32x((const float*) P.q + row + d, y, 8);
+                        else {
+                            const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*) P.q + row + d);
+                            if (P.q_dt == H3S_BF16) Vec<H3S_BF16>::unpack(u, y);
+                            else Vec<H3S_F16>::unpack(u, y);
+                        }
+                    }
+                } else if (valid) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (d + i < P.kv.dim) y[i] = load_any(P.q, P.q_dt, row + d + i);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(y[i]));
+            }
+        top = kv_max4(top);
+        // 2^k takes top to [2^14, 2^15) (a row of zeros, infinities or NaN: left as it is)
+        const int k = top > 0.0f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+        rowf[e] = __builtin_ldexpf(P.scale, -k);
+#pragma unroll
+        for (int c = 0; c < WC; ++c)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float y = __builtin_ldexpf(f[2 * c + s][i], k);
+                    pin(y);
+                    const _Float16 hi = (_Float16) y;
+                    qf[e][c][s][0][i] = hi;
+                    if constexpr (TWO) qf[e][c][s][1][i] = (_Float16) (y - (float) hi);
+                }
+    }
+
+    // the cache blocks this wavefront walks: those that any of its rows can see, a part of them, every KS-th
+    const int posmin = len - n + (int) (rw / group), posmax = len - n + (int) ((min(R, rw + 16 * NQ) - 1) / group);
+    const int kb0 = P.window > 0 ? max(posmin - P.window + 1, 0) / kKvB : 0;
+    const int count = posmax >= 0 ? posmax / kKvB + 1 - kb0 : 0;
+    const int per = (count + P.nsplit - 1) / P.nsplit;
+    const int last = kb0 + min(count, (split + 1) * per);
+    const int32_t* table = P.kv.table + (int64_t) b * P.kv.width;
+    // the first present block from kb on (its page), or `last`
+    auto present = [&](int& kb, int& page) {
+        for (; kb < last; kb += KS) {
+            page = table[kb];
+            if (page >= 0 && page < P.kv.blocks) return;
+        }
+    };
+    uint4 kr[4][WC], vr[DT];
+    const int koff = ((l15 >> 2) * 16 + (l15 & 3)) * W + g * 16, voff = l15 * 64 + g * 16;
+    auto load_k = [&](int page) {
+        const int8_t* p = P.kv.k + ((int64_t) page * P.kv.heads + h) * (kKvB * W) + koff;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < WC; ++c) kr[t][c] = *reinterpret_cast<const uint4*>(p + t * 4 * W + c * 64);
+    };
+    auto load_v = [&](int page) {
+        const int8_t* p = P.kv.v + ((int64_t) page * P.kv.heads + h) * (kKvB * W) + voff;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) vr[t] = *reinterpret_cast<const uint4*>(p + t * 1024);
+    };
+
+    float m[NQ], l[NQ];
+    v4f_kv o[NQ][DT];
+#pragma unroll
+    for (int e = 0; e < NQ; ++e) {
+        m[e] = kKvUnset;
+        l[e] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[e][t] = v4f_kv{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    int kb = kb0 + split * per + (KS == 1 ? 0 : wave), page = 0;
+    present(kb, page);
+    float ks = 0.0f, vs = 0.0f;
+    if (kb < last) {
+        load_k(page);
+        load_v(page);
+        ks = P.kv.ks[(int64_t) page * P.kv.heads + h];
+        vs = P.kv.vs[(int64_t) page * P.kv.heads + h];
+    }
+    while (kb < last) {
+        int nkb = kb + KS, npage = 0;
+        present(nkb, npage);
+        const bool more = nkb < last;
+        // S^T: register t, i of lane group g is the key 16 g + 4 t + i of the block
+        v4f_kv s[NQ][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int e = 0; e < NQ; ++e) s[e][t] = v4f_kv{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < WC; ++c) {
+                const v8h_kv a0 = kv_half8(kr[t][c].x, kr[t][c].y), a1 = kv_half8(kr[t][c].z, kr[t][c].w);
+#pragma unroll
+                for (int e = 0; e < NQ; ++e) {
+#pragma unroll
+                    for (int w = 0; w < PARTS; ++w) {
+                        s[e][t] = kv_mma(a0, qf[e][c][0][w], s[e][t]);
+                        s[e][t] = kv_mma(a1, qf[e][c][1][w], s[e][t]);
+                    }
+                }
+            }
+        }
+        const float ks_now = ks, vs_now = vs;
+        if (more) {
+            load_k(npage);
+            ks = P.kv.ks[(int64_t) npage * P.kv.heads + h];
+            vs = P.kv.vs[(int64_t) npage * P.kv.heads + h];
+        }
+        const int key0 = kb * kKvB;
+        const bool whole = key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window) && !P.mask;
+        v8h_kv pf[NQ][2][PARTS];
+        float vsl[NQ];
+        uint32_t hidden = 0;                        // by the mask: bit 4 t + i
+        if (!whole && P.mask) {
+            const int k0 = key0 + g * 16;
+            const uint8_t* mp = P.mask + (int64_t) b * P.mask_stride + k0;
+            if (P.mask_vec && k0 + 16 <= P.mask_stride) {
+                const uint4 u = *reinterpret_cast<const uint4*>(mp);
+                const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int i = 0; i < 16; ++i) hidden |= ((w4[i >> 2] >> (8 * (i & 3))) & 0xffu) == 0 ? 1u << i : 0u;
+            } else {
+                for (int i = 0; i < 16; ++i)
+                    if (k0 + i >= P.mask_stride || mp[i] == 0) hidden |= 1u << i;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < NQ; ++e) {
+            float f = rowf[e] * ks_now;
+            f = f < 1e-37f ? 1e-37f : f;            // (minus infinity times it stays minus infinity)
+            uint32_t off = hidden;
+            if (!whole) {
+                const int hi = pos[e] - key0 - g * 16;                  // the lane's keys 0 .. hi of 16 are not ahead of the row
+                off |= hi >= 15 ? 0u : hi < 0 ? 0xffffu : 0xffffu & (0xfffeu << hi);
+                if (P.window > 0) {
+                    const int lo = hi - P.window + 1;                    // and lo .. are inside the window
+                    off |= lo <= 0 ? 0u : lo > 15 ? 0xffffu : (1u << lo) - 1;
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if ((off >> (4 * t + i)) & 1) s[e][t][i] = -__builtin_inff();
+            }
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, s[e][t][i]);
+            top = kv_max4(top);
+            // a block that the row does not see at all has no part in it, whatever its scales are
+            vsl[e] = whole || top > -__builtin_inff() ? vs_now : 0.0f;
+            const float mn = fmaxf(m[e], top * f);
+            if (__any(mn > m[e])) {
+                const float alpha = __builtin_amdgcn_exp2f(m[e] - mn);
+                l[e] *= alpha;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[e][t] *= alpha;
+                m[e] = mn;
+            }
+            const float ref = kKvShift - m[e];
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e][t][i], f, ref));
+                    if (!whole && ((off >> (4 * t + i)) & 1)) p = 0.0f;
+                    sum += p;
+                    const int at = 4 * (t & 1) + i;
+                    const _Float16 hi = (_Float16) p;
+                    pf[e][t >> 1][0][at] = hi;
+                    if constexpr (TWO) pf[e][t >> 1][1][at] = (_Float16) (p - (float) hi);
+                }
+            l[e] += sum;
+        }
+        // O^T
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            const v8h_kv a0 = kv_half8(vr[t].x, vr[t].y), a1 = kv_half8(vr[t].z, vr[t].w);
+#pragma unroll
+            for (int e = 0; e < NQ; ++e) {
+                v4f_kv y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < PARTS; ++w) {
+                    y = kv_mma(a0, pf[e][0][w], y);
+                    y = kv_mma(a1, pf[e][1][w], y);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[e][t][i] = __builtin_fmaf(y[i], vsl[e], o[e][t][i]);
+            }
+        }
+        if (more) load_v(npage);
+        kb = nkb;
+        page = npage;
+    }
+
+#pragma unroll
+    for (int e = 0; e < NQ; ++e) l[e] = kv_sum4(l[e]);
+    const int64_t item = ((int64_t) tile * P.kv.seqs + b) * P.kv.heads + h;
+    if constexpr (KS == 1) {
+#pragma unroll
+        for (int e = 0; e < NQ; ++e) {
+            if (tok[e] < 0) continue;
+            if (P.nsplit == 1) {
+                const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
+                const int64_t at = (tok[e] * P.q_heads + head[e]) * P.kv.dim;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+                    kv_store4(P, at, 16 * t + 4 * g, o[e][t][0] * inv, o[e][t][1] * inv, o[e][t][2] * inv, o[e][t][3] * inv);
+                if (P.lse && g == 0) P.lse[tok[e] * P.q_heads + head[e]] = kv_lse(m[e], l[e]);
+            } else {
+                const int64_t row = (item * P.nsplit + split) * RT + (rw - rt0) + 16 * e + l15;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+                    *reinterpret_cast<float4*>(P.po + row * W + 16 * t + 4 * g) = make_float4(o[e][t][0], o[e][t][1], o[e][t][2], o[e][t][3]);
+                if (g == 0) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(m[e], l[e]);
+            }
+        }
+    } else {
+        // the four wavefronts' sums, 16 rows at a time
+        __shared__ float so[4][16][W + 4];
+        __shared__ float sm[4][16], sl[4][16];
+#pragma unroll
+        for (int e = 0; e < NQ; ++e) {
+            if (e) __syncthreads();
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+                *reinterpret_cast<float4*>(&so[wave][l15][16 * t + 4 * g]) = make_float4(o[e][t][0], o[e][t][1], o[e][t][2], o[e][t][3]);
+            if (g == 0) { sm[wave][l15] = m[e]; sl[wave][l15] = l[e]; }
+            __syncthreads();
+            const int r = threadIdx.x >> 4, c = threadIdx.x & 15;
+            const uint32_t rr = rw + 16 * e + r;
+            if (rr < R) {
+                const float mx = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+                float wt[4], lt = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    wt[w] = __builtin_amdgcn_exp2f(sm[w][r] - mx);
+                    lt += sl[w][r] * wt[w];
+                }
+                const int64_t at = ((int64_t) r0 + rr / group) * P.q_heads + h * group + rr % group;
+                const int64_t row = (item * P.nsplit + split) * RT + 16 * e + r;
+                const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+#pragma unroll
+                for (int t = 0; t < WC; ++t) {
+                    const int d = 64 * t + 4 * c;
+                    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const float4 v = *reinterpret_cast<const float4*>(&so[w][r][d]);
+                        y[0] = __builtin_fmaf(v.x, wt[w], y[0]);
+                        y[1] = __builtin_fmaf(v.y, wt[w], y[1]);
+                        y[2] = __builtin_fmaf(v.z, wt[w], y[2]);
+                        y[3] = __builtin_fmaf(v.w, wt[w], y[3]);
+                    }
+                    if (P.nsplit == 1) kv_store4(P, at * P.kv.dim, d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+                    else *reinterpret_cast<float4*>(P.po + row * W + d) = make_float4(y[0], y[1], y[2], y[3]);
+                }
+                if (c == 0) {
+                    if (P.nsplit > 1) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(mx, lt);
+                    else if (P.lse) P.lse[at] = kv_lse(mx, lt);
+                }
+            }
+        }
+    }
+}
+
+// joins the parts of one row: one block of 256 threads a row, its wavefronts taking every fourth part, in that order
+template <int WC, int RT>
+__global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
+    constexpr int W = 64 * WC;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t item = blockIdx.x / RT;
+    const int r = (int) (blockIdx.x % RT);
+    const int h = (int) (item % P.kv.heads), b = (int) (item / P.kv.heads % P.kv.seqs);
+    int r0, n;
+    kv_rows_of(P.kv, b, r0, n);
+    const uint32_t rr = (uint32_t) (item / P.kv.heads / P.kv.seqs) * RT + r, group = P.group;
+    if (rr >= (uint32_t) n * group) return;
+    const int64_t row0 = item * P.nsplit * RT + r;
+    float mx = kKvUnset;
+    for (int s = lane; s < P.nsplit; s += 64) mx = fmaxf(mx, P.pml[(row0 + (int64_t) s * RT) * 2]);
+    mx = wave_max<64>(mx);
+    float lt = 0.0f;
+    for (int s = lane; s < P.nsplit; s += 64) {
+        const float2 ml = *reinterpret_cast<const float2*>(P.pml + (row0 + (int64_t) s * RT) * 2);
+        lt += ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
+    }
+    lt = wave_sum<64>(lt);
+    float y[WC];
+#pragma unroll
+    for (int t = 0; t < WC; ++t) y[t] = 0.0f;
+#pragma unroll 4
+    for (int s = wave; s < P.nsplit; s += 4) {
+        const int64_t row = row0 + (int64_t) s * RT;
+        const float w = __builtin_amdgcn_exp2f(P.pml[row * 2] - mx);
+#pragma unroll
+        for (int t = 0; t < WC; ++t) y[t] = __builtin_fmaf(P.po[row * W + 64 * t + lane], w, y[t]);
+    }
+    __shared__ float sy[4][W];
+#pragma unroll
+    for (int t = 0; t < WC; ++t) sy[wave][64 * t + lane] = y[t];
+    __syncthreads();
+    const int64_t at = ((int64_t) r0 + rr / group) * P.q_heads + h * group + rr % group;
+    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+    for (int d = threadIdx.x; d < P.kv.dim; d += 256)
+        store_any(P.out, P.out_dt, at * P.kv.dim + d, ((sy[0][d] + sy[1][d]) + (sy[2][d] + sy[3][d])) * inv);
+    if (P.lse && threadIdx.x == 0) P.lse[at] = kv_lse(mx, lt);
+}
+
+// which kernel takes the call, and in how many parts
+struct KvPlan {
+    int nq, ks, rt;       // kv_attn_kernel's, and the rows a block of threads takes
+    int64_t tiles;
+    int nsplit;
+    int64_t blocks;       // of threads, without the parts
+};
+
+template <int WC, int NQ, int KS>
+static void kv_attn_run(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two) {
+    const unsigned grid = (unsigned) (plan.blocks * plan.nsplit);
+    if (two) kv_attn_kernel<WC, NQ, KS, true><<<grid, 256, 0, c->stream>>>(P);
+    else kv_attn_kernel<WC, NQ, KS, false><<<grid, 256, 0, c->stream>>>(P);
+    constexpr int RT = 16 * NQ * (KS == 1 ? 4 : 1);
+    if (plan.nsplit > 1) kv_merge_kernel<WC, RT><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
+}
+
+// heads of up to 64 WC features (kv_attn_64.hip .. kv_attn_256.hip)
+void kv_attn_64(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
+void kv_attn_128(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
+void kv_attn_192(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
+void kv_attn_256(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
+
+template <int WC>
+static void kv_attn_width(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two) {
+    if (plan.ks == 4 && plan.nq == 1) kv_attn_run<WC, 1, 4>(c, P, plan, two);
+    else if (plan.ks == 4) kv_attn_run<WC, 2, 4>(c, P, plan, two);
+    else kv_attn_run<WC, 2, 1>(c, P, plan, two);
+}
+
+}  // namespace h3

@@ -1,0 +1,363 @@
+// kv_cache.hip - the 8-bit key/value cache's own operators (h3lm.h): kv_write (new tokens into their blocks) and kv_read
+// (tokens out of them as values), and the table of function pointers that reaches all of h3lm.h.
+//
+// Mathematics: a block is 64 tokens of one head, keys or values, with one scale s = max|x| / 127 over all of it, so a code is
+// off by at most s / 2. A block that tokens join later keeps its scale unless a larger token comes: then s' = max|x| / 127 of
+// the newcomers, and the old codes are rounded again at s' (c' = rint(c s / s')). One block of threads owns one cache block of
+// one head and side, so it finds the maximum, rescales and writes with no other writer and no atomics.
+#include <algorithm>
+
+#include "kv.h"
+
+namespace h3 {
+
+int kv_args(const std::string& fn, const h3_kv_cache* cache, const h3_kv_batch* batch, KvArgs& P) {
+    if (!cache || !batch) return fail(fn + ": the cache and the batch are required");
+    const h3_kv_cache& c = *cache;
+    const h3_kv_batch& q = *batch;
+    if (c.blocks <= 0 || c.heads <= 0 || c.dim <= 0 || c.dim > 256) return fail(fn + ": a cache has blocks, heads and 1 to 256 features a head");
+    if (c.blocks > INT32_MAX || c.heads > 65535) return fail(fn + ": too many blocks or heads");
+    if (q.seqs < 0 || q.rows < 0 || q.width < 0 || q.most < 0) return fail(fn + ": a negative size");
+    if (q.rows > INT32_MAX || q.seqs >= INT32_MAX || q.width > (INT32_MAX - 64) / kKvB) return fail(fn + ": sizes past 32 bits");
+    if (!c.k || !c.v || !c.k_scale || !c.v_scale) return fail(fn + ": the cache's codes and scales are required");
+    if (!aligned16(c.k) || !aligned16(c.v)) return fail(fn + ": the cache's codes must be 16-byte aligned");
+    if (q.seqs > 0 && (!q.starts || (q.width > 0 && !q.table))) return fail(fn + ": the table and the starts are required");
+    P = KvArgs{c.k, c.v, c.k_scale, c.v_scale, c.blocks, (int) c.heads, (int) c.dim, q.table, q.starts, (int) q.width, (int) q.seqs, (int) q.rows};
+    return 0;
+}
+
+// the maximum over a block of 256 threads, on every thread; a NaN anywhere gives NaN
+__device__ __forceinline__ float block_max(float m, bool nan) {
+    __shared__ float red[4];
+    __shared__ int bad[4];
+    m = wave_max<64>(m);
+    const int any = __any(nan);
+    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = m; bad[threadIdx.x >> 6] = any; }
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    return (bad[0] | bad[1] | bad[2] | bad[3]) ? __builtin_nanf("") : m;
+}
+
+// 16 consecutive elements of a row from feature d0 on, zeros from `dim` on; vec: 16-byte loads (dim and the row's start allow
+// them: dim a multiple of 8, so a run of 8 features is all in or all out)
+__device__ __forceinline__ void load16(const void* p, int dt, int64_t row, int d0, int dim, bool vec, float* f) {
+    if (vec) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int d = d0 + 8 * h;
+            if (d < dim) {
+                if (dt == H3S_F32) load_f32x((const float*) p + row + d, f + 8 * h, 8);
+                else {
+                    const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*) p + row + d);
+                    if (dt == H3S_BF16) Vec<H3S_BF16>::unpack(u, f + 8 * h);
+                    else Vec<H3S_F16>::unpack(u, f + 8 * h);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[8 * h + i] = 0.0f;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = d0 + i < dim ? load_any(p, dt, row + d0 + i) : 0.0f;
+    }
+}
+
+__device__ __forceinline__ uint32_t byte_of(const uint4& u, int i) {
+    const uint32_t w = i < 4 ? u.x : i < 8 ? u.y : i < 12 ? u.z : u.w;
+    return w >> (8 * (i & 3));
+}
+// the old codes of a 16-byte piece at the new scale, at the places where `keep` has a bit; zeros elsewhere
+__device__ __forceinline__ uint4 rescaled(const uint4& u, float ratio, uint32_t keep) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float v = __builtin_rintf((float) (int8_t) byte_of(u, 4 * q + i) * ratio);
+            // (a ratio that is not finite belongs to a scale that is not: the code then says nothing, and 0 is as good)
+            c[i] = (keep >> (4 * q + i)) & 1 ? fminf(fmaxf(v, -127.0f), 127.0f) : 0.0f;
+        }
+        w[q] = pack_i8x4(c[0], c[1], c[2], c[3]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct KvWriteArgs {
+    KvArgs kv;
+    const int32_t* past;
+    const void *xk, *xv;
+    int64_t k_stride, v_stride;
+    int dt, nb;              // nb: blocks a sequence may touch
+    int k_vec, v_vec;        // whole 16-byte pieces
+};
+// (Chosen between, never indexed by the side: an index into the kernel's arguments became a scalar load whose base and offset
+// were no multiples of 4 by themselves, and scalar loads drop the two low bits of each.)
+
+// One block of threads: one cache block of one head, keys (side 0) or values (side 1). Thread t holds the
+// pieces t + 256 p of 16 features, 4 WC pieces a token. Bound by latency for single tokens (one load, a maximum over the block, one store)
+// and by the rows' bytes for prompts. 8 heads of 128, bfloat16: see the table of cases.
+template <int WC>
+__global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs A) {
+    constexpr int W = 64 * WC, TPR = 4 * WC;                                // 16-feature pieces a token
+    const KvArgs& P = A.kv;
+    __shared__ __align__(16) uint8_t codes[W * (kKvB + 4)];                               // values: the new codes, a feature's tokens side by side
+    int64_t id = blockIdx.x;
+    const int side = (int) (id & 1);
+    id >>= 1;
+    const int h = (int) (id % P.heads);
+    id /= P.heads;
+    const int i = (int) (id % A.nb), b = (int) (id / A.nb);
+    int r0, n;
+    kv_rows_of(P, b, r0, n);
+    const int64_t past = max(A.past[b], 0), end = min(past + n, (int64_t) P.width * kKvB);
+    const int64_t j = past / kKvB + i;                                      // the sequence's block
+    if (end <= past || j * kKvB >= end) return;                             // (no new token: the block is not touched)
+    const int page = P.table[(int64_t) b * P.width + j];
+    if (page < 0 || page >= P.blocks) return;
+    const int kept = (int) max(past - j * kKvB, (int64_t) 0);               // its tokens [0, kept) were there
+    const int last = (int) min(end - j * kKvB, (int64_t) kKvB);             // and [kept, last) are new
+    const int64_t row0 = r0 + (j * kKvB - past);                            // the row of its token 0 (with kept > 0: before r0)
+    const int64_t tile = ((int64_t) page * P.heads + h);
+    const int t = threadIdx.x;
+    const void* x = side ? A.xv : A.xk;
+    const int64_t stride = side ? A.v_stride : A.k_stride;
+    const bool vec = (side ? A.v_vec : A.k_vec) != 0;
+
+    float f[WC][16];
+    float m = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int p = 0; p < WC; ++p) {
+        const int tok = (t + 256 * p) / TPR, d0 = (t + 256 * p) % TPR * 16;
+        if (tok >= kept && tok < last) {
+            load16(x, A.dt, (row0 + tok) * stride + (int64_t) h * P.dim, d0, P.dim, vec, f[p]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) f[p][e] = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            m = fmaxf(m, fabsf(f[p][e]));
+            nan = nan || f[p][e] != f[p][e];
+        }
+    }
+    m = block_max(m, nan);
+    float* scale = (side ? P.vs : P.ks) + tile;
+    const float was = kept ? *scale : 0.0f;
+    float s = m / 127.0f;
+    // (a NaN on either side wins)
+    s = s != s ? s : was > s || was != was ? was : s;
+    s = s < 1e-30f ? 1e-30f : s;
+    const bool moved = kept && s != was;                                    // (NaN: rescaled, to no effect)
+    const float ratio = was / s;
+    __syncthreads();                                                        // every thread has read the old scale
+    if (t == 0) *scale = s;
+
+    int8_t* base = (side ? P.v : P.k) + tile * kKvB * W;
+#pragma unroll
+    for (int p = 0; p < WC; ++p) {
+        const int tok = (t + 256 * p) / TPR, d0 = (t + 256 * p) % TPR * 16;
+        uint32_t w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float c[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] = fminf(fmaxf(__builtin_rintf(f[p][4 * q + e] / s), -127.0f), 127.0f);
+            w[q] = pack_i8x4(c[0], c[1], c[2], c[3]);
+        }
+        if (side == 0) {
+            uint4* dst = reinterpret_cast<uint4*>(base + (int64_t) tok * W + d0);
+            if (tok >= kept) *dst = make_uint4(w[0], w[1], w[2], w[3]);
+            else if (moved) *dst = rescaled(*dst, ratio, 0xffffu);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) codes[(d0 + e) * (kKvB + 4) + tok] = (uint8_t) (w[e / 4] >> (8 * (e & 3)));
+        }
+    }
+    if (side == 0) return;
+    __syncthreads();
+    // values: 16-byte pieces of 16 tokens of one feature; pieces of old tokens only are left alone unless the scale moved
+#pragma unroll
+    for (int p = 0; p < WC; ++p) {
+        const int piece = t + 256 * p, d = piece / 4, k0 = (piece % 4) * 16;
+        const int old = min(max(kept - k0, 0), 16);
+        if (old == 16 && !moved) continue;
+        uint4* dst = reinterpret_cast<uint4*>(base + (int64_t) d * kKvB + k0);
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (old) {
+            u = *dst;
+            if (moved) u = rescaled(u, ratio, (1u << old) - 1);
+        }
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(codes + d * (kKvB + 4) + k0);
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int o = min(max(old - 4 * q, 0), 4);                      // old tokens in this word
+            const uint32_t mask = o == 4 ? 0xffffffffu : (1u << (8 * o)) - 1;
+            w[q] = (w[q] & mask) | (src[q] & ~mask);
+        }
+        *dst = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+struct KvReadArgs {
+    KvArgs kv;
+    const int32_t* first;
+    void *xk, *xv;
+    int64_t k_stride, v_stride;
+    int dt, nb;
+    int k_vec, v_vec;
+};
+
+__device__ __forceinline__ void store16(void* p, int dt, int64_t row, int d0, int dim, bool vec, const float* f) {
+    if (vec) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int d = d0 + 8 * h;
+            if (d >= dim) continue;
+            if (dt == H3S_F32) {
+                float4* o = reinterpret_cast<float4*>((float*) p + row + d);
+                o[0] = make_float4(f[8 * h], f[8 * h + 1], f[8 * h + 2], f[8 * h + 3]);
+                o[1] = make_float4(f[8 * h + 4], f[8 * h + 5], f[8 * h + 6], f[8 * h + 7]);
+            } else {
+                *reinterpret_cast<uint4*>((uint16_t*) p + row + d) =
+                    dt == H3S_BF16 ? Vec<H3S_BF16>::pack(f + 8 * h) : Vec<H3S_F16>::pack(f + 8 * h);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (d0 + i < dim) store_any(p, dt, row + d0 + i, f[i]);
+    }
+}
+
+// One block of threads: the tokens that a read takes out of one cache block of one head and side (layout as kv_write_kernel).
+template <int WC>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs A) {
+    constexpr int W = 64 * WC, TPR = 4 * WC;
+    const KvArgs& P = A.kv;
+    __shared__ __align__(16) uint8_t codes[W * (kKvB + 4)];
+    int64_t id = blockIdx.x;
+    const int side = (int) (id & 1);
+    id >>= 1;
+    const int h = (int) (id % P.heads);
+    id /= P.heads;
+    const int i = (int) (id % A.nb), b = (int) (id / A.nb);
+    int r0, n;
+    kv_rows_of(P, b, r0, n);
+    const int64_t first = max(A.first[b], 0), end = first + n;
+    const int64_t j = first / kKvB + i;
+    if (j * kKvB >= end) return;
+    const int page = j < P.width ? P.table[(int64_t) b * P.width + j] : -1;
+    const bool there = page >= 0 && page < P.blocks;
+    const int from = (int) max(first - j * kKvB, (int64_t) 0), to = (int) min(end - j * kKvB, (int64_t) kKvB);
+    const int64_t row0 = r0 + (j * kKvB - first), tile = (int64_t) (there ? page : 0) * P.heads + h;
+    const float s = there ? (side ? P.vs : P.ks)[tile] : 0.0f;
+    const int8_t* base = (side ? P.v : P.k) + tile * kKvB * W;
+    const int t = threadIdx.x;
+    void* x = side ? A.xv : A.xk;
+    const int64_t stride = side ? A.v_stride : A.k_stride;
+    const bool vec = (side ? A.v_vec : A.k_vec) != 0;
+    if (side == 1) {
+#pragma unroll
+        for (int p = 0; p < WC; ++p) {
+            const int piece = t + 256 * p, d = piece / 4, k0 = (piece % 4) * 16;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (there) u = *reinterpret_cast<const uint4*>(base + (int64_t) d * kKvB + k0);
+            uint32_t* dst = reinterpret_cast<uint32_t*>(codes + d * (kKvB + 4) + k0);
+            dst[0] = u.x; dst[1] = u.y; dst[2] = u.z; dst[3] = u.w;
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int p = 0; p < WC; ++p) {
+        const int tok = (t + 256 * p) / TPR, d0 = (t + 256 * p) % TPR * 16;
+        if (tok < from || tok >= to) continue;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (side == 0 && there) u = *reinterpret_cast<const uint4*>(base + (int64_t) tok * W + d0);
+        float f[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            f[e] = there ? (float) (int8_t) (side ? codes[(d0 + e) * (kKvB + 4) + tok] : byte_of(u, e)) * s : 0.0f;
+        store16(x, A.dt, (row0 + tok) * stride + (int64_t) h * P.dim, d0, P.dim, vec, f);
+    }
+}
+
+// what kv_write and kv_read check alike; nb: the blocks that `most` rows of a sequence can lie in
+static int row_checks(const std::string& fn, const KvArgs& P, const h3_kv_batch& q, const int32_t* at, const char* at_name, const void* k,
+                      int64_t k_stride, const void* v, int64_t v_stride, int dt, int64_t* nb) {
+    const int64_t feats = (int64_t) P.heads * P.dim;
+    if (!dt_ok(dt)) return fail(fn + ": unknown element type");
+    if (!at || !k || !v) return fail(fn + ": k, v and " + at_name + " are required");
+    if (k_stride < feats || v_stride < feats) return fail(fn + ": a row stride is shorter than a row");
+    *nb = (std::min<int64_t>(q.most, P.rows) + kKvB - 2) / kKvB + 1;
+    if (*nb * P.seqs > 0x7fffffff / 2 / P.heads) return fail(fn + ": too many blocks of work");
+    return 0;
+}
+// whether rows of k or v can be taken in 16-byte pieces
+static bool rows_vec(const void* p, int64_t stride, int dim, int dt) {
+    return aligned16(p) && dim % 8 == 0 && (stride * elem_size(dt)) % 16 == 0;
+}
+
+int kv_write(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* past, const void* k, int64_t k_stride,
+             const void* v, int64_t v_stride, int dt) try {
+    const char* fn = "kv_write";
+    KvWriteArgs A;
+    if (kv_args(fn, cache, batch, A.kv)) return -1;
+    if (A.kv.seqs == 0 || A.kv.rows == 0 || batch->most == 0 || A.kv.width == 0) return 0;
+    int64_t nb;
+    if (row_checks(fn, A.kv, *batch, past, "past", k, k_stride, v, v_stride, dt, &nb)) return -1;
+    Ctx* c = ctx_of(ctx, fn);
+    if (!c) return -1;
+    A.past = past;
+    A.xk = k; A.xv = v;
+    A.k_stride = k_stride; A.v_stride = v_stride;
+    A.dt = dt; A.nb = (int) nb;
+    A.k_vec = rows_vec(k, k_stride, A.kv.dim, dt);
+    A.v_vec = rows_vec(v, v_stride, A.kv.dim, dt);
+    const unsigned grid = (unsigned) (nb * A.kv.seqs * A.kv.heads * 2);
+    switch (kv_width(A.kv.dim) / 64) {
+        case 1: kv_write_kernel<1><<<grid, 256, 0, c->stream>>>(A); break;
+        case 2: kv_write_kernel<2><<<grid, 256, 0, c->stream>>>(A); break;
+        case 3: kv_write_kernel<3><<<grid, 256, 0, c->stream>>>(A); break;
+        default: kv_write_kernel<4><<<grid, 256, 0, c->stream>>>(A); break;
+    }
+    return launched(fn);
+} catch (const std::exception& e) { return fail(e.what()); }
+
+int kv_read(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* first, void* k, int64_t k_stride, void* v,
+            int64_t v_stride, int dt) try {
+    const char* fn = "kv_read";
+    KvReadArgs A;
+    if (kv_args(fn, cache, batch, A.kv)) return -1;
+    if (A.kv.seqs == 0 || A.kv.rows == 0 || batch->most == 0) return 0;
+    int64_t nb;
+    if (row_checks(fn, A.kv, *batch, first, "first", k, k_stride, v, v_stride, dt, &nb)) return -1;
+    Ctx* c = ctx_of(ctx, fn);
+    if (!c) return -1;
+    A.first = first;
+    A.xk = k; A.xv = v;
+    A.k_stride = k_stride; A.v_stride = v_stride;
+    A.dt = dt; A.nb = (int) nb;
+    A.k_vec = rows_vec(k, k_stride, A.kv.dim, dt);
+    A.v_vec = rows_vec(v, v_stride, A.kv.dim, dt);
+    const unsigned grid = (unsigned) (nb * A.kv.seqs * A.kv.heads * 2);
+    switch (kv_width(A.kv.dim) / 64) {
+        case 1: kv_read_kernel<1><<<grid, 256, 0, c->stream>>>(A); break;
+        case 2: kv_read_kernel<2><<<grid, 256, 0, c->stream>>>(A); break;
+        case 3: kv_read_kernel<3><<<grid, 256, 0, c->stream>>>(A); break;
+        default: kv_read_kernel<4><<<grid, 256, 0, c->stream>>>(A); break;
+    }
+    return launched(fn);
+} catch (const std::exception& e) { return fail(e.what()); }
+
+}  // namespace h3
+
+// (host only: a constant of function addresses would otherwise be emitted into the device code as well)
+#ifndef __HIP_DEVICE_COMPILE__
+extern "C" __attribute__((visibility("default"))) const h3_lm_api h3lm = {
+    (int64_t) sizeof(h3_lm_api), h3::kv_write, h3::kv_read, h3::kv_attention, h3::kv_attention_work, h3::linear4,
+};
+#endif

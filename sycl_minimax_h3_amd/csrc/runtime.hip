@@ -109,6 +109,7 @@ static const char* region_name(Ctx::Region r) {
         case Ctx::ATT_V: return "attention scratch (v)";
         case Ctx::ATT_AUX: return "attention scratch (scales and k's mean)";
         case Ctx::ATT_PART: return "attention scratch (partial sums)";
+        case Ctx::KV_PART: return "cached attention scratch (partial sums)";
         case Ctx::LIN_F32: return "linear scratch (float32 product)";
         default: return "scratch";
     }

@@ -7,6 +7,7 @@ entry points of include/h3hip.h come after the reference's operations.
 """
 from __future__ import annotations
 
+import ctypes as _C
 from dataclasses import dataclass
 
 from . import api as _api
@@ -401,3 +402,159 @@ def int8_quantize(x: Tensor, q: Tensor, s: Tensor, group: int = 0) -> None:
         raise Error(f"int8_quantize: q {q.dtype} {q.shape} / s {s.dtype} {s.shape} for x {x.shape}")
     dev = _dev(x)
     dev.check(dev.api.int8_quantize(dev.ctx, x.ptr(), x.dtype.kernel_code(), m, k, group, q.ptr(), s.ptr()))
+
+
+# ---- the operators of include/h3lm.h: an 8-bit key/value cache, the attention over it, linear layers with 4-bit weights ----
+
+KV_BLOCK = _api.KV_BLOCK   # tokens in a block of the cache
+
+
+def _i32(t: Tensor, what: str, n: int) -> int:
+    if t.dtype != DType.I32 or t.elements() < n:
+        raise Error(f"{what} must be int32 with at least {n} values, got {t.dtype} {t.shape}")
+    return t.ptr()
+
+
+class KvCache:
+    """One layer's key/value cache in blocks of KV_BLOCK tokens (h3_kv_cache): codes k int8 [blocks, heads, 64, w] and v
+    int8 [blocks, heads, w, 64], w = dim up to a multiple of 64, and float32 scales [blocks, heads]."""
+
+    def __init__(self, k: Tensor, v: Tensor, k_scale: Tensor, v_scale: Tensor, dim: int):
+        w = KvCache.width(dim)
+        if len(k.shape) != 4 or k.dtype != DType.I8 or k.shape[2] != KV_BLOCK or k.shape[3] != w:
+            raise Error(f"kv cache: k must be int8 [blocks, heads, {KV_BLOCK}, {w}], got {k.dtype} {k.shape}")
+        blocks, heads = int(k.shape[0]), int(k.shape[1])
+        if v.dtype != DType.I8 or list(v.shape) != [blocks, heads, w, KV_BLOCK]:
+            raise Error(f"kv cache: v must be int8 {[blocks, heads, w, KV_BLOCK]}, got {v.dtype} {v.shape}")
+        for t, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t.dtype != DType.F32 or t.elements() != blocks * heads:
+                raise Error(f"kv cache: {what} must be float32 {[blocks, heads]}, got {t.dtype} {t.shape}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.blocks, self.heads, self.dim = blocks, heads, int(dim)
+        self._c = _api.KvCache(k.ptr(), v.ptr(), k_scale.ptr(), v_scale.ptr(), blocks, heads, dim)
+
+    @staticmethod
+    def width(dim: int) -> int:
+        """The features that a head's codes hold: dim up to a multiple of 64."""
+        if not 1 <= dim <= 256:
+            raise Error(f"kv cache: {dim} features a head (1 to 256)")
+        return (int(dim) + 63) // 64 * 64
+
+    @staticmethod
+    def new(dev, blocks: int, heads: int, dim: int) -> "KvCache":
+        """A cache of its own memory; a block's contents are undefined until tokens are written into it."""
+        w = KvCache.width(dim)
+        return KvCache(Tensor.new(dev, DType.I8, [blocks, heads, KV_BLOCK, w]), Tensor.new(dev, DType.I8, [blocks, heads, w, KV_BLOCK]),
+                       Tensor.new(dev, DType.F32, [blocks, heads]), Tensor.new(dev, DType.F32, [blocks, heads]), dim)
+
+
+def _kv_batch(table: Tensor, starts: Tensor, rows: int, most: int):
+    """The batch of a call: table int32 [seqs, width], starts int32 [seqs + 1]."""
+    if table.dtype != DType.I32 or len(table.shape) != 2:
+        raise Error(f"the block table must be int32 [sequences, blocks], got {table.dtype} {table.shape}")
+    seqs, width = int(table.shape[0]), int(table.shape[1])
+    if starts.dtype != DType.I32 or starts.elements() != seqs + 1:
+        raise Error(f"starts must be int32 [{seqs + 1}], got {starts.dtype} {starts.shape}")
+    if most < 0:
+        raise Error(f"the most rows of a sequence: {most}")
+    return _api.KvBatch(table.ptr(), starts.ptr(), seqs, width, rows, most)
+
+
+def _kv_rows(fn: str, cache: KvCache, k: Rows, v: Rows) -> None:
+    if (k.heads, k.dim) != (cache.heads, cache.dim) or (v.heads, v.dim) != (cache.heads, cache.dim):
+        raise Error(f"{fn}: k and v of {k.heads} x {k.dim} and {v.heads} x {v.dim} for a cache of {cache.heads} x {cache.dim}")
+    if k.tokens != v.tokens or k.t.dtype != v.t.dtype:
+        raise Error(f"{fn}: k and v must share their rows and their type")
+
+
+def kv_write(cache: KvCache, table: Tensor, k: Rows, v: Rows, starts: Tensor, past: Tensor, most: int) -> None:
+    """New tokens into the cache: row starts[b] + j of k and v becomes token past[b] + j of sequence b, in block table[b, p // 64].
+    starts int32 [sequences + 1], past int32 [sequences] (the tokens that each has in the cache already), most: at least the
+    most rows of any sequence. A block has one scale for each head; where larger tokens join old ones, those are rounded again."""
+    _kv_rows("kv_write", cache, k, v)
+    batch = _kv_batch(table, starts, k.tokens, most)
+    args = (_i32(past, "past", batch.seqs), k.ptr(), k.stride, v.ptr(), v.stride, k.t.dtype.kernel_code())
+    dev = _dev(cache.k)
+    dev.check(dev.api.lm.kv_write(dev.ctx, _C.byref(cache._c), _C.byref(batch), *args))
+
+
+def kv_read(cache: KvCache, table: Tensor, starts: Tensor, first: Tensor, most: int, k: Rows, v: Rows) -> None:
+    """Tokens out of the cache as values: row starts[b] + j of k and v receives token first[b] + j of sequence b."""
+    _kv_rows("kv_read", cache, k, v)
+    batch = _kv_batch(table, starts, k.tokens, most)
+    args = (_i32(first, "first", batch.seqs), k.ptr(), k.stride, v.ptr(), v.stride, k.t.dtype.kernel_code())
+    dev = _dev(cache.k)
+    dev.check(dev.api.lm.kv_read(dev.ctx, _C.byref(cache._c), _C.byref(batch), *args))
+
+
+def kv_attention_work(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, most: int, *, max_len: int = 0, window: int = 0) -> int:
+    """The bytes of workspace that kv_attention takes for these arguments (0: none)."""
+    batch = _kv_batch(table, starts, q.tokens, most)
+    dev = _dev(cache.k)
+    n = dev.api.lm.kv_attention_work(dev.ctx, _C.byref(cache._c), _C.byref(batch), max_len, q.heads, window)
+    if n < 0:
+        raise Error(dev.api.error())
+    return n
+
+
+def kv_attention(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, lengths: Tensor, most: int, out: Tensor, *, max_len: int = 0,
+                 window: int = 0, mask: Tensor | None = None, scale: float = 0.0, lse: Tensor | None = None,
+                 work: Tensor | None = None) -> None:
+    """Causal attention of each sequence's newest tokens (rows starts[b] .. of q) over its lengths[b] tokens in the cache, those
+    newest ones among them: softmax(q k^T scale) v per head, query head h reading head h // (q.heads // cache.heads). out
+    [rows, q.heads * dim]. scale 0: 1 / sqrt(dim). window: only the last so many tokens; mask uint8 [sequences, n]: only tokens
+    whose byte is not 0 (tokens from n on are hidden); a row that sees nothing gets zeros. lse float32 [rows, q.heads]: the
+    logarithm of each row's sum of exponentials. max_len: about the longest length (0: the table's width). work: a workspace of
+    kv_attention_work() bytes, which a call recorded into a graph has to bring if that is not 0."""
+    if q.dim != cache.dim:
+        raise Error(f"kv_attention: q heads of {q.dim} for a cache of {cache.dim}")
+    if out.elements() != q.tokens * q.heads * q.dim:
+        raise Error(f"kv_attention: out {out.shape} for {q.tokens} rows of {q.heads} x {q.dim}")
+    batch = _kv_batch(table, starts, q.tokens, most)
+    mask_p, mask_n = None, 0
+    if mask is not None:
+        if mask.dtype not in (DType.U8, DType.I8) or len(mask.shape) != 2 or mask.shape[0] != batch.seqs:
+            raise Error(f"kv_attention: the mask must be uint8 [{batch.seqs}, tokens], got {mask.dtype} {mask.shape}")
+        mask_p, mask_n = mask.ptr(), int(mask.shape[1])
+    if lse is not None and (lse.dtype != DType.F32 or lse.elements() != q.tokens * q.heads):
+        raise Error(f"kv_attention: lse must be float32 [{q.tokens}, {q.heads}], got {lse.dtype} {lse.shape}")
+    args = (_i32(lengths, "lengths", batch.seqs), max_len, q.ptr(), q.stride, q.t.dtype.kernel_code(), q.heads, scale, window, mask_p,
+            mask_n, out.ptr(), out.dtype.kernel_code(), _p(lse), _p(work), work.nbytes() if work is not None else 0)
+    dev = _dev(cache.k)
+    dev.check(dev.api.lm.kv_attention(dev.ctx, _C.byref(cache._c), _C.byref(batch), *args))
+
+
+@dataclass
+class Int4Linear:
+    """A linear layer with 4-bit weights: codes uint8 [N, K / 2] (byte i of a row: inputs 2 i in the low four bits, 2 i + 1), scale
+    [N, K / group] in a float type; weight = scale * (code - 8), or scale * code - mins with mins like scale."""
+
+    weight: Tensor
+    scale: Tensor
+    mins: Tensor | None = None
+    bias: Tensor | None = None
+
+    def inputs(self) -> int:
+        return 2 * self.weight.shape[1]
+
+    def outputs(self) -> int:
+        return self.weight.shape[0]
+
+    def forward(self, x: Tensor, out: Tensor) -> None:
+        """out = linear(x): x [M, K] in a float type, out [M, N] in out's type."""
+        if self.weight.dtype != DType.U8 or len(self.weight.shape) != 2:
+            raise Error(f"int4_linear: the weight must be uint8 [N, K / 2], got {self.weight.dtype} {self.weight.shape}")
+        n, k = self.outputs(), self.inputs()
+        if k == 0 or n == 0:
+            raise Error(f"int4_linear: an empty weight {self.weight.shape}")
+        m = x.elements() // k
+        if x.elements() != m * k or out.elements() != m * n:
+            raise Error(f"int4_linear: x {x.shape} and out {out.shape} do not fit a [{n}, {k}] weight")
+        if len(self.scale.shape) != 2 or self.scale.shape[0] != n or self.scale.shape[1] == 0 or k % self.scale.shape[1]:
+            raise Error(f"int4_linear: scales {self.scale.shape} for a [{n}, {k}] weight")
+        if self.mins is not None and (list(self.mins.shape) != list(self.scale.shape) or self.mins.dtype != self.scale.dtype):
+            raise Error(f"int4_linear: minima {self.mins.dtype} {self.mins.shape} for scales {self.scale.dtype} {self.scale.shape}")
+        bias = _floats(self.bias, "the bias", n) if self.bias is not None else None
+        dev = _dev(x)
+        dev.check(dev.api.lm.linear4(dev.ctx, x.ptr(), x.dtype.kernel_code(), m, k, self.weight.ptr(), n, self.scale.ptr(), _p(self.mins),
+                                     self.scale.dtype.kernel_code(), k // self.scale.shape[1], bias, out.ptr(), out.dtype.kernel_code()))

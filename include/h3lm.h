@@ -90,7 +90,7 @@ typedef struct {
      * a row holds the codes of inputs 2 i (low four bits) and 2 i + 1. With g = k / group and scale [N, K / group] of type scale_dt:
      *     W[n, k] = scale[n, g] * (code - 8)            mins NULL
      *     W[n, k] = scale[n, g] * code - mins[n, g]     mins [N, K / group] of type scale_dt
-     * group: a multiple of 32 that divides K. Float32 sums; bias float32 [N] or NULL, added before the one rounding. codes and x
+     * group: a multiple of 32 that divides K, and K at most 2^20. Float32 sums; bias float32 [N] or NULL, added before the one rounding. codes and x
      * 16-byte aligned, rows whole 16-byte pieces (K a multiple of 32 makes them so). out may not overlap x. No workspace. */
     int (*linear4)(void* ctx, const void* x, int dt, int64_t M, int64_t K, const uint8_t* codes, int64_t N, const void* scale,
                    const void* mins, int scale_dt, int64_t group, const float* bias, void* out, int out_dt);

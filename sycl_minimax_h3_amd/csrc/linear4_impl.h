@@ -1,0 +1,749 @@
+// linear4_impl.h - linear layers with 4-bit weights and group scales (h3lm.h, linear4).
+//
+// Mathematics: with w = s c - z in each group of inputs (z the group's minimum, or 8 s),
+//     y = sum over groups of  s (sum x c) - z (sum x)  =  s (sum x (16 + c)) - (16 s + z) (sum x).
+// A code put into the top four bits of the mantissa of a bfloat16 or half with the exponent of 16 is the number 16 + c, exactly:
+// a shift and one and-or for two codes, with no conversion. The products sum x (16 + c) of a run of 32 inputs are one matrix
+// instruction (16 x 16 x 32, float32 sums) with x as it stands (bfloat16, half; float32 as three bfloat16 parts). A run's sum of x is one
+// more, with a first operand of ones in one row, shared by all columns of the wavefront; it leaves the sums of four runs as the
+// first operand of a float32 instruction (16 x 16 x 4) whose second is the four 16 s + z: their products are one instruction for 128
+// inputs. What is left for the vector units is one multiply-add by s a group and output. (16 against c of 0 .. 15: the two terms are
+// at most some five times their difference, so float32 sums lose little over two bits.)
+//
+// Layout: a lane loads 16 bytes of a weight row, 32 codes; the four lanes of a row (16 apart) hold 128 consecutive inputs. A 4 x 4
+// exchange between them (four lane swaps) leaves each with eight codes of each of four runs of 32 inputs, so that an instruction's 32
+// inputs lie in one group.
+//
+// Work. Up to 16 rows (linear4_few_kernel): a wavefront takes 16 NT columns and every KW-th 128 inputs; the KW wavefronts of a block
+// are joined through LDS in wavefront order. Bound by the codes' bytes: everything that a step needs is loaded a step ahead.
+// More rows (linear4_many_kernel): a block takes 16 MT rows x 128 columns, in two groups of four wavefronts that take every other 128
+// inputs; x goes through LDS, in the order of the instructions' operands, and each wavefront has 32 columns.
+#pragma once
+
+#include "kv.h"
+
+namespace h3 {
+
+typedef __bf16 v8bf_l4 __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h_l4 __attribute__((ext_vector_type(8)));
+typedef float v4f_l4 __attribute__((ext_vector_type(4)));
+
+struct L4Args {
+    const void* x;
+    int64_t M, N;
+    int K;                            // at most kL4MostK
+    const uint8_t* codes;
+    const void *scale, *mins;         // without minima: mins is scale (and not used)
+    int scale_dt, has_mins;
+    int group, groups;                // inputs a group; groups a row
+    uint32_t magic;                   // 2^32 / (group / 32), rounded up (0: groups of 32)
+    const float* bias;
+    void* out;
+    int out_dt;
+};
+
+constexpr int kL4MostK = 1 << 20;
+// the group of the run r of 32 inputs: r / (group / 32) by a multiplication. With g = group / 32 and magic = (2^32 + e) / g, e < g, the
+// product is r / g + r e / (2^32 g): the quotient is right where r e < 2^32, and r and g are at most 2^15
+__device__ __forceinline__ int l4_group(const L4Args& P, int r) { return P.magic ? (int) __umulhi((uint32_t) r, P.magic) : r; }
+
+template <int OP> __device__ __forceinline__ v4f_l4 l4_mma(const uint4& a, const uint4& b, const v4f_l4& c) {
+    if constexpr (OP == H3S_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h_l4, a), __builtin_bit_cast(v8h_l4, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf_l4, a), __builtin_bit_cast(v8bf_l4, b), c, 0, 0, 0);
+}
+// eight codes of a word as 16 + code, in the order 0 4 1 5 2 6 3 7. m and e: the codes' bits and the exponent, in registers (as literals
+// the and and the or would be two instructions: one takes only one literal)
+template <int OP> __device__ __forceinline__ void l4_constants(uint32_t& m, uint32_t& e) {
+    m = OP == H3S_F16 ? 0x03C003C0u : 0x00780078u;
+    e = OP == H3S_F16 ? 0x4C004C00u : 0x41804180u;
+    asm volatile("" : "+s"(m));
+    asm volatile("" : "+v"(e));
+}
+template <int OP> __device__ __forceinline__ uint4 l4_codes(uint32_t w, uint32_t m, uint32_t e) {
+    if constexpr (OP == H3S_F16) return make_uint4(((w << 6) & m) | e, ((w << 2) & m) | e, ((w >> 2) & m) | e, ((w >> 6) & m) | e);
+    else return make_uint4(((w << 3) & m) | e, ((w >> 1) & m) | e, ((w >> 5) & m) | e, ((w >> 9) & m) | e);
+}
+// eight 16-bit values in that order
+__device__ __forceinline__ uint4 l4_order(const uint4& u) {
+    return make_uint4(__builtin_amdgcn_perm(u.z, u.x, 0x05040100u), __builtin_amdgcn_perm(u.z, u.x, 0x07060302u),
+                      __builtin_amdgcn_perm(u.w, u.y, 0x05040100u), __builtin_amdgcn_perm(u.w, u.y, 0x07060302u));
+}
+
+// eight values of x as loaded, and as the parts of an instruction's operand
+template <int DT> struct L4X {
+    static constexpr int PARTS = 1;
+    uint4 u;
+    __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(const void* x, int64_t at) { u = *reinterpret_cast<const uint4*>((const uint16_t*) x + at); }
+    __device__ __forceinline__ void parts(uint4 (&f)[1]) const { f[0] = l4_order(u); }
+};
+template <> struct L4X<H3S_F32> {
+    static constexpr int PARTS = 3;
+    float4 a, b;
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    __device__ __forceinline__ void load(const void* x, int64_t at) {
+        a = *reinterpret_cast<const float4*>((const float*) x + at);
+        b = *reinterpret_cast<const float4*>((const float*) x + at + 4);
+    }
+    __device__ __forceinline__ void parts(uint4 (&f)[3]) const {
+        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const uint4 u = Vec<H3S_BF16>::pack(v);
+            float r[8];
+            Vec<H3S_BF16>::unpack(u, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = v[i] - r[i];
+            f[p] = l4_order(u);
+        }
+    }
+};
+
+// How a 128-input step's scales of one column are loaded: 16-bit or float32 types with the step's scales in one load (they start
+// on a boundary of their size), or any type one by one
+enum { L4_S16 = 0, L4_S32 = 1, L4_SANY = 2 };
+
+// one column's scales of a step (one for each 32 J inputs), and the lane's own (the run 32 g ..) minimum, as loaded
+template <int J, int SM> struct L4S {
+    static constexpr int CNT = 4 / J, RAW = SM == L4_S16 ? (CNT + 1) / 2 : CNT;
+    uint32_t s[RAW], z;
+    __device__ __forceinline__ uint32_t one(const L4Args& P, const char* p, int64_t i) const {
+        if (SM == L4_S32 || (SM == L4_SANY && P.scale_dt == H3S_F32)) return ((const uint32_t*) p)[i];
+        return ((const uint16_t*) p)[i];
+    }
+    // scale, mins: the first column's (uniform); off: the bytes from there to the lane's column; r: the step's first run of 32 inputs.
+    // (A uniform address and a lane's 32-bit offset, which is the same in every step, take no vector instructions.)
+    __device__ __forceinline__ void load(const L4Args& P, const char* scale, const char* mins, uint32_t off, int r, int g) {
+        if constexpr (SM == L4_SANY) {
+            const int most = P.K / 32 - 1;
+#pragma unroll
+            for (int c = 0; c < CNT; ++c) s[c] = one(P, scale + off, l4_group(P, min(r + J * c, most)));
+            z = one(P, mins + off, l4_group(P, min(r + g, most)));
+        } else {
+            constexpr int ES = SM == L4_S32 ? 4 : 2;
+            const int64_t at = (J == 1 ? r : J == 2 ? r / 2 : l4_group(P, r)) * ES;
+            const char* p = scale + at;
+            if constexpr (SM == L4_S32) {
+                if constexpr (CNT == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p + off); s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w; }
+                else if constexpr (CNT == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p + off); s[0] = v.x; s[1] = v.y; }
+                else s[0] = *reinterpret_cast<const uint32_t*>(p + off);
+                z = *reinterpret_cast<const uint32_t*>(mins + at + (off + (J == 1 ? g : J == 2 ? g >> 1 : 0) * ES));
+            } else {
+                if constexpr (CNT == 4) { const uint2 v = *reinterpret_cast<const uint2*>(p + off); s[0] = v.x; s[1] = v.y; }
+                else if constexpr (CNT == 2) s[0] = *reinterpret_cast<const uint32_t*>(p + off);
+                else s[0] = *reinterpret_cast<const uint16_t*>(p + off);
+                z = *reinterpret_cast<const uint16_t*>(mins + at + (off + (J == 1 ? g : J == 2 ? g >> 1 : 0) * ES));
+            }
+        }
+    }
+    __device__ __forceinline__ float number(const L4Args& P, uint32_t u) const {
+        if (SM == L4_S32 || (SM == L4_SANY && P.scale_dt == H3S_F32)) return __uint_as_float(u);
+        const float a = bf16_lo(u), b = f16_lo(u);        // (both, and a select: a branch a scale costs more)
+        return P.scale_dt == H3S_BF16 ? a : b;
+    }
+    __device__ __forceinline__ float scale(const L4Args& P, int c) const {
+        if constexpr (SM == L4_S16 && CNT > 1) return number(P, c & 1 ? s[c >> 1] >> 16 : s[c >> 1] & 0xffffu);
+        else return number(P, s[c]);
+    }
+    // 16 s + z of the lane's own run
+    __device__ __forceinline__ float offset(const L4Args& P, const float* sc, int g) const {
+        float own = sc[0];
+        if constexpr (CNT == 2) own = g < 2 ? sc[0] : sc[1];
+        else if constexpr (CNT == 4) own = g < 2 ? (g ? sc[1] : sc[0]) : (g == 2 ? sc[2] : sc[3]);
+        const float a = __builtin_fmaf(16.0f, own, number(P, z)), b = 24.0f * own;
+        return P.has_mins ? a : b;
+    }
+};
+
+// a step's codes of one column, the run of 32 inputs j in word j
+__device__ __forceinline__ void l4_exchange(const uint4& w, uint32_t (&c)[4]) {
+    const auto p = __builtin_amdgcn_permlane32_swap(w.x, w.z, false, false);
+    const auto q = __builtin_amdgcn_permlane32_swap(w.y, w.w, false, false);
+    const auto r = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false);
+    const auto s = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
+    c[0] = r[0]; c[1] = r[1]; c[2] = s[0]; c[3] = s[1];
+}
+
+// a step's codes and scales of NT columns, from what was loaded: c the codes, the run j of 32 inputs in word j; sc a scale for each 32 J
+// inputs; off 16 s + z of the lane's own run (zeros past the row's end)
+template <int NT, int J, int SM>
+__device__ __forceinline__ void l4_decode(const L4Args& P, int kk, int g, const uint4 (&w)[NT], const L4S<J, SM> (&sr)[NT], uint32_t (&c)[NT][4],
+                                          float (&sc)[NT][4 / J], float (&off)[NT]) {
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+        l4_exchange(w[b], c[b]);
+#pragma unroll
+        for (int q = 0; q < 4 / J; ++q) sc[b][q] = sr[b].scale(P, q);
+        off[b] = sr[b].offset(P, sc[b], g);
+    }
+    // (the last step of a row that is no multiple of 128: its scales do not come in one load)
+    if (SM == L4_SANY && kk + 128 > P.K) {
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+#pragma unroll
+            for (int q = 0; q < 4 / J; ++q) sc[b][q] = kk + 32 * J * q < P.K ? sc[b][q] : 0.0f;
+            off[b] = kk + 32 * g < P.K ? off[b] : 0.0f;
+        }
+    }
+}
+
+// The products of one step of 128 inputs: NT columns' codes and scales against MT x 16 rows. frag(a, j, f): the operand of the rows
+// 16 a .. and the run j (zeros past the row's end). Rows: place l of an operand is row 4 (l % 4) + l / 4, so that register i of lane
+// group g sums row 4 i + g and up to four rows take one multiply-add (NI of them).
+template <int OP, int PARTS, int MT, int NT, int NI, int J, typename F>
+__device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, uint32_t e, const uint32_t (&c)[NT][4], const float (&sc)[NT][4 / J], const float (&off)[NT],
+                                            F frag, v4f_l4 (&acc)[MT][NT]) {
+    v4f_l4 sx[MT];
+#pragma unroll
+    for (int a = 0; a < MT; ++a) sx[a] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int q = 0; q < 4 / J; ++q) {
+        v4f_l4 y[MT][NT];
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int b = 0; b < NT; ++b) y[a][b] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = q * J; j < (q + 1) * J; ++j) {
+            uint4 f[NT];
+#pragma unroll
+            for (int b = 0; b < NT; ++b) f[b] = l4_codes<OP>(c[b][j], m, e);
+#pragma unroll
+            for (int a = 0; a < MT; ++a) {
+                uint4 xf[PARTS];
+                frag(a, j, xf);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    sx[a] = l4_mma<OP>(sel[j], xf[p], sx[a]);
+#pragma unroll
+                    for (int b = 0; b < NT; ++b) y[a][b] = l4_mma<OP>(xf[p], f[b], y[a][b]);
+                }
+            }
+        }
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int b = 0; b < NT; ++b)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) acc[a][b][i] = __builtin_fmaf(sc[b][q], y[a][b][i], acc[a][b][i]);
+    }
+#pragma unroll
+    for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int b = 0; b < NT; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(-sx[a][0], off[b], acc[a][b], 0, 0, 0);
+}
+
+// the first operands whose row 4 j is ones: the sums of x of run j then end in lane group j
+template <int OP> __device__ __forceinline__ void l4_select(int l15, uint4 (&sel)[4]) {
+    const uint32_t one = OP == H3S_F16 ? 0x3C003C00u : 0x3F803F80u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t u = l15 == 4 * j ? one : 0;
+        sel[j] = make_uint4(u, u, u, u);
+    }
+}
+
+// (loaded whether there is one or not: a load in a branch would have every wavefront wait for all its loads where the branch ends)
+__device__ __forceinline__ float l4_bias(const L4Args& P, int64_t n) {
+    const float* p = P.bias ? P.bias + min(n, P.N - 1) : (const float*) P.codes;
+    return *p;
+}
+template <int NI> __device__ __forceinline__ void l4_store(const L4Args& P, int64_t m0, int64_t n, int g, const v4f_l4& y, float read) {
+    const float bias = P.bias ? read : 0.0f;
+    if (n >= P.N) return;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int64_t m = m0 + 4 * i + g;
+        if (m < P.M) store_any(P.out, P.out_dt, m * P.N + n, y[i] + bias);
+    }
+}
+
+// ---- up to four rows of x: multiply-adds of pairs of codes --------------------------------------------------------------------
+
+// c + a.lo b.lo + a.hi b.hi
+template <int OP> __device__ __forceinline__ float l4_dot(uint32_t a, uint32_t b, float c) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    if constexpr (OP == H3S_F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, a), __builtin_bit_cast(h2, b), c, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, a), __builtin_bit_cast(bf2, b), c, false);
+}
+
+constexpr int kL4DotWaves = 11;       // wavefronts of a block, at most
+
+// A row of weights is cut into chunks of 512 inputs; a wavefront has U of them (every KW-th), with x's values for them in registers, and
+// walks down the rows: 16 lanes take a row's chunk, 32 codes each, four rows at a time. So its loads are runs of 256 bytes, the scale of a
+// lane's codes is one 2-byte load beside its neighbours', and no operand goes through LDS. (As matrix instructions' operands - 16
+// rows a load, 64 bytes of each, a scale gathered from 16 rows - the same loads alone took 94 us where the codes come in 62.) Per tile of
+// 16 rows the wavefronts' sums are joined through LDS, in wavefront order; the loads go on across tiles, DP row steps ahead.
+template <int DT, int M, int U, bool MINS>
+__global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P) {
+    constexpr int OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS, DP = U == 1 ? 4 : U == 2 ? 3 : 2;
+    const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4, KW = (int) (blockDim.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
+    const int tiles = (int) ((P.N + 15) / 16), grid = (int) gridDim.x;
+    const int ses = P.scale_dt == H3S_F32 ? 4 : 2;
+    // the lane's inputs k .. k + 31 of each chunk (past the row's end: its last ones, against zeros)
+    uint32_t kofs[U], gofs[U];
+    bool in[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int k = (wave + u * KW) * 512 + l * 32;
+        in[u] = k < P.K;
+        kofs[u] = (uint32_t) (min(k, P.K - 32) / 2);
+        gofs[u] = (uint32_t) (l4_group(P, min(k, P.K - 32) / 32) * ses);
+    }
+    uint4 w[DP][U];
+    uint32_t sr[DP][U], zr[DP][U];
+    int ltile = blockIdx.x, lrs = 0;
+    // (never skipped, so that the loads in flight are counted; past the last tile: the last rows again)
+    auto load = [&](int d) {
+        const int64_t rb = min((int64_t) ltile * 16 + lrs * 4, P.N - 1);
+        const int qe = (int) min<int64_t>(q, P.N - 1 - rb);
+        const uint8_t* cp = P.codes + rb * (P.K / 2);
+        const char *sp = (const char*) P.scale + rb * P.groups * ses, *zp = (const char*) P.mins + rb * P.groups * ses;
+        const uint32_t co = (uint32_t) (qe * (P.K / 2)), so = (uint32_t) (qe * P.groups * ses);
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[d][u] = *reinterpret_cast<const uint4*>(cp + (co + kofs[u]));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (ses == 4) {
+                sr[d][u] = *reinterpret_cast<const uint32_t*>(sp + (so + gofs[u]));
+                if constexpr (MINS) zr[d][u] = *reinterpret_cast<const uint32_t*>(zp + (so + gofs[u]));
+            } else {
+                sr[d][u] = *reinterpret_cast<const uint16_t*>(sp + (so + gofs[u]));
+                if constexpr (MINS) zr[d][u] = *reinterpret_cast<const uint16_t*>(zp + (so + gofs[u]));
+            }
+        }
+        if (++lrs == 4) {
+            lrs = 0;
+            ltile = min(ltile + grid, tiles - 1);
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < DP; ++d) load(d);
+    // x as operands: the pairs in the order of l4_codes, and the sum of each lane's 32 values
+    uint32_t x[M][U][PARTS][16];
+    float sx[M][U];
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const char* xp = (const char*) P.x + ((int64_t) min(m, (int) P.M - 1) * P.K + 2 * (int) kofs[u]) * (DT == H3S_F32 ? 4 : 2);
+            sx[m][u] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                L4X<DT> v;
+                v.load(xp, 8 * e);
+                if (!in[u]) v.zero();
+                uint4 f[PARTS];
+                v.parts(f);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    x[m][u][p][4 * e] = f[p].x; x[m][u][p][4 * e + 1] = f[p].y; x[m][u][p][4 * e + 2] = f[p].z; x[m][u][p][4 * e + 3] = f[p].w;
+                    float y[8];
+                    Vec<OP>::unpack(f[p], y);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sx[m][u] += y[i];
+                }
+            }
+        }
+    uint32_t cm, ce;
+    l4_constants<OP>(cm, ce);
+    const bool bf = P.scale_dt == H3S_BF16, wide = ses == 4;
+    auto number = [&](uint32_t r) {
+        const float a = bf16_lo(r), b = f16_lo(r), c = __uint_as_float(r);
+        return wide ? c : bf ? a : b;
+    };
+    __shared__ float part[2][M][16][kL4DotWaves + 1];
+    int turn = 0, rs = 0, tile = blockIdx.x;
+    while (tile < tiles) {
+#pragma unroll
+        for (int d = 0; d < DP; ++d) {
+            float acc[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) acc[m] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t c[4] = {w[d][u].x, w[d][u].y, w[d][u].z, w[d][u].w};
+                float y[M];
+#pragma unroll
+                for (int m = 0; m < M; ++m) y[m] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint4 f = l4_codes<OP>(c[e], cm, ce);
+#pragma unroll
+                    for (int m = 0; m < M; ++m)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            y[m] = l4_dot<OP>(x[m][u][p][4 * e], f.x, y[m]);
+                            y[m] = l4_dot<OP>(x[m][u][p][4 * e + 1], f.y, y[m]);
+                            y[m] = l4_dot<OP>(x[m][u][p][4 * e + 2], f.z, y[m]);
+                            y[m] = l4_dot<OP>(x[m][u][p][4 * e + 3], f.w, y[m]);
+                        }
+                }
+                const float s = number(sr[d][u]), off = MINS ? __builtin_fmaf(16.0f, s, number(zr[d][u])) : 24.0f * s;
+#pragma unroll
+                for (int m = 0; m < M; ++m) acc[m] = __builtin_fmaf(-off, sx[m][u], __builtin_fmaf(s, y[m], acc[m]));
+            }
+            load(d);
+#pragma unroll
+            for (int m = 0; m < M; ++m) acc[m] = wave_sum<16>(acc[m]);
+            if (l == 0) {
+#pragma unroll
+                for (int m = 0; m < M; ++m) part[turn & 1][m][rs * 4 + q][wave] = acc[m];
+            }
+            if (++rs == 4) {
+                // (the area is written again two tiles later, behind the next tile's barrier)
+                lds_barrier();
+                const int n = threadIdx.x & 15, m = threadIdx.x >> 4;
+                const int64_t col = (int64_t) tile * 16 + n;
+                if (m < M && m < P.M && tile < tiles && col < P.N) {
+                    float y = part[turn & 1][m][n][0];
+                    for (int v = 1; v < KW; ++v) y += part[turn & 1][m][n][v];
+                    store_any(P.out, P.out_dt, m * P.N + col, y + (P.bias ? P.bias[col] : 0.0f));
+                }
+                ++turn;
+                rs = 0;
+                tile += grid;
+            }
+        }
+    }
+}
+
+// ---- up to 16 rows ------------------------------------------------------------------------------------------------------------
+
+// Up to 16 rows. J: runs of 32 inputs to one scale (4: groups are multiples of 128 inputs, 2: of 64, 1: of 32).
+// A block walks the tiles of 16 NT columns that are its own, its KW wavefronts side by side along the inputs, and joins their sums
+// through LDS at the end of each; the loads go on across tiles, DP steps ahead. So a tile's codes, one run of memory, are asked for
+// together, and the device streams through the weights.
+// XL (up to four rows that fit kL4Lds): x is put into LDS once, as operands. Otherwise x's operands are loaded in the step that uses
+// them (from the L2); vector loads return in order, so only one step's codes are then asked for behind them.
+template <int DT, int NT, int KW, int NI, int J, int SM, bool XL>
+__global__ __launch_bounds__(64 * KW) void linear4_few_kernel(L4Args P) {
+    constexpr int OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS, DP = XL ? 3 : 1;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
+    const int steps = (P.K + 127) / 128, rounds = (steps + KW - 1) / KW;          // rounds a tile
+    const int tiles = (int) ((P.N + 16 * NT - 1) / (16 * NT));
+    const int row = min((l15 & 3) * 4 + (l15 >> 2), (int) P.M - 1);              // (places without a row: the last again, not stored)
+    const uint32_t xoff = (uint32_t) (row * P.K + 8 * g) * (DT == H3S_F32 ? 4 : 2);
+    const int ses = SM == L4_S32 || (SM == L4_SANY && P.scale_dt == H3S_F32) ? 4 : 2;
+    uint4 w[DP][NT];
+    L4S<J, SM> sr[DP][NT];
+    float bias[DP][NT];
+    // where the loads are: the tile and the round; the tile's first column's codes and scales, and the lane's bytes from there
+    int ltile = blockIdx.x, lround = 0;
+    const uint8_t* cbase;
+    const char *sbase, *zbase;
+    const char* bbase;                                                            // (no bias: anything that is there)
+    uint32_t coff[NT], soff[NT], boff[NT];
+    auto enter = [&]() {
+        const int64_t n0 = (int64_t) ltile * (16 * NT);
+        cbase = P.codes + n0 * (P.K / 2);
+        sbase = (const char*) P.scale + n0 * P.groups * ses;
+        zbase = (const char*) P.mins + n0 * P.groups * ses;
+        bbase = P.bias ? (const char*) (P.bias + n0) : (const char*) P.codes;
+        const int left = (int) min<int64_t>(P.N - 1 - n0, 16 * NT);               // (columns past the last: the last again, not stored)
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            const int n = min(16 * b + l15, left);
+            coff[b] = (uint32_t) (n * (P.K / 2) + 16 * g);
+            soff[b] = (uint32_t) (n * P.groups * ses);
+            boff[b] = P.bias ? 4 * n : 0;
+        }
+    };
+    // (Never skipped: with the same loads in every round the compiler counts the ones in flight; where there is nothing to load it is
+    // the last step or the last tile again.)
+    auto load = [&](uint4 (&wd)[NT], L4S<J, SM> (&sd)[NT], float (&bd)[NT]) {
+        const int step = min(lround * KW + wave, steps - 1);
+        const uint8_t* cp = cbase + step * 64;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            uint32_t at = coff[b];
+            if (SM == L4_SANY) at = min(at, coff[b] - 16 * g + (uint32_t) (P.K / 2 - 16 - step * 64));   // (within the row)
+            wd[b] = *reinterpret_cast<const uint4*>(cp + at);
+        }
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            sd[b].load(P, sbase, zbase, soff[b], step * 4, g);
+            bd[b] = *(const float*) (bbase + boff[b]);
+        }
+        if (++lround == rounds) {
+            lround = 0;
+            ltile = min(ltile + (int) gridDim.x, tiles - 1);
+            enter();
+        }
+    };
+    enter();
+#pragma unroll
+    for (int u = 0; u < DP; ++u) load(w[u], sr[u], bias[u]);
+    uint4 sel[4];
+    l4_select<OP>(l15, sel);
+    uint32_t cm, ce;
+    l4_constants<OP>(cm, ce);
+    extern __shared__ uint4 lds[];
+    __shared__ v4f_l4 part[2][NT][KW][64];
+    const int pieces = steps * 16;                                                // 8-input pieces of a row, zeros past its end
+    if constexpr (XL) {
+        for (int i = threadIdx.x; i < pieces * (int) P.M; i += 64 * KW) {
+            const int r = i / pieces, p = i - r * pieces;
+            L4X<DT> v;
+            v.zero();
+            if (8 * p < P.K) v.load((const char*) P.x + (int64_t) r * P.K * (DT == H3S_F32 ? 4 : 2), 8 * p);
+            uint4 f[PARTS];
+            v.parts(f);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) lds[(r * PARTS + q) * pieces + p] = f[q];
+        }
+        lds_barrier();
+    }
+    v4f_l4 acc[1][NT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b) acc[0][b] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+    int tile = blockIdx.x, round = 0, turn = 0;
+    while (tile < tiles) {
+#pragma unroll
+        for (int u = 0; u < DP; ++u) {
+            const int step = round * KW + wave;
+            uint32_t c[NT][4];
+            float sc[NT][4 / J], off[NT];
+            L4X<DT> xr[4];
+            if constexpr (!XL) {
+                const char* xp = (const char*) P.x + (int64_t) min(step, steps - 1) * 128 * (DT == H3S_F32 ? 4 : 2);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t at = xoff + 32 * j * (DT == H3S_F32 ? 4 : 2);
+                    if (SM == L4_SANY) at = min(at, (uint32_t) (row * P.K + P.K - 8 - min(step, steps - 1) * 128) * (DT == H3S_F32 ? 4 : 2));
+                    xr[j].load(xp + at, 0);
+                }
+            }
+            l4_decode<NT, J, SM>(P, step * 128, g, w[u], sr[u], c, sc, off);
+            float bn[NT];
+#pragma unroll
+            for (int b = 0; b < NT; ++b) bn[b] = bias[u][b];
+            load(w[u], sr[u], bias[u]);
+            if (step < steps && tile < tiles) {
+                if constexpr (!XL && SM == L4_SANY) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (step * 128 + 32 * j >= P.K) xr[j].zero();
+                }
+                l4_products<OP, PARTS, 1, NT, NI, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
+                    if constexpr (XL) {
+#pragma unroll
+                        for (int q = 0; q < PARTS; ++q) f[q] = lds[(row * PARTS + q) * pieces + step * 16 + 4 * j + g];
+                    } else xr[j].parts(f);
+                }, acc);
+            }
+            if (++round == rounds) {
+                // the wavefronts' sums, in wavefront order, by one of them in turn; the others go on (the area is used again two tiles
+                // later, behind the next tile's barrier)
+#pragma unroll
+                for (int b = 0; b < NT; ++b) {
+                    part[turn & 1][b][wave][lane] = acc[0][b];
+                    acc[0][b] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                lds_barrier();
+                if (wave == turn % KW && tile < tiles) {
+#pragma unroll
+                    for (int b = 0; b < NT; ++b) {
+                        v4f_l4 y = part[turn & 1][b][0][lane];
+#pragma unroll
+                        for (int v = 1; v < KW; ++v) y += part[turn & 1][b][v][lane];
+                        l4_store<NI>(P, 0, (int64_t) tile * (16 * NT) + 16 * b + l15, g, y, bn[b]);
+                    }
+                }
+                ++turn;
+                round = 0;
+                tile += gridDim.x;
+            }
+        }
+    }
+}
+constexpr int kL4Lds = 64 * 1024;      // bytes of x in LDS
+
+constexpr int kL4Cols = 128;      // columns of a block of linear4_many_kernel
+
+template <int DT, int MT, int J, int SM>
+__global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
+    constexpr int NT = 2, OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS;
+    constexpr int PIECES = 16 * MT * 16 / 256;                                    // 8-input pieces of x a thread stages
+    __shared__ uint4 xs[2][2][MT][4][PARTS][64];                                  // [K group][stage][rows][run][part][lane]
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6)), kg = wave >> 2;
+    // blocks eight apart run on one XCD: the row tiles of a column block lie there one after another and share its codes
+    const int64_t mt = (P.M + 16 * MT - 1) / (16 * MT), id = blockIdx.x;
+    const int64_t nb = id / (8 * mt) * 8 + id % 8, n0 = nb * kL4Cols + (wave & 3) * (16 * NT), m0 = id / 8 % mt * (16 * MT);
+    if (nb * kL4Cols >= P.N) return;
+    const int steps = (P.K + 127) / 128;
+    const int ses = SM == L4_S32 || (SM == L4_SANY && P.scale_dt == H3S_F32) ? 4 : 2;
+    const int64_t from = min(n0, P.N - 1);                                        // (a wavefront past the columns: the last one, not stored)
+    const uint8_t* cbase = P.codes + from * (P.K / 2);
+    const char *sbase = (const char*) P.scale + from * P.groups * ses, *zbase = (const char*) P.mins + from * P.groups * ses;
+    uint32_t coff[NT], soff[NT];
+    v4f_l4 acc[MT][NT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+        const int n = (int) min<int64_t>(16 * b + l15, P.N - 1 - from);
+        coff[b] = (uint32_t) (n * (P.K / 2) + 16 * g);
+        soff[b] = (uint32_t) (n * P.groups * ses);
+#pragma unroll
+        for (int a = 0; a < MT; ++a) acc[a][b] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    uint4 sel[4];
+    l4_select<OP>(l15, sel);
+    uint32_t cm, ce;
+    l4_constants<OP>(cm, ce);
+    // x: piece t + 256 p of the K group's step is 8 inputs (16 pieces a row)
+    constexpr int XES = DT == H3S_F32 ? 4 : 2;
+    const int t = threadIdx.x & 255;
+    L4X<DT> xr[PIECES];
+    const char* xbase = (const char*) P.x + m0 * P.K * XES;
+    uint32_t xoff[PIECES];
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) xoff[p] = (uint32_t) ((int) min<int64_t>((t + 256 * p) / 16, P.M - 1 - m0) * P.K + t % 16 * 8) * XES;
+    uint4 w[NT];
+    L4S<J, SM> sr[NT];
+    auto load_x = [&](int step) {
+        const char* xp = xbase + (int64_t) step * 128 * XES;
+        const bool out = SM == L4_SANY && step * 128 + t % 16 * 8 >= P.K;
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            xr[p].load(xp + (out ? xoff[p] - t % 16 * 8 * XES : xoff[p]), 0);
+            if (out) xr[p].zero();
+        }
+    };
+    auto store_x = [&](int stage) {
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int at = t + 256 * p, r = at / 16, k8 = at % 16;                // place: row 4 (l % 4) + l / 4 at l
+            uint4 f[PARTS];
+            xr[p].parts(f);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) xs[kg][stage][r / 16][k8 / 4][q][k8 % 4 * 16 + (r % 4) * 4 + r % 16 / 4] = f[q];
+        }
+    };
+    auto load_w = [&](int step) {
+        const uint8_t* cp = cbase + step * 64;
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            uint32_t at = coff[b];
+            if (SM == L4_SANY) at = min(at, coff[b] - 16 * g + (uint32_t) (P.K / 2 - 16 - step * 64));   // (within the row)
+            w[b] = *reinterpret_cast<const uint4*>(cp + at);
+        }
+#pragma unroll
+        for (int b = 0; b < NT; ++b) sr[b].load(P, sbase, zbase, soff[b], step * 4, g);
+    };
+    // both K groups make the same number of rounds (the second's last may have no step)
+    // (Loads are never skipped, see linear4_few_kernel: past the end it is the last step again.)
+    load_x(min(kg, steps - 1));
+    load_w(min(kg, steps - 1));
+    store_x(0);
+    load_x(min(kg + 2, steps - 1));
+    lds_barrier();
+    int stage = 0;
+    for (int first = 0; first < steps; first += 2) {
+        const int step = first + kg;
+        if (step < steps) {
+            uint32_t c[NT][4];
+            float sc[NT][4 / J], off[NT];
+            l4_decode<NT, J, SM>(P, step * 128, g, w, sr, c, sc, off);
+            load_w(min(step + 2, steps - 1));
+            l4_products<OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][stage][a][j][q][lane];
+            }, acc);
+            store_x(stage ^ 1);
+            load_x(min(step + 4, steps - 1));
+        }
+        lds_barrier();
+        stage ^= 1;
+    }
+    // the second group's sums to the first's
+    v4f_l4* part = reinterpret_cast<v4f_l4*>(&xs[0][0][0][0][0][0]);
+    static_assert(sizeof(xs) >= 4 * MT * NT * 64 * 16, "the sums fit x's stages");
+    if (kg == 1) {
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int b = 0; b < NT; ++b) part[((wave & 3) * MT * NT + a * NT + b) * 64 + lane] = acc[a][b];
+    }
+    __syncthreads();
+    if (kg == 0) {
+        float bias[NT];
+#pragma unroll
+        for (int b = 0; b < NT; ++b) bias[b] = l4_bias(P, n0 + 16 * b + l15);
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int b = 0; b < NT; ++b)
+                l4_store<4>(P, m0 + 16 * a, n0 + 16 * b + l15, g, acc[a][b] + part[((wave & 3) * MT * NT + a * NT + b) * 64 + lane], bias[b]);
+    }
+}
+
+// which kernel a call takes (linear4.hip): rows 4, 16 (few: the registers of sums), 32 or 64 (many: the tile)
+struct L4Plan { int rows; };
+
+template <int DT, int NT, int KW, int NI, int J, int SM, bool XL>
+static void l4_few(Ctx* c, const L4Args& P, int per_cu, size_t lds) {
+    // a block walks as many tiles as any other, or one less
+    const int64_t tiles = (P.N + 16 * NT - 1) / (16 * NT), turns = (tiles + per_cu * c->cus - 1) / (per_cu * c->cus);
+    linear4_few_kernel<DT, NT, KW, NI, J, SM, XL><<<(unsigned) ((tiles + turns - 1) / turns), 64 * KW, lds, c->stream>>>(P);
+}
+template <int DT, int J, int SM>
+static void l4_run(Ctx* c, const L4Args& P, const L4Plan& plan) {
+    if (plan.rows <= 16) {
+        l4_few<DT, 2, 8, 4, J, SM, false>(c, P, 2, 0);
+    } else {
+        const int64_t mt = (P.M + plan.rows - 1) / plan.rows, nb = ((P.N + kL4Cols - 1) / kL4Cols + 7) / 8 * 8;
+        if (plan.rows == 32) linear4_many_kernel<DT, 2, J, SM><<<(unsigned) (mt * nb), 512, 0, c->stream>>>(P);
+        else if constexpr (DT != H3S_F32) linear4_many_kernel<DT, 4, J, SM><<<(unsigned) (mt * nb), 512, 0, c->stream>>>(P);
+    }
+}
+template <int DT, int M, int U>
+static void l4_dot_run(Ctx* c, const L4Args& P, int per_cu) {
+    const int64_t tiles = (P.N + 15) / 16, turns = (tiles + per_cu * c->cus - 1) / (per_cu * c->cus);
+    const unsigned grid = (unsigned) ((tiles + turns - 1) / turns);
+    const int chunks = (P.K + 511) / 512, kw = (chunks + U - 1) / U;
+    if (P.has_mins) linear4_dot_kernel<DT, M, U, true><<<grid, 64 * kw, 0, c->stream>>>(P);
+    else linear4_dot_kernel<DT, M, U, false><<<grid, 64 * kw, 0, c->stream>>>(P);
+}
+// whether the rows are few enough for multiply-adds and x's values for registers (the last run starts it)
+template <int DT> static bool l4_dot_takes(Ctx* c, const L4Args& P) {
+    const int chunks = (P.K + 511) / 512;
+    constexpr int PARTS = L4X<DT>::PARTS;
+    if (P.M > 4 || (P.N + 15) / 16 > 0x7fffffff / 2) return false;
+    const int u = chunks <= kL4DotWaves ? 1 : chunks <= 2 * kL4DotWaves ? 2 : chunks <= 4 * kL4DotWaves ? 4 : 0, m = P.M == 3 ? 4 : (int) P.M;
+    if (u == 0 || 16 * PARTS * u * m > 96) return false;
+    if (m == 1) {
+        if (u == 1) l4_dot_run<DT, 1, 1>(c, P, 2);
+        else if (u == 2) l4_dot_run<DT, 1, 2>(c, P, 2);
+        else if constexpr (PARTS == 1) l4_dot_run<DT, 1, 4>(c, P, 2);
+    } else if (m == 2) {
+        if (u == 1) l4_dot_run<DT, 2, 1>(c, P, 2);
+        else if constexpr (PARTS == 1) l4_dot_run<DT, 2, 2>(c, P, 2);
+    } else if constexpr (PARTS == 1) l4_dot_run<DT, 4, 1>(c, P, 2);
+    return true;
+}
+template <int DT>
+static void l4_type(Ctx* c, const L4Args& P, const L4Plan& plan) {
+    if (l4_dot_takes<DT>(c, P)) return;
+    // a step of 128 inputs has 4, 2 or 1 scales: one load where every column's lie on a boundary of their size
+    const int64_t cnt = P.group % 128 == 0 ? 1 : P.group == 64 ? 2 : P.group == 32 ? 4 : 0;
+    const bool vec = cnt && P.groups % cnt == 0 && (uintptr_t) P.scale % (uintptr_t) (cnt * elem_size(P.scale_dt)) == 0;
+    if (!vec) l4_run<DT, 1, L4_SANY>(c, P, plan);
+    else if (P.scale_dt == H3S_F32) {
+        if (cnt == 1) l4_run<DT, 4, L4_S32>(c, P, plan);
+        else if (cnt == 2) l4_run<DT, 2, L4_S32>(c, P, plan);
+        else l4_run<DT, 1, L4_S32>(c, P, plan);
+    } else {
+        if (cnt == 1) l4_run<DT, 4, L4_S16>(c, P, plan);
+        else if (cnt == 2) l4_run<DT, 2, L4_S16>(c, P, plan);
+        else l4_run<DT, 1, L4_S16>(c, P, plan);
+    }
+}
+void l4_bf16(Ctx* c, const L4Args& P, const L4Plan& plan);
+void l4_f16(Ctx* c, const L4Args& P, const L4Plan& plan);
+void l4_f32(Ctx* c, const L4Args& P, const L4Plan& plan);
+
+}  // namespace h3

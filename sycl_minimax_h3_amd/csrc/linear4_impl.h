@@ -412,155 +412,205 @@ __global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P)
 
 // ---- up to 16 rows ------------------------------------------------------------------------------------------------------------
 
-// Up to 16 rows. J: runs of 32 inputs to one scale (4: groups are multiples of 128 inputs, 2: of 64, 1: of 32).
-// A block walks the tiles of 16 NT columns that are its own, its KW wavefronts side by side along the inputs, and joins their sums
-// through LDS at the end of each; the loads go on across tiles, DP steps ahead. So a tile's codes, one run of memory, are asked for
-// together, and the device streams through the weights.
-// XL (up to four rows that fit kL4Lds): x is put into LDS once, as operands. Otherwise x's operands are loaded in the step that uses
-// them (from the L2); vector loads return in order, so only one step's codes are then asked for behind them.
-template <int DT, int NT, int KW, int NI, int J, int SM, bool XL>
-__global__ __launch_bounds__(64 * KW) void linear4_few_kernel(L4Args P) {
-    constexpr int OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS, DP = XL ? 3 : 1;
-    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+// The scales and minima of four steps of one column: lane group g loads those of step first + g (one gather for four steps: a gather
+// from 16 rows of weights costs about as much as 16 x 64 bytes of codes), and a step's are passed on from its group.
+template <int J, int SM> struct L4Q {
+    static constexpr int CNT = 4 / J, RAW = SM == L4_S16 ? (CNT + 1) / 2 : CNT;
+    uint32_t s[RAW], z[RAW];
+    // scale, mins: the tile's first column's; off: the bytes from there to the lane's column; r: the first run of the lane's step
+    __device__ __forceinline__ void load(const L4Args& P, const char* scale, const char* mins, uint32_t off, int r) {
+        if constexpr (SM == L4_SANY) {
+            const int most = P.K / 32 - 1, es = P.scale_dt == H3S_F32 ? 4 : 2;
+#pragma unroll
+            for (int c = 0; c < CNT; ++c) {
+                const uint32_t at = off + (uint32_t) (l4_group(P, min(r + J * c, most)) * es);
+                s[c] = es == 4 ? *reinterpret_cast<const uint32_t*>(scale + at) : *reinterpret_cast<const uint16_t*>(scale + at);
+                z[c] = es == 4 ? *reinterpret_cast<const uint32_t*>(mins + at) : *reinterpret_cast<const uint16_t*>(mins + at);
+            }
+        } else {
+            const uint32_t at = off + (uint32_t) (J == 1 ? r : J == 2 ? r / 2 : l4_group(P, r)) * (SM == L4_S32 ? 4 : 2);
+            take(scale + at, s);
+            take(mins + at, z);
+        }
+    }
+    __device__ __forceinline__ void take(const char* p, uint32_t (&u)[RAW]) const {
+        if constexpr (RAW == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); u[0] = v.x; u[1] = v.y; u[2] = v.z; u[3] = v.w; }
+        else if constexpr (RAW == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); u[0] = v.x; u[1] = v.y; }
+        else if constexpr (SM == L4_S16 && CNT == 1) u[0] = *reinterpret_cast<const uint16_t*>(p);
+        else u[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+    // those of the step of lane group `from` (lane: 4 (16 from + lane % 16)), for every lane
+    __device__ __forceinline__ void pass(const L4Args& P, int lane, int g, float (&sc)[CNT], float& off) const {
+        uint32_t a[RAW], b[RAW];
+#pragma unroll
+        for (int i = 0; i < RAW; ++i) {
+            a[i] = (uint32_t) __builtin_amdgcn_ds_bpermute(lane, (int) s[i]);
+            b[i] = (uint32_t) __builtin_amdgcn_ds_bpermute(lane, (int) z[i]);
+        }
+        float zc[CNT];
+#pragma unroll
+        for (int c = 0; c < CNT; ++c) {
+            sc[c] = number(P, a, c);
+            zc[c] = number(P, b, c);
+        }
+        float own = sc[0], least = zc[0];
+        if constexpr (CNT == 2) { own = g < 2 ? sc[0] : sc[1]; least = g < 2 ? zc[0] : zc[1]; }
+        else if constexpr (CNT == 4) { own = g < 2 ? (g ? sc[1] : sc[0]) : (g == 2 ? sc[2] : sc[3]); least = g < 2 ? (g ? zc[1] : zc[0]) : (g == 2 ? zc[2] : zc[3]); }
+        const float x = __builtin_fmaf(16.0f, own, least), y = 24.0f * own;
+        off = P.has_mins ? x : y;
+    }
+    __device__ __forceinline__ float number(const L4Args& P, const uint32_t* u, int c) const {
+        const uint32_t v = SM == L4_S16 && CNT > 1 ? (c & 1 ? u[c >> 1] >> 16 : u[c >> 1] & 0xffffu) : u[c];
+        const float x = __uint_as_float(v), a = bf16_lo(v), b = f16_lo(v);
+        if (SM == L4_S32) return x;
+        const float h = P.scale_dt == H3S_BF16 ? a : b;
+        return SM == L4_SANY && P.scale_dt == H3S_F32 ? x : h;
+    }
+};
+
+constexpr int kL4FewWaves = 12;       // wavefronts of a block, at most
+
+// J: runs of 32 inputs to one scale (4: groups are multiples of 128 inputs, 2: of 64, 1: of 32).
+// A block walks the tiles of 16 NT columns that are its own. Its KW wavefronts have 4 quads x 4 steps of 128 inputs each, one run of
+// memory in a weight row, and are joined through LDS at the end of a tile; the loads go on across tiles.
+// XR (one quad: up to 12 x 512 inputs): a wavefront's operands of x stay in registers. Otherwise they are loaded in the step that uses
+// them (from the L2).
+template <int DT, int NT, int J, int SM, bool XR>
+__global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P, int quads) {
+    constexpr int OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS, XES = DT == H3S_F32 ? 4 : 2, DP = XR ? 4 : 2;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, KW = (int) (blockDim.x >> 6);
     const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
-    const int steps = (P.K + 127) / 128, rounds = (steps + KW - 1) / KW;          // rounds a tile
+    const int steps = (P.K + 127) / 128, first = wave * quads * 4, grid = (int) gridDim.x;
     const int tiles = (int) ((P.N + 16 * NT - 1) / (16 * NT));
     const int row = min((l15 & 3) * 4 + (l15 >> 2), (int) P.M - 1);              // (places without a row: the last again, not stored)
-    const uint32_t xoff = (uint32_t) (row * P.K + 8 * g) * (DT == H3S_F32 ? 4 : 2);
     const int ses = SM == L4_S32 || (SM == L4_SANY && P.scale_dt == H3S_F32) ? 4 : 2;
-    uint4 w[DP][NT];
-    L4S<J, SM> sr[DP][NT];
-    float bias[DP][NT];
-    // where the loads are: the tile and the round; the tile's first column's codes and scales, and the lane's bytes from there
-    int ltile = blockIdx.x, lround = 0;
-    const uint8_t* cbase;
-    const char *sbase, *zbase;
-    const char* bbase;                                                            // (no bias: anything that is there)
-    uint32_t coff[NT], soff[NT], boff[NT];
-    auto enter = [&]() {
-        const int64_t n0 = (int64_t) ltile * (16 * NT);
-        cbase = P.codes + n0 * (P.K / 2);
-        sbase = (const char*) P.scale + n0 * P.groups * ses;
-        zbase = (const char*) P.mins + n0 * P.groups * ses;
-        bbase = P.bias ? (const char*) (P.bias + n0) : (const char*) P.codes;
+    // the operand of run j of a step (zeros past the row's end)
+    auto load_x = [&](int step, int j, L4X<DT>& x) {
+        const int k = step * 128 + 32 * j + 8 * g;
+        x.load((const char*) P.x + (uint32_t) (row * P.K + min(k, P.K - 8)) * XES, 0);
+        if (SM == L4_SANY && k >= P.K) x.zero();
+    };
+    uint4 w[DP][NT];                                                              // DP steps in flight
+    L4Q<J, SM> now[NT], next[NT];
+    // where the loads of the codes are (the scales': one quad ahead of the step in hand): a tile's first column, the lane's bytes from there
+    struct At {
+        const uint8_t* codes;
+        const char *scale, *mins;
+        uint32_t coff[NT], soff[NT];
+    };
+    auto enter = [&](int tile, At& a) {
+        const int64_t n0 = (int64_t) tile * (16 * NT);
+        a.codes = P.codes + n0 * (P.K / 2);
+        a.scale = (const char*) P.scale + n0 * P.groups * ses;
+        a.mins = (const char*) P.mins + n0 * P.groups * ses;
         const int left = (int) min<int64_t>(P.N - 1 - n0, 16 * NT);               // (columns past the last: the last again, not stored)
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
             const int n = min(16 * b + l15, left);
-            coff[b] = (uint32_t) (n * (P.K / 2) + 16 * g);
-            soff[b] = (uint32_t) (n * P.groups * ses);
-            boff[b] = P.bias ? 4 * n : 0;
+            a.coff[b] = (uint32_t) (n * (P.K / 2) + 16 * g);
+            a.soff[b] = (uint32_t) (n * P.groups * ses);
         }
     };
-    // (Never skipped: with the same loads in every round the compiler counts the ones in flight; where there is nothing to load it is
+    // (Loads are never skipped: with the same ones in every round the compiler counts those in flight; where there is nothing to load it is
     // the last step or the last tile again.)
-    auto load = [&](uint4 (&wd)[NT], L4S<J, SM> (&sd)[NT], float (&bd)[NT]) {
-        const int step = min(lround * KW + wave, steps - 1);
-        const uint8_t* cp = cbase + step * 64;
+    auto load_w = [&](const At& a, int step, uint4 (&wd)[NT]) {
+        const int st = min(step, steps - 1);
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-            uint32_t at = coff[b];
-            if (SM == L4_SANY) at = min(at, coff[b] - 16 * g + (uint32_t) (P.K / 2 - 16 - step * 64));   // (within the row)
-            wd[b] = *reinterpret_cast<const uint4*>(cp + at);
-        }
-#pragma unroll
-        for (int b = 0; b < NT; ++b) {
-            sd[b].load(P, sbase, zbase, soff[b], step * 4, g);
-            bd[b] = *(const float*) (bbase + boff[b]);
-        }
-        if (++lround == rounds) {
-            lround = 0;
-            ltile = min(ltile + (int) gridDim.x, tiles - 1);
-            enter();
+            uint32_t at = a.coff[b];
+            if (SM == L4_SANY) at = min(at, a.coff[b] - 16 * g + (uint32_t) (P.K / 2 - 16 - st * 64));    // (within the row)
+            wd[b] = *reinterpret_cast<const uint4*>(a.codes + st * 64 + at);
         }
     };
-    enter();
+    auto load_s = [&](const At& a, int step) {
 #pragma unroll
-    for (int u = 0; u < DP; ++u) load(w[u], sr[u], bias[u]);
+        for (int b = 0; b < NT; ++b) next[b].load(P, a.scale, a.mins, a.soff[b], min(step + g, steps - 1) * 4);
+    };
+    int tile = blockIdx.x, quad = 0, turn = 0;
+    At here, then;                                                                // this quad's tile and the next quad's
+    enter(tile, here);
+    load_s(here, first);
+#pragma unroll
+    for (int r = 0; r < DP; ++r) load_w(here, first + r, w[r]);
+    L4X<DT> xr[XR ? 4 : 1][4];
+    if constexpr (XR) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                load_x(min(first + r, steps - 1), j, xr[r][j]);
+                if constexpr (DT != H3S_F32) xr[r][j].u = l4_order(xr[r][j].u);
+            }
+    }
     uint4 sel[4];
     l4_select<OP>(l15, sel);
     uint32_t cm, ce;
     l4_constants<OP>(cm, ce);
-    extern __shared__ uint4 lds[];
-    __shared__ v4f_l4 part[2][NT][KW][64];
-    const int pieces = steps * 16;                                                // 8-input pieces of a row, zeros past its end
-    if constexpr (XL) {
-        for (int i = threadIdx.x; i < pieces * (int) P.M; i += 64 * KW) {
-            const int r = i / pieces, p = i - r * pieces;
-            L4X<DT> v;
-            v.zero();
-            if (8 * p < P.K) v.load((const char*) P.x + (int64_t) r * P.K * (DT == H3S_F32 ? 4 : 2), 8 * p);
-            uint4 f[PARTS];
-            v.parts(f);
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q) lds[(r * PARTS + q) * pieces + p] = f[q];
-        }
-        lds_barrier();
-    }
+    __shared__ v4f_l4 part[2][NT][kL4FewWaves][64];
     v4f_l4 acc[1][NT];
 #pragma unroll
     for (int b = 0; b < NT; ++b) acc[0][b] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
-    int tile = blockIdx.x, round = 0, turn = 0;
     while (tile < tiles) {
+        const bool end = quad + 1 == quads;
+        const int ntile = end ? min(tile + grid, tiles - 1) : tile, nfirst = end ? first : first + 4 * (quad + 1);
+        enter(ntile, then);
 #pragma unroll
-        for (int u = 0; u < DP; ++u) {
-            const int step = round * KW + wave;
+        for (int b = 0; b < NT; ++b) now[b] = next[b];
+        load_s(then, nfirst);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int step = first + 4 * quad + r;
+            if constexpr (!XR) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) load_x(min(step, steps - 1), j, xr[0][j]);
+            }
             uint32_t c[NT][4];
             float sc[NT][4 / J], off[NT];
-            L4X<DT> xr[4];
-            if constexpr (!XL) {
-                const char* xp = (const char*) P.x + (int64_t) min(step, steps - 1) * 128 * (DT == H3S_F32 ? 4 : 2);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t at = xoff + 32 * j * (DT == H3S_F32 ? 4 : 2);
-                    if (SM == L4_SANY) at = min(at, (uint32_t) (row * P.K + P.K - 8 - min(step, steps - 1) * 128) * (DT == H3S_F32 ? 4 : 2));
-                    xr[j].load(xp + at, 0);
+            for (int b = 0; b < NT; ++b) {
+                l4_exchange(w[r % DP][b], c[b]);
+                now[b].pass(P, 4 * (16 * r + l15), g, sc[b], off[b]);
+                if (SM == L4_SANY && step * 128 + 128 > P.K) {
+#pragma unroll
+                    for (int q = 0; q < 4 / J; ++q) sc[b][q] = step * 128 + 32 * J * q < P.K ? sc[b][q] : 0.0f;
+                    off[b] = step * 128 + 32 * g < P.K ? off[b] : 0.0f;
                 }
             }
-            l4_decode<NT, J, SM>(P, step * 128, g, w[u], sr[u], c, sc, off);
-            float bn[NT];
-#pragma unroll
-            for (int b = 0; b < NT; ++b) bn[b] = bias[u][b];
-            load(w[u], sr[u], bias[u]);
-            if (step < steps && tile < tiles) {
-                if constexpr (!XL && SM == L4_SANY) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (step * 128 + 32 * j >= P.K) xr[j].zero();
-                }
-                l4_products<OP, PARTS, 1, NT, NI, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
-                    if constexpr (XL) {
-#pragma unroll
-                        for (int q = 0; q < PARTS; ++q) f[q] = lds[(row * PARTS + q) * pieces + step * 16 + 4 * j + g];
-                    } else xr[j].parts(f);
+            if (r + DP < 4) load_w(here, step + DP, w[r % DP]);
+            else load_w(then, nfirst + r + DP - 4, w[r % DP]);
+            if (step < steps) {
+                l4_products<OP, PARTS, 1, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
+                    if constexpr (XR && DT != H3S_F32) f[0] = xr[r][j].u;
+                    else xr[XR ? r : 0][j].parts(f);
                 }, acc);
             }
-            if (++round == rounds) {
-                // the wavefronts' sums, in wavefront order, by one of them in turn; the others go on (the area is used again two tiles
-                // later, behind the next tile's barrier)
+        }
+        here = then;
+        ++quad;
+        if (end) {
+            // the wavefronts' sums, in wavefront order, by one of them in turn; the others go on (the area is used again two tiles later,
+            // behind the next tile's barrier)
+#pragma unroll
+            for (int b = 0; b < NT; ++b) {
+                part[turn & 1][b][wave][lane] = acc[0][b];
+                acc[0][b] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            lds_barrier();
+            if (wave == turn % KW) {
 #pragma unroll
                 for (int b = 0; b < NT; ++b) {
-                    part[turn & 1][b][wave][lane] = acc[0][b];
-                    acc[0][b] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+                    const int64_t n = (int64_t) tile * (16 * NT) + 16 * b + l15;
+                    v4f_l4 y = part[turn & 1][b][0][lane];
+                    for (int v = 1; v < KW; ++v) y += part[turn & 1][b][v][lane];
+                    l4_store<4>(P, 0, n, g, y, l4_bias(P, n));
                 }
-                lds_barrier();
-                if (wave == turn % KW && tile < tiles) {
-#pragma unroll
-                    for (int b = 0; b < NT; ++b) {
-                        v4f_l4 y = part[turn & 1][b][0][lane];
-#pragma unroll
-                        for (int v = 1; v < KW; ++v) y += part[turn & 1][b][v][lane];
-                        l4_store<NI>(P, 0, (int64_t) tile * (16 * NT) + 16 * b + l15, g, y, bn[b]);
-                    }
-                }
-                ++turn;
-                round = 0;
-                tile += gridDim.x;
             }
+            ++turn;
+            quad = 0;
+            tile += grid;
         }
     }
 }
-constexpr int kL4Lds = 64 * 1024;      // bytes of x in LDS
 
 constexpr int kL4Cols = 128;      // columns of a block of linear4_many_kernel
 
@@ -616,11 +666,12 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
     auto store_x = [&](int stage) {
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int at = t + 256 * p, r = at / 16, k8 = at % 16;                // place: row 4 (l % 4) + l / 4 at l
+            const int at = t + 256 * p, r = at / 16, k8 = at % 16;                // place: row 4 (l % 4) + l / 4 at l,
+                                                                                  // its low bits by the lane group (banks)
             uint4 f[PARTS];
             xr[p].parts(f);
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q) xs[kg][stage][r / 16][k8 / 4][q][k8 % 4 * 16 + (r % 4) * 4 + r % 16 / 4] = f[q];
+            for (int q = 0; q < PARTS; ++q) xs[kg][stage][r / 16][k8 / 4][q][k8 % 4 * 16 + (r % 4) * 4 + (r % 16 / 4 ^ k8 % 4)] = f[q];
         }
     };
     auto load_w = [&](int step) {
@@ -651,7 +702,7 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
             load_w(min(step + 2, steps - 1));
             l4_products<OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
 #pragma unroll
-                for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][stage][a][j][q][lane];
+                for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][stage][a][j][q][lane ^ g];
             }, acc);
             store_x(stage ^ 1);
             load_x(min(step + 4, steps - 1));
@@ -681,19 +732,28 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
     }
 }
 
-// which kernel a call takes (linear4.hip): rows 4, 16 (few: the registers of sums), 32 or 64 (many: the tile)
+// which kernel a call takes (linear4.hip): rows 16 (few), 32 or 64 (many: the tile)
 struct L4Plan { int rows; };
 
-template <int DT, int NT, int KW, int NI, int J, int SM, bool XL>
-static void l4_few(Ctx* c, const L4Args& P, int per_cu, size_t lds) {
+template <int DT, int NT, int J, int SM, bool XR>
+static void l4_few_run(Ctx* c, const L4Args& P, int quads, int kw) {
     // a block walks as many tiles as any other, or one less
-    const int64_t tiles = (P.N + 16 * NT - 1) / (16 * NT), turns = (tiles + per_cu * c->cus - 1) / (per_cu * c->cus);
-    linear4_few_kernel<DT, NT, KW, NI, J, SM, XL><<<(unsigned) ((tiles + turns - 1) / turns), 64 * KW, lds, c->stream>>>(P);
+    const int64_t tiles = (P.N + 16 * NT - 1) / (16 * NT), turns = (tiles + c->cus - 1) / c->cus;
+    linear4_few_kernel<DT, NT, J, SM, XR><<<(unsigned) ((tiles + turns - 1) / turns), 64 * kw, 0, c->stream>>>(P, quads);
+}
+template <int DT, int J, int SM>
+static void l4_few(Ctx* c, const L4Args& P) {
+    // the fewest quads of steps a wavefront that 12 wavefronts can share the inputs in
+    const int steps = (P.K + 127) / 128, quads = (steps + 4 * kL4FewWaves - 1) / (4 * kL4FewWaves), kw = (steps + 4 * quads - 1) / (4 * quads);
+    if constexpr (DT != H3S_F32) {
+        if (quads == 1) return l4_few_run<DT, 1, J, SM, true>(c, P, quads, kw);
+    }
+    l4_few_run<DT, 2, J, SM, false>(c, P, quads, kw);
 }
 template <int DT, int J, int SM>
 static void l4_run(Ctx* c, const L4Args& P, const L4Plan& plan) {
     if (plan.rows <= 16) {
-        l4_few<DT, 2, 8, 4, J, SM, false>(c, P, 2, 0);
+        l4_few<DT, J, SM>(c, P);
     } else {
         const int64_t mt = (P.M + plan.rows - 1) / plan.rows, nb = ((P.N + kL4Cols - 1) / kL4Cols + 7) / 8 * 8;
         if (plan.rows == 32) linear4_many_kernel<DT, 2, J, SM><<<(unsigned) (mt * nb), 512, 0, c->stream>>>(P);

@@ -14,15 +14,15 @@ namespace h3 {
 static KvPlan kv_plan(const KvArgs& P, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
     KvPlan plan;
     const int64_t rows = std::min<int64_t>(most, P.rows) * group;
-    plan.ks = rows <= 64 ? 4 : 1;
+    plan.rows = rows > 64;
     plan.nq = rows <= 16 ? 1 : 2;
-    plan.rt = 16 * plan.nq * (plan.ks == 1 ? 4 : 1);
+    plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
     plan.tiles = (rows + plan.rt - 1) / plan.rt;
     plan.blocks = plan.tiles * P.seqs * P.heads;
     int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     if (window > 0) keys = std::min(keys, window + most + 2 * kKvB);
     const int64_t blocks = (keys + kKvB - 1) / kKvB;
-    const int64_t least = plan.ks == 4 ? 4 : 8;
+    const int64_t least = plan.rows ? 8 : 4;
     int64_t ns = std::min(blocks / least, 2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1));
     plan.nsplit = (int) std::max<int64_t>(1, std::min<int64_t>(ns, 1024));
     return plan;

@@ -13,11 +13,11 @@
 // Layout: S^T = K Q^T, with the keys as the first operand, leaves one query row a lane (lane % 16) and four keys a register
 // group; the row statistics are the lane's own but for two exchanges (lanes 16 and 32 apart). The rows of K are taken in the order
 // that makes those keys, as they stand, the second operand of O^T = V^T P^T: lane group g = lane / 16 holds the keys 16 g .. 16 g + 15
-// of a block, which is also the 16 bytes of a V row that it loads. Nothing goes through LDS on the way.
+// of a block, which is also the 16 bytes of a V row that it loads. Probabilities never leave their registers.
 //
 // Work: a block of threads takes one key/value head of one sequence, a tile of its rows (tokens x the heads that share the
-// key/value head) and a range of the cache blocks. KS = 4: its four wavefronts share 16 NQ rows and take every fourth cache block
-// (few rows: answered tokens; bound by the cache's bytes), joined through LDS. KS = 1: each has 16 NQ rows of its own (prompts).
+// key/value head) and a range of the cache blocks. Few rows (kv_attn_kernel): its four wavefronts share 16 NQ rows and take every fourth cache block
+// (answered tokens; bound by the cache's bytes), joined through LDS. KS = 1: each has 16 NQ rows of its own (prompts).
 // Where that leaves the device idle, the cache blocks are split over several blocks of threads, whose sums kv_merge_kernel
 // joins in split order.
 #pragma once
@@ -101,166 +101,81 @@ __device__ __forceinline__ float kv_lse(float m, float l) {
     return l > 0.0f ? (m + (__builtin_log2f(l) - kKvShift)) * 0.69314718055994531f : l == 0.0f ? -__builtin_inff() : l;
 }
 
-template <int WC, int NQ, int KS, bool TWO>
-__global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
-    constexpr int W = 64 * WC, DT = 4 * WC, RT = 16 * NQ * (KS == 1 ? 4 : 1), PARTS = TWO ? 2 : 1;
-    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
-    int64_t id = blockIdx.x;
-    const int h = (int) (id % P.kv.heads);
-    id /= P.kv.heads;
-    const int split = (int) (id % P.nsplit);
-    id /= P.nsplit;
-    const int b = (int) (id % P.kv.seqs), tile = P.tiles - 1 - (int) (id / P.kv.seqs);      // the longest rows first
-    int r0, n;
-    kv_rows_of(P.kv, b, r0, n);
-    const uint32_t R = (uint32_t) n * P.group, rt0 = (uint32_t) tile * RT;                    // (rows * group is below 2^31)
-    if (rt0 >= R) return;
-    const uint32_t rw = rt0 + (KS == 1 ? wave * 16 * NQ : 0), group = P.group;
-    if (KS == 1 && rw >= R) return;                                                          // (no barrier below for KS = 1)
-    const int len = min(max(P.lengths[b], 0), P.kv.width * kKvB);
-
-    // the query rows: lane % 16 of each of the NQ tiles
-    int pos[NQ];
-    int64_t tok[NQ];
-    int head[NQ];
-    float rowf[NQ];
+// What a wavefront holds of its 16 NQ query rows: row lane % 16 of each tile
+template <int WC, int NQ, bool TWO> struct KvRows {
+    static constexpr int W = 64 * WC, DT = 4 * WC, PARTS = TWO ? 2 : 1;
+    int pos[NQ], head[NQ];                          // the row's token (-1: no row), its query head
+    int64_t tok[NQ];                                // its row of q and out (-1: none)
+    float rowf[NQ], m[NQ], l[NQ];
     v8h_kv qf[NQ][WC][2][PARTS];
-#pragma unroll
-    for (int e = 0; e < NQ; ++e) {
-        const bool valid = rw + 16 * e + l15 < R;
-        const uint32_t r = valid ? rw + 16 * e + l15 : 0;
-        const int j = (int) (r / group);
-        head[e] = (int) (h * group + r % group);
-        tok[e] = valid ? (int64_t) r0 + j : -1;
-        pos[e] = valid ? len - n + j : -1;
-        const int64_t row = ((int64_t) r0 + j) * P.q_stride + (int64_t) head[e] * P.kv.dim;
-        float f[WC * 2][8];
-        float top = 0.0f;
-#pragma unroll
-        for (int c = 0; c < WC; ++c)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int d = c * 64 + g * 16 + s * 8;
-                float* y = f[2 * c + s];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = 0.0f;
-                if (valid && P.q_vec) {
-                    if (d < P.kv.dim) {
-                        if (P.q_dt == H3S_F32) load_f32x((const float*) P.q + row + d, y, 8);
-                        else {
-                            const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*) P.q + row + d);
-                            if (P.q_dt == H3S_BF16) Vec<H3S_BF16>::unpack(u, y);
-                            else Vec<H3S_F16>::unpack(u, y);
-                        }
-                    }
-                } else if (valid) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (d + i < P.kv.dim) y[i] = load_any(P.q, P.q_dt, row + d + i);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(y[i]));
-            }
-        top = kv_max4(top);
-        // 2^k takes top to [2^14, 2^15) (a row of zeros, infinities or NaN: left as it is)
-        const int k = top > 0.0f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-        rowf[e] = __builtin_ldexpf(P.scale, -k);
-#pragma unroll
-        for (int c = 0; c < WC; ++c)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float y = __builtin_ldexpf(f[2 * c + s][i], k);
-                    pin(y);
-                    const _Float16 hi = (_Float16) y;
-                    qf[e][c][s][0][i] = hi;
-                    if constexpr (TWO) qf[e][c][s][1][i] = (_Float16) (y - (float) hi);
-                }
-    }
-
-    // the cache blocks this wavefront walks: those that any of its rows can see, a part of them, every KS-th
-    const int posmin = len - n + (int) (rw / group), posmax = len - n + (int) ((min(R, rw + 16 * NQ) - 1) / group);
-    const int kb0 = P.window > 0 ? max(posmin - P.window + 1, 0) / kKvB : 0;
-    const int count = posmax >= 0 ? posmax / kKvB + 1 - kb0 : 0;
-    const int per = (count + P.nsplit - 1) / P.nsplit;
-    const int last = kb0 + min(count, (split + 1) * per);
-    const int32_t* table = P.kv.table + (int64_t) b * P.kv.width;
-    // the first present block from kb on (its page), or `last`
-    auto present = [&](int& kb, int& page) {
-        for (; kb < last; kb += KS) {
-            page = table[kb];
-            if (page >= 0 && page < P.kv.blocks) return;
-        }
-    };
-    uint4 kr[4][WC], vr[DT];
-    const int koff = ((l15 >> 2) * 16 + (l15 & 3)) * W + g * 16, voff = l15 * 64 + g * 16;
-    auto load_k = [&](int page) {
-        const int8_t* p = P.kv.k + ((int64_t) page * P.kv.heads + h) * (kKvB * W) + koff;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int c = 0; c < WC; ++c) kr[t][c] = *reinterpret_cast<const uint4*>(p + t * 4 * W + c * 64);
-    };
-    auto load_v = [&](int page) {
-        const int8_t* p = P.kv.v + ((int64_t) page * P.kv.heads + h) * (kKvB * W) + voff;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) vr[t] = *reinterpret_cast<const uint4*>(p + t * 1024);
-    };
-
-    float m[NQ], l[NQ];
     v4f_kv o[NQ][DT];
+
+    // rows rw .. of the R of a sequence with n rows from r0 on and len tokens, for key/value head h
+    __device__ __forceinline__ void load(const KvAttnArgs& P, int h, int r0, int n, int len, uint32_t R, uint32_t rw, int l15, int g) {
+        const uint32_t group = P.group;
 #pragma unroll
-    for (int e = 0; e < NQ; ++e) {
-        m[e] = kKvUnset;
-        l[e] = 0.0f;
+        for (int e = 0; e < NQ; ++e) {
+            const bool valid = rw + 16 * e + l15 < R;
+            const uint32_t r = valid ? rw + 16 * e + l15 : 0;
+            const int j = (int) (r / group);
+            head[e] = (int) (h * group + r % group);
+            tok[e] = valid ? (int64_t) r0 + j : -1;
+            pos[e] = valid ? len - n + j : -1;
+            const int64_t row = ((int64_t) r0 + j) * P.q_stride + (int64_t) head[e] * P.kv.dim;
+            float f[WC * 2][8];
+            float top = 0.0f;
 #pragma unroll
-        for (int t = 0; t < DT; ++t) o[e][t] = v4f_kv{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int c = 0; c < WC; ++c)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const int d = c * 64 + g * 16 + s * 8;
+                    float* y = f[2 * c + s];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = 0.0f;
+                    if (valid && P.q_vec) {
+                        if (d < P.kv.dim) {
+                            if (P.q_dt == H3S_F32) load_f32x((const float*) P.q + row + d, y, 8);
+                            else {
+                                const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*) P.q + row + d);
+                                if (P.q_dt == H3S_BF16) Vec<H3S_BF16>::unpack(u, y);
+                                else Vec<H3S_F16>::unpack(u, y);
+                            }
+                        }
+                    } else if (valid) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (d + i < P.kv.dim) y[i] = load_any(P.q, P.q_dt, row + d + i);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(y[i]));
+                }
+            top = kv_max4(top);
+            // 2^k takes top to [2^14, 2^15) (a row of zeros, infinities or NaN: left as it is)
+            const int k = top > 0.0f && top < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+            rowf[e] = __builtin_ldexpf(P.scale, -k);
+#pragma unroll
+            for (int c = 0; c < WC; ++c)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float y = __builtin_ldexpf(f[2 * c + s][i], k);
+                        pin(y);
+                        const _Float16 hi = (_Float16) y;
+                        qf[e][c][s][0][i] = hi;
+                        if constexpr (TWO) qf[e][c][s][1][i] = (_Float16) (y - (float) hi);
+                    }
+            m[e] = kKvUnset;
+            l[e] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[e][t] = v4f_kv{0.0f, 0.0f, 0.0f, 0.0f};
+        }
     }
 
-    int kb = kb0 + split * per + (KS == 1 ? 0 : wave), page = 0;
-    present(kb, page);
-    float ks = 0.0f, vs = 0.0f;
-    if (kb < last) {
-        load_k(page);
-        load_v(page);
-        ks = P.kv.ks[(int64_t) page * P.kv.heads + h];
-        vs = P.kv.vs[(int64_t) page * P.kv.heads + h];
-    }
-    while (kb < last) {
-        int nkb = kb + KS, npage = 0;
-        present(nkb, npage);
-        const bool more = nkb < last;
-        // S^T: register t, i of lane group g is the key 16 g + 4 t + i of the block
-        v4f_kv s[NQ][4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int e = 0; e < NQ; ++e) s[e][t] = v4f_kv{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int c = 0; c < WC; ++c) {
-                const v8h_kv a0 = kv_half8(kr[t][c].x, kr[t][c].y), a1 = kv_half8(kr[t][c].z, kr[t][c].w);
-#pragma unroll
-                for (int e = 0; e < NQ; ++e) {
-#pragma unroll
-                    for (int w = 0; w < PARTS; ++w) {
-                        s[e][t] = kv_mma(a0, qf[e][c][0][w], s[e][t]);
-                        s[e][t] = kv_mma(a1, qf[e][c][1][w], s[e][t]);
-                    }
-                }
-            }
-        }
-        const float ks_now = ks, vs_now = vs;
-        if (more) {
-            load_k(npage);
-            ks = P.kv.ks[(int64_t) npage * P.kv.heads + h];
-            vs = P.kv.vs[(int64_t) npage * P.kv.heads + h];
-        }
-        const int key0 = kb * kKvB;
-        const bool whole = key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window) && !P.mask;
-        v8h_kv pf[NQ][2][PARTS];
-        float vsl[NQ];
+    // One cache block's scores to probabilities: s (register t, i of lane group g: the key 16 g + 4 t + i of the block) to the operands
+    // pf, times 2^15, and vsl, the factor of the block's values for each row. whole: every row sees every key.
+    __device__ __forceinline__ void softmax(const KvAttnArgs& P, int b, int g, int key0, bool whole, float ks, float vs, v4f_kv (&s)[NQ][4],
+                                            v8h_kv (&pf)[NQ][2][PARTS], float (&vsl)[NQ]) {
         uint32_t hidden = 0;                        // by the mask: bit 4 t + i
         if (!whole && P.mask) {
             const int k0 = key0 + g * 16;
@@ -277,7 +192,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
         }
 #pragma unroll
         for (int e = 0; e < NQ; ++e) {
-            float f = rowf[e] * ks_now;
+            float f = rowf[e] * ks;
             f = f < 1e-37f ? 1e-37f : f;            // (minus infinity times it stays minus infinity)
             uint32_t off = hidden;
             if (!whole) {
@@ -300,7 +215,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, s[e][t][i]);
             top = kv_max4(top);
             // a block that the row does not see at all has no part in it, whatever its scales are
-            vsl[e] = whole || top > -__builtin_inff() ? vs_now : 0.0f;
+            vsl[e] = whole || top > -__builtin_inff() ? vs : 0.0f;
             const float mn = fmaxf(m[e], top * f);
             if (__any(mn > m[e])) {
                 const float alpha = __builtin_amdgcn_exp2f(m[e] - mn);
@@ -325,94 +240,320 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
                 }
             l[e] += sum;
         }
-        // O^T
+    }
+
+    // O^T += v_scale V^T P^T for the feature tile t, whose codes of the keys 8 .. of each 16 are a1
+    __device__ __forceinline__ void values(int t, const v8h_kv& a0, const v8h_kv& a1, const v8h_kv (&pf)[NQ][2][PARTS], const float (&vsl)[NQ]) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            const v8h_kv a0 = kv_half8(vr[t].x, vr[t].y), a1 = kv_half8(vr[t].z, vr[t].w);
+        for (int e = 0; e < NQ; ++e) {
+            v4f_kv y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int e = 0; e < NQ; ++e) {
-                v4f_kv y = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int w = 0; w < PARTS; ++w) {
+                y = kv_mma(a0, pf[e][0][w], y);
+                y = kv_mma(a1, pf[e][1][w], y);
+            }
 #pragma unroll
-                for (int w = 0; w < PARTS; ++w) {
-                    y = kv_mma(a0, pf[e][0][w], y);
-                    y = kv_mma(a1, pf[e][1][w], y);
+            for (int i = 0; i < 4; ++i) o[e][t][i] = __builtin_fmaf(y[i], vsl[e], o[e][t][i]);
+        }
+    }
+};
+
+// which rows, head, sequence and part of the cache a block of threads has
+struct KvItem {
+    int h, split, b, tile, r0, n, len;
+    uint32_t R;
+    __device__ __forceinline__ void take(const KvAttnArgs& P) {
+        int64_t id = blockIdx.x;
+        h = (int) (id % P.kv.heads);
+        id /= P.kv.heads;
+        split = (int) (id % P.nsplit);
+        id /= P.nsplit;
+        b = (int) (id % P.kv.seqs);
+        tile = P.tiles - 1 - (int) (id / P.kv.seqs);                      // the longest rows first
+        kv_rows_of(P.kv, b, r0, n);
+        R = (uint32_t) n * P.group;                                       // (rows * group is below 2^31)
+        len = min(max(P.lengths[b], 0), P.kv.width * kKvB);
+    }
+    // the item's place among the parts' sums
+    __device__ __forceinline__ int64_t part(const KvAttnArgs& P) const {
+        return (((int64_t) tile * P.kv.seqs + b) * P.kv.heads + h) * P.nsplit + split;
+    }
+};
+
+// Few rows (up to 64 of a sequence and head): the four wavefronts of a block share 16 NQ rows and take every fourth cache block.
+// Bound by the cache's bytes: the next block's codes are on their way while one is worked on.
+template <int WC, int NQ, bool TWO>
+__global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
+    constexpr int W = 64 * WC, DT = 4 * WC, RT = 16 * NQ, KS = 4, PARTS = TWO ? 2 : 1;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
+    KvItem it;
+    it.take(P);
+    const int h = it.h, b = it.b;
+    const uint32_t R = it.R, rw = (uint32_t) it.tile * RT, group = P.group;
+    if (rw >= R) return;
+    KvRows<WC, NQ, TWO> q;
+    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
+
+    // the cache blocks that any of the rows can see, a part of them, every KS-th
+    const int posmin = it.len - it.n + (int) (rw / group), posmax = it.len - it.n + (int) ((min(R, rw + RT) - 1) / group);
+    const int kb0 = P.window > 0 ? max(posmin - P.window + 1, 0) / kKvB : 0;
+    const int count = posmax >= 0 ? posmax / kKvB + 1 - kb0 : 0;
+    const int per = (count + P.nsplit - 1) / P.nsplit;
+    const int last = kb0 + min(count, (it.split + 1) * per);
+    const int32_t* table = P.kv.table + (int64_t) b * P.kv.width;
+    // the first present block from kb on (its page), or `last`
+    auto present = [&](int& kb, int& page) {
+        for (; kb < last; kb += KS) {
+            page = table[kb];
+            if (page >= 0 && page < P.kv.blocks) return;
+        }
+    };
+    uint4 kr[4][WC], vr[DT];
+    const int koff = ((l15 >> 2) * 16 + (l15 & 3)) * W + g * 16, voff = l15 * 64 + g * 16;
+    auto load_k = [&](int page) {
+        const int8_t* p = P.kv.k + ((int64_t) page * P.kv.heads + h) * (kKvB * W) + koff;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int c = 0; c < WC; ++c) kr[t][c] = *reinterpret_cast<const uint4*>(p + t * 4 * W + c * 64);
+    };
+    auto load_v = [&](int page) {
+        const int8_t* p = P.kv.v + ((int64_t) page * P.kv.heads + h) * (kKvB * W) + voff;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) vr[t] = *reinterpret_cast<const uint4*>(p + t * 1024);
+    };
+    int kb = kb0 + it.split * per + wave, page = 0;
+    present(kb, page);
+    float ks = 0.0f, vs = 0.0f;
+    if (kb < last) {
+        load_k(page);
+        load_v(page);
+        ks = P.kv.ks[(int64_t) page * P.kv.heads + h];
+        vs = P.kv.vs[(int64_t) page * P.kv.heads + h];
+    }
+    while (kb < last) {
+        int nkb = kb + KS, npage = 0;
+        present(nkb, npage);
+        const bool more = nkb < last;
+        v4f_kv s[NQ][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int e = 0; e < NQ; ++e) s[e][t] = v4f_kv{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < WC; ++c) {
+                const v8h_kv a0 = kv_half8(kr[t][c].x, kr[t][c].y), a1 = kv_half8(kr[t][c].z, kr[t][c].w);
+#pragma unroll
+                for (int e = 0; e < NQ; ++e) {
+#pragma unroll
+                    for (int w = 0; w < PARTS; ++w) {
+                        s[e][t] = kv_mma(a0, q.qf[e][c][0][w], s[e][t]);
+                        s[e][t] = kv_mma(a1, q.qf[e][c][1][w], s[e][t]);
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[e][t][i] = __builtin_fmaf(y[i], vsl[e], o[e][t][i]);
             }
         }
+        const float ks_now = ks, vs_now = vs;
+        if (more) {
+            load_k(npage);
+            ks = P.kv.ks[(int64_t) npage * P.kv.heads + h];
+            vs = P.kv.vs[(int64_t) npage * P.kv.heads + h];
+        }
+        const int key0 = kb * kKvB;
+        const bool whole = key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window) && !P.mask;
+        v8h_kv pf[NQ][2][PARTS];
+        float vsl[NQ];
+        q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            q.values(t, kv_half8(vr[t].x, vr[t].y), kv_half8(vr[t].z, vr[t].w), pf, vsl);
         if (more) load_v(npage);
         kb = nkb;
         page = npage;
     }
 
+    // the four wavefronts' sums, 16 rows at a time
+    __shared__ float so[4][16][W + 4];
+    __shared__ float sm[4][16], sl[4][16];
 #pragma unroll
-    for (int e = 0; e < NQ; ++e) l[e] = kv_sum4(l[e]);
-    const int64_t item = ((int64_t) tile * P.kv.seqs + b) * P.kv.heads + h;
-    if constexpr (KS == 1) {
+    for (int e = 0; e < NQ; ++e) {
+        const float l = kv_sum4(q.l[e]);
+        if (e) __syncthreads();
 #pragma unroll
-        for (int e = 0; e < NQ; ++e) {
-            if (tok[e] < 0) continue;
-            if (P.nsplit == 1) {
-                const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
-                const int64_t at = (tok[e] * P.q_heads + head[e]) * P.kv.dim;
+        for (int t = 0; t < DT; ++t)
+            *reinterpret_cast<float4*>(&so[wave][l15][16 * t + 4 * g]) = make_float4(q.o[e][t][0], q.o[e][t][1], q.o[e][t][2], q.o[e][t][3]);
+        if (g == 0) { sm[wave][l15] = q.m[e]; sl[wave][l15] = l; }
+        __syncthreads();
+        const int r = threadIdx.x >> 4, c = threadIdx.x & 15;
+        const uint32_t rr = rw + 16 * e + r;
+        if (rr < R) {
+            const float mx = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+            float wt[4], lt = 0.0f;
 #pragma unroll
-                for (int t = 0; t < DT; ++t)
-                    kv_store4(P, at, 16 * t + 4 * g, o[e][t][0] * inv, o[e][t][1] * inv, o[e][t][2] * inv, o[e][t][3] * inv);
-                if (P.lse && g == 0) P.lse[tok[e] * P.q_heads + head[e]] = kv_lse(m[e], l[e]);
-            } else {
-                const int64_t row = (item * P.nsplit + split) * RT + (rw - rt0) + 16 * e + l15;
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-                    *reinterpret_cast<float4*>(P.po + row * W + 16 * t + 4 * g) = make_float4(o[e][t][0], o[e][t][1], o[e][t][2], o[e][t][3]);
-                if (g == 0) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(m[e], l[e]);
+            for (int w = 0; w < 4; ++w) {
+                wt[w] = __builtin_amdgcn_exp2f(sm[w][r] - mx);
+                lt += sl[w][r] * wt[w];
             }
-        }
-    } else {
-        // the four wavefronts' sums, 16 rows at a time
-        __shared__ float so[4][16][W + 4];
-        __shared__ float sm[4][16], sl[4][16];
+            const int64_t at = ((int64_t) it.r0 + rr / group) * P.q_heads + h * group + rr % group;
+            const int64_t row = it.part(P) * RT + 16 * e + r;
+            const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
 #pragma unroll
-        for (int e = 0; e < NQ; ++e) {
-            if (e) __syncthreads();
-#pragma unroll
-            for (int t = 0; t < DT; ++t)
-                *reinterpret_cast<float4*>(&so[wave][l15][16 * t + 4 * g]) = make_float4(o[e][t][0], o[e][t][1], o[e][t][2], o[e][t][3]);
-            if (g == 0) { sm[wave][l15] = m[e]; sl[wave][l15] = l[e]; }
-            __syncthreads();
-            const int r = threadIdx.x >> 4, c = threadIdx.x & 15;
-            const uint32_t rr = rw + 16 * e + r;
-            if (rr < R) {
-                const float mx = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-                float wt[4], lt = 0.0f;
+            for (int t = 0; t < WC; ++t) {
+                const int d = 64 * t + 4 * c;
+                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    wt[w] = __builtin_amdgcn_exp2f(sm[w][r] - mx);
-                    lt += sl[w][r] * wt[w];
+                    const float4 v = *reinterpret_cast<const float4*>(&so[w][r][d]);
+                    y[0] = __builtin_fmaf(v.x, wt[w], y[0]);
+                    y[1] = __builtin_fmaf(v.y, wt[w], y[1]);
+                    y[2] = __builtin_fmaf(v.z, wt[w], y[2]);
+                    y[3] = __builtin_fmaf(v.w, wt[w], y[3]);
                 }
-                const int64_t at = ((int64_t) r0 + rr / group) * P.q_heads + h * group + rr % group;
-                const int64_t row = (item * P.nsplit + split) * RT + 16 * e + r;
-                const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-#pragma unroll
-                for (int t = 0; t < WC; ++t) {
-                    const int d = 64 * t + 4 * c;
-                    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const float4 v = *reinterpret_cast<const float4*>(&so[w][r][d]);
-                        y[0] = __builtin_fmaf(v.x, wt[w], y[0]);
-                        y[1] = __builtin_fmaf(v.y, wt[w], y[1]);
-                        y[2] = __builtin_fmaf(v.z, wt[w], y[2]);
-                        y[3] = __builtin_fmaf(v.w, wt[w], y[3]);
-                    }
-                    if (P.nsplit == 1) kv_store4(P, at * P.kv.dim, d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
-                    else *reinterpret_cast<float4*>(P.po + row * W + d) = make_float4(y[0], y[1], y[2], y[3]);
-                }
-                if (c == 0) {
-                    if (P.nsplit > 1) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(mx, lt);
-                    else if (P.lse) P.lse[at] = kv_lse(mx, lt);
-                }
+                if (P.nsplit == 1) kv_store4(P, at * P.kv.dim, d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+                else *reinterpret_cast<float4*>(P.po + row * W + d) = make_float4(y[0], y[1], y[2], y[3]);
             }
+            if (c == 0) {
+                if (P.nsplit > 1) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(mx, lt);
+                else if (P.lse) P.lse[at] = kv_lse(mx, lt);
+            }
+        }
+    }
+}
+
+// Many rows: each of a block's four wavefronts has 16 NQ rows of its own, and all go through the same cache blocks. A block's codes
+// are turned to half once, by all four, into LDS in the order of the products' operands (two stages, one barrier a cache block), where
+// doing it in every wavefront took more vector instructions than the softmax. Bound by vector instructions beside the products.
+template <int WC, int NQ, bool TWO>
+__global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs P) {
+    constexpr int W = 64 * WC, DT = 4 * WC, RT = 64 * NQ, PARTS = TWO ? 2 : 1;
+    __shared__ v8h_kv sk[2][4][WC][2][64], sv[2][DT][2][64];              // [stage][key tile or feature tile][...][half][lane]
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
+    KvItem it;
+    it.take(P);
+    const int h = it.h, b = it.b;
+    const uint32_t R = it.R, rt0 = (uint32_t) it.tile * RT, rw = rt0 + wave * 16 * NQ, group = P.group;
+    if (rt0 >= R) return;
+    KvRows<WC, NQ, TWO> q;
+    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
+    // the cache blocks that any of the block's rows can see, a part of them; the wavefront's own rows see posmin .. posmax
+    const int base = it.len - it.n, bmin = base + (int) (rt0 / group), bmax = base + (int) ((min(R, rt0 + RT) - 1) / group);
+    const bool rows = rw < R;
+    const int posmin = base + (int) (rw / group), posmax = rows ? base + (int) ((min(R, rw + 16 * NQ) - 1) / group) : -1;
+    const int kb0 = P.window > 0 ? max(bmin - P.window + 1, 0) / kKvB : 0;
+    const int count = bmax >= 0 ? bmax / kKvB + 1 - kb0 : 0;
+    const int per = (count + P.nsplit - 1) / P.nsplit;
+    const int last = kb0 + min(count, (it.split + 1) * per);
+    const int32_t* table = P.kv.table + (int64_t) b * P.kv.width;
+    auto present = [&](int& kb, int& page) {
+        for (; kb < last; ++kb) {
+            page = table[kb];
+            if (page >= 0 && page < P.kv.blocks) return;
+        }
+        page = -1;
+    };
+    // the thread's 16-byte pieces of a block's codes: piece t + 256 i
+    uint4 kr[WC], vr[WC];
+    float ks = 0.0f, vs = 0.0f;
+    auto load = [&](int page) {
+        const int64_t at = (int64_t) page * P.kv.heads + h;
+        const uint4 *kp = reinterpret_cast<const uint4*>(P.kv.k + at * (kKvB * W)), *vp = reinterpret_cast<const uint4*>(P.kv.v + at * (kKvB * W));
+#pragma unroll
+        for (int i = 0; i < WC; ++i) {
+            kr[i] = kp[threadIdx.x + 256 * i];
+            vr[i] = vp[threadIdx.x + 256 * i];
+        }
+        ks = P.kv.ks[at];
+        vs = P.kv.vs[at];
+    };
+    auto stage = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < WC; ++i) {
+            const int p = threadIdx.x + 256 * i;
+            // keys: token p / 4 WC, the features 16 (p % 4 WC) ..; the token is row 4 (token / 16) + token % 4 of the key tile token / 4 % 4.
+            // (the low bits of its place are mixed with the lane group's: else a store's lanes lie on a quarter of the banks)
+            const int key = p / (4 * WC), c = p % (4 * WC) / 4, kg = p % 4, at = (key >> 4) * 4 + (key & 3), t = (key >> 2) & 3;
+            sk[st][t][c][0][16 * kg + (at ^ (4 * kg))] = kv_half8(kr[i].x, kr[i].y);
+            sk[st][t][c][1][16 * kg + (at ^ (4 * kg))] = kv_half8(kr[i].z, kr[i].w);
+            // values: feature p / 4, the tokens 16 (p % 4) ..
+            sv[st][p / 64][0][16 * (p & 3) + p / 4 % 16] = kv_half8(vr[i].x, vr[i].y);
+            sv[st][p / 64][1][16 * (p & 3) + p / 4 % 16] = kv_half8(vr[i].z, vr[i].w);
+        }
+    };
+    int kb = kb0 + it.split * per, page = -1, st = 0;
+    present(kb, page);
+    int nkb = kb, npage = -1;
+    float ks_now = 0.0f, vs_now = 0.0f;
+    if (page >= 0) {
+        load(page);
+        stage(0);
+        ks_now = ks;
+        vs_now = vs;
+        nkb = kb + 1;
+        present(nkb, npage);
+        if (npage >= 0) load(npage);
+    }
+    lds_barrier();
+    while (kb < last) {
+        const int key0 = kb * kKvB;
+        if (key0 <= posmax) {
+            v4f_kv s[NQ][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int e = 0; e < NQ; ++e) s[e][t] = v4f_kv{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < WC; ++c)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const v8h_kv a = sk[st][t][c][u][16 * g + (l15 ^ (4 * g))];
+#pragma unroll
+                        for (int e = 0; e < NQ; ++e)
+#pragma unroll
+                            for (int w = 0; w < PARTS; ++w) s[e][t] = kv_mma(a, q.qf[e][c][u][w], s[e][t]);
+                    }
+            }
+            const bool whole = key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window) && !P.mask;
+            v8h_kv pf[NQ][2][PARTS];
+            float vsl[NQ];
+            q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) q.values(t, sv[st][t][0][lane], sv[st][t][1][lane], pf, vsl);
+        }
+        // the next block's codes, loaded a block ago, to the other stage, and the loads of the one after
+        if (npage >= 0) {
+            stage(st ^ 1);
+            ks_now = ks;
+            vs_now = vs;
+        }
+        kb = nkb;
+        page = npage;
+        if (npage >= 0) {
+            nkb = kb + 1;
+            present(nkb, npage);
+            if (npage >= 0) load(npage);
+        }
+        lds_barrier();
+        st ^= 1;
+    }
+#pragma unroll
+    for (int e = 0; e < NQ; ++e) {
+        const float l = kv_sum4(q.l[e]);
+        if (q.tok[e] < 0) continue;
+        if (P.nsplit == 1) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t at = q.tok[e] * P.q_heads + q.head[e];
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+                kv_store4(P, at * P.kv.dim, 16 * t + 4 * g, q.o[e][t][0] * inv, q.o[e][t][1] * inv, q.o[e][t][2] * inv, q.o[e][t][3] * inv);
+            if (P.lse && g == 0) P.lse[at] = kv_lse(q.m[e], l);
+        } else {
+            const int64_t row = it.part(P) * RT + (rw - rt0) + 16 * e + l15;
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+                *reinterpret_cast<float4*>(P.po + row * W + 16 * t + 4 * g) = make_float4(q.o[e][t][0], q.o[e][t][1], q.o[e][t][2], q.o[e][t][3]);
+            if (g == 0) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(q.m[e], l);
         }
     }
 }
@@ -462,18 +603,24 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
 
 // which kernel takes the call, and in how many parts
 struct KvPlan {
-    int nq, ks, rt;       // kv_attn_kernel's, and the rows a block of threads takes
+    bool rows;            // kv_attn_rows_kernel (else kv_attn_kernel)
+    int nq, rt;           // its tiles of 16 rows a wavefront, and the rows a block of threads takes
     int64_t tiles;
     int nsplit;
     int64_t blocks;       // of threads, without the parts
 };
 
-template <int WC, int NQ, int KS>
+template <int WC, int NQ, bool ROWS>
 static void kv_attn_run(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two) {
     const unsigned grid = (unsigned) (plan.blocks * plan.nsplit);
-    if (two) kv_attn_kernel<WC, NQ, KS, true><<<grid, 256, 0, c->stream>>>(P);
-    else kv_attn_kernel<WC, NQ, KS, false><<<grid, 256, 0, c->stream>>>(P);
-    constexpr int RT = 16 * NQ * (KS == 1 ? 4 : 1);
+    constexpr int RT = (ROWS ? 64 : 16) * NQ;
+    if constexpr (ROWS) {
+        if (two) kv_attn_rows_kernel<WC, NQ, true><<<grid, 256, 0, c->stream>>>(P);
+        else kv_attn_rows_kernel<WC, NQ, false><<<grid, 256, 0, c->stream>>>(P);
+    } else {
+        if (two) kv_attn_kernel<WC, NQ, true><<<grid, 256, 0, c->stream>>>(P);
+        else kv_attn_kernel<WC, NQ, false><<<grid, 256, 0, c->stream>>>(P);
+    }
     if (plan.nsplit > 1) kv_merge_kernel<WC, RT><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
 }
 
@@ -485,9 +632,9 @@ void kv_attn_256(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
 
 template <int WC>
 static void kv_attn_width(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two) {
-    if (plan.ks == 4 && plan.nq == 1) kv_attn_run<WC, 1, 4>(c, P, plan, two);
-    else if (plan.ks == 4) kv_attn_run<WC, 2, 4>(c, P, plan, two);
-    else kv_attn_run<WC, 2, 1>(c, P, plan, two);
+    if (plan.rows) kv_attn_run<WC, 2, true>(c, P, plan, two);
+    else if (plan.nq == 1) kv_attn_run<WC, 1, false>(c, P, plan, two);
+    else kv_attn_run<WC, 2, false>(c, P, plan, two);
 }
 
 }  // namespace h3

@@ -475,11 +475,11 @@ def test_attention_kernels_taken(dev):
         return launches(dev, lambda: ops.kv_attention(c, t, rq, st, lt, max(n for n, _ in seqs), out, work=work))
 
     few = names([(1, 200)] * 3, 2, 8, 128, "BF16", {})
-    assert len(few) == 1 and few[0][0].startswith("kv_attn_kernel<2, 1, 4, false") and few[0][1] == 6, few
+    assert len(few) == 1 and few[0][0].startswith("kv_attn_kernel<2, 1, false") and few[0][1] == 6, few
     split = names([(1, 2000)], 1, 8, 128, "F32", {})
-    assert len(split) == 2 and split[0][0].startswith("kv_attn_kernel<2, 1, 4, true") and split[0][1] > 4, split
+    assert len(split) == 2 and split[0][0].startswith("kv_attn_kernel<2, 1, true") and split[0][1] > 4, split
     many = names([(100, 100)], 2, 4, 64, "F16", {})
-    assert many[0][0].startswith("kv_attn_kernel<1, 2, 1, false"), many
+    assert many[0][0].startswith("kv_attn_rows_kernel<1, 2, false"), many
 
 
 # ---- linear4 -------------------------------------------------------------------------------------------------------------------

@@ -8,23 +8,26 @@
 namespace h3 {
 
 // Rows: `most` tokens of a sequence times the heads that share a key/value head. Up to 64 rows the four wavefronts of a block
-// share 16 or 32 of them and the cache is read by all four (an answered token is bound by the cache's bytes); beyond, each has 32
-// rows of its own. Parts: as many as give each CU two blocks of threads, but at least four cache blocks each (one a
-// wavefront), because every part costs its sums, written and read, and the merge's launch.
+// share 16 or 32 of them and the cache is read by all four (an answered token is bound by the cache's bytes); beyond, each has 16 or 32
+// rows of its own (16 where 32 would leave CUs without a block).
+// Parts: of the same number of cache blocks for every sequence (at least four), as many as give each CU the two blocks of threads that
+// it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up to 8192 tokens, 64
+// heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and their merge 4, 7
+// and 11 us more.)
 static KvPlan kv_plan(const KvArgs& P, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
     KvPlan plan;
-    const int64_t rows = std::min<int64_t>(most, P.rows) * group;
+    const int64_t rows = std::min<int64_t>(most, P.rows) * group, each = (int64_t) P.seqs * P.heads;
     plan.rows = rows > 64;
-    plan.nq = rows <= 16 ? 1 : 2;
+    plan.nq = plan.rows ? ((rows + 127) / 128 * each < cus ? 1 : 2) : rows <= 16 ? 1 : 2;
     plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
     plan.tiles = (rows + plan.rt - 1) / plan.rt;
-    plan.blocks = plan.tiles * P.seqs * P.heads;
+    plan.blocks = plan.tiles * each;
     int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     if (window > 0) keys = std::min(keys, window + most + 2 * kKvB);
-    const int64_t blocks = (keys + kKvB - 1) / kKvB;
-    const int64_t least = plan.rows ? 8 : 4;
-    int64_t ns = std::min(blocks / least, 2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1));
-    plan.nsplit = (int) std::max<int64_t>(1, std::min<int64_t>(ns, 1024));
+    const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = 4;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
+    plan.per = (int) std::max(least, (blocks + want - 1) / want);
+    plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
     return plan;
 }
 static int64_t kv_part_floats(const KvPlan& plan, int64_t W) { return plan.nsplit > 1 ? plan.blocks * plan.nsplit * plan.rt * (W + 2) : 0; }
@@ -88,7 +91,7 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     A.window = (int) std::min<int64_t>(window, INT32_MAX / 2);
     A.mask = mask; A.mask_stride = mask_stride;
     A.out = out; A.out_dt = out_dt; A.lse = lse;
-    A.tiles = (int) plan.tiles; A.nsplit = plan.nsplit;
+    A.tiles = (int) plan.tiles; A.nsplit = plan.nsplit; A.per = plan.per;
     A.q_vec = aligned16(q) && dim % 8 == 0 && (q_stride * elem_size(dt)) % 16 == 0;
     A.out_vec = aligned16(out) && dim % 4 == 0;
     A.mask_vec = mask && aligned16(mask) && mask_stride % 16 == 0;

@@ -46,7 +46,7 @@ struct KvAttnArgs {
     void* out;
     int out_dt;
     float* lse;
-    int tiles, nsplit;                              // row tiles a sequence and head; parts of the cache blocks
+    int tiles, nsplit, per;                         // row tiles a sequence and head; parts, of `per` cache blocks each (the last: the rest)
     float *po, *pml;                                // the parts' sums [item, part, rows, W] and (m, l) [item, part, rows, 2]
     bool q_vec, out_vec, mask_vec;
 };
@@ -274,6 +274,16 @@ struct KvItem {
         R = (uint32_t) n * P.group;                                       // (rows * group is below 2^31)
         len = min(max(P.lengths[b], 0), P.kv.width * kKvB);
     }
+    // the cache blocks kb0 .. kb0 + count that any of the rows rt0 .. rt0 + rt can see
+    __device__ __forceinline__ void range(const KvAttnArgs& P, uint32_t rt0, int rt, int& kb0, int& count) const {
+        const int base = len - n, bmin = base + (int) (rt0 / P.group), bmax = base + (int) ((min(R, rt0 + rt) - 1) / P.group);
+        kb0 = P.window > 0 ? max(bmin - P.window + 1, 0) / kKvB : 0;
+        count = bmax >= 0 ? max(bmax / kKvB + 1 - kb0, 0) : 0;
+    }
+    // the end of this part's blocks (from kb0 + split * per on); parts past the first that have none leave nothing
+    __device__ __forceinline__ int end(const KvAttnArgs& P, int kb0, int count) const {
+        return split + 1 == P.nsplit ? kb0 + count : kb0 + min(count, (split + 1) * P.per);
+    }
     // the item's place among the parts' sums
     __device__ __forceinline__ int64_t part(const KvAttnArgs& P) const {
         return (((int64_t) tile * P.kv.seqs + b) * P.kv.heads + h) * P.nsplit + split;
@@ -297,10 +307,10 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
 
     // the cache blocks that any of the rows can see, a part of them, every KS-th
     const int posmin = it.len - it.n + (int) (rw / group), posmax = it.len - it.n + (int) ((min(R, rw + RT) - 1) / group);
-    const int kb0 = P.window > 0 ? max(posmin - P.window + 1, 0) / kKvB : 0;
-    const int count = posmax >= 0 ? posmax / kKvB + 1 - kb0 : 0;
-    const int per = (count + P.nsplit - 1) / P.nsplit;
-    const int last = kb0 + min(count, (it.split + 1) * per);
+    int kb0, count;
+    it.range(P, rw, RT, kb0, count);
+    if (it.split && it.split * P.per >= count) return;
+    const int last = it.end(P, kb0, count);
     const int32_t* table = P.kv.table + (int64_t) b * P.kv.width;
     // the first present block from kb on (its page), or `last`
     auto present = [&](int& kb, int& page) {
@@ -323,7 +333,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) vr[t] = *reinterpret_cast<const uint4*>(p + t * 1024);
     };
-    int kb = kb0 + it.split * per + wave, page = 0;
+    int kb = kb0 + it.split * P.per + wave, page = 0;
     present(kb, page);
     float ks = 0.0f, vs = 0.0f;
     if (kb < last) {
@@ -438,13 +448,12 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
     KvRows<WC, NQ, TWO> q;
     q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
     // the cache blocks that any of the block's rows can see, a part of them; the wavefront's own rows see posmin .. posmax
-    const int base = it.len - it.n, bmin = base + (int) (rt0 / group), bmax = base + (int) ((min(R, rt0 + RT) - 1) / group);
-    const bool rows = rw < R;
-    const int posmin = base + (int) (rw / group), posmax = rows ? base + (int) ((min(R, rw + 16 * NQ) - 1) / group) : -1;
-    const int kb0 = P.window > 0 ? max(bmin - P.window + 1, 0) / kKvB : 0;
-    const int count = bmax >= 0 ? bmax / kKvB + 1 - kb0 : 0;
-    const int per = (count + P.nsplit - 1) / P.nsplit;
-    const int last = kb0 + min(count, (it.split + 1) * per);
+    const int base = it.len - it.n;
+    const int posmin = base + (int) (rw / group), posmax = rw < R ? base + (int) ((min(R, rw + 16 * NQ) - 1) / group) : -1;
+    int kb0, count;
+    it.range(P, rt0, RT, kb0, count);
+    if (it.split && it.split * P.per >= count) return;
+    const int last = it.end(P, kb0, count);
     const int32_t* table = P.kv.table + (int64_t) b * P.kv.width;
     auto present = [&](int& kb, int& page) {
         for (; kb < last; ++kb) {
@@ -481,7 +490,7 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
             sv[st][p / 64][1][16 * (p & 3) + p / 4 % 16] = kv_half8(vr[i].z, vr[i].w);
         }
     };
-    int kb = kb0 + it.split * per, page = -1, st = 0;
+    int kb = kb0 + it.split * P.per, page = -1, st = 0;
     present(kb, page);
     int nkb = kb, npage = -1;
     float ks_now = 0.0f, vs_now = 0.0f;
@@ -565,17 +574,24 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t item = blockIdx.x / RT;
     const int r = (int) (blockIdx.x % RT);
-    const int h = (int) (item % P.kv.heads), b = (int) (item / P.kv.heads % P.kv.seqs);
-    int r0, n;
-    kv_rows_of(P.kv, b, r0, n);
-    const uint32_t rr = (uint32_t) (item / P.kv.heads / P.kv.seqs) * RT + r, group = P.group;
-    if (rr >= (uint32_t) n * group) return;
+    KvItem it;
+    it.h = (int) (item % P.kv.heads);
+    it.b = (int) (item / P.kv.heads % P.kv.seqs);
+    it.tile = (int) (item / P.kv.heads / P.kv.seqs);
+    kv_rows_of(P.kv, it.b, it.r0, it.n);
+    it.R = (uint32_t) it.n * P.group;
+    it.len = min(max(P.lengths[it.b], 0), P.kv.width * kKvB);
+    const uint32_t rr = (uint32_t) it.tile * RT + r, group = P.group;
+    if (rr >= it.R) return;
+    int kb0, count;
+    it.range(P, (uint32_t) it.tile * RT, RT, kb0, count);
+    const int parts = min(max((count + P.per - 1) / P.per, 1), P.nsplit);
     const int64_t row0 = item * P.nsplit * RT + r;
     float mx = kKvUnset;
-    for (int s = lane; s < P.nsplit; s += 64) mx = fmaxf(mx, P.pml[(row0 + (int64_t) s * RT) * 2]);
+    for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, P.pml[(row0 + (int64_t) s * RT) * 2]);
     mx = wave_max<64>(mx);
     float lt = 0.0f;
-    for (int s = lane; s < P.nsplit; s += 64) {
+    for (int s = lane; s < parts; s += 64) {
         const float2 ml = *reinterpret_cast<const float2*>(P.pml + (row0 + (int64_t) s * RT) * 2);
         lt += ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
     }
@@ -584,7 +600,7 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
 #pragma unroll
     for (int t = 0; t < WC; ++t) y[t] = 0.0f;
 #pragma unroll 4
-    for (int s = wave; s < P.nsplit; s += 4) {
+    for (int s = wave; s < parts; s += 4) {
         const int64_t row = row0 + (int64_t) s * RT;
         const float w = __builtin_amdgcn_exp2f(P.pml[row * 2] - mx);
 #pragma unroll
@@ -594,7 +610,7 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
 #pragma unroll
     for (int t = 0; t < WC; ++t) sy[wave][64 * t + lane] = y[t];
     __syncthreads();
-    const int64_t at = ((int64_t) r0 + rr / group) * P.q_heads + h * group + rr % group;
+    const int64_t at = ((int64_t) it.r0 + rr / group) * P.q_heads + it.h * group + rr % group;
     const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
     for (int d = threadIdx.x; d < P.kv.dim; d += 256)
         store_any(P.out, P.out_dt, at * P.kv.dim + d, ((sy[0][d] + sy[1][d]) + (sy[2][d] + sy[3][d])) * inv);
@@ -606,7 +622,7 @@ struct KvPlan {
     bool rows;            // kv_attn_rows_kernel (else kv_attn_kernel)
     int nq, rt;           // its tiles of 16 rows a wavefront, and the rows a block of threads takes
     int64_t tiles;
-    int nsplit;
+    int nsplit, per;      // parts, and the cache blocks of each
     int64_t blocks;       // of threads, without the parts
 };
 
@@ -632,7 +648,8 @@ void kv_attn_256(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
 
 template <int WC>
 static void kv_attn_width(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two) {
-    if (plan.rows) kv_attn_run<WC, 2, true>(c, P, plan, two);
+    if (plan.rows && plan.nq == 1) kv_attn_run<WC, 1, true>(c, P, plan, two);
+    else if (plan.rows) kv_attn_run<WC, 2, true>(c, P, plan, two);
     else if (plan.nq == 1) kv_attn_run<WC, 1, false>(c, P, plan, two);
     else kv_attn_run<WC, 2, false>(c, P, plan, two);
 }

@@ -8,7 +8,7 @@ from helpers import launches, new, up
 
 pytestmark = pytest.mark.gpu
 
-from sycl_minimax_h3_amd import Error, Tensor, ops  # noqa: E402
+from sycl_minimax_h3_amd import Device, Error, Tensor, ops  # noqa: E402
 
 BLOCK = ref.BLOCK
 
@@ -221,8 +221,28 @@ def check_attn(got, lse, want, used, what=""):
         assert (lse[used:] == 44.0).all()
 
 
+@pytest.fixture(scope="module")
+def dev_cus2():
+    """A context that sizes its grids for two compute units: calls of any size then take the tiles of large ones, without parts."""
+    import os
+
+    old = os.environ.get("H3S_CUS")
+    os.environ["H3S_CUS"] = "2"
+    try:
+        d = Device.open()
+    finally:
+        if old is None:
+            del os.environ["H3S_CUS"]
+        else:
+            os.environ["H3S_CUS"] = old
+    yield d
+    d.close()
+
+
+@pytest.mark.parametrize("where", ["dev", "dev_cus2"])
 @pytest.mark.parametrize("seqs,heads,group,dim,dt,out_dt,opts", ATTN)
-def test_attention(dev, seqs, heads, group, dim, dt, out_dt, opts):
+def test_attention(request, where, seqs, heads, group, dim, dt, out_dt, opts):
+    dev = request.getfixturevalue(where)
     case = attn_case(dev, seqs, heads, group, dim, dt, opts)
     cache, table, starts, lengths, bits, q, rows, stride, mask = case
     got, lse = run_attn(dev, *case, group, dt, out_dt, opts)
@@ -477,9 +497,11 @@ def test_attention_kernels_taken(dev):
     few = names([(1, 200)] * 3, 2, 8, 128, "BF16", {})
     assert len(few) == 1 and few[0][0].startswith("kv_attn_kernel<2, 1, false") and few[0][1] == 6, few
     split = names([(1, 2000)], 1, 8, 128, "F32", {})
-    assert len(split) == 2 and split[0][0].startswith("kv_attn_kernel<2, 1, true") and split[0][1] > 4, split
-    many = names([(100, 100)], 2, 4, 64, "F16", {})
-    assert many[0][0].startswith("kv_attn_rows_kernel<1, 2, false"), many
+    assert len(split) == 2 and split[0][0].startswith("kv_attn_kernel<2, 1, true") and split[0][1] >= 4, split
+    some = names([(100, 100)], 2, 4, 64, "F16", {})
+    assert len(some) == 1 and some[0][0].startswith("kv_attn_rows_kernel<1, 1, false") and some[0][1] == 14, some
+    many = names([(130, 130)], 16, 16, 64, "F16", {})
+    assert len(many) == 1 and many[0][0].startswith("kv_attn_rows_kernel<1, 2, false") and many[0][1] == 17 * 16, many
 
 
 # ---- linear4 -------------------------------------------------------------------------------------------------------------------

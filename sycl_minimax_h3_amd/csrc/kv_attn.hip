@@ -10,7 +10,7 @@ namespace h3 {
 // Rows: `most` tokens of a sequence times the heads that share a key/value head. Up to 64 rows the four wavefronts of a block
 // share 16 or 32 of them and the cache is read by all four (an answered token is bound by the cache's bytes); beyond, each has 16 or 32
 // rows of its own (16 where 32 would leave CUs without a block).
-// Parts: of the same number of cache blocks for every sequence (at least four), as many as give each CU the two blocks of threads that
+// Parts: of the same number of cache blocks for every sequence (at least eight, or four of a prompt's), as many as give each CU the two blocks of threads that
 // it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up to 8192 tokens, 64
 // heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and their merge 4, 7
 // and 11 us more.)
@@ -24,7 +24,7 @@ static KvPlan kv_plan(const KvArgs& P, int64_t most, int64_t group, int64_t max_
     plan.blocks = plan.tiles * each;
     int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     if (window > 0) keys = std::min(keys, window + most + 2 * kKvB);
-    const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = 4;
+    const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
     plan.per = (int) std::max(least, (blocks + want - 1) / want);
     plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);

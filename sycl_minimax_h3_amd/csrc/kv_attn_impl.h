@@ -192,8 +192,6 @@ template <int WC, int NQ, bool TWO> struct KvRows {
         }
 #pragma unroll
         for (int e = 0; e < NQ; ++e) {
-            float f = rowf[e] * ks;
-            f = f < 1e-37f ? 1e-37f : f;            // (minus infinity times it stays minus infinity)
             uint32_t off = hidden;
             if (!whole) {
                 const int hi = pos[e] - key0 - g * 16;                  // the lane's keys 0 .. hi of 16 are not ahead of the row
@@ -214,8 +212,13 @@ template <int WC, int NQ, bool TWO> struct KvRows {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, s[e][t][i]);
             top = kv_max4(top);
-            // a block that the row does not see at all has no part in it, whatever its scales are
-            vsl[e] = whole || top > -__builtin_inff() ? vs : 0.0f;
+            // Hidden scores are minus infinity, and a factor above 0 keeps them so. Where the row sees none of the block, the block has no
+            // part in it whatever its scales are (NaN times minus infinity would be NaN).
+            const bool seen = top > -__builtin_inff();
+            float f = rowf[e] * ks;
+            f = f < 1e-37f ? 1e-37f : f;
+            f = seen ? f : 1.0f;
+            vsl[e] = seen ? vs : 0.0f;
             const float mn = fmaxf(m[e], top * f);
             if (__any(mn > m[e])) {
                 const float alpha = __builtin_amdgcn_exp2f(m[e] - mn);
@@ -230,8 +233,7 @@ template <int WC, int NQ, bool TWO> struct KvRows {
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e][t][i], f, ref));
-                    if (!whole && ((off >> (4 * t + i)) & 1)) p = 0.0f;
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e][t][i], f, ref));
                     sum += p;
                     const int at = 4 * (t & 1) + i;
                     const _Float16 hi = (_Float16) p;
@@ -431,6 +433,10 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     }
 }
 
+// A 16-byte place among the 16 of a lane group is mixed with the group and the feature chunk: 16 lanes that store side by side (four
+// tokens' or one token's pieces) then lie on all banks. Reads stay 16 places of one group.
+template <int WC> __device__ __forceinline__ int kv_mix(int g, int c) { return (4 * g) ^ (WC == 2 ? 2 * c : c); }
+
 // Many rows: each of a block's four wavefronts has 16 NQ rows of its own, and all go through the same cache blocks. A block's codes
 // are turned to half once, by all four, into LDS in the order of the products' operands (two stages, one barrier a cache block), where
 // doing it in every wavefront took more vector instructions than the softmax. Bound by vector instructions beside the products.
@@ -481,13 +487,14 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
         for (int i = 0; i < WC; ++i) {
             const int p = threadIdx.x + 256 * i;
             // keys: token p / 4 WC, the features 16 (p % 4 WC) ..; the token is row 4 (token / 16) + token % 4 of the key tile token / 4 % 4.
-            // (the low bits of its place are mixed with the lane group's: else a store's lanes lie on a quarter of the banks)
-            const int key = p / (4 * WC), c = p % (4 * WC) / 4, kg = p % 4, at = (key >> 4) * 4 + (key & 3), t = (key >> 2) & 3;
-            sk[st][t][c][0][16 * kg + (at ^ (4 * kg))] = kv_half8(kr[i].x, kr[i].y);
-            sk[st][t][c][1][16 * kg + (at ^ (4 * kg))] = kv_half8(kr[i].z, kr[i].w);
+            const int key = p / (4 * WC), c = p % (4 * WC) / 4, kg = p % 4, at = 16 * kg + (((key >> 4) * 4 + (key & 3)) ^ kv_mix<WC>(kg, c));
+            const int t = (key >> 2) & 3;
+            sk[st][t][c][0][at] = kv_half8(kr[i].x, kr[i].y);
+            sk[st][t][c][1][at] = kv_half8(kr[i].z, kr[i].w);
             // values: feature p / 4, the tokens 16 (p % 4) ..
-            sv[st][p / 64][0][16 * (p & 3) + p / 4 % 16] = kv_half8(vr[i].x, vr[i].y);
-            sv[st][p / 64][1][16 * (p & 3) + p / 4 % 16] = kv_half8(vr[i].z, vr[i].w);
+            const int av = 16 * kg + (p / 4 % 16 ^ (4 * kg));
+            sv[st][p / 64][0][av] = kv_half8(vr[i].x, vr[i].y);
+            sv[st][p / 64][1][av] = kv_half8(vr[i].z, vr[i].w);
         }
     };
     int kb = kb0 + it.split * P.per, page = -1, st = 0;
@@ -516,7 +523,7 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
                 for (int c = 0; c < WC; ++c)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const v8h_kv a = sk[st][t][c][u][16 * g + (l15 ^ (4 * g))];
+                        const v8h_kv a = sk[st][t][c][u][16 * g + (l15 ^ kv_mix<WC>(g, c))];
 #pragma unroll
                         for (int e = 0; e < NQ; ++e)
 #pragma unroll
@@ -528,7 +535,7 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
             float vsl[NQ];
             q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
 #pragma unroll
-            for (int t = 0; t < DT; ++t) q.values(t, sv[st][t][0][lane], sv[st][t][1][lane], pf, vsl);
+            for (int t = 0; t < DT; ++t) q.values(t, sv[st][t][0][16 * g + (l15 ^ (4 * g))], sv[st][t][1][16 * g + (l15 ^ (4 * g))], pf, vsl);
         }
         // the next block's codes, loaded a block ago, to the other stage, and the loads of the one after
         if (npage >= 0) {

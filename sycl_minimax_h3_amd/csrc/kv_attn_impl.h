@@ -304,8 +304,6 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     const int h = it.h, b = it.b;
     const uint32_t R = it.R, rw = (uint32_t) it.tile * RT, group = P.group;
     if (rw >= R) return;
-    KvRows<WC, NQ, TWO> q;
-    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
 
     // the cache blocks that any of the rows can see, a part of them, every KS-th
     const int posmin = it.len - it.n + (int) (rw / group), posmax = it.len - it.n + (int) ((min(R, rw + RT) - 1) / group);
@@ -344,6 +342,8 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
         ks = P.kv.ks[(int64_t) page * P.kv.heads + h];
         vs = P.kv.vs[(int64_t) page * P.kv.heads + h];
     }
+    KvRows<WC, NQ, TWO> q;                          // (behind the first loads of the cache, which take longer)
+    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
     while (kb < last) {
         int nkb = kb + KS, npage = 0;
         present(nkb, npage);
@@ -451,8 +451,6 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
     const int h = it.h, b = it.b;
     const uint32_t R = it.R, rt0 = (uint32_t) it.tile * RT, rw = rt0 + wave * 16 * NQ, group = P.group;
     if (rt0 >= R) return;
-    KvRows<WC, NQ, TWO> q;
-    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
     // the cache blocks that any of the block's rows can see, a part of them; the wavefront's own rows see posmin .. posmax
     const int base = it.len - it.n;
     const int posmin = base + (int) (rw / group), posmax = rw < R ? base + (int) ((min(R, rw + 16 * NQ) - 1) / group) : -1;
@@ -501,8 +499,10 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
     present(kb, page);
     int nkb = kb, npage = -1;
     float ks_now = 0.0f, vs_now = 0.0f;
+    if (page >= 0) load(page);
+    KvRows<WC, NQ, TWO> q;
+    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
     if (page >= 0) {
-        load(page);
         stage(0);
         ks_now = ks;
         vs_now = vs;

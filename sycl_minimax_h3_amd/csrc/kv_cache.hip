@@ -26,7 +26,7 @@ int kv_args(const std::string& fn, const h3_kv_cache* cache, const h3_kv_batch* 
     return 0;
 }
 
-// the maximum over a block of 256 threads, on every thread; a NaN anywhere gives NaN
+// the maximum over a block of 256 threads, on every thread (with a barrier); a NaN anywhere gives NaN
 __device__ __forceinline__ float block_max(float m, bool nan) {
     __shared__ float red[4];
     __shared__ int bad[4];
@@ -38,50 +38,49 @@ __device__ __forceinline__ float block_max(float m, bool nan) {
     return (bad[0] | bad[1] | bad[2] | bad[3]) ? __builtin_nanf("") : m;
 }
 
-// 16 consecutive elements of a row from feature d0 on, zeros from `dim` on; vec: 16-byte loads (dim and the row's start allow
-// them: dim a multiple of 8, so a run of 8 features is all in or all out)
-__device__ __forceinline__ void load16(const void* p, int dt, int64_t row, int d0, int dim, bool vec, float* f) {
+// four consecutive elements of a row from feature d on, zeros from `dim` on; vec: in one load (dim a multiple of 4, so they are all in
+// or all out)
+__device__ __forceinline__ void load4(const void* p, int dt, int64_t row, int d, int dim, bool vec, float* f) {
     if (vec) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int d = d0 + 8 * h;
-            if (d < dim) {
-                if (dt == H3S_F32) load_f32x((const float*) p + row + d, f + 8 * h, 8);
-                else {
-                    const uint4 u = *reinterpret_cast<const uint4*>((const uint16_t*) p + row + d);
-                    if (dt == H3S_BF16) Vec<H3S_BF16>::unpack(u, f + 8 * h);
-                    else Vec<H3S_F16>::unpack(u, f + 8 * h);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[8 * h + i] = 0.0f;
-            }
+        if (d >= dim) {
+            f[0] = f[1] = f[2] = f[3] = 0.0f;
+        } else if (dt == H3S_F32) {
+            load_f32x((const float*) p + row + d, f, 4);
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*) p + row + d);
+            float g[8];
+            if (dt == H3S_BF16) Vec<H3S_BF16>::unpack(make_uint4(u.x, u.y, 0, 0), g);
+            else Vec<H3S_F16>::unpack(make_uint4(u.x, u.y, 0, 0), g);
+            f[0] = g[0]; f[1] = g[1]; f[2] = g[2]; f[3] = g[3];
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = d0 + i < dim ? load_any(p, dt, row + d0 + i) : 0.0f;
+        for (int i = 0; i < 4; ++i) f[i] = d + i < dim ? load_any(p, dt, row + d + i) : 0.0f;
+    }
+}
+__device__ __forceinline__ void store4(void* p, int dt, int64_t row, int d, int dim, bool vec, const float* f) {
+    if (vec) {
+        if (d >= dim) return;
+        if (dt == H3S_F32) *reinterpret_cast<float4*>((float*) p + row + d) = make_float4(f[0], f[1], f[2], f[3]);
+        else *reinterpret_cast<uint2*>((uint16_t*) p + row + d) =
+                 dt == H3S_BF16 ? make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3])) : make_uint2(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < dim) store_any(p, dt, row + d + i, f[i]);
     }
 }
 
-__device__ __forceinline__ uint32_t byte_of(const uint4& u, int i) {
-    const uint32_t w = i < 4 ? u.x : i < 8 ? u.y : i < 12 ? u.z : u.w;
-    return w >> (8 * (i & 3));
-}
-// the old codes of a 16-byte piece at the new scale, at the places where `keep` has a bit; zeros elsewhere
-__device__ __forceinline__ uint4 rescaled(const uint4& u, float ratio, uint32_t keep) {
-    uint32_t w[4];
+// four old codes at the new scale, those where `keep` has a bit; zeros elsewhere
+__device__ __forceinline__ uint32_t rescaled(uint32_t u, float ratio, uint32_t keep) {
+    float c[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        float c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float v = __builtin_rintf((float) (int8_t) byte_of(u, 4 * q + i) * ratio);
-            // (a ratio that is not finite belongs to a scale that is not: the code then says nothing, and 0 is as good)
-            c[i] = (keep >> (4 * q + i)) & 1 ? fminf(fmaxf(v, -127.0f), 127.0f) : 0.0f;
-        }
-        w[q] = pack_i8x4(c[0], c[1], c[2], c[3]);
+    for (int i = 0; i < 4; ++i) {
+        const float v = __builtin_rintf((float) (int8_t) (u >> (8 * i)) * ratio);
+        // (a ratio that is not finite belongs to a scale that is not: the code then says nothing, and any is as good)
+        c[i] = (keep >> i) & 1 ? fminf(fmaxf(v, -127.0f), 127.0f) : 0.0f;
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return pack_i8x4(c[0], c[1], c[2], c[3]);
 }
 
 struct KvWriteArgs {
@@ -90,19 +89,22 @@ struct KvWriteArgs {
     const void *xk, *xv;
     int64_t k_stride, v_stride;
     int dt, nb;              // nb: blocks a sequence may touch
-    int k_vec, v_vec;        // whole 16-byte pieces
+    int k_vec, v_vec;        // rows four elements at a time
 };
 // (Chosen between, never indexed by the side: an index into the kernel's arguments became a scalar load whose base and offset
 // were no multiples of 4 by themselves, and scalar loads drop the two low bits of each.)
 
-// One block of threads: one cache block of one head, keys (side 0) or values (side 1). Thread t holds the
-// pieces t + 256 p of 16 features, 4 WC pieces a token. Bound by latency for single tokens (one load, a maximum over the block, one store)
-// and by the rows' bytes for prompts. 8 heads of 128, bfloat16: see the table of cases.
+constexpr int kKvRow = kKvB / 4 + 1;      // words of a feature's 64 tokens in LDS, one more than they are (banks)
+
+// One block of threads: one cache block of one head, keys (side 0) or values (side 1). Thread t holds the pieces t + 256 p, p < WC, of
+// four tokens x four features, W / 4 pieces side by side: its loads of the rows and its stores of keys are whole runs of them, and a
+// piece's codes are four words either way round. Values go through LDS into a feature's tokens. Bound by latency for single tokens (the
+// sequence's place, the rows, a maximum over the block, one store: 5 us) and by the rows' bytes for prompts.
 template <int WC>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs A) {
-    constexpr int W = 64 * WC, TPR = 4 * WC;                                // 16-feature pieces a token
+    constexpr int W = 64 * WC;
     const KvArgs& P = A.kv;
-    __shared__ __align__(16) uint8_t codes[W * (kKvB + 4)];                               // values: the new codes, a feature's tokens side by side
+    __shared__ uint32_t codes[W * kKvRow];
     int64_t id = blockIdx.x;
     const int side = (int) (id & 1);
     id >>= 1;
@@ -115,65 +117,72 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs A) {
     const int64_t j = past / kKvB + i;                                      // the sequence's block
     if (end <= past || j * kKvB >= end) return;                             // (no new token: the block is not touched)
     const int page = P.table[(int64_t) b * P.width + j];
-    if (page < 0 || page >= P.blocks) return;
     const int kept = (int) max(past - j * kKvB, (int64_t) 0);               // its tokens [0, kept) were there
     const int last = (int) min(end - j * kKvB, (int64_t) kKvB);             // and [kept, last) are new
     const int64_t row0 = r0 + (j * kKvB - past);                            // the row of its token 0 (with kept > 0: before r0)
-    const int64_t tile = ((int64_t) page * P.heads + h);
     const int t = threadIdx.x;
     const void* x = side ? A.xv : A.xk;
     const int64_t stride = side ? A.v_stride : A.k_stride;
     const bool vec = (side ? A.v_vec : A.k_vec) != 0;
 
-    float f[WC][16];
+    float f[WC][4][4];                                                      // [piece][token][feature]
     float m = 0.0f;
     bool nan = false;
 #pragma unroll
     for (int p = 0; p < WC; ++p) {
-        const int tok = (t + 256 * p) / TPR, d0 = (t + 256 * p) % TPR * 16;
-        if (tok >= kept && tok < last) {
-            load16(x, A.dt, (row0 + tok) * stride + (int64_t) h * P.dim, d0, P.dim, vec, f[p]);
-        } else {
+        const int tok = (t + 256 * p) / (W / 4) * 4, d = (t + 256 * p) % (W / 4) * 4;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) f[p][e] = 0.0f;
-        }
+        for (int k = 0; k < 4; ++k) {
+            if (tok + k >= kept && tok + k < last) {
+                load4(x, A.dt, (row0 + tok + k) * stride + (int64_t) h * P.dim, d, P.dim, vec, f[p][k]);
+            } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            m = fmaxf(m, fabsf(f[p][e]));
-            nan = nan || f[p][e] != f[p][e];
+                for (int e = 0; e < 4; ++e) f[p][k][e] = 0.0f;
+            }
         }
     }
-    m = block_max(m, nan);
+    if (page < 0 || page >= P.blocks) return;                               // (after the rows' loads, which need not wait for it)
+    const int64_t tile = (int64_t) page * P.heads + h;
     float* scale = (side ? P.vs : P.ks) + tile;
     const float was = kept ? *scale : 0.0f;
+#pragma unroll
+    for (int p = 0; p < WC; ++p)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m = fmaxf(m, fabsf(f[p][k][e]));
+                nan = nan || f[p][k][e] != f[p][k][e];
+            }
+    m = block_max(m, nan);                                                  // (a barrier: every thread has read the old scale)
     float s = m / 127.0f;
     // (a NaN on either side wins)
     s = s != s ? s : was > s || was != was ? was : s;
     s = s < 1e-30f ? 1e-30f : s;
     const bool moved = kept && s != was;                                    // (NaN: rescaled, to no effect)
-    const float ratio = was / s;
-    __syncthreads();                                                        // every thread has read the old scale
+    const float ratio = was / s, inv = 1.0f / s;                            // (quant_code: x / s as the IEEE division gives it)
     if (t == 0) *scale = s;
 
     int8_t* base = (side ? P.v : P.k) + tile * kKvB * W;
 #pragma unroll
     for (int p = 0; p < WC; ++p) {
-        const int tok = (t + 256 * p) / TPR, d0 = (t + 256 * p) % TPR * 16;
-        uint32_t w[4];
+        const int tok = (t + 256 * p) / (W / 4) * 4, d = (t + 256 * p) % (W / 4) * 4;
+        if (side == 0 && tok + 4 <= kept && !moved) continue;               // (old tokens only, unchanged)
+        float c[4][4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float c[4];
+        for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[e] = fminf(fmaxf(__builtin_rintf(f[p][4 * q + e] / s), -127.0f), 127.0f);
-            w[q] = pack_i8x4(c[0], c[1], c[2], c[3]);
-        }
+            for (int e = 0; e < 4; ++e) c[k][e] = fmaxf(quant_code(f[p][k][e], s, inv), -127.0f);
         if (side == 0) {
-            uint4* dst = reinterpret_cast<uint4*>(base + (int64_t) tok * W + d0);
-            if (tok >= kept) *dst = make_uint4(w[0], w[1], w[2], w[3]);
-            else if (moved) *dst = rescaled(*dst, ratio, 0xffffu);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t* dst = reinterpret_cast<uint32_t*>(base + (int64_t) (tok + k) * W + d);
+                if (tok + k >= kept) *dst = pack_i8x4(c[k][0], c[k][1], c[k][2], c[k][3]);
+                else if (moved) *dst = rescaled(*dst, ratio, 15u);
+            }
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) codes[(d0 + e) * (kKvB + 4) + tok] = (uint8_t) (w[e / 4] >> (8 * (e & 3)));
+            for (int e = 0; e < 4; ++e) codes[(d + e) * kKvRow + tok / 4] = pack_i8x4(c[0][e], c[1][e], c[2][e], c[3][e]);
         }
     }
     if (side == 0) return;
@@ -186,17 +195,14 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs A) {
         if (old == 16 && !moved) continue;
         uint4* dst = reinterpret_cast<uint4*>(base + (int64_t) d * kKvB + k0);
         uint4 u = make_uint4(0, 0, 0, 0);
-        if (old) {
-            u = *dst;
-            if (moved) u = rescaled(u, ratio, (1u << old) - 1);
-        }
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(codes + d * (kKvB + 4) + k0);
+        if (old) u = *dst;
         uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int o = min(max(old - 4 * q, 0), 4);                      // old tokens in this word
+            if (moved) w[q] = rescaled(w[q], ratio, (1u << o) - 1);
             const uint32_t mask = o == 4 ? 0xffffffffu : (1u << (8 * o)) - 1;
-            w[q] = (w[q] & mask) | (src[q] & ~mask);
+            w[q] = (w[q] & mask) | (codes[d * kKvRow + k0 / 4 + q] & ~mask);
         }
         *dst = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -211,34 +217,12 @@ struct KvReadArgs {
     int k_vec, v_vec;
 };
 
-__device__ __forceinline__ void store16(void* p, int dt, int64_t row, int d0, int dim, bool vec, const float* f) {
-    if (vec) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int d = d0 + 8 * h;
-            if (d >= dim) continue;
-            if (dt == H3S_F32) {
-                float4* o = reinterpret_cast<float4*>((float*) p + row + d);
-                o[0] = make_float4(f[8 * h], f[8 * h + 1], f[8 * h + 2], f[8 * h + 3]);
-                o[1] = make_float4(f[8 * h + 4], f[8 * h + 5], f[8 * h + 6], f[8 * h + 7]);
-            } else {
-                *reinterpret_cast<uint4*>((uint16_t*) p + row + d) =
-                    dt == H3S_BF16 ? Vec<H3S_BF16>::pack(f + 8 * h) : Vec<H3S_F16>::pack(f + 8 * h);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (d0 + i < dim) store_any(p, dt, row + d0 + i, f[i]);
-    }
-}
-
-// One block of threads: the tokens that a read takes out of one cache block of one head and side (layout as kv_write_kernel).
+// One block of threads: the tokens that a read takes out of one cache block of one head and side (pieces as in kv_write_kernel).
 template <int WC>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs A) {
-    constexpr int W = 64 * WC, TPR = 4 * WC;
+    constexpr int W = 64 * WC;
     const KvArgs& P = A.kv;
-    __shared__ __align__(16) uint8_t codes[W * (kKvB + 4)];
+    __shared__ uint32_t codes[W * kKvRow];
     int64_t id = blockIdx.x;
     const int side = (int) (id & 1);
     id >>= 1;
@@ -260,28 +244,39 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs A) {
     void* x = side ? A.xv : A.xk;
     const int64_t stride = side ? A.v_stride : A.k_stride;
     const bool vec = (side ? A.v_vec : A.k_vec) != 0;
+    uint32_t w[WC][4];                                                      // a piece's codes: by token for keys, by feature for values
     if (side == 1) {
 #pragma unroll
         for (int p = 0; p < WC; ++p) {
             const int piece = t + 256 * p, d = piece / 4, k0 = (piece % 4) * 16;
             uint4 u = make_uint4(0, 0, 0, 0);
-            if (there) u = *reinterpret_cast<const uint4*>(base + (int64_t) d * kKvB + k0);
-            uint32_t* dst = reinterpret_cast<uint32_t*>(codes + d * (kKvB + 4) + k0);
+            if (there && k0 < to && k0 + 16 > from) u = *reinterpret_cast<const uint4*>(base + (int64_t) d * kKvB + k0);
+            uint32_t* dst = codes + d * kKvRow + k0 / 4;
             dst[0] = u.x; dst[1] = u.y; dst[2] = u.z; dst[3] = u.w;
         }
         __syncthreads();
     }
 #pragma unroll
     for (int p = 0; p < WC; ++p) {
-        const int tok = (t + 256 * p) / TPR, d0 = (t + 256 * p) % TPR * 16;
-        if (tok < from || tok >= to) continue;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (side == 0 && there) u = *reinterpret_cast<const uint4*>(base + (int64_t) tok * W + d0);
-        float f[16];
+        const int tok = (t + 256 * p) / (W / 4) * 4, d = (t + 256 * p) % (W / 4) * 4;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            f[e] = there ? (float) (int8_t) (side ? codes[(d0 + e) * (kKvB + 4) + tok] : byte_of(u, e)) * s : 0.0f;
-        store16(x, A.dt, (row0 + tok) * stride + (int64_t) h * P.dim, d0, P.dim, vec, f);
+        for (int k = 0; k < 4; ++k) {
+            w[p][k] = 0;
+            if (side == 1) w[p][k] = codes[(d + k) * kKvRow + tok / 4];
+            else if (there && tok + k >= from && tok + k < to) w[p][k] = *reinterpret_cast<const uint32_t*>(base + (int64_t) (tok + k) * W + d);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < WC; ++p) {
+        const int tok = (t + 256 * p) / (W / 4) * 4, d = (t + 256 * p) % (W / 4) * 4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (tok + k < from || tok + k >= to) continue;
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = there ? (float) (int8_t) (side ? w[p][e] >> (8 * k) : w[p][k] >> (8 * e)) * s : 0.0f;
+            store4(x, A.dt, (row0 + tok + k) * stride + (int64_t) h * P.dim, d, P.dim, vec, f);
+        }
     }
 }
 
@@ -296,9 +291,10 @@ static int row_checks(const std::string& fn, const KvArgs& P, const h3_kv_batch&
     if (*nb * P.seqs > 0x7fffffff / 2 / P.heads) return fail(fn + ": too many blocks of work");
     return 0;
 }
-// whether rows of k or v can be taken in 16-byte pieces
+// whether rows of k or v can be taken four elements at a time
 static bool rows_vec(const void* p, int64_t stride, int dim, int dt) {
-    return aligned16(p) && dim % 8 == 0 && (stride * elem_size(dt)) % 16 == 0;
+    const int piece = 4 * elem_size(dt);
+    return (uintptr_t) p % piece == 0 && dim % 4 == 0 && stride % 4 == 0;
 }
 
 int kv_write(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* past, const void* k, int64_t k_stride,

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 F32, F16, BF16 = 0, 1, 2
 ROT_NONE, ROT_REGULAR, ROT_SYLVESTER = 0, 1, 2
@@ -104,7 +105,10 @@ class KvBatch(C.Structure):
 
 
 KV_BLOCK = 64
-_cache, _batch = C.POINTER(KvCache), C.POINTER(KvBatch)
+# h3_kv_batch's fields as bytes, which go through a pointer argument faster than a structure is made
+_batch_fields = struct.Struct("PPqqqq")
+kv_batch = _batch_fields.pack   # (table, starts, seqs, width, rows, most)
+assert _batch_fields.size == C.sizeof(KvBatch)
 
 
 class LmApi(C.Structure):
@@ -112,10 +116,10 @@ class LmApi(C.Structure):
 
     _fields_ = [
         ("size", i64),
-        ("kv_write", C.CFUNCTYPE(i32, vp, _cache, _batch, vp, vp, i64, vp, i64, i32)),
-        ("kv_read", C.CFUNCTYPE(i32, vp, _cache, _batch, vp, vp, i64, vp, i64, i32)),
-        ("kv_attention", C.CFUNCTYPE(i32, vp, _cache, _batch, vp, i64, vp, i64, i32, i64, f32, i64, vp, i64, vp, i32, vp, vp, u64)),
-        ("kv_attention_work", C.CFUNCTYPE(i64, vp, _cache, _batch, i64, i64, i64)),
+        ("kv_write", C.CFUNCTYPE(i32, vp, vp, vp, vp, vp, i64, vp, i64, i32)),
+        ("kv_read", C.CFUNCTYPE(i32, vp, vp, vp, vp, vp, i64, vp, i64, i32)),
+        ("kv_attention", C.CFUNCTYPE(i32, vp, vp, vp, vp, i64, vp, i64, i32, i64, f32, i64, vp, i64, vp, i32, vp, vp, u64)),
+        ("kv_attention_work", C.CFUNCTYPE(i64, vp, vp, vp, i64, i64, i64)),
         ("linear4", C.CFUNCTYPE(i32, vp, vp, i32, i64, i64, vp, i64, vp, vp, i32, i64, vp, vp, i32)),
     ]
 
@@ -149,6 +153,8 @@ class Api:
             raise OSError(f"h3lm is missing from the library ({path})") from None
         if self.lm.size < C.sizeof(LmApi):
             raise OSError(f"h3lm is an older library's ({path})")
+        for name, _ in LmApi._fields_[1:]:   # (a field read makes a function object: once here, not at every call)
+            setattr(self, "lm_" + name, getattr(self.lm, name))
 
     def error(self) -> str:
         """The library's last error on this thread."""

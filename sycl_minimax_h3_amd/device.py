@@ -8,6 +8,7 @@ dtype and a row-major shape over a ``Buf`` or over a PyTorch tensor's storage.
 from __future__ import annotations
 
 import enum
+import math
 from typing import Sequence
 
 import numpy as np
@@ -32,19 +33,25 @@ class DType(enum.Enum):
     F64 = "F64"
 
     def size(self) -> int:
-        return {"I8": 1, "U8": 1, "F16": 2, "BF16": 2, "F32": 4, "I32": 4, "I64": 8, "F64": 8}[self.value]
+        return self._size
 
     def kernel_code(self) -> int:
         """The library's code for a floating-point type (dtype.rs:43-50)."""
-        codes = {"F32": _api.F32, "F16": _api.F16, "BF16": _api.BF16}
-        if self.value not in codes:
+        code = self._code
+        if code is None:
             raise Error(f"{self} is not a floating-point tensor type")
-        return codes[self.value]
+        return code
 
     def numpy(self):
         """The numpy type that carries the bits (16-bit floats as uint16 bit patterns)."""
         return {"F32": np.float32, "F16": np.uint16, "BF16": np.uint16, "I8": np.int8, "U8": np.uint8,
                 "I32": np.int32, "I64": np.int64, "F64": np.float64}[self.value]
+
+
+# (as attributes: a call asks for them several times, and a table by value costs more than the rest of its checks)
+for _t, _size, _code in ((DType.F32, 4, _api.F32), (DType.F16, 2, _api.F16), (DType.BF16, 2, _api.BF16), (DType.I8, 1, None), (DType.U8, 1, None),
+                         (DType.I32, 4, None), (DType.I64, 8, None), (DType.F64, 8, None)):
+    _t._size, _t._code = _size, _code
 
 
 class Device:
@@ -155,10 +162,7 @@ class Tensor:
         self.dtype, self.shape, self._ptr, self._owner, self.dev = dtype, list(shape), ptr, owner, dev
 
     def elements(self) -> int:
-        n = 1
-        for s in self.shape:
-            n *= int(s)
-        return n
+        return int(math.prod(self.shape))
 
     def nbytes(self) -> int:
         return self.elements() * self.dtype.size()

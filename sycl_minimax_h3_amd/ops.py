@@ -410,7 +410,7 @@ KV_BLOCK = _api.KV_BLOCK   # tokens in a block of the cache
 
 
 def _i32(t: Tensor, what: str, n: int) -> int:
-    if t.dtype != DType.I32 or t.elements() < n:
+    if t.dtype is not DType.I32 or t.elements() < n:
         raise Error(f"{what} must be int32 with at least {n} values, got {t.dtype} {t.shape}")
     return t.ptr()
 
@@ -432,6 +432,7 @@ class KvCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.blocks, self.heads, self.dim = blocks, heads, int(dim)
         self._c = _api.KvCache(k.ptr(), v.ptr(), k_scale.ptr(), v_scale.ptr(), blocks, heads, dim)
+        self._p = _C.addressof(self._c)
 
     @staticmethod
     def width(dim: int) -> int:
@@ -449,21 +450,21 @@ class KvCache:
 
 
 def _kv_batch(table: Tensor, starts: Tensor, rows: int, most: int):
-    """The batch of a call: table int32 [seqs, width], starts int32 [seqs + 1]."""
-    if table.dtype != DType.I32 or len(table.shape) != 2:
+    """The batch of a call (table int32 [seqs, width], starts int32 [seqs + 1]) and its sequences."""
+    if table.dtype is not DType.I32 or len(table.shape) != 2:
         raise Error(f"the block table must be int32 [sequences, blocks], got {table.dtype} {table.shape}")
-    seqs, width = int(table.shape[0]), int(table.shape[1])
-    if starts.dtype != DType.I32 or starts.elements() != seqs + 1:
+    seqs, width = table.shape
+    if starts.dtype is not DType.I32 or starts.elements() != seqs + 1:
         raise Error(f"starts must be int32 [{seqs + 1}], got {starts.dtype} {starts.shape}")
     if most < 0:
         raise Error(f"the most rows of a sequence: {most}")
-    return _api.KvBatch(table.ptr(), starts.ptr(), seqs, width, rows, most)
+    return _api.kv_batch(table.ptr(), starts.ptr(), seqs, width, rows, most), seqs
 
 
 def _kv_rows(fn: str, cache: KvCache, k: Rows, v: Rows) -> None:
-    if (k.heads, k.dim) != (cache.heads, cache.dim) or (v.heads, v.dim) != (cache.heads, cache.dim):
+    if k.heads != cache.heads or k.dim != cache.dim or v.heads != cache.heads or v.dim != cache.dim:
         raise Error(f"{fn}: k and v of {k.heads} x {k.dim} and {v.heads} x {v.dim} for a cache of {cache.heads} x {cache.dim}")
-    if k.tokens != v.tokens or k.t.dtype != v.t.dtype:
+    if k.tokens != v.tokens or k.t.dtype is not v.t.dtype:
         raise Error(f"{fn}: k and v must share their rows and their type")
 
 
@@ -472,26 +473,26 @@ def kv_write(cache: KvCache, table: Tensor, k: Rows, v: Rows, starts: Tensor, pa
     starts int32 [sequences + 1], past int32 [sequences] (the tokens that each has in the cache already), most: at least the
     most rows of any sequence. A block has one scale for each head; where larger tokens join old ones, those are rounded again."""
     _kv_rows("kv_write", cache, k, v)
-    batch = _kv_batch(table, starts, k.tokens, most)
-    args = (_i32(past, "past", batch.seqs), k.ptr(), k.stride, v.ptr(), v.stride, k.t.dtype.kernel_code())
+    batch, seqs = _kv_batch(table, starts, k.tokens, most)
+    args = (_i32(past, "past", seqs), k.ptr(), k.stride, v.ptr(), v.stride, k.t.dtype.kernel_code())
     dev = _dev(cache.k)
-    dev.check(dev.api.lm.kv_write(dev.ctx, _C.byref(cache._c), _C.byref(batch), *args))
+    dev.check(dev.api.lm_kv_write(dev.ctx, cache._p, batch, *args))
 
 
 def kv_read(cache: KvCache, table: Tensor, starts: Tensor, first: Tensor, most: int, k: Rows, v: Rows) -> None:
     """Tokens out of the cache as values: row starts[b] + j of k and v receives token first[b] + j of sequence b."""
     _kv_rows("kv_read", cache, k, v)
-    batch = _kv_batch(table, starts, k.tokens, most)
-    args = (_i32(first, "first", batch.seqs), k.ptr(), k.stride, v.ptr(), v.stride, k.t.dtype.kernel_code())
+    batch, seqs = _kv_batch(table, starts, k.tokens, most)
+    args = (_i32(first, "first", seqs), k.ptr(), k.stride, v.ptr(), v.stride, k.t.dtype.kernel_code())
     dev = _dev(cache.k)
-    dev.check(dev.api.lm.kv_read(dev.ctx, _C.byref(cache._c), _C.byref(batch), *args))
+    dev.check(dev.api.lm_kv_read(dev.ctx, cache._p, batch, *args))
 
 
 def kv_attention_work(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, most: int, *, max_len: int = 0, window: int = 0) -> int:
     """The bytes of workspace that kv_attention takes for these arguments (0: none)."""
-    batch = _kv_batch(table, starts, q.tokens, most)
+    batch, _ = _kv_batch(table, starts, q.tokens, most)
     dev = _dev(cache.k)
-    n = dev.api.lm.kv_attention_work(dev.ctx, _C.byref(cache._c), _C.byref(batch), max_len, q.heads, window)
+    n = dev.api.lm_kv_attention_work(dev.ctx, cache._p, batch, max_len, q.heads, window)
     if n < 0:
         raise Error(dev.api.error())
     return n
@@ -510,18 +511,18 @@ def kv_attention(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, lengths
         raise Error(f"kv_attention: q heads of {q.dim} for a cache of {cache.dim}")
     if out.elements() != q.tokens * q.heads * q.dim:
         raise Error(f"kv_attention: out {out.shape} for {q.tokens} rows of {q.heads} x {q.dim}")
-    batch = _kv_batch(table, starts, q.tokens, most)
+    batch, seqs = _kv_batch(table, starts, q.tokens, most)
     mask_p, mask_n = None, 0
     if mask is not None:
-        if mask.dtype not in (DType.U8, DType.I8) or len(mask.shape) != 2 or mask.shape[0] != batch.seqs:
-            raise Error(f"kv_attention: the mask must be uint8 [{batch.seqs}, tokens], got {mask.dtype} {mask.shape}")
+        if mask.dtype not in (DType.U8, DType.I8) or len(mask.shape) != 2 or mask.shape[0] != seqs:
+            raise Error(f"kv_attention: the mask must be uint8 [{seqs}, tokens], got {mask.dtype} {mask.shape}")
         mask_p, mask_n = mask.ptr(), int(mask.shape[1])
     if lse is not None and (lse.dtype != DType.F32 or lse.elements() != q.tokens * q.heads):
         raise Error(f"kv_attention: lse must be float32 [{q.tokens}, {q.heads}], got {lse.dtype} {lse.shape}")
-    args = (_i32(lengths, "lengths", batch.seqs), max_len, q.ptr(), q.stride, q.t.dtype.kernel_code(), q.heads, scale, window, mask_p,
+    args = (_i32(lengths, "lengths", seqs), max_len, q.ptr(), q.stride, q.t.dtype.kernel_code(), q.heads, scale, window, mask_p,
             mask_n, out.ptr(), out.dtype.kernel_code(), _p(lse), _p(work), work.nbytes() if work is not None else 0)
     dev = _dev(cache.k)
-    dev.check(dev.api.lm.kv_attention(dev.ctx, _C.byref(cache._c), _C.byref(batch), *args))
+    dev.check(dev.api.lm_kv_attention(dev.ctx, cache._p, batch, *args))
 
 
 @dataclass
@@ -542,19 +543,23 @@ class Int4Linear:
 
     def forward(self, x: Tensor, out: Tensor) -> None:
         """out = linear(x): x [M, K] in a float type, out [M, N] in out's type."""
-        if self.weight.dtype != DType.U8 or len(self.weight.shape) != 2:
-            raise Error(f"int4_linear: the weight must be uint8 [N, K / 2], got {self.weight.dtype} {self.weight.shape}")
-        n, k = self.outputs(), self.inputs()
+        weight, scale, mins, bias = self.weight, self.scale, self.mins, self.bias
+        if weight.dtype is not DType.U8 or len(weight.shape) != 2:
+            raise Error(f"int4_linear: the weight must be uint8 [N, K / 2], got {weight.dtype} {weight.shape}")
+        n, half = weight.shape
+        k = 2 * half
         if k == 0 or n == 0:
-            raise Error(f"int4_linear: an empty weight {self.weight.shape}")
-        m = x.elements() // k
-        if x.elements() != m * k or out.elements() != m * n:
+            raise Error(f"int4_linear: an empty weight {weight.shape}")
+        count = x.elements()
+        m = count // k
+        if count != m * k or out.elements() != m * n:
             raise Error(f"int4_linear: x {x.shape} and out {out.shape} do not fit a [{n}, {k}] weight")
-        if len(self.scale.shape) != 2 or self.scale.shape[0] != n or self.scale.shape[1] == 0 or k % self.scale.shape[1]:
-            raise Error(f"int4_linear: scales {self.scale.shape} for a [{n}, {k}] weight")
-        if self.mins is not None and (list(self.mins.shape) != list(self.scale.shape) or self.mins.dtype != self.scale.dtype):
-            raise Error(f"int4_linear: minima {self.mins.dtype} {self.mins.shape} for scales {self.scale.dtype} {self.scale.shape}")
-        bias = _floats(self.bias, "the bias", n) if self.bias is not None else None
+        shape = scale.shape
+        if len(shape) != 2 or shape[0] != n or shape[1] == 0 or k % shape[1]:
+            raise Error(f"int4_linear: scales {shape} for a [{n}, {k}] weight")
+        if mins is not None and (mins.shape != shape or mins.dtype is not scale.dtype):
+            raise Error(f"int4_linear: minima {mins.dtype} {mins.shape} for scales {scale.dtype} {shape}")
+        args = (x.ptr(), x.dtype.kernel_code(), m, k, weight.ptr(), n, scale.ptr(), _p(mins), scale.dtype.kernel_code(), k // shape[1],
+                _floats(bias, "the bias", n) if bias is not None else None, out.ptr(), out.dtype.kernel_code())
         dev = _dev(x)
-        dev.check(dev.api.lm.linear4(dev.ctx, x.ptr(), x.dtype.kernel_code(), m, k, self.weight.ptr(), n, self.scale.ptr(), _p(self.mins),
-                                     self.scale.dtype.kernel_code(), k // self.scale.shape[1], bias, out.ptr(), out.dtype.kernel_code()))
+        dev.check(dev.api.lm_linear4(dev.ctx, *args))

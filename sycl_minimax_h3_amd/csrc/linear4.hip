@@ -24,7 +24,7 @@ int linear4(void* ctx, const void* x, int dt, int64_t M, int64_t K, const uint8_
     // Rows: up to 4 take one register of sums a lane, up to 16 one operand. Few columns: 16 a block and sixteen wavefronts
     // along the inputs, so that the device is covered; many: 32 a block, which share x's operands.
     L4Plan plan;
-    plan.rows = M <= 16 ? 16 : M <= 32 || dt == H3S_F32 || getenv("L4R") ? 32 : 64;
+    plan.rows = M <= 16 ? 16 : M <= 32 || dt == H3S_F32 ? 32 : 64;
     if (dt == H3S_BF16) l4_bf16(c, P, plan);
     else if (dt == H3S_F16) l4_f16(c, P, plan);
     else l4_f32(c, P, plan);

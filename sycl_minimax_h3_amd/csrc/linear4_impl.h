@@ -103,58 +103,6 @@ template <> struct L4X<H3S_F32> {
 // on a boundary of their size), or any type one by one
 enum { L4_S16 = 0, L4_S32 = 1, L4_SANY = 2 };
 
-// one column's scales of a step (one for each 32 J inputs), and the lane's own (the run 32 g ..) minimum, as loaded
-template <int J, int SM> struct L4S {
-    static constexpr int CNT = 4 / J, RAW = SM == L4_S16 ? (CNT + 1) / 2 : CNT;
-    uint32_t s[RAW], z;
-    __device__ __forceinline__ uint32_t one(const L4Args& P, const char* p, int64_t i) const {
-        if (SM == L4_S32 || (SM == L4_SANY && P.scale_dt == H3S_F32)) return ((const uint32_t*) p)[i];
-        return ((const uint16_t*) p)[i];
-    }
-    // scale, mins: the first column's (uniform); off: the bytes from there to the lane's column; r: the step's first run of 32 inputs.
-    // (A uniform address and a lane's 32-bit offset, which is the same in every step, take no vector instructions.)
-    __device__ __forceinline__ void load(const L4Args& P, const char* scale, const char* mins, uint32_t off, int r, int g) {
-        if constexpr (SM == L4_SANY) {
-            const int most = P.K / 32 - 1;
-#pragma unroll
-            for (int c = 0; c < CNT; ++c) s[c] = one(P, scale + off, l4_group(P, min(r + J * c, most)));
-            z = one(P, mins + off, l4_group(P, min(r + g, most)));
-        } else {
-            constexpr int ES = SM == L4_S32 ? 4 : 2;
-            const int64_t at = (J == 1 ? r : J == 2 ? r / 2 : l4_group(P, r)) * ES;
-            const char* p = scale + at;
-            if constexpr (SM == L4_S32) {
-                if constexpr (CNT == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p + off); s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w; }
-                else if constexpr (CNT == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p + off); s[0] = v.x; s[1] = v.y; }
-                else s[0] = *reinterpret_cast<const uint32_t*>(p + off);
-                z = *reinterpret_cast<const uint32_t*>(mins + at + (off + (J == 1 ? g : J == 2 ? g >> 1 : 0) * ES));
-            } else {
-                if constexpr (CNT == 4) { const uint2 v = *reinterpret_cast<const uint2*>(p + off); s[0] = v.x; s[1] = v.y; }
-                else if constexpr (CNT == 2) s[0] = *reinterpret_cast<const uint32_t*>(p + off);
-                else s[0] = *reinterpret_cast<const uint16_t*>(p + off);
-                z = *reinterpret_cast<const uint16_t*>(mins + at + (off + (J == 1 ? g : J == 2 ? g >> 1 : 0) * ES));
-            }
-        }
-    }
-    __device__ __forceinline__ float number(const L4Args& P, uint32_t u) const {
-        if (SM == L4_S32 || (SM == L4_SANY && P.scale_dt == H3S_F32)) return __uint_as_float(u);
-        const float a = bf16_lo(u), b = f16_lo(u);        // (both, and a select: a branch a scale costs more)
-        return P.scale_dt == H3S_BF16 ? a : b;
-    }
-    __device__ __forceinline__ float scale(const L4Args& P, int c) const {
-        if constexpr (SM == L4_S16 && CNT > 1) return number(P, c & 1 ? s[c >> 1] >> 16 : s[c >> 1] & 0xffffu);
-        else return number(P, s[c]);
-    }
-    // 16 s + z of the lane's own run
-    __device__ __forceinline__ float offset(const L4Args& P, const float* sc, int g) const {
-        float own = sc[0];
-        if constexpr (CNT == 2) own = g < 2 ? sc[0] : sc[1];
-        else if constexpr (CNT == 4) own = g < 2 ? (g ? sc[1] : sc[0]) : (g == 2 ? sc[2] : sc[3]);
-        const float a = __builtin_fmaf(16.0f, own, number(P, z)), b = 24.0f * own;
-        return P.has_mins ? a : b;
-    }
-};
-
 // a step's codes of one column, the run of 32 inputs j in word j
 __device__ __forceinline__ void l4_exchange(const uint4& w, uint32_t (&c)[4]) {
     const auto p = __builtin_amdgcn_permlane32_swap(w.x, w.z, false, false);
@@ -162,29 +110,6 @@ __device__ __forceinline__ void l4_exchange(const uint4& w, uint32_t (&c)[4]) {
     const auto r = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false);
     const auto s = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
     c[0] = r[0]; c[1] = r[1]; c[2] = s[0]; c[3] = s[1];
-}
-
-// a step's codes and scales of NT columns, from what was loaded: c the codes, the run j of 32 inputs in word j; sc a scale for each 32 J
-// inputs; off 16 s + z of the lane's own run (zeros past the row's end)
-template <int NT, int J, int SM>
-__device__ __forceinline__ void l4_decode(const L4Args& P, int kk, int g, const uint4 (&w)[NT], const L4S<J, SM> (&sr)[NT], uint32_t (&c)[NT][4],
-                                          float (&sc)[NT][4 / J], float (&off)[NT]) {
-#pragma unroll
-    for (int b = 0; b < NT; ++b) {
-        l4_exchange(w[b], c[b]);
-#pragma unroll
-        for (int q = 0; q < 4 / J; ++q) sc[b][q] = sr[b].scale(P, q);
-        off[b] = sr[b].offset(P, sc[b], g);
-    }
-    // (the last step of a row that is no multiple of 128: its scales do not come in one load)
-    if (SM == L4_SANY && kk + 128 > P.K) {
-#pragma unroll
-        for (int b = 0; b < NT; ++b) {
-#pragma unroll
-            for (int q = 0; q < 4 / J; ++q) sc[b][q] = kk + 32 * J * q < P.K ? sc[b][q] : 0.0f;
-            off[b] = kk + 32 * g < P.K ? off[b] : 0.0f;
-        }
-    }
 }
 
 // The products of one step of 128 inputs: NT columns' codes and scales against MT x 16 rows. frag(a, j, f): the operand of the rows
@@ -653,7 +578,7 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) xoff[p] = (uint32_t) ((int) min<int64_t>((t + 256 * p) / 16, P.M - 1 - m0) * P.K + t % 16 * 8) * XES;
     uint4 w[NT];
-    L4S<J, SM> sr[NT];
+    L4Q<J, SM> now[NT], next[NT];                                                 // the scales of four of the K group's steps
     auto load_x = [&](int step) {
         const char* xp = xbase + (int64_t) step * 128 * XES;
         const bool out = SM == L4_SANY && step * 128 + t % 16 * 8 >= P.K;
@@ -682,33 +607,49 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
             if (SM == L4_SANY) at = min(at, coff[b] - 16 * g + (uint32_t) (P.K / 2 - 16 - step * 64));   // (within the row)
             w[b] = *reinterpret_cast<const uint4*>(cp + at);
         }
+    };
+    auto load_s = [&](int step) {
 #pragma unroll
-        for (int b = 0; b < NT; ++b) sr[b].load(P, sbase, zbase, soff[b], step * 4, g);
+        for (int b = 0; b < NT; ++b) next[b].load(P, sbase, zbase, soff[b], min(step + 2 * g, steps - 1) * 4);
     };
     // both K groups make the same number of rounds (the second's last may have no step)
     // (Loads are never skipped, see linear4_few_kernel: past the end it is the last step again.)
+    load_s(kg);
     load_x(min(kg, steps - 1));
     load_w(min(kg, steps - 1));
     store_x(0);
     load_x(min(kg + 2, steps - 1));
     lds_barrier();
-    int stage = 0;
-    for (int first = 0; first < steps; first += 2) {
-        const int step = first + kg;
-        if (step < steps) {
-            uint32_t c[NT][4];
-            float sc[NT][4 / J], off[NT];
-            l4_decode<NT, J, SM>(P, step * 128, g, w, sr, c, sc, off);
-            load_w(min(step + 2, steps - 1));
-            l4_products<OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
+    for (int first = 0; first < steps; first += 8) {
 #pragma unroll
-                for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][stage][a][j][q][lane ^ g];
-            }, acc);
-            store_x(stage ^ 1);
-            load_x(min(step + 4, steps - 1));
+        for (int b = 0; b < NT; ++b) now[b] = next[b];
+        load_s(first + 8 + kg);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int step = first + 2 * r + kg;
+            if (step < steps) {
+                uint32_t c[NT][4];
+                float sc[NT][4 / J], off[NT];
+#pragma unroll
+                for (int b = 0; b < NT; ++b) {
+                    l4_exchange(w[b], c[b]);
+                    now[b].pass(P, 4 * (16 * r + l15), g, sc[b], off[b]);
+                    if (SM == L4_SANY && step * 128 + 128 > P.K) {
+#pragma unroll
+                        for (int q = 0; q < 4 / J; ++q) sc[b][q] = step * 128 + 32 * J * q < P.K ? sc[b][q] : 0.0f;
+                        off[b] = step * 128 + 32 * g < P.K ? off[b] : 0.0f;
+                    }
+                }
+                load_w(min(step + 2, steps - 1));
+                l4_products<OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][r & 1][a][j][q][lane ^ g];
+                }, acc);
+                store_x((r & 1) ^ 1);
+                load_x(min(step + 4, steps - 1));
+            }
+            lds_barrier();
         }
-        lds_barrier();
-        stage ^= 1;
     }
     // the second group's sums to the first's
     v4f_l4* part = reinterpret_cast<v4f_l4*>(&xs[0][0][0][0][0][0]);

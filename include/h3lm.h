@@ -57,12 +57,13 @@ typedef struct {
      * in float32 with IEEE division; codes behind the last token are zero. So a block's old tokens lose precision when a larger
      * one joins them, and writing tokens one by one may give other codes than writing them together. An infinity or NaN in a new
      * token makes its block's scale infinite or NaN, and the block's tokens read as such. Tokens past the table's end are
-     * dropped. No two sequences may write into one block; blocks they share may only be read. */
+     * dropped; a past below 0 counts as 0. No two sequences may write into one block; blocks they share may only be read. */
     int (*kv_write)(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* past, const void* k,
                     int64_t k_stride, const void* v, int64_t v_stride, int dt);
 
     /* Tokens out of the cache as values: row starts[b] + j of k and v (heads * dim features of type dt) receives token
-     * first[b] + j of sequence b, zeros where that is not in the cache's blocks. code * scale in float32, rounded to dt. */
+     * first[b] + j of sequence b, zeros where that is not in the cache's blocks (a first below 0 counts
+     * as 0). code * scale in float32, rounded to dt. */
     int (*kv_read)(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* first, void* k,
                    int64_t k_stride, void* v, int64_t v_stride, int dt);
 
@@ -75,6 +76,7 @@ typedef struct {
      * that sees nothing gets zeros (lse -infinity). Hidden tokens have no effect, whatever their codes, scales and mask say.
      * Products, softmax and sums are float32 (q to 11 bits of each value for 16-bit types, which is all they have, 22 for float32;
      * probabilities likewise), rounded once to out_dt.
+     * Lengths count as at least 0 and at most the table's 64 * width tokens. out may not overlap q.
      * max_len: about the longest of the lengths (0: the table's width); it only decides how the work is split.
      * work: a device workspace of at least kv_attention_work(...) bytes, 16-byte aligned, in use until the call's work is done;
      * NULL: the context's own scratch. A call recorded into a graph has to bring its own (two graphs, or a graph and eager calls,
@@ -91,7 +93,9 @@ typedef struct {
      *     W[n, k] = scale[n, g] * (code - 8)            mins NULL
      *     W[n, k] = scale[n, g] * code - mins[n, g]     mins [N, K / group] of type scale_dt
      * group: a multiple of 32 that divides K, and K at most 2^20. Float32 sums; bias float32 [N] or NULL, added before the one rounding. codes and x
-     * 16-byte aligned, rows whole 16-byte pieces (K a multiple of 32 makes them so). out may not overlap x. No workspace. */
+     * 16-byte aligned, rows whole 16-byte pieces (K a multiple of 32 makes them so). out may not overlap x. No workspace.
+     * The sums run over x * (16 + code), with 16 times x's sum taken off again: an infinity or NaN in a row of x makes that row of out
+     * NaN (of no other row), and so may values whose sums times 31 leave float32. */
     int (*linear4)(void* ctx, const void* x, int dt, int64_t M, int64_t K, const uint8_t* codes, int64_t N, const void* scale,
                    const void* mins, int scale_dt, int64_t group, const float* bias, void* out, int out_dt);
 } h3_lm_api;

@@ -23,7 +23,7 @@ static KvPlan kv_plan(const KvArgs& P, int64_t most, int64_t group, int64_t max_
     plan.tiles = (rows + plan.rt - 1) / plan.rt;
     plan.blocks = plan.tiles * each;
     int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
-    if (window > 0) keys = std::min(keys, window + most + 2 * kKvB);
+    if (window > 0) keys = std::min(keys, std::min<int64_t>(window, INT32_MAX) + std::min<int64_t>(most, P.rows) + 2 * kKvB);
     const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
     plan.per = (int) std::max(least, (blocks + want - 1) / want);

@@ -713,7 +713,7 @@ static void l4_dot_run(Ctx* c, const L4Args& P, int per_cu) {
 template <int DT> static bool l4_dot_takes(Ctx* c, const L4Args& P) {
     const int chunks = (P.K + 511) / 512;
     constexpr int PARTS = L4X<DT>::PARTS;
-    if (P.M > 4 || (P.N + 15) / 16 > 0x7fffffff / 2) return false;
+    if (P.M > 4) return false;
     const int u = chunks <= kL4DotWaves ? 1 : chunks <= 2 * kL4DotWaves ? 2 : chunks <= 4 * kL4DotWaves ? 4 : 0, m = P.M == 3 ? 4 : (int) P.M;
     if (u == 0 || 16 * PARTS * u * m > 96) return false;
     if (m == 1) {
@@ -731,7 +731,7 @@ static void l4_type(Ctx* c, const L4Args& P, const L4Plan& plan) {
     if (l4_dot_takes<DT>(c, P)) return;
     // a step of 128 inputs has 4, 2 or 1 scales: one load where every column's lie on a boundary of their size
     const int64_t cnt = P.group % 128 == 0 ? 1 : P.group == 64 ? 2 : P.group == 32 ? 4 : 0;
-    const bool vec = cnt && P.groups % cnt == 0 && (uintptr_t) P.scale % (uintptr_t) (cnt * elem_size(P.scale_dt)) == 0;
+    const bool vec = cnt && P.groups % cnt == 0 && ((uintptr_t) P.scale | (uintptr_t) P.mins) % (uintptr_t) (cnt * elem_size(P.scale_dt)) == 0;
     if (!vec) l4_run<DT, 1, L4_SANY>(c, P, plan);
     else if (P.scale_dt == H3S_F32) {
         if (cnt == 1) l4_run<DT, 4, L4_S32>(c, P, plan);

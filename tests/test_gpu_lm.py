@@ -355,6 +355,43 @@ def test_cache_past_32_bits(dev):
         t._owner.free()
 
 
+def test_attention_window_past_every_length(dev):
+    """A window of any size is the largest that matters; the work is split as without one."""
+    seqs = [(1, 1500), (1, 700)]
+    cache, table, starts, lengths, bits, q, rows, stride, _ = attn_case(dev, seqs, 2, 4, 64, "BF16", {}, seed=61)
+    c, t, x = upload(dev, cache), i32(dev, table), up(dev, bits, "BF16", [rows, stride])
+    r, st, ln = ops.Rows(x, 8, stride, rows, 8, 64), i32(dev, starts), i32(dev, lengths)
+    got = []
+    for window in (0, 1 << 31, (1 << 63) - 1):
+        assert ops.kv_attention_work(c, t, r, st, 1, window=window) == ops.kv_attention_work(c, t, r, st, 1)
+        out = new(dev, "F32", [rows, 8 * 64])
+        ops.kv_attention(c, t, r, st, ln, 1, out, window=window)
+        got.append(out.to_numpy()[:int(starts[-1])])
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+
+
+def test_attention_two_contexts_at_once(dev):
+    """Two contexts' calls, queued in turn without a wait, each with its own split and its own scratch."""
+    other = Device.open()
+    made = []
+    for d in (dev, other):
+        for seed, seqs in ((71, [(1, 1900)]), (72, [(1, 900), (2, 1300)])):
+            cache, table, starts, lengths, bits, q, rows, stride, _ = attn_case(d, seqs, 2, 4, 64, "BF16", {}, seed=seed)
+            out = up(d, np.full((rows, 8 * 64), 55.0, np.float32), "F32", [rows, 8 * 64])
+            args = (upload(d, cache), i32(d, table), ops.Rows(up(d, bits, "BF16", [rows, stride]), 8, stride, rows, 8, 64),
+                    i32(d, starts), i32(d, lengths), max(n for n, _ in seqs), out)
+            made.append((args, ref.attention(cache, table, starts, lengths, q, 4, "BF16", "F32"), int(starts[-1])))
+    for _ in range(3):
+        for i in (0, 2, 1, 3):
+            ops.kv_attention(*made[i][0])
+    for d in (dev, other):
+        d.wait()
+    for args, want, used in made:
+        check_attn(args[6].to_numpy().reshape(-1, 8, 64), None, want, used, str(used))
+    del made, args
+    other.close()
+
+
 class Recorded:
     """What `call` queues on the context's stream, recorded into a HIP graph (and not run)."""
 
@@ -523,6 +560,23 @@ LINEAR4 = [
     (300, 640, 130, 32, True, "BF16", "F32", "F16", True),
     (64, 256, 1, 32, False, "F16", "F32", "F16", True),
 ]
+# rows of weights in several chunks or steps a wavefront, and more columns than the blocks of a grid take at once
+LINEAR4_LONG = [
+    (1, 14336, 40, 64, True, "BF16", "BF16", "F16", True),
+    (1, 8192, 40, 128, False, "F32", "F32", "F32", True),
+    (1, 20000 * 32, 5, 32, True, "BF16", "F32", "F16", False),
+    (1, 512, 20011, 128, False, "F16", "F32", "F16", True),
+    (2, 6400, 33, 32, True, "F16", "F16", "F16", True),
+    (2, 544, 9001, 32, True, "F32", "F32", "F32", False),
+    (4, 5632, 18, 256, False, "BF16", "BF16", "BF16", True),
+    (3, 8192, 50, 64, True, "BF16", "F32", "F16", True),
+    (9, 14336, 35, 32, True, "BF16", "BF16", "F16", True),
+    (16, 512, 20011, 64, False, "BF16", "BF16", "F16", True),
+    (7, 1 << 20, 3, 128, False, "F16", "F32", "F32", True),
+    (12, 6176, 100, 32, True, "F32", "F32", "F16", True),
+    (33, 14336, 150, 64, True, "BF16", "BF16", "F16", True),
+    (70, 6240, 140, 96, False, "F16", "F32", "F32", True),
+]
 
 
 def linear4_case(dev, M, K, N, group, mins, dt, scale_dt, bias, seed=5):
@@ -537,7 +591,7 @@ def linear4_case(dev, M, K, N, group, mins, dt, scale_dt, bias, seed=5):
     return layer, xb, codes, ref.from_bits(sb, scale_dt), ref.from_bits(mb, scale_dt) if mins else None, b
 
 
-@pytest.mark.parametrize("M,K,N,group,mins,dt,out_dt,scale_dt,bias", LINEAR4)
+@pytest.mark.parametrize("M,K,N,group,mins,dt,out_dt,scale_dt,bias", LINEAR4 + LINEAR4_LONG)
 def test_linear4(dev, M, K, N, group, mins, dt, out_dt, scale_dt, bias):
     layer, xb, codes, s, z, b = linear4_case(dev, M, K, N, group, mins, dt, scale_dt, bias)
     mark = ref.to_bits(np.full((M + 1, N), 9.0), out_dt)
@@ -549,6 +603,25 @@ def test_linear4(dev, M, K, N, group, mins, dt, out_dt, scale_dt, bias):
     off = np.abs(got[:M] - want)
     assert (off <= tol).all(), f"worst {np.max(off / tol):.3g} of the bound at {np.argwhere(off > tol)[:3].tolist()}"
     assert (got[M] == 9.0).all()
+
+
+@pytest.mark.parametrize("M", [1, 9, 33])
+@pytest.mark.parametrize("at", ["scale", "mins"])
+def test_linear4_scales_off_a_boundary(dev, M, at):
+    """Scales or minima that start on a 2-byte boundary only."""
+    K, N, group = 512, 40, 32
+    layer, xb, codes, s, z, b = linear4_case(dev, M, K, N, group, True, "BF16", "F16", True, seed=9)
+    bits = ref.to_bits(s if at == "scale" else z, "F16").ravel()
+    whole = up(dev, np.concatenate([bits[:1], bits]), "F16", [bits.size + 1])
+    moved = Tensor(whole.dtype, [N, K // group], whole.ptr() + 2, whole, dev)
+    if at == "scale":
+        layer.scale = moved
+    else:
+        layer.mins = moved
+    out = new(dev, "F32", [M, N])
+    layer.forward(up(dev, xb, "BF16", [M, K]), out)
+    want, tol = ref.linear4(ref.from_bits(xb, "BF16"), codes, s, z, b, "F32")
+    assert (np.abs(out.to_numpy() - want) <= tol).all()
 
 
 def test_linear4_odd_values(dev):

@@ -292,6 +292,31 @@ struct KvItem {
     }
 };
 
+// The walk over a sequence's blocks that are there. The wavefront holds 64 entries of the table, one a lane, so that a block's number is
+// known without a wait for memory: read entry by entry, its latency stood before every block's loads (64 sequences of up to 8192 tokens
+// 133.4 us, 130.7 so; 601 float32 tokens 33.8 and 33.1).
+struct KvPages {
+    const int32_t* table;
+    int width, base, entry;
+    __device__ __forceinline__ void take(const KvAttnArgs& P, int b) {
+        table = P.kv.table + (int64_t) b * P.kv.width;
+        width = P.kv.width;
+        base = -64;
+    }
+    // the first block from kb on, in steps of BY, that is there (its page), or `last`
+    template <int BY> __device__ __forceinline__ bool next(const KvAttnArgs& P, int& kb, int& page, int last, int lane) {
+        for (; kb < last; kb += BY) {
+            if (kb - base >= 64) {
+                base = kb;
+                entry = table[min(kb + lane, width - 1)];
+            }
+            page = __builtin_amdgcn_readlane(entry, kb - base);
+            if (page >= 0 && page < P.kv.blocks) return true;
+        }
+        return false;
+    }
+};
+
 // Few rows (up to 64 of a sequence and head): the four wavefronts of a block share 16 NQ rows and take every fourth cache block.
 // Bound by the cache's bytes: the next block's codes are on their way while one is worked on.
 template <int WC, int NQ, bool TWO>
@@ -311,14 +336,8 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     it.range(P, rw, RT, kb0, count);
     if (it.split && it.split * P.per >= count) return;
     const int last = it.end(P, kb0, count);
-    const int32_t* table = P.kv.table + (int64_t) b * P.kv.width;
-    // the first present block from kb on (its page), or `last`
-    auto present = [&](int& kb, int& page) {
-        for (; kb < last; kb += KS) {
-            page = table[kb];
-            if (page >= 0 && page < P.kv.blocks) return;
-        }
-    };
+    KvPages pages;
+    pages.take(P, b);
     uint4 kr[4][WC], vr[DT];
     const int koff = ((l15 >> 2) * 16 + (l15 & 3)) * W + g * 16, voff = l15 * 64 + g * 16;
     auto load_k = [&](int page) {
@@ -334,9 +353,8 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
         for (int t = 0; t < DT; ++t) vr[t] = *reinterpret_cast<const uint4*>(p + t * 1024);
     };
     int kb = kb0 + it.split * P.per + wave, page = 0;
-    present(kb, page);
     float ks = 0.0f, vs = 0.0f;
-    if (kb < last) {
+    if (pages.next<KS>(P, kb, page, last, lane)) {
         load_k(page);
         load_v(page);
         ks = P.kv.ks[(int64_t) page * P.kv.heads + h];
@@ -346,8 +364,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
     while (kb < last) {
         int nkb = kb + KS, npage = 0;
-        present(nkb, npage);
-        const bool more = nkb < last;
+        const bool more = pages.next<KS>(P, nkb, npage, last, lane);
         v4f_kv s[NQ][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -382,7 +399,6 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
             q.values(t, kv_half8(vr[t].x, vr[t].y), kv_half8(vr[t].z, vr[t].w), pf, vsl);
         if (more) load_v(npage);
         kb = nkb;
-        page = npage;
     }
 
     // the four wavefronts' sums, 16 rows at a time
@@ -458,14 +474,8 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
     it.range(P, rt0, RT, kb0, count);
     if (it.split && it.split * P.per >= count) return;
     const int last = it.end(P, kb0, count);
-    const int32_t* table = P.kv.table + (int64_t) b * P.kv.width;
-    auto present = [&](int& kb, int& page) {
-        for (; kb < last; ++kb) {
-            page = table[kb];
-            if (page >= 0 && page < P.kv.blocks) return;
-        }
-        page = -1;
-    };
+    KvPages pages;
+    pages.take(P, b);
     // the thread's 16-byte pieces of a block's codes: piece t + 256 i
     uint4 kr[WC], vr[WC];
     float ks = 0.0f, vs = 0.0f;
@@ -495,20 +505,21 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
             sv[st][p / 64][1][av] = kv_half8(vr[i].z, vr[i].w);
         }
     };
-    int kb = kb0 + it.split * P.per, page = -1, st = 0;
-    present(kb, page);
-    int nkb = kb, npage = -1;
+    int kb = kb0 + it.split * P.per, page = 0, st = 0;
+    const bool any = pages.next<1>(P, kb, page, last, lane);
+    int nkb = kb, npage = 0;
+    bool more = false;
     float ks_now = 0.0f, vs_now = 0.0f;
-    if (page >= 0) load(page);
+    if (any) load(page);
     KvRows<WC, NQ, TWO> q;
     q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
-    if (page >= 0) {
+    if (any) {
         stage(0);
         ks_now = ks;
         vs_now = vs;
         nkb = kb + 1;
-        present(nkb, npage);
-        if (npage >= 0) load(npage);
+        more = pages.next<1>(P, nkb, npage, last, lane);
+        if (more) load(npage);
     }
     lds_barrier();
     while (kb < last) {
@@ -538,17 +549,16 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
             for (int t = 0; t < DT; ++t) q.values(t, sv[st][t][0][16 * g + (l15 ^ (4 * g))], sv[st][t][1][16 * g + (l15 ^ (4 * g))], pf, vsl);
         }
         // the next block's codes, loaded a block ago, to the other stage, and the loads of the one after
-        if (npage >= 0) {
+        if (more) {
             stage(st ^ 1);
             ks_now = ks;
             vs_now = vs;
         }
         kb = nkb;
-        page = npage;
-        if (npage >= 0) {
+        if (more) {
             nkb = kb + 1;
-            present(nkb, npage);
-            if (npage >= 0) load(npage);
+            more = pages.next<1>(P, nkb, npage, last, lane);
+            if (more) load(npage);
         }
         lds_barrier();
         st ^= 1;

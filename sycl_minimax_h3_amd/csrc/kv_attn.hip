@@ -7,18 +7,22 @@
 
 namespace h3 {
 
-// Rows: `most` tokens of a sequence times the heads that share a key/value head. Up to 64 rows the four wavefronts of a block
-// share 16 or 32 of them and the cache is read by all four (an answered token is bound by the cache's bytes); beyond, each has 16 or 32
-// rows of its own (16 where 32 would leave CUs without a block).
+// Rows: `most` tokens of a sequence times the heads that share a key/value head. Up to 32 (heads of up to 128 features) or 16 the four
+// wavefronts of a block share 16 or 32 of them and the cache is read by all four (an answered token is bound by the cache's bytes);
+// beyond, each has 16 or 32 rows of its own. With more rows shared, or wider heads, a wavefront holds so much that one runs on a SIMD: 16
+// sequences of 4096 tokens, 8 heads, 64 rows: 65 us shared, 50 not; 32 rows 44 and 45; 32 rows of 256 features, 2048 tokens, 72 and 66.
+// 32 rows of its own: where blocks of 128 rows still give each CU one and less than a quarter of their rows is none, and never for float32
+// queries, whose two halves leave room for one wavefront a SIMD only (2048 tokens over 4096, 64 heads over 8 of 128: 16-bit 265 us
+// with 32 rows, 356 with 16; float32 588 and 460; 64 sequences of 72 rows over 2048 tokens: 86 and 75).
 // Parts: of the same number of cache blocks for every sequence (at least eight, or four of a prompt's), as many as give each CU the two blocks of threads that
 // it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up to 8192 tokens, 64
 // heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and their merge 4, 7
 // and 11 us more.)
-static KvPlan kv_plan(const KvArgs& P, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
+static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
     KvPlan plan;
     const int64_t rows = std::min<int64_t>(most, P.rows) * group, each = (int64_t) P.seqs * P.heads;
-    plan.rows = rows > 64;
-    plan.nq = plan.rows ? ((rows + 127) / 128 * each < cus ? 1 : 2) : rows <= 16 ? 1 : 2;
+    plan.rows = rows > (P.dim <= 128 ? 32 : 16);
+    plan.nq = plan.rows ? (two || rows <= 96 || (rows + 127) / 128 * each < cus ? 1 : 2) : rows <= 16 ? 1 : 2;
     plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
     plan.tiles = (rows + plan.rt - 1) / plan.rt;
     plan.blocks = plan.tiles * each;
@@ -46,7 +50,11 @@ int64_t kv_attention_work(void* ctx, const h3_kv_cache* cache, const h3_kv_batch
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
     if (P.seqs == 0 || P.rows == 0 || batch->most == 0) return 0;
-    return 4 * kv_part_floats(kv_plan(P, batch->most, q_heads / P.heads, max_len, window, c->cus), kv_width(P.dim));
+    // (the more of what 16-bit and float32 queries take)
+    int64_t floats = 0;
+    for (bool two : {false, true})
+        floats = std::max(floats, kv_part_floats(kv_plan(P, two, batch->most, q_heads / P.heads, max_len, window, c->cus), kv_width(P.dim)));
+    return 4 * floats;
 } catch (const std::exception& e) { return fail(e.what()); }
 
 int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* lengths, int64_t max_len, const void* q,
@@ -67,7 +75,8 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
     if (A.kv.rows * group > INT32_MAX) return fail(std::string(fn) + ": too many rows");
-    const KvPlan plan = kv_plan(A.kv, batch->most, group, max_len, window, c->cus);
+    const bool two = dt == H3S_F32;
+    const KvPlan plan = kv_plan(A.kv, two, batch->most, group, max_len, window, c->cus);
     const int64_t W = kv_width(dim);
     if (plan.blocks * plan.nsplit > 0x7fffffff || plan.blocks * plan.rt > 0x7fffffff) return fail(std::string(fn) + ": too many blocks of work");
     const int64_t floats = kv_part_floats(plan, W);
@@ -95,7 +104,6 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     A.q_vec = aligned16(q) && dim % 8 == 0 && (q_stride * elem_size(dt)) % 16 == 0;
     A.out_vec = aligned16(out) && dim % 4 == 0;
     A.mask_vec = mask && aligned16(mask) && mask_stride % 16 == 0;
-    const bool two = dt == H3S_F32;
     switch (W / 64) {
         case 1: kv_attn_64(c, A, plan, two); break;
         case 2: kv_attn_128(c, A, plan, two); break;

@@ -17,7 +17,7 @@
 //
 // Work: a block of threads takes one key/value head of one sequence, a tile of its rows (tokens x the heads that share the
 // key/value head) and a range of the cache blocks. Few rows (kv_attn_kernel): its four wavefronts share 16 NQ rows and take every fourth cache block
-// (answered tokens; bound by the cache's bytes), joined through LDS. KS = 1: each has 16 NQ rows of its own (prompts).
+// (answered tokens; bound by the cache's bytes), joined through LDS. Many (kv_attn_rows_kernel): each has 16 NQ rows of its own (prompts).
 // Where that leaves the device idle, the cache blocks are split over several blocks of threads, whose sums kv_merge_kernel
 // joins in split order.
 #pragma once
@@ -317,7 +317,7 @@ struct KvPages {
     }
 };
 
-// Few rows (up to 64 of a sequence and head): the four wavefronts of a block share 16 NQ rows and take every fourth cache block.
+// Few rows (up to 32 of a sequence and head): the four wavefronts of a block share 16 NQ rows and take every fourth cache block.
 // Bound by the cache's bytes: the next block's codes are on their way while one is worked on.
 template <int WC, int NQ, bool TWO>
 __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
@@ -648,8 +648,8 @@ static void kv_attn_run(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool tw
     const unsigned grid = (unsigned) (plan.blocks * plan.nsplit);
     constexpr int RT = (ROWS ? 64 : 16) * NQ;
     if constexpr (ROWS) {
-        if (two) kv_attn_rows_kernel<WC, NQ, true><<<grid, 256, 0, c->stream>>>(P);
-        else kv_attn_rows_kernel<WC, NQ, false><<<grid, 256, 0, c->stream>>>(P);
+        if (!two) kv_attn_rows_kernel<WC, NQ, false><<<grid, 256, 0, c->stream>>>(P);
+        else if constexpr (NQ == 1) kv_attn_rows_kernel<WC, 1, true><<<grid, 256, 0, c->stream>>>(P);
     } else {
         if (two) kv_attn_kernel<WC, NQ, true><<<grid, 256, 0, c->stream>>>(P);
         else kv_attn_kernel<WC, NQ, false><<<grid, 256, 0, c->stream>>>(P);
@@ -668,7 +668,7 @@ static void kv_attn_width(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool 
     if (plan.rows && plan.nq == 1) kv_attn_run<WC, 1, true>(c, P, plan, two);
     else if (plan.rows) kv_attn_run<WC, 2, true>(c, P, plan, two);
     else if (plan.nq == 1) kv_attn_run<WC, 1, false>(c, P, plan, two);
-    else kv_attn_run<WC, 2, false>(c, P, plan, two);
+    else if constexpr (WC <= 2) kv_attn_run<WC, 2, false>(c, P, plan, two);
 }
 
 }  // namespace h3

@@ -14,20 +14,16 @@ int linear4(void* ctx, const void* x, int dt, int64_t M, int64_t K, const uint8_
     if (K > kL4MostK) return fail(std::string(fn) + ": at most " + std::to_string(kL4MostK) + " inputs");
     if (!x || !codes || !scale || !out) return fail(std::string(fn) + ": x, codes, scale and out are required");
     if (!aligned16(x) || !aligned16(codes)) return fail(std::string(fn) + ": x and codes must be 16-byte aligned");
-    if (M > ((int64_t) 1 << 31) || N > ((int64_t) 1 << 31) || (M + 31) / 32 * ((N + kL4Cols - 1) / kL4Cols + 8) > 0x7fffffff)
+    if (M > ((int64_t) 1 << 31) || N > ((int64_t) 1 << 31) || (M + 31) / 32 * ((N + 127) / 128 + 8) > 0x7fffffff)
         return fail(std::string(fn) + ": too many rows or columns");
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
     const uint64_t runs = (uint64_t) group / 32;
     const L4Args P{x, M, N, (int) K, codes, scale, mins ? mins : scale, scale_dt, mins != nullptr, (int) group, (int) (K / group),
                    runs == 1 ? 0u : (uint32_t) (((1ull << 32) + runs - 1) / runs), bias, out, out_dt};
-    // Rows: up to 4 take one register of sums a lane, up to 16 one operand. Few columns: 16 a block and sixteen wavefronts
-    // along the inputs, so that the device is covered; many: 32 a block, which share x's operands.
-    L4Plan plan;
-    plan.rows = M <= 16 ? 16 : M <= 32 || dt == H3S_F32 ? 32 : 64;
-    if (dt == H3S_BF16) l4_bf16(c, P, plan);
-    else if (dt == H3S_F16) l4_f16(c, P, plan);
-    else l4_f32(c, P, plan);
+    if (dt == H3S_BF16) l4_bf16(c, P);
+    else if (dt == H3S_F16) l4_f16(c, P);
+    else l4_f32(c, P);
     return launched(fn);
 } catch (const std::exception& e) { return fail(e.what()); }
 

@@ -2,5 +2,5 @@
 #include "linear4_impl.h"
 
 namespace h3 {
-void l4_bf16(Ctx* c, const L4Args& P, const L4Plan& plan) { l4_type<H3S_BF16>(c, P, plan); }
+void l4_bf16(Ctx* c, const L4Args& P) { l4_type<H3S_BF16>(c, P); }
 }  // namespace h3

@@ -14,10 +14,11 @@
 // exchange between them (four lane swaps) leaves each with eight codes of each of four runs of 32 inputs, so that an instruction's 32
 // inputs lie in one group.
 //
-// Work. Up to 16 rows (linear4_few_kernel): a wavefront takes 16 NT columns and every KW-th 128 inputs; the KW wavefronts of a block
+// Work. One row (linear4_dot_kernel): the codes as above, multiplied by pairs on the vector units, with x in registers.
+// Two to 16 rows (linear4_few_kernel): a wavefront takes 16 NT columns and every KW-th 128 inputs; the KW wavefronts of a block
 // are joined through LDS in wavefront order. Bound by the codes' bytes: everything that a step needs is loaded a step ahead.
-// More rows (linear4_many_kernel): a block takes 16 MT rows x 128 columns, in two groups of four wavefronts that take every other 128
-// inputs; x goes through LDS, in the order of the instructions' operands, and each wavefront has 32 columns.
+// More rows (linear4_many_kernel): a block takes 16 MT rows x 128 columns (64 or 32 where that leaves CUs idle), in two groups of four
+// wavefronts (four of two, eight of one) that take every other (fourth, eighth) 128 inputs; x goes through LDS, in the order of the instructions' operands, and each wavefront has 32 columns.
 #pragma once
 
 #include "kv.h"
@@ -183,7 +184,7 @@ template <int NI> __device__ __forceinline__ void l4_store(const L4Args& P, int6
     }
 }
 
-// ---- up to four rows of x: multiply-adds of pairs of codes --------------------------------------------------------------------
+// ---- one row of x: multiply-adds of pairs of codes -----------------------------------------------------------------------------
 
 // c + a.lo b.lo + a.hi b.hi
 template <int OP> __device__ __forceinline__ float l4_dot(uint32_t a, uint32_t b, float c) {
@@ -200,7 +201,7 @@ constexpr int kL4DotWaves = 11;       // wavefronts of a block, at most
 // lane's codes is one 2-byte load beside its neighbours', and no operand goes through LDS. (As matrix instructions' operands - 16
 // rows a load, 64 bytes of each, a scale gathered from 16 rows - the same loads alone took 94 us where the codes come in 62.) Per tile of
 // 16 rows the wavefronts' sums are joined through LDS, in wavefront order; the loads go on across tiles, DP row steps ahead.
-template <int DT, int M, int U, bool MINS>
+template <int DT, int U, bool MINS>
 __global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P) {
     constexpr int OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS, DP = U == 1 ? 4 : U == 2 ? 3 : 2;
     const int lane = threadIdx.x & 63, l = lane & 15, q = lane >> 4, KW = (int) (blockDim.x >> 6);
@@ -247,31 +248,29 @@ __global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P)
 #pragma unroll
     for (int d = 0; d < DP; ++d) load(d);
     // x as operands: the pairs in the order of l4_codes, and the sum of each lane's 32 values
-    uint32_t x[M][U][PARTS][16];
-    float sx[M][U];
+    uint32_t x[U][PARTS][16];
+    float sx[U];
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+    for (int u = 0; u < U; ++u) {
+        const char* xp = (const char*) P.x + 2 * kofs[u] * (DT == H3S_F32 ? 4 : 2);
+        sx[u] = 0.0f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const char* xp = (const char*) P.x + ((int64_t) min(m, (int) P.M - 1) * P.K + 2 * (int) kofs[u]) * (DT == H3S_F32 ? 4 : 2);
-            sx[m][u] = 0.0f;
+        for (int e = 0; e < 4; ++e) {
+            L4X<DT> v;
+            v.load(xp, 8 * e);
+            if (!in[u]) v.zero();
+            uint4 f[PARTS];
+            v.parts(f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                L4X<DT> v;
-                v.load(xp, 8 * e);
-                if (!in[u]) v.zero();
-                uint4 f[PARTS];
-                v.parts(f);
+            for (int p = 0; p < PARTS; ++p) {
+                x[u][p][4 * e] = f[p].x; x[u][p][4 * e + 1] = f[p].y; x[u][p][4 * e + 2] = f[p].z; x[u][p][4 * e + 3] = f[p].w;
+                float y[8];
+                Vec<OP>::unpack(f[p], y);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    x[m][u][p][4 * e] = f[p].x; x[m][u][p][4 * e + 1] = f[p].y; x[m][u][p][4 * e + 2] = f[p].z; x[m][u][p][4 * e + 3] = f[p].w;
-                    float y[8];
-                    Vec<OP>::unpack(f[p], y);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sx[m][u] += y[i];
-                }
+                for (int i = 0; i < 8; ++i) sx[u] += y[i];
             }
         }
+    }
     uint32_t cm, ce;
     l4_constants<OP>(cm, ce);
     const bool bf = P.scale_dt == H3S_BF16, wide = ses == 4;
@@ -279,53 +278,41 @@ __global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P)
         const float a = bf16_lo(r), b = f16_lo(r), c = __uint_as_float(r);
         return wide ? c : bf ? a : b;
     };
-    __shared__ float part[2][M][16][kL4DotWaves + 1];
+    __shared__ float part[2][16][kL4DotWaves + 1];
     int turn = 0, rs = 0, tile = blockIdx.x;
     while (tile < tiles) {
 #pragma unroll
         for (int d = 0; d < DP; ++d) {
-            float acc[M];
-#pragma unroll
-            for (int m = 0; m < M; ++m) acc[m] = 0.0f;
+            float acc = 0.0f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t c[4] = {w[d][u].x, w[d][u].y, w[d][u].z, w[d][u].w};
-                float y[M];
-#pragma unroll
-                for (int m = 0; m < M; ++m) y[m] = 0.0f;
+                float y = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint4 f = l4_codes<OP>(c[e], cm, ce);
 #pragma unroll
-                    for (int m = 0; m < M; ++m)
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            y[m] = l4_dot<OP>(x[m][u][p][4 * e], f.x, y[m]);
-                            y[m] = l4_dot<OP>(x[m][u][p][4 * e + 1], f.y, y[m]);
-                            y[m] = l4_dot<OP>(x[m][u][p][4 * e + 2], f.z, y[m]);
-                            y[m] = l4_dot<OP>(x[m][u][p][4 * e + 3], f.w, y[m]);
-                        }
+                    for (int p = 0; p < PARTS; ++p) {
+                        y = l4_dot<OP>(x[u][p][4 * e], f.x, y);
+                        y = l4_dot<OP>(x[u][p][4 * e + 1], f.y, y);
+                        y = l4_dot<OP>(x[u][p][4 * e + 2], f.z, y);
+                        y = l4_dot<OP>(x[u][p][4 * e + 3], f.w, y);
+                    }
                 }
                 const float s = number(sr[d][u]), off = MINS ? __builtin_fmaf(16.0f, s, number(zr[d][u])) : 24.0f * s;
-#pragma unroll
-                for (int m = 0; m < M; ++m) acc[m] = __builtin_fmaf(-off, sx[m][u], __builtin_fmaf(s, y[m], acc[m]));
+                acc = __builtin_fmaf(-off, sx[u], __builtin_fmaf(s, y, acc));
             }
             load(d);
-#pragma unroll
-            for (int m = 0; m < M; ++m) acc[m] = wave_sum<16>(acc[m]);
-            if (l == 0) {
-#pragma unroll
-                for (int m = 0; m < M; ++m) part[turn & 1][m][rs * 4 + q][wave] = acc[m];
-            }
+            acc = wave_sum<16>(acc);
+            if (l == 0) part[turn & 1][rs * 4 + q][wave] = acc;
             if (++rs == 4) {
                 // (the area is written again two tiles later, behind the next tile's barrier)
                 lds_barrier();
-                const int n = threadIdx.x & 15, m = threadIdx.x >> 4;
-                const int64_t col = (int64_t) tile * 16 + n;
-                if (m < M && m < P.M && tile < tiles && col < P.N) {
-                    float y = part[turn & 1][m][n][0];
-                    for (int v = 1; v < KW; ++v) y += part[turn & 1][m][n][v];
-                    store_any(P.out, P.out_dt, m * P.N + col, y + (P.bias ? P.bias[col] : 0.0f));
+                const int64_t col = (int64_t) tile * 16 + threadIdx.x;
+                if (threadIdx.x < 16 && tile < tiles && col < P.N) {
+                    float y = part[turn & 1][threadIdx.x][0];
+                    for (int v = 1; v < KW; ++v) y += part[turn & 1][threadIdx.x][v];
+                    store_any(P.out, P.out_dt, col, y + (P.bias ? P.bias[col] : 0.0f));
                 }
                 ++turn;
                 rs = 0;
@@ -537,19 +524,19 @@ __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P,
     }
 }
 
-constexpr int kL4Cols = 128;      // columns of a block of linear4_many_kernel
-
-template <int DT, int MT, int J, int SM>
+// CG: wavefronts side by side, of 32 columns each; the block's 8 / CG groups of them take every (8 / CG)th step of 128 inputs
+template <int DT, int MT, int CG, int J, int SM>
 __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
     constexpr int NT = 2, OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS;
-    constexpr int PIECES = 16 * MT * 16 / 256;                                    // 8-input pieces of x a thread stages
-    __shared__ uint4 xs[2][2][MT][4][PARTS][64];                                  // [K group][stage][rows][run][part][lane]
+    constexpr int KG = 8 / CG, COLS = 16 * NT * CG;
+    constexpr int PIECES = 16 * MT * 16 / (64 * CG);                              // 8-input pieces of x a thread stages
+    __shared__ uint4 xs[KG][2][MT][4][PARTS][64];                                 // [K group][stage][rows][run][part][lane]
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6)), kg = wave >> 2;
+    const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6)), kg = wave / CG;
     // blocks eight apart run on one XCD: the row tiles of a column block lie there one after another and share its codes
     const int64_t mt = (P.M + 16 * MT - 1) / (16 * MT), id = blockIdx.x;
-    const int64_t nb = id / (8 * mt) * 8 + id % 8, n0 = nb * kL4Cols + (wave & 3) * (16 * NT), m0 = id / 8 % mt * (16 * MT);
-    if (nb * kL4Cols >= P.N) return;
+    const int64_t nb = id / (8 * mt) * 8 + id % 8, n0 = nb * COLS + wave % CG * (16 * NT), m0 = id / 8 % mt * (16 * MT);
+    if (nb * COLS >= P.N) return;
     const int steps = (P.K + 127) / 128;
     const int ses = SM == L4_S32 || (SM == L4_SANY && P.scale_dt == H3S_F32) ? 4 : 2;
     const int64_t from = min(n0, P.N - 1);                                        // (a wavefront past the columns: the last one, not stored)
@@ -569,14 +556,14 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
     l4_select<OP>(l15, sel);
     uint32_t cm, ce;
     l4_constants<OP>(cm, ce);
-    // x: piece t + 256 p of the K group's step is 8 inputs (16 pieces a row)
+    // x: piece t + 64 CG p of the K group's step is 8 inputs (16 pieces a row)
     constexpr int XES = DT == H3S_F32 ? 4 : 2;
-    const int t = threadIdx.x & 255;
+    const int t = threadIdx.x % (64 * CG);
     L4X<DT> xr[PIECES];
     const char* xbase = (const char*) P.x + m0 * P.K * XES;
     uint32_t xoff[PIECES];
 #pragma unroll
-    for (int p = 0; p < PIECES; ++p) xoff[p] = (uint32_t) ((int) min<int64_t>((t + 256 * p) / 16, P.M - 1 - m0) * P.K + t % 16 * 8) * XES;
+    for (int p = 0; p < PIECES; ++p) xoff[p] = (uint32_t) ((int) min<int64_t>((t + 64 * CG * p) / 16, P.M - 1 - m0) * P.K + t % 16 * 8) * XES;
     uint4 w[NT];
     L4Q<J, SM> now[NT], next[NT];                                                 // the scales of four of the K group's steps
     auto load_x = [&](int step) {
@@ -591,7 +578,7 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
     auto store_x = [&](int stage) {
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int at = t + 256 * p, r = at / 16, k8 = at % 16;                // place: row 4 (l % 4) + l / 4 at l,
+            const int at = t + 64 * CG * p, r = at / 16, k8 = at % 16;                // place: row 4 (l % 4) + l / 4 at l,
                                                                                   // its low bits by the lane group (banks)
             uint4 f[PARTS];
             xr[p].parts(f);
@@ -610,23 +597,23 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
     };
     auto load_s = [&](int step) {
 #pragma unroll
-        for (int b = 0; b < NT; ++b) next[b].load(P, sbase, zbase, soff[b], min(step + 2 * g, steps - 1) * 4);
+        for (int b = 0; b < NT; ++b) next[b].load(P, sbase, zbase, soff[b], min(step + KG * g, steps - 1) * 4);
     };
-    // both K groups make the same number of rounds (the second's last may have no step)
+    // all K groups make the same number of rounds (their last may have no step)
     // (Loads are never skipped, see linear4_few_kernel: past the end it is the last step again.)
     load_s(kg);
     load_x(min(kg, steps - 1));
     load_w(min(kg, steps - 1));
     store_x(0);
-    load_x(min(kg + 2, steps - 1));
+    load_x(min(kg + KG, steps - 1));
     lds_barrier();
-    for (int first = 0; first < steps; first += 8) {
+    for (int first = 0; first < steps; first += 4 * KG) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) now[b] = next[b];
-        load_s(first + 8 + kg);
+        load_s(first + 4 * KG + kg);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int step = first + 2 * r + kg;
+            const int step = first + KG * r + kg;
             if (step < steps) {
                 uint32_t c[NT][4];
                 float sc[NT][4 / J], off[NT];
@@ -640,25 +627,25 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
                         off[b] = step * 128 + 32 * g < P.K ? off[b] : 0.0f;
                     }
                 }
-                load_w(min(step + 2, steps - 1));
+                load_w(min(step + KG, steps - 1));
                 l4_products<OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][r & 1][a][j][q][lane ^ g];
                 }, acc);
                 store_x((r & 1) ^ 1);
-                load_x(min(step + 4, steps - 1));
+                load_x(min(step + 2 * KG, steps - 1));
             }
             lds_barrier();
         }
     }
-    // the second group's sums to the first's
+    // the groups' sums to the first's, in their order
     v4f_l4* part = reinterpret_cast<v4f_l4*>(&xs[0][0][0][0][0][0]);
-    static_assert(sizeof(xs) >= 4 * MT * NT * 64 * 16, "the sums fit x's stages");
-    if (kg == 1) {
+    static_assert(sizeof(xs) >= (size_t) (KG - 1) * CG * MT * NT * 64 * 16, "the sums fit x's stages");
+    if (kg) {
 #pragma unroll
         for (int a = 0; a < MT; ++a)
 #pragma unroll
-            for (int b = 0; b < NT; ++b) part[((wave & 3) * MT * NT + a * NT + b) * 64 + lane] = acc[a][b];
+            for (int b = 0; b < NT; ++b) part[(((wave - CG) * MT + a) * NT + b) * 64 + lane] = acc[a][b];
     }
     __syncthreads();
     if (kg == 0) {
@@ -668,13 +655,14 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
 #pragma unroll
         for (int a = 0; a < MT; ++a)
 #pragma unroll
-            for (int b = 0; b < NT; ++b)
-                l4_store<4>(P, m0 + 16 * a, n0 + 16 * b + l15, g, acc[a][b] + part[((wave & 3) * MT * NT + a * NT + b) * 64 + lane], bias[b]);
+            for (int b = 0; b < NT; ++b) {
+                v4f_l4 y = acc[a][b];
+#pragma unroll
+                for (int k = 0; k + 1 < KG; ++k) y += part[(((k * CG + wave) * MT + a) * NT + b) * 64 + lane];
+                l4_store<4>(P, m0 + 16 * a, n0 + 16 * b + l15, g, y, bias[b]);
+            }
     }
 }
-
-// which kernel a call takes (linear4.hip): rows 16 (few), 32 or 64 (many: the tile)
-struct L4Plan { int rows; };
 
 template <int DT, int NT, int J, int SM, bool XR>
 static void l4_few_run(Ctx* c, const L4Args& P, int quads, int kw) {
@@ -691,60 +679,77 @@ static void l4_few(Ctx* c, const L4Args& P) {
     }
     l4_few_run<DT, 2, J, SM, false>(c, P, quads, kw);
 }
+// the blocks of tiles of `rows` rows and 32 cg columns; those of a column tile go to one XCD of eight, so an eighth of them is a whole number
+static int64_t l4_blocks(const L4Args& P, int rows, int cg) {
+    return (P.M + rows - 1) / rows * (((P.N + 32 * cg - 1) / (32 * cg) + 7) / 8 * 8);
+}
+template <int DT, int MT, int CG, int J, int SM>
+static void l4_many_run(Ctx* c, const L4Args& P) {
+    linear4_many_kernel<DT, MT, CG, J, SM><<<(unsigned) l4_blocks(P, 16 * MT, CG), 512, 0, c->stream>>>(P);
+}
+// Half as many columns a block, and twice the groups along the inputs, while the blocks still run at once (as far as x's stages fit LDS):
+// 5376 -> 5376, 32 rows 38 to 18 us, 128 rows 52 to 34; 14336 -> 5376, 32 rows 92 to 34 us, 128 rows 126 to 75.
+template <int DT, int MT, int J, int SM>
+static void l4_many(Ctx* c, const L4Args& P) {
+    if constexpr (DT != H3S_F32) {
+        if constexpr (MT == 2) {
+            if (l4_blocks(P, 32, 1) <= c->cus) return l4_many_run<DT, MT, 1, J, SM>(c, P);
+        }
+        if (l4_blocks(P, 16 * MT, 2) <= c->cus) return l4_many_run<DT, MT, 2, J, SM>(c, P);
+    }
+    l4_many_run<DT, MT, 4, J, SM>(c, P);
+}
 template <int DT, int J, int SM>
-static void l4_run(Ctx* c, const L4Args& P, const L4Plan& plan) {
-    if (plan.rows <= 16) {
-        l4_few<DT, J, SM>(c, P);
+static void l4_run(Ctx* c, const L4Args& P) {
+    if constexpr (DT == H3S_F32) {
+        if (P.M <= 16) l4_few<DT, J, SM>(c, P);
+        else l4_many<DT, 2, J, SM>(c, P);
     } else {
-        const int64_t mt = (P.M + plan.rows - 1) / plan.rows, nb = ((P.N + kL4Cols - 1) / kL4Cols + 7) / 8 * 8;
-        if (plan.rows == 32) linear4_many_kernel<DT, 2, J, SM><<<(unsigned) (mt * nb), 512, 0, c->stream>>>(P);
-        else if constexpr (DT != H3S_F32) linear4_many_kernel<DT, 4, J, SM><<<(unsigned) (mt * nb), 512, 0, c->stream>>>(P);
+        // Up to 16 rows as one operand, unless x's operands do not fit the wavefronts' registers there and few columns leave the inputs to
+        // split (14336 -> 5376: 16 rows 41 us, in tiles of 32 rows 33). Tiles of 32 rows up to 32 rows, and beyond while the device runs
+        // all blocks of 64 columns of them at once (64 rows: 5376 -> 5376 34 to 25 us, 14336 -> 5376 75 to 55).
+        if (P.M <= 4 || (P.M <= 16 && (P.K <= 512 * kL4FewWaves || l4_blocks(P, 32, 1) > c->cus))) l4_few<DT, J, SM>(c, P);
+        else if (P.M <= 32 || l4_blocks(P, 32, 2) <= c->cus) l4_many<DT, 2, J, SM>(c, P);
+        else l4_many<DT, 4, J, SM>(c, P);
     }
 }
-template <int DT, int M, int U>
-static void l4_dot_run(Ctx* c, const L4Args& P, int per_cu) {
-    const int64_t tiles = (P.N + 15) / 16, turns = (tiles + per_cu * c->cus - 1) / (per_cu * c->cus);
+template <int DT, int U>
+static void l4_dot_run(Ctx* c, const L4Args& P) {
+    const int64_t tiles = (P.N + 15) / 16, turns = (tiles + 2 * c->cus - 1) / (2 * c->cus);
     const unsigned grid = (unsigned) ((tiles + turns - 1) / turns);
     const int chunks = (P.K + 511) / 512, kw = (chunks + U - 1) / U;
-    if (P.has_mins) linear4_dot_kernel<DT, M, U, true><<<grid, 64 * kw, 0, c->stream>>>(P);
-    else linear4_dot_kernel<DT, M, U, false><<<grid, 64 * kw, 0, c->stream>>>(P);
+    if (P.has_mins) linear4_dot_kernel<DT, U, true><<<grid, 64 * kw, 0, c->stream>>>(P);
+    else linear4_dot_kernel<DT, U, false><<<grid, 64 * kw, 0, c->stream>>>(P);
 }
-// whether the rows are few enough for multiply-adds and x's values for registers (the last run starts it)
+// whether the call has one row, whose values for a wavefront's chunks fit its registers (the last run starts it)
 template <int DT> static bool l4_dot_takes(Ctx* c, const L4Args& P) {
     const int chunks = (P.K + 511) / 512;
-    constexpr int PARTS = L4X<DT>::PARTS;
-    if (P.M > 4) return false;
-    const int u = chunks <= kL4DotWaves ? 1 : chunks <= 2 * kL4DotWaves ? 2 : chunks <= 4 * kL4DotWaves ? 4 : 0, m = P.M == 3 ? 4 : (int) P.M;
-    if (u == 0 || 16 * PARTS * u * m > 96) return false;
-    if (m == 1) {
-        if (u == 1) l4_dot_run<DT, 1, 1>(c, P, 2);
-        else if (u == 2) l4_dot_run<DT, 1, 2>(c, P, 2);
-        else if constexpr (PARTS == 1) l4_dot_run<DT, 1, 4>(c, P, 2);
-    } else if (m == 2) {
-        if (u == 1) l4_dot_run<DT, 2, 1>(c, P, 2);
-        else if constexpr (PARTS == 1) l4_dot_run<DT, 2, 2>(c, P, 2);
-    } else if constexpr (PARTS == 1) l4_dot_run<DT, 4, 1>(c, P, 2);
+    if (P.M > 1) return false;
+    if (chunks <= kL4DotWaves) l4_dot_run<DT, 1>(c, P);
+    else if (chunks <= 2 * kL4DotWaves) l4_dot_run<DT, 2>(c, P);
+    else if (chunks <= 4 * kL4DotWaves && L4X<DT>::PARTS == 1) l4_dot_run<DT, L4X<DT>::PARTS == 1 ? 4 : 1>(c, P);
+    else return false;
     return true;
 }
 template <int DT>
-static void l4_type(Ctx* c, const L4Args& P, const L4Plan& plan) {
+static void l4_type(Ctx* c, const L4Args& P) {
     if (l4_dot_takes<DT>(c, P)) return;
     // a step of 128 inputs has 4, 2 or 1 scales: one load where every column's lie on a boundary of their size
     const int64_t cnt = P.group % 128 == 0 ? 1 : P.group == 64 ? 2 : P.group == 32 ? 4 : 0;
     const bool vec = cnt && P.groups % cnt == 0 && ((uintptr_t) P.scale | (uintptr_t) P.mins) % (uintptr_t) (cnt * elem_size(P.scale_dt)) == 0;
-    if (!vec) l4_run<DT, 1, L4_SANY>(c, P, plan);
+    if (!vec) l4_run<DT, 1, L4_SANY>(c, P);
     else if (P.scale_dt == H3S_F32) {
-        if (cnt == 1) l4_run<DT, 4, L4_S32>(c, P, plan);
-        else if (cnt == 2) l4_run<DT, 2, L4_S32>(c, P, plan);
-        else l4_run<DT, 1, L4_S32>(c, P, plan);
+        if (cnt == 1) l4_run<DT, 4, L4_S32>(c, P);
+        else if (cnt == 2) l4_run<DT, 2, L4_S32>(c, P);
+        else l4_run<DT, 1, L4_S32>(c, P);
     } else {
-        if (cnt == 1) l4_run<DT, 4, L4_S16>(c, P, plan);
-        else if (cnt == 2) l4_run<DT, 2, L4_S16>(c, P, plan);
-        else l4_run<DT, 1, L4_S16>(c, P, plan);
+        if (cnt == 1) l4_run<DT, 4, L4_S16>(c, P);
+        else if (cnt == 2) l4_run<DT, 2, L4_S16>(c, P);
+        else l4_run<DT, 1, L4_S16>(c, P);
     }
 }
-void l4_bf16(Ctx* c, const L4Args& P, const L4Plan& plan);
-void l4_f16(Ctx* c, const L4Args& P, const L4Plan& plan);
-void l4_f32(Ctx* c, const L4Args& P, const L4Plan& plan);
+void l4_bf16(Ctx* c, const L4Args& P);
+void l4_f16(Ctx* c, const L4Args& P);
+void l4_f32(Ctx* c, const L4Args& P);
 
 }  // namespace h3

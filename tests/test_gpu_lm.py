@@ -177,6 +177,17 @@ ATTN = [
     ([(20, 64)], 1, 8, 128, "F32", "BF16", {"scale": 0.37}),
     ([(9, 4)], 1, 2, 64, "BF16", "BF16", {"lse": True}),                       # fewer tokens than rows: the first see nothing
 ]
+# the number of rows on both sides of each kernel's
+ATTN_ROWS = [
+    ([(4, 300), (1, 90)], 2, 8, 64, "BF16", "BF16", {"lse": True}),            # 32 rows
+    ([(11, 250)], 2, 3, 128, "F16", "F16", {"mask": 0.6}),                     # 33
+    ([(2, 600), (2, 2)], 1, 16, 128, "F32", "F32", {"window": 100}),           # 32
+    ([(3, 200)], 2, 6, 250, "BF16", "F32", {"lse": True}),                     # 18 wide rows
+    ([(16, 400), (5, 5)], 1, 1, 200, "F32", "BF16", {"lse": True}),            # 16 wide rows
+    ([(97, 300), (20, 500)], 3, 1, 64, "BF16", "BF16", {"lse": True}),
+    ([(96, 96)], 3, 1, 64, "F16", "BF16", {"window": 40}),
+    ([(150, 190), (1, 70)], 2, 2, 128, "F32", "F32", {"lse": True, "mask": 0.9}),
+]
 
 
 def attn_case(dev, seqs, heads, group, dim, dt, opts, seed=11, spread=1.0):
@@ -240,7 +251,7 @@ def dev_cus2():
 
 
 @pytest.mark.parametrize("where", ["dev", "dev_cus2"])
-@pytest.mark.parametrize("seqs,heads,group,dim,dt,out_dt,opts", ATTN)
+@pytest.mark.parametrize("seqs,heads,group,dim,dt,out_dt,opts", ATTN + ATTN_ROWS)
 def test_attention(request, where, seqs, heads, group, dim, dt, out_dt, opts):
     dev = request.getfixturevalue(where)
     case = attn_case(dev, seqs, heads, group, dim, dt, opts)
@@ -537,6 +548,14 @@ def test_attention_kernels_taken(dev):
     assert len(split) == 2 and split[0][0].startswith("kv_attn_kernel<2, 1, true") and split[0][1] >= 4, split
     some = names([(100, 100)], 2, 4, 64, "F16", {})
     assert len(some) == 1 and some[0][0].startswith("kv_attn_rows_kernel<1, 1, false") and some[0][1] == 14, some
+    shared = names([(4, 100)] * 3, 2, 8, 128, "BF16", {})
+    assert len(shared) == 1 and shared[0][0].startswith("kv_attn_kernel<2, 2, false") and shared[0][1] == 6, shared
+    own = names([(5, 100)] * 3, 2, 8, 128, "BF16", {})
+    assert len(own) == 1 and own[0][0].startswith("kv_attn_rows_kernel<2, 1, false") and own[0][1] == 6, own
+    wide = names([(4, 100)] * 3, 2, 8, 256, "F32", {})
+    assert len(wide) == 1 and wide[0][0].startswith("kv_attn_rows_kernel<4, 1, true") and wide[0][1] == 6, wide
+    halves = names([(130, 130)], 16, 16, 64, "F32", {})
+    assert len(halves) == 1 and halves[0][0].startswith("kv_attn_rows_kernel<1, 1, true") and halves[0][1] == 33 * 16, halves
     many = names([(130, 130)], 16, 16, 64, "F16", {})
     assert len(many) == 1 and many[0][0].startswith("kv_attn_rows_kernel<1, 2, false") and many[0][1] == 17 * 16, many
 
@@ -576,6 +595,11 @@ LINEAR4_LONG = [
     (12, 6176, 100, 32, True, "F32", "F32", "F16", True),
     (33, 14336, 150, 64, True, "BF16", "BF16", "F16", True),
     (70, 6240, 140, 96, False, "F16", "F32", "F32", True),
+    (20, 5376, 5376, 32, True, "BF16", "BF16", "F16", True),                    # 42 blocks of 128 columns: in 168 of 32
+    (50, 1568, 4100, 32, True, "F16", "F16", "F16", True),                      # 33 blocks: in 66 of 64
+    (32, 2048, 8200, 128, False, "BF16", "BF16", "F32", False),                 # 65: in 130 of 64
+    (100, 640, 17000, 64, True, "BF16", "BF16", "F16", True),                   # 266: as they are
+    (33, 1024, 5000, 64, False, "F32", "F32", "F16", True),
 ]
 
 

@@ -691,19 +691,19 @@ static void l4_many_run(Ctx* c, const L4Args& P) {
 // 5376 -> 5376, 32 rows 38 to 18 us, 128 rows 52 to 34; 14336 -> 5376, 32 rows 92 to 34 us, 128 rows 126 to 75.
 template <int DT, int MT, int J, int SM>
 static void l4_many(Ctx* c, const L4Args& P) {
-    if constexpr (DT != H3S_F32) {
-        if constexpr (MT == 2) {
-            if (l4_blocks(P, 32, 1) <= c->cus) return l4_many_run<DT, MT, 1, J, SM>(c, P);
-        }
-        if (l4_blocks(P, 16 * MT, 2) <= c->cus) return l4_many_run<DT, MT, 2, J, SM>(c, P);
+    if constexpr (MT == 2) {
+        if (l4_blocks(P, 32, 1) <= c->cus) return l4_many_run<DT, MT, 1, J, SM>(c, P);
     }
-    l4_many_run<DT, MT, 4, J, SM>(c, P);
+    if (l4_blocks(P, 16 * MT, 2) <= c->cus) l4_many_run<DT, MT, 2, J, SM>(c, P);
+    else l4_many_run<DT, MT, 4, J, SM>(c, P);
 }
 template <int DT, int J, int SM>
 static void l4_run(Ctx* c, const L4Args& P) {
     if constexpr (DT == H3S_F32) {
+        // (three parts: x's stages of 32 rows and more than two groups do not fit LDS, those of 16 rows do: 32 rows 5376 -> 5376 56 to 26 us, 14336 -> 5376 140 to 58)
         if (P.M <= 16) l4_few<DT, J, SM>(c, P);
-        else l4_many<DT, 2, J, SM>(c, P);
+        else if (l4_blocks(P, 16, 2) <= c->cus) l4_many_run<DT, 1, 2, J, SM>(c, P);
+        else l4_many_run<DT, 2, 4, J, SM>(c, P);
     } else {
         // Up to 16 rows as one operand, unless x's operands do not fit the wavefronts' registers there and few columns leave the inputs to
         // split (14336 -> 5376: 16 rows 41 us, in tiles of 32 rows 33). Tiles of 32 rows up to 32 rows, and beyond while the device runs

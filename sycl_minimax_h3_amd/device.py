@@ -162,7 +162,7 @@ class Tensor:
         self.dtype, self.shape, self._ptr, self._owner, self.dev = dtype, list(shape), ptr, owner, dev
 
     def elements(self) -> int:
-        return int(math.prod(self.shape))
+        return math.prod(map(int, self.shape))
 
     def nbytes(self) -> int:
         return self.elements() * self.dtype.size()

@@ -600,6 +600,7 @@ LINEAR4_LONG = [
     (32, 2048, 8200, 128, False, "BF16", "BF16", "F32", False),                 # 65: in 130 of 64
     (100, 640, 17000, 64, True, "BF16", "BF16", "F16", True),                   # 266: as they are
     (33, 1024, 5000, 64, False, "F32", "F32", "F16", True),
+    (27, 5376, 5300, 32, True, "F32", "F32", "F16", True),                      # in 166 blocks of 16 rows x 64 columns
 ]
 
 

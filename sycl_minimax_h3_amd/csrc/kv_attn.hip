@@ -14,10 +14,10 @@ namespace h3 {
 // 32 rows of its own: where blocks of 128 rows still give each CU one and less than a quarter of their rows is none, and never for float32
 // queries, whose two halves leave room for one wavefront a SIMD only (2048 tokens over 4096, 64 heads over 8 of 128: 16-bit 265 us
 // with 32 rows, 356 with 16; float32 588 and 460; 64 sequences of 72 rows over 2048 tokens: 86 and 75).
-// Parts: of the same number of cache blocks for every sequence (at least eight, or four of a prompt's), as many as give each CU the two blocks of threads that
-// it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up to 8192 tokens, 64
-// heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and their merge 4, 7
-// and 11 us more.)
+// Parts: of the same number of cache blocks for every sequence (at least eight, or four of a prompt's), as many as give each CU the two
+// blocks of threads that it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up
+// to 8192 tokens, 64 heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and
+// their merge 4, 7 and 11 us more.)
 static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
     KvPlan plan;
     const int64_t rows = std::min<int64_t>(most, P.rows) * group, each = (int64_t) P.seqs * P.heads;

@@ -99,7 +99,8 @@ constexpr int kKvRow = kKvB / 4 + 1;      // words of a feature's 64 tokens in L
 // One block of threads: one cache block of one head, keys (side 0) or values (side 1). Thread t holds the pieces t + 256 p, p < WC, of
 // four tokens x four features, W / 4 pieces side by side: its loads of the rows and its stores of keys are whole runs of them, and a
 // piece's codes are four words either way round. Values go through LDS into a feature's tokens. Bound by latency for single tokens (the
-// sequence's place, the rows, a maximum over the block, one store: 5 us) and by the rows' bytes for prompts.
+// sequence's place, the rows, a maximum over the block, one store: 4.5 us; 64 sequences' 7.8) and by the rows' bytes for prompts (four of
+// 5734 tokens in all 12.8 us).
 template <int WC>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs A) {
     constexpr int W = 64 * WC;
@@ -217,7 +218,8 @@ struct KvReadArgs {
     int k_vec, v_vec;
 };
 
-// One block of threads: the tokens that a read takes out of one cache block of one head and side (pieces as in kv_write_kernel).
+// One block of threads: the tokens that a read takes out of one cache block of one head and side (pieces as in kv_write_kernel). Bound as
+// there: one token 4.9 us, the four prompts 10.4.
 template <int WC>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs A) {
     constexpr int W = 64 * WC;

@@ -16,9 +16,13 @@
 //
 // Work. One row (linear4_dot_kernel): the codes as above, multiplied by pairs on the vector units, with x in registers.
 // Two to 16 rows (linear4_few_kernel): a wavefront takes 16 NT columns and every KW-th 128 inputs; the KW wavefronts of a block
-// are joined through LDS in wavefront order. Bound by the codes' bytes: everything that a step needs is loaded a step ahead.
+// are joined through LDS in wavefront order. Bound by the codes' bytes: everything that a step needs is loaded a step ahead
+// (16 rows, 28672 columns of 5376: 26.5 us, 3.1 TB/s).
 // More rows (linear4_many_kernel): a block takes 16 MT rows x 128 columns (64 or 32 where that leaves CUs idle), in two groups of four
-// wavefronts (four of two, eight of one) that take every other (fourth, eighth) 128 inputs; x goes through LDS, in the order of the instructions' operands, and each wavefront has 32 columns.
+// wavefronts (four of two, eight of one) that take every other (fourth, eighth) 128 inputs; x goes through LDS, in the order of the
+// instructions' operands, and each wavefront has 32 columns. Bound by vector instructions beside the products (300 rows 14336 -> 5376,
+// groups of 32: 126-138 us, 0.34-0.37 PFLOP/s: a multiply-add for each register of a product, the codes, and 24 more product
+// instructions beside each 32, for the sums of x and the minima).
 #pragma once
 
 #include "kv.h"
@@ -200,7 +204,9 @@ constexpr int kL4DotWaves = 11;       // wavefronts of a block, at most
 // walks down the rows: 16 lanes take a row's chunk, 32 codes each, four rows at a time. So its loads are runs of 256 bytes, the scale of a
 // lane's codes is one 2-byte load beside its neighbours', and no operand goes through LDS. (As matrix instructions' operands - 16
 // rows a load, 64 bytes of each, a scale gathered from 16 rows - the same loads alone took 94 us where the codes come in 62.) Per tile of
-// 16 rows the wavefronts' sums are joined through LDS, in wavefront order; the loads go on across tiles, DP row steps ahead.
+// 16 rows the wavefronts' sums are joined through LDS, in wavefront order; the loads go on across tiles, DP row steps ahead. Bound by the
+// codes' bytes: 131072 columns of 5376 67-72 us by the card, 5.0-5.4 TB/s. (One row of x only: with two 28672 columns took 32 us, with
+// four 43, where linear4_few_kernel takes 24.)
 template <int DT, int U, bool MINS>
 __global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P) {
     constexpr int OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS, DP = U == 1 ? 4 : U == 2 ? 3 : 2;
@@ -700,7 +706,8 @@ static void l4_many(Ctx* c, const L4Args& P) {
 template <int DT, int J, int SM>
 static void l4_run(Ctx* c, const L4Args& P) {
     if constexpr (DT == H3S_F32) {
-        // (three parts: x's stages of 32 rows and more than two groups do not fit LDS, those of 16 rows do: 32 rows 5376 -> 5376 56 to 26 us, 14336 -> 5376 140 to 58)
+        // (three parts: x's stages of 32 rows and more than two groups do not fit LDS, those of 16 rows do: 32 rows 5376 -> 5376 56 to
+        // 26 us, 14336 -> 5376 140 to 58)
         if (P.M <= 16) l4_few<DT, J, SM>(c, P);
         else if (l4_blocks(P, 16, 2) <= c->cus) l4_many_run<DT, 1, 2, J, SM>(c, P);
         else l4_many_run<DT, 2, 4, J, SM>(c, P);

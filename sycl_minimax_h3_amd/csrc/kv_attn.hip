@@ -17,7 +17,7 @@ namespace h3 {
 // Parts: of the same number of cache blocks for every sequence (at least eight, or four of a prompt's), as many as give each CU the two
 // blocks of threads that it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up
 // to 8192 tokens, 64 heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and
-// their merge 4, 7 and 11 us more.)
+// their merge 4, 7 and 11 us more. Longer parts: one sequence of 2000 tokens in parts of 8, 16 and 32 blocks 12.6, 15.5 and 18.5 us.)
 static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
     KvPlan plan;
     const int64_t rows = std::min<int64_t>(most, P.rows) * group, each = (int64_t) P.seqs * P.heads;

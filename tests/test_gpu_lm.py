@@ -187,6 +187,11 @@ ATTN_ROWS = [
     ([(97, 300), (20, 500)], 3, 1, 64, "BF16", "BF16", {"lse": True}),
     ([(96, 96)], 3, 1, 64, "F16", "BF16", {"window": 40}),
     ([(150, 190), (1, 70)], 2, 2, 128, "F32", "F32", {"lse": True, "mask": 0.9}),
+    # short caches beside none
+    ([(1, 1000), (2, 321), (0, 9), (1, 0)], 2, 8, 128, "BF16", "BF16", {"lse": True}),
+    ([(1, 700), (1, 1)], 3, 12, 64, "F32", "F32", {"lse": True, "mask": 0.5}),
+    ([(3, 500)], 2, 5, 75, "F16", "F16", {"window": 130}),
+    ([(1, 900)], 1, 1, 128, "F32", "F32", {"max_len": 300}),                    # longer than said
 ]
 
 

@@ -245,19 +245,22 @@ template <int WC, int NQ, bool TWO> struct KvRows {
         }
     }
 
-    // O^T += v_scale V^T P^T for the feature tile t, whose codes of the keys 8 .. of each 16 are a1
-    __device__ __forceinline__ void values(int t, const v8h_kv& a0, const v8h_kv& a1, const v8h_kv (&pf)[NQ][2][PARTS], const float (&vsl)[NQ]) {
+    // V^T P^T of a feature tile, whose codes of the keys 8 .. of each 16 are a1
+    __device__ __forceinline__ void products(const v8h_kv& a0, const v8h_kv& a1, const v8h_kv (&pf)[NQ][2][PARTS], v4f_kv (&y)[NQ]) const {
 #pragma unroll
-        for (int e = 0; e < NQ; ++e) {
-            v4f_kv y = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < PARTS; ++w) {
 #pragma unroll
-            for (int w = 0; w < PARTS; ++w) {
-                y = kv_mma(a0, pf[e][0][w], y);
-                y = kv_mma(a1, pf[e][1][w], y);
-            }
+            for (int e = 0; e < NQ; ++e) y[e] = kv_mma(a0, pf[e][0][w], w ? y[e] : v4f_kv{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[e][t][i] = __builtin_fmaf(y[i], vsl[e], o[e][t][i]);
+            for (int e = 0; e < NQ; ++e) y[e] = kv_mma(a1, pf[e][1][w], y[e]);
         }
+    }
+    // O^T += v_scale of it, for the feature tile t
+    __device__ __forceinline__ void add(int t, const v4f_kv (&y)[NQ], const float (&vsl)[NQ]) {
+#pragma unroll
+        for (int e = 0; e < NQ; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[e][t][i] = __builtin_fmaf(y[e][i], vsl[e], o[e][t][i]);
     }
 };
 
@@ -397,8 +400,11 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
         float vsl[NQ];
         q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-            q.values(t, kv_half8(vr[t].x, vr[t].y), kv_half8(vr[t].z, vr[t].w), pf, vsl);
+        for (int t = 0; t < DT; ++t) {
+            v4f_kv y[NQ];
+            q.products(kv_half8(vr[t].x, vr[t].y), kv_half8(vr[t].z, vr[t].w), pf, y);
+            q.add(t, y, vsl);
+        }
         if (more) load_v(npage);
         kb = nkb;
     }
@@ -458,9 +464,10 @@ template <int WC> __device__ __forceinline__ int kv_mix(int g, int c) { return (
 // Many rows: each of a block's four wavefronts has 16 NQ rows of its own, and all go through the same cache blocks. A block's codes
 // are turned to half once, by all four, into LDS in the order of the products' operands (two stages, one barrier a cache block), where
 // doing it in every wavefront took more vector instructions than the softmax. Bound by vector instructions beside the products (4096 tokens
-// over 8192, 64 heads over 8 of 128: 960-1080 us by the card, 0.77-0.86 PFLOP/s, the matrix cores 34 % busy).
+// over 8192, 64 heads over 8 of 128: 940-1060 us by the card, 0.78-0.87 PFLOP/s, the matrix cores 35 % busy). Operands are read from LDS a
+// step ahead of their products (960 us without, 16 sequences of 100 tokens of 256 features 203 to 181).
 template <int WC, int NQ, bool TWO>
-__global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs P) {
+__global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC, DT = 4 * WC, RT = 64 * NQ, PARTS = TWO ? 2 : 1;
     __shared__ v8h_kv sk[2][4][WC][2][64], sv[2][DT][2][64];              // [stage][key tile or feature tile][...][half][lane]
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
@@ -528,28 +535,47 @@ __global__ __launch_bounds__(256, WC <= 2 && !TWO ? 2 : 1) void kv_attn_rows_ker
     while (kb < last) {
         const int key0 = kb * kKvB;
         if (key0 <= posmax) {
+            // a feature chunk's operands of all four key tiles are read while the one before is multiplied: four tiles' sums in turn
+            // leave no product waiting for the last
             v4f_kv s[NQ][4];
+            v8h_kv a[2][4];
+            auto keys = [&](int i) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+                for (int t = 0; t < 4; ++t) a[i & 1][t] = sk[st][t][i / 2][i % 2][16 * g + (l15 ^ kv_mix<WC>(g, i / 2))];
+            };
+            keys(0);
 #pragma unroll
-                for (int e = 0; e < NQ; ++e) s[e][t] = v4f_kv{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < 2 * WC; ++i) {
+                if (i + 1 < 2 * WC) keys(i + 1);
 #pragma unroll
-                for (int c = 0; c < WC; ++c)
+                for (int w = 0; w < PARTS; ++w)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const v8h_kv a = sk[st][t][c][u][16 * g + (l15 ^ kv_mix<WC>(g, c))];
+                    for (int t = 0; t < 4; ++t)
 #pragma unroll
                         for (int e = 0; e < NQ; ++e)
-#pragma unroll
-                            for (int w = 0; w < PARTS; ++w) s[e][t] = kv_mma(a, q.qf[e][c][u][w], s[e][t]);
-                    }
+                            s[e][t] = kv_mma(a[i & 1][t], q.qf[e][i / 2][i % 2][w], i + w ? s[e][t] : v4f_kv{0.0f, 0.0f, 0.0f, 0.0f});
+                __builtin_amdgcn_sched_barrier(0);
             }
             const bool whole = key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window) && !P.mask;
             v8h_kv pf[NQ][2][PARTS];
             float vsl[NQ];
             q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
+            // likewise a feature tile's operands, and the sums of the tile before are added to o meanwhile
+            v8h_kv x[2][2];
+            auto feats = [&](int t) {
+                x[t & 1][0] = sv[st][t][0][16 * g + (l15 ^ (4 * g))];
+                x[t & 1][1] = sv[st][t][1][16 * g + (l15 ^ (4 * g))];
+            };
+            v4f_kv y[2][NQ];
+            feats(0);
 #pragma unroll
-            for (int t = 0; t < DT; ++t) q.values(t, sv[st][t][0][16 * g + (l15 ^ (4 * g))], sv[st][t][1][16 * g + (l15 ^ (4 * g))], pf, vsl);
+            for (int t = 0; t < DT; ++t) {
+                if (t + 1 < DT) feats(t + 1);
+                q.products(x[t & 1][0], x[t & 1][1], pf, y[t & 1]);
+                if (t) q.add(t - 1, y[(t & 1) ^ 1], vsl);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            q.add(DT - 1, y[(DT - 1) & 1], vsl);
         }
         // the next block's codes, loaded a block ago, to the other stage, and the loads of the one after
         if (more) {

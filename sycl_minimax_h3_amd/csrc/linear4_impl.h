@@ -21,7 +21,7 @@
 // More rows (linear4_many_kernel): a block takes 16 MT rows x 128 columns (64 or 32 where that leaves CUs idle), in two groups of four
 // wavefronts (four of two, eight of one) that take every other (fourth, eighth) 128 inputs; x goes through LDS, in the order of the
 // instructions' operands, and each wavefront has 32 columns. Bound by vector instructions beside the products (300 rows 14336 -> 5376,
-// groups of 32: 126-138 us, 0.34-0.37 PFLOP/s: a multiply-add for each register of a product, the codes, and 24 more product
+// groups of 32: 119-130 us, 0.36-0.39 PFLOP/s: a multiply-add for each register of a product, the codes, and 24 more product
 // instructions beside each 32, for the sums of x and the minima).
 #pragma once
 
@@ -118,14 +118,19 @@ __device__ __forceinline__ void l4_exchange(const uint4& w, uint32_t (&c)[4]) {
 }
 
 // The products of one step of 128 inputs: NT columns' codes and scales against MT x 16 rows. frag(a, j, f): the operand of the rows
-// 16 a .. and the run j (zeros past the row's end). Rows: place l of an operand is row 4 (l % 4) + l / 4, so that register i of lane
+// 16 a .. and the run j (zeros past the row's end); AHEAD: a run's operands are asked for before the products of the one
+// before (from LDS: 300 rows 5376 -> 28672 247 to 211 us, 14336 -> 5376 127 to 120). Rows: place l of an operand is row 4 (l % 4) + l / 4, so that register i of lane
 // group g sums row 4 i + g and up to four rows take one multiply-add (NI of them).
-template <int OP, int PARTS, int MT, int NT, int NI, int J, typename F>
+template <bool AHEAD, int OP, int PARTS, int MT, int NT, int NI, int J, typename F>
 __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, uint32_t e, const uint32_t (&c)[NT][4], const float (&sc)[NT][4 / J], const float (&off)[NT],
                                             F frag, v4f_l4 (&acc)[MT][NT]) {
     v4f_l4 sx[MT];
+    uint4 x[2][MT][PARTS];
 #pragma unroll
-    for (int a = 0; a < MT; ++a) sx[a] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int a = 0; a < MT; ++a) {
+        sx[a] = v4f_l4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (AHEAD) frag(a, 0, x[0][a]);
+    }
 #pragma unroll
     for (int q = 0; q < 4 / J; ++q) {
         v4f_l4 y[MT][NT];
@@ -138,10 +143,14 @@ __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, u
             uint4 f[NT];
 #pragma unroll
             for (int b = 0; b < NT; ++b) f[b] = l4_codes<OP>(c[b][j], m, e);
+            if (AHEAD && j < 3) {
+#pragma unroll
+                for (int a = 0; a < MT; ++a) frag(a, j + 1, x[(j & 1) ^ 1][a]);
+            }
 #pragma unroll
             for (int a = 0; a < MT; ++a) {
-                uint4 xf[PARTS];
-                frag(a, j, xf);
+                uint4 (&xf)[PARTS] = x[AHEAD ? j & 1 : 0][a];
+                if (!AHEAD) frag(a, j, xf);
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) {
                     sx[a] = l4_mma<OP>(sel[j], xf[p], sx[a]);
@@ -149,6 +158,7 @@ __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, u
                     for (int b = 0; b < NT; ++b) y[a][b] = l4_mma<OP>(xf[p], f[b], y[a][b]);
                 }
             }
+            if (AHEAD) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int a = 0; a < MT; ++a)
@@ -497,7 +507,7 @@ __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P,
             if (r + DP < 4) load_w(here, step + DP, w[r % DP]);
             else load_w(then, nfirst + r + DP - 4, w[r % DP]);
             if (step < steps) {
-                l4_products<OP, PARTS, 1, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
+                l4_products<false, OP, PARTS, 1, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
                     if constexpr (XR && DT != H3S_F32) f[0] = xr[r][j].u;
                     else xr[XR ? r : 0][j].parts(f);
                 }, acc);
@@ -634,7 +644,7 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
                     }
                 }
                 load_w(min(step + KG, steps - 1));
-                l4_products<OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
+                l4_products<PARTS == 1, OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][r & 1][a][j][q][lane ^ g];
                 }, acc);
@@ -694,7 +704,7 @@ static void l4_many_run(Ctx* c, const L4Args& P) {
     linear4_many_kernel<DT, MT, CG, J, SM><<<(unsigned) l4_blocks(P, 16 * MT, CG), 512, 0, c->stream>>>(P);
 }
 // Half as many columns a block, and twice the groups along the inputs, while the blocks still run at once (as far as x's stages fit LDS):
-// 5376 -> 5376, 32 rows 38 to 18 us, 128 rows 52 to 34; 14336 -> 5376, 32 rows 92 to 34 us, 128 rows 126 to 75.
+// 5376 -> 5376, 32 rows 38 to 18 us, 128 rows 52 to 34; 14336 -> 5376, 32 rows 92 to 33 us, 128 rows 126 to 72.
 template <int DT, int MT, int J, int SM>
 static void l4_many(Ctx* c, const L4Args& P) {
     if constexpr (MT == 2) {
@@ -713,8 +723,8 @@ static void l4_run(Ctx* c, const L4Args& P) {
         else l4_many_run<DT, 2, 4, J, SM>(c, P);
     } else {
         // Up to 16 rows as one operand, unless x's operands do not fit the wavefronts' registers there and few columns leave the inputs to
-        // split (14336 -> 5376: 16 rows 41 us, in tiles of 32 rows 33). Tiles of 32 rows up to 32 rows, and beyond while the device runs
-        // all blocks of 64 columns of them at once (64 rows: 5376 -> 5376 34 to 25 us, 14336 -> 5376 75 to 55).
+        // split (14336 -> 5376: 16 rows 41 us, in tiles of 32 rows 32). Tiles of 32 rows up to 32 rows, and beyond while the device runs
+        // all blocks of 64 columns of them at once (64 rows: 5376 -> 5376 34 to 22 us, 14336 -> 5376 75 to 47).
         if (P.M <= 4 || (P.M <= 16 && (P.K <= 512 * kL4FewWaves || l4_blocks(P, 32, 1) > c->cus))) l4_few<DT, J, SM>(c, P);
         else if (P.M <= 32 || l4_blocks(P, 32, 2) <= c->cus) l4_many<DT, 2, J, SM>(c, P);
         else l4_many<DT, 4, J, SM>(c, P);

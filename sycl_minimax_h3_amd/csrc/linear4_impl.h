@@ -119,8 +119,8 @@ __device__ __forceinline__ void l4_exchange(const uint4& w, uint32_t (&c)[4]) {
 
 // The products of one step of 128 inputs: NT columns' codes and scales against MT x 16 rows. frag(a, j, f): the operand of the rows
 // 16 a .. and the run j (zeros past the row's end); AHEAD: a run's operands are asked for before the products of the one
-// before (from LDS: 300 rows 5376 -> 28672 247 to 211 us, 14336 -> 5376 127 to 120). Rows: place l of an operand is row 4 (l % 4) + l / 4, so that register i of lane
-// group g sums row 4 i + g and up to four rows take one multiply-add (NI of them).
+// before (from LDS: 300 rows 5376 -> 28672 247 to 211 us, 14336 -> 5376 127 to 120). Rows: place l of an operand is row 4 (l % 4) + l / 4,
+// so that register i of lane group g sums row 4 i + g and up to four rows take one multiply-add (NI of them).
 template <bool AHEAD, int OP, int PARTS, int MT, int NT, int NI, int J, typename F>
 __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, uint32_t e, const uint32_t (&c)[NT][4], const float (&sc)[NT][4 / J], const float (&off)[NT],
                                             F frag, v4f_l4 (&acc)[MT][NT]) {

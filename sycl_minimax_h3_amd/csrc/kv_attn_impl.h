@@ -1,7 +1,7 @@
 // kv_attn_impl.h - the attention over the 8-bit key/value cache (h3lm.h, kv_attention).
 //
 // Mathematics, for one query row with scores s_j = q . k_j * scale over the tokens j it sees: p_j = 2^(s_j log2(e) - m), m the
-// running maximum, l = sum p_j, o = sum p_j v_j / l, in one pass over the cache: where a block raises m, l and o are
+// running maximum (less 15, kKvShift), l = sum p_j, o = sum p_j v_j / l, in one pass over the cache: where a block raises m, l and o are
 // multiplied by 2^(m_old - m). Keys are codes times a block's scale, so s = (q . codes) * (k_scale * scale * log2 e): one factor a
 // block. Values likewise: a block's sum of p_j codes_j is added to o with v_scale as the factor.
 //
@@ -33,7 +33,10 @@ typedef float v4f_kv __attribute__((ext_vector_type(4)));
 
 // where m starts: below every score, and finite, so that m_old - m is never infinity minus infinity
 constexpr float kKvUnset = -3e38f;
-constexpr float kKvShift = 15.0f;                   // probabilities are held times 2^15
+// Probabilities are held times 2^15: m is 15 below the running maximum. Where a block's largest score is 2^19 or more from zero (its steps
+// 2^-4 and more) m is that score itself, and scores are rounded before m is taken off: the fused difference would be off by half a step of
+// the score, past what half holds above 2^15 from 2^23 on, and without bound beyond.
+constexpr float kKvShift = 15.0f, kKvFar = 524288.0f;
 
 struct KvAttnArgs {
     KvArgs kv;
@@ -97,9 +100,9 @@ __device__ __forceinline__ void kv_store4(const KvAttnArgs& P, int64_t at, int d
             if (d + i < dim) store_any(P.out, P.out_dt, at + d + i, f[i]);
     }
 }
-// the logarithm of the row's sum of exponentials from the maximum (base 2) and the sum times 2^15
+// the logarithm of the row's sum of exponentials from m and the sum of 2^(score - m)
 __device__ __forceinline__ float kv_lse(float m, float l) {
-    return l > 0.0f ? (m + (__builtin_log2f(l) - kKvShift)) * 0.69314718055994531f : l == 0.0f ? -__builtin_inff() : l;
+    return l > 0.0f ? (m + __builtin_log2f(l)) * 0.69314718055994531f : l == 0.0f ? -__builtin_inff() : l;
 }
 
 // What a wavefront holds of its 16 NQ query rows: row lane % 16 of each tile
@@ -220,7 +223,19 @@ template <int WC, int NQ, bool TWO> struct KvRows {
             f = f < 1e-37f ? 1e-37f : f;
             f = seen ? f : 1.0f;
             vsl[e] = seen ? vs : 0.0f;
-            const float mn = fmaxf(m[e], top * f);
+            const float big = top * f;
+            const bool far = seen && fabsf(big) >= kKvFar;
+            float from = big - kKvShift;
+            if (__builtin_expect(__any(far), 0)) {
+                from = far ? big : from;
+                const float once = far ? f : 1.0f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[e][t][i] *= once;
+                f = far ? 1.0f : f;
+            }
+            const float mn = fmaxf(m[e], from);
             if (__any(mn > m[e])) {
                 const float alpha = __builtin_amdgcn_exp2f(m[e] - mn);
                 l[e] *= alpha;
@@ -228,13 +243,12 @@ template <int WC, int NQ, bool TWO> struct KvRows {
                 for (int t = 0; t < DT; ++t) o[e][t] *= alpha;
                 m[e] = mn;
             }
-            const float ref = kKvShift - m[e];
             float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e][t][i], f, ref));
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e][t][i], f, -m[e]));
                     sum += p;
                     const int at = 4 * (t & 1) + i;
                     const _Float16 hi = (_Float16) p;

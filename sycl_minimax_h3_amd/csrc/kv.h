@@ -26,6 +26,31 @@ __device__ __forceinline__ void kv_rows_of(const KvArgs& P, int b, int& r0, int&
     n = min(max(e, r0), P.rows) - r0;
 }
 
+// The blocks of 256 threads that one launch takes: a launch of 2^32 threads or more is cut without an error.
+constexpr int64_t kKvMostBlocks = 0xffffff;
+
+// Work laid out by the rows there are, for batches where `most` rows of every sequence would be far more: sequence b's items begin at
+// floor(start * num / den) + each * b, and the last sequence that begins at or before item `at` has it. Found by the whole wavefront, 64
+// sequences at a time (up to 63 sequences: one load, which the rows need anyway). Returns the item's number in its sequence b,
+// whose rows are [r0, r0 + n); below 0 where the item is nobody's (rows before the first sequence). Whatever `starts` says, b is a
+// sequence and the rows are within the call's.
+__device__ __forceinline__ int kv_find(const KvArgs& P, int at, uint32_t num, uint32_t den, int each, int& b, int& r0, int& n) {
+    const int lane = threadIdx.x & 63;
+    int step = 1;                                                           // (fewer sequences than kKvMostBlocks: 64 step is an int)
+    while (step * 64 < P.seqs) step *= 64;
+    for (b = 0;; step /= 64) {
+        const int c = b + lane * step;
+        const int s = min(max(P.starts[min(c, P.seqs)], 0), P.rows);
+        const int first = (int) ((uint32_t) s * num / den) + each * min(c, P.seqs);
+        const int k = (int) __popcll(__ballot(c < P.seqs && first <= at) & ~1ull);   // (lane 0 is where none is)
+        b += k * step;
+        if (step > 1) continue;
+        r0 = __builtin_amdgcn_readlane(s, k);
+        n = min(max(k < 63 ? __builtin_amdgcn_readlane(s, k + 1) : P.starts[b + 1], r0), P.rows) - r0;
+        return at - __builtin_amdgcn_readlane(first, k);
+    }
+}
+
 // checks cache and batch and fills P: 0, or -1 with the reason
 int kv_args(const std::string& fn, const h3_kv_cache* cache, const h3_kv_batch* batch, KvArgs& P);
 

@@ -88,11 +88,31 @@ struct KvWriteArgs {
     const int32_t* past;
     const void *xk, *xv;
     int64_t k_stride, v_stride;
-    int dt, nb;              // nb: blocks a sequence may touch
+    int dt, nb;              // nb: blocks a sequence may touch (0: laid out by the rows, see kv_place)
     int k_vec, v_vec;        // rows four elements at a time
 };
 // (Chosen between, never indexed by the side: an index into the kernel's arguments became a scalar load whose base and offset
 // were no multiples of 4 by themselves, and scalar loads drop the two low bits of each.)
+
+// A block of threads: one head and side of the i-th cache block that sequence b's rows [r0, r0 + n) lie in. Where sequences have about
+// as many rows each, a sequence has nb of them; else its share of the rows: n rows lie in at most floor(n / 64) + 2 blocks.
+struct KvPlace { int side, h, i, b, r0, n; };
+__device__ __forceinline__ KvPlace kv_place(const KvArgs& P, int nb) {
+    KvPlace o;
+    uint32_t id = blockIdx.x;
+    o.side = (int) (id & 1);
+    id >>= 1;
+    o.h = (int) (id % (uint32_t) P.heads);
+    id /= (uint32_t) P.heads;
+    if (nb) {
+        o.i = (int) (id % (uint32_t) nb);
+        o.b = (int) (id / (uint32_t) nb);
+        kv_rows_of(P, o.b, o.r0, o.n);
+    } else {
+        o.i = kv_find(P, (int) id, 1, kKvB, 2, o.b, o.r0, o.n);
+    }
+    return o;
+}
 
 constexpr int kKvRow = kKvB / 4 + 1;      // words of a feature's 64 tokens in LDS, one more than they are (banks)
 
@@ -106,17 +126,10 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvWriteArgs A) {
     constexpr int W = 64 * WC;
     const KvArgs& P = A.kv;
     __shared__ uint32_t codes[W * kKvRow];
-    int64_t id = blockIdx.x;
-    const int side = (int) (id & 1);
-    id >>= 1;
-    const int h = (int) (id % P.heads);
-    id /= P.heads;
-    const int i = (int) (id % A.nb), b = (int) (id / A.nb);
-    int r0, n;
-    kv_rows_of(P, b, r0, n);
+    const auto [side, h, i, b, r0, n] = kv_place(P, A.nb);
     const int64_t past = max(A.past[b], 0), end = min(past + n, (int64_t) P.width * kKvB);
     const int64_t j = past / kKvB + i;                                      // the sequence's block
-    if (end <= past || j * kKvB >= end) return;                             // (no new token: the block is not touched)
+    if (i < 0 || end <= past || j * kKvB >= end) return;                    // (no new token: the block is not touched)
     const int page = P.table[(int64_t) b * P.width + j];
     const int kept = (int) max(past - j * kKvB, (int64_t) 0);               // its tokens [0, kept) were there
     const int last = (int) min(end - j * kKvB, (int64_t) kKvB);             // and [kept, last) are new
@@ -225,17 +238,10 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs A) {
     constexpr int W = 64 * WC;
     const KvArgs& P = A.kv;
     __shared__ uint32_t codes[W * kKvRow];
-    int64_t id = blockIdx.x;
-    const int side = (int) (id & 1);
-    id >>= 1;
-    const int h = (int) (id % P.heads);
-    id /= P.heads;
-    const int i = (int) (id % A.nb), b = (int) (id / A.nb);
-    int r0, n;
-    kv_rows_of(P, b, r0, n);
+    const auto [side, h, i, b, r0, n] = kv_place(P, A.nb);
     const int64_t first = max(A.first[b], 0), end = first + n;
     const int64_t j = first / kKvB + i;
-    if (j * kKvB >= end) return;
+    if (i < 0 || j * kKvB >= end) return;
     const int page = j < P.width ? P.table[(int64_t) b * P.width + j] : -1;
     const bool there = page >= 0 && page < P.blocks;
     const int from = (int) max(first - j * kKvB, (int64_t) 0), to = (int) min(end - j * kKvB, (int64_t) kKvB);
@@ -282,15 +288,19 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvReadArgs A) {
     }
 }
 
-// what kv_write and kv_read check alike; nb: the blocks that `most` rows of a sequence can lie in
+// what kv_write and kv_read check alike, and their grid: `most` rows of a sequence can lie in nb blocks, all rows in rows / 64 + 2 seqs
+// (one sequence of 16400 rows among 1024 of one: 1281 cache blocks in 2304 places instead of 263168)
 static int row_checks(const std::string& fn, const KvArgs& P, const h3_kv_batch& q, const int32_t* at, const char* at_name, const void* k,
-                      int64_t k_stride, const void* v, int64_t v_stride, int dt, int64_t* nb) {
+                      int64_t k_stride, const void* v, int64_t v_stride, int dt, int* nb, unsigned* grid) {
     const int64_t feats = (int64_t) P.heads * P.dim;
     if (!dt_ok(dt)) return fail(fn + ": unknown element type");
     if (!at || !k || !v) return fail(fn + ": k, v and " + at_name + " are required");
     if (k_stride < feats || v_stride < feats) return fail(fn + ": a row stride is shorter than a row");
-    *nb = (std::min<int64_t>(q.most, P.rows) + kKvB - 2) / kKvB + 1;
-    if (*nb * P.seqs > 0x7fffffff / 2 / P.heads) return fail(fn + ": too many blocks of work");
+    const int64_t each = (std::min<int64_t>(q.most, P.rows) + kKvB - 2) / kKvB + 1, all = P.rows / kKvB + 2 * (int64_t) P.seqs;
+    *nb = each * P.seqs <= all ? (int) each : 0;
+    const int64_t places = *nb ? each * P.seqs : all;
+    if (places > kKvMostBlocks / 2 / P.heads) return fail(fn + ": too many blocks of work");
+    *grid = (unsigned) (places * P.heads * 2);
     return 0;
 }
 // whether rows of k or v can be taken four elements at a time
@@ -305,17 +315,16 @@ int kv_write(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, cons
     KvWriteArgs A;
     if (kv_args(fn, cache, batch, A.kv)) return -1;
     if (A.kv.seqs == 0 || A.kv.rows == 0 || batch->most == 0 || A.kv.width == 0) return 0;
-    int64_t nb;
-    if (row_checks(fn, A.kv, *batch, past, "past", k, k_stride, v, v_stride, dt, &nb)) return -1;
+    unsigned grid;
+    if (row_checks(fn, A.kv, *batch, past, "past", k, k_stride, v, v_stride, dt, &A.nb, &grid)) return -1;
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
     A.past = past;
     A.xk = k; A.xv = v;
     A.k_stride = k_stride; A.v_stride = v_stride;
-    A.dt = dt; A.nb = (int) nb;
+    A.dt = dt;
     A.k_vec = rows_vec(k, k_stride, A.kv.dim, dt);
     A.v_vec = rows_vec(v, v_stride, A.kv.dim, dt);
-    const unsigned grid = (unsigned) (nb * A.kv.seqs * A.kv.heads * 2);
     switch (kv_width(A.kv.dim) / 64) {
         case 1: kv_write_kernel<1><<<grid, 256, 0, c->stream>>>(A); break;
         case 2: kv_write_kernel<2><<<grid, 256, 0, c->stream>>>(A); break;
@@ -331,17 +340,16 @@ int kv_read(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const
     KvReadArgs A;
     if (kv_args(fn, cache, batch, A.kv)) return -1;
     if (A.kv.seqs == 0 || A.kv.rows == 0 || batch->most == 0) return 0;
-    int64_t nb;
-    if (row_checks(fn, A.kv, *batch, first, "first", k, k_stride, v, v_stride, dt, &nb)) return -1;
+    unsigned grid;
+    if (row_checks(fn, A.kv, *batch, first, "first", k, k_stride, v, v_stride, dt, &A.nb, &grid)) return -1;
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
     A.first = first;
     A.xk = k; A.xv = v;
     A.k_stride = k_stride; A.v_stride = v_stride;
-    A.dt = dt; A.nb = (int) nb;
+    A.dt = dt;
     A.k_vec = rows_vec(k, k_stride, A.kv.dim, dt);
     A.v_vec = rows_vec(v, v_stride, A.kv.dim, dt);
-    const unsigned grid = (unsigned) (nb * A.kv.seqs * A.kv.heads * 2);
     switch (kv_width(A.kv.dim) / 64) {
         case 1: kv_read_kernel<1><<<grid, 256, 0, c->stream>>>(A); break;
         case 2: kv_read_kernel<2><<<grid, 256, 0, c->stream>>>(A); break;

@@ -1,11 +1,14 @@
-"""The 8-bit key/value cache and the attention over it at scores far from zero."""
+"""The 8-bit key/value cache and the attention over it at scores far from zero and for batches of one long sequence among many short ones."""
 import numpy as np
 import pytest
 
 import lm_reference as ref
-from test_gpu_lm import attn_case, run_attn
+from helpers import up
+from test_gpu_lm import attn_case, compare_cache, i32, run_attn, tables, upload
 
 pytestmark = pytest.mark.gpu
+
+from sycl_minimax_h3_amd import ops  # noqa: E402
 
 BLOCK = ref.BLOCK
 
@@ -46,3 +49,49 @@ def test_attention_scores_past_the_steps_of_float32(dev, seqs, dt, sign):
         assert (np.abs(out[at] - want) <= rel * np.abs(want)).all(), np.abs(out[at] - want).max()
         # float32 queries as two halves (2^-22) and some six roundings of the score (2^-24 each)
         assert (np.abs(lse[at] - score) <= 2.0 ** -20 * np.abs(score)).all()
+
+
+# ---- one long sequence among many short ones ------------------------------------------------------------------------------------
+
+def ragged(news, pasts, seed):
+    """The block table, the blocks of the pool and the starts of sequences with so many new tokens behind so many cached ones."""
+    g = np.random.default_rng(seed)
+    table, blocks = tables([(p + n + BLOCK - 1) // BLOCK for p, n in zip(pasts, news)], seed=seed)
+    starts = np.concatenate([[0], np.cumsum(news)])
+    return g, table, blocks, starts
+
+
+@pytest.mark.parametrize("heads,dim,seqs,long", [
+    (32, 8, 1024, 16400),        # 1024 times the longest would be more than a launch takes
+    (2, 64, 3, 700),
+    (1, 100, 64, 300),
+    (2, 192, 65, 300),           # more sequences than a wavefront has lanes
+    (1, 256, 130, 500),
+    (1, 16, 4100, 200),          # more than 64 times as many
+])
+def test_write_and_read_of_one_long_sequence_among_many(dev, heads, dim, seqs, long):
+    """The work is that of the rows there are, whichever sequences have them. Rows before the first sequence and behind the last stay."""
+    news, pasts = np.ones(seqs, int), np.arange(seqs) % 67
+    news[seqs // 2], news[seqs - 1] = long, 130
+    if seqs > 8:
+        news[3], news[4], news[6] = 0, 64, 65
+    g, table, blocks, starts = ragged(news, pasts, 83)
+    starts = starts + 200
+    cache = ref.Cache(blocks, heads, dim, 83)
+    rows = int(starts[-1]) + 2
+    val = g.standard_normal((rows, 2 * heads * dim)).astype(np.float32)
+    x = up(dev, val, "F32", [rows, 2 * heads * dim])
+    r = [ops.Rows(x, i * heads * dim, 2 * heads * dim, rows, heads, dim) for i in (0, 1)]
+    c, t, st = upload(dev, cache), i32(dev, table), i32(dev, starts)
+    ops.kv_write(c, t, r[0], r[1], st, i32(dev, pasts), long)
+    cache.write(table, starts, pasts, [val[:, i * heads * dim:(i + 1) * heads * dim].reshape(rows, heads, dim) for i in (0, 1)])
+    compare_cache(c, cache)
+    y = up(dev, np.full((rows, 2 * heads * dim), 77.0, np.float32), "F32", [rows, 2 * heads * dim])
+    o = [ops.Rows(y, i * heads * dim, 2 * heads * dim, rows, heads, dim) for i in (0, 1)]
+    ops.kv_read(c, t, st, i32(dev, pasts), long, o[0], o[1])
+    want = np.full((rows, 2 * heads * dim), 77.0, np.float32)
+    for b in range(seqs):
+        for i in (0, 1):
+            v, _ = cache.values(i, table[b], pasts[b] + np.arange(news[b]))
+            want[starts[b]:starts[b + 1], i * heads * dim:(i + 1) * heads * dim] = v.transpose(1, 0, 2).reshape(-1, heads * dim)
+    assert np.array_equal(y.to_numpy(), want)

@@ -10,6 +10,8 @@
  *     #include "h3lm.h"
  *     h3lm.kv_write(ctx, &cache, &batch, past, k, k_stride, v, v_stride, H3S_BF16);
  *
+ * A call whose work would take 2^32 threads of the device or more is refused ("too many blocks of work").
+ *
  * All of them can be recorded into a HIP graph (kv_attention with a workspace of the caller's, below). The values behind
  * device pointers - block tables, starts, lengths - are read on the device when the work runs, so a recorded graph is replayed
  * on new ones. No value there makes a kernel read or write outside its buffers: entries out of range are treated as stated.

@@ -14,18 +14,23 @@ namespace h3 {
 // 32 rows of its own: where blocks of 128 rows still give each CU one and less than a quarter of their rows is none, and never for float32
 // queries, whose two halves leave room for one wavefront a SIMD only (2048 tokens over 4096, 64 heads over 8 of 128: 16-bit 265 us
 // with 32 rows, 356 with 16; float32 588 and 460; 64 sequences of 72 rows over 2048 tokens: 86 and 75).
+// Places: a tile of rows each; as many as the rows of all sequences can lie in, where that is fewer than `most` rows of each take (one
+// prompt of 8192 tokens among 1024 sequences of a token, 8 heads a key/value head: 1599 instead of 524288).
 // Parts: of the same number of cache blocks for every sequence (at least eight, or four of a prompt's), as many as give each CU the two
 // blocks of threads that it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up
 // to 8192 tokens, 64 heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and
 // their merge 4, 7 and 11 us more. Longer parts: one sequence of 2000 tokens in parts of 8, 16 and 32 blocks 12.6, 15.5 and 18.5 us.)
 static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
     KvPlan plan;
-    const int64_t rows = std::min<int64_t>(most, P.rows) * group, each = (int64_t) P.seqs * P.heads;
+    const int64_t rows = std::min<int64_t>(most, P.rows) * group;
+    auto even = [&](int64_t rt) { return (rows + rt - 1) / rt * P.seqs; };
+    auto ragged = [&](int64_t rt) { return P.rows * group / rt + P.seqs; };
     plan.rows = rows > (P.dim <= 128 ? 32 : 16);
-    plan.nq = plan.rows ? (two || rows <= 96 || (rows + 127) / 128 * each < cus ? 1 : 2) : rows <= 16 ? 1 : 2;
+    plan.nq = plan.rows ? (two || rows <= 96 || std::min(even(128), ragged(128)) * P.heads < cus ? 1 : 2) : rows <= 16 ? 1 : 2;
     plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
-    plan.tiles = (rows + plan.rt - 1) / plan.rt;
-    plan.blocks = plan.tiles * each;
+    plan.tiles = even(plan.rt) <= ragged(plan.rt) ? (rows + plan.rt - 1) / plan.rt : 0;
+    plan.places = std::min(even(plan.rt), ragged(plan.rt));
+    plan.blocks = plan.places * P.heads;
     int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     if (window > 0) keys = std::min(keys, std::min<int64_t>(window, INT32_MAX) + std::min<int64_t>(most, P.rows) + 2 * kKvB);
     const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
@@ -78,7 +83,9 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     const bool two = dt == H3S_F32;
     const KvPlan plan = kv_plan(A.kv, two, batch->most, group, max_len, window, c->cus);
     const int64_t W = kv_width(dim);
-    if (plan.blocks * plan.nsplit > 0x7fffffff || plan.blocks * plan.rt > 0x7fffffff) return fail(std::string(fn) + ": too many blocks of work");
+    // (the merge has a block of threads a row)
+    if (plan.blocks > kKvMostBlocks || plan.blocks * (plan.nsplit > 1 ? std::max(plan.nsplit, plan.rt) : 1) > kKvMostBlocks)
+        return fail(std::string(fn) + ": too many blocks of work");
     const int64_t floats = kv_part_floats(plan, W);
     A.po = nullptr;
     if (floats) {
@@ -100,7 +107,7 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     A.window = (int) std::min<int64_t>(window, INT32_MAX / 2);
     A.mask = mask; A.mask_stride = mask_stride;
     A.out = out; A.out_dt = out_dt; A.lse = lse;
-    A.tiles = (int) plan.tiles; A.nsplit = plan.nsplit; A.per = plan.per;
+    A.tiles = (int) plan.tiles; A.places = (int) plan.places; A.nsplit = plan.nsplit; A.per = plan.per;
     A.q_vec = aligned16(q) && dim % 8 == 0 && (q_stride * elem_size(dt)) % 16 == 0;
     A.out_vec = aligned16(out) && dim % 4 == 0;
     A.mask_vec = mask && aligned16(mask) && mask_stride % 16 == 0;

@@ -50,8 +50,9 @@ struct KvAttnArgs {
     void* out;
     int out_dt;
     float* lse;
-    int tiles, nsplit, per;                         // row tiles a sequence and head; parts, of `per` cache blocks each (the last: the rest)
-    float *po, *pml;                                // the parts' sums [item, part, rows, W] and (m, l) [item, part, rows, 2]
+    int tiles, places;                              // row tiles a sequence (0: laid out by the rows, see KvItem); row tiles of all sequences
+    int nsplit, per;                                // parts, of `per` cache blocks each (the last: the rest)
+    float *po, *pml;                                // the parts' sums [place, head, part, rows, W] and (m, l) [place, head, part, rows, 2]
     bool q_vec, out_vec, mask_vec;
 };
 
@@ -278,19 +279,28 @@ template <int WC, int NQ, bool TWO> struct KvRows {
     }
 };
 
-// which rows, head, sequence and part of the cache a block of threads has
+// Which rows, head, sequence and part of the cache a block of threads has. Sequences with about as many rows each have P.tiles tiles of RT
+// rows; else each has its share: R of all sequences' rows lie in at most floor(R / RT) + 1 of the places from floor(its first / RT) + its number on.
 struct KvItem {
-    int h, split, b, tile, r0, n, len;
+    int h, split, place, b, tile, r0, n, len;
     uint32_t R;
-    __device__ __forceinline__ void take(const KvAttnArgs& P) {
-        int64_t id = blockIdx.x;
-        h = (int) (id % P.kv.heads);
-        id /= P.kv.heads;
-        split = (int) (id % P.nsplit);
-        id /= P.nsplit;
-        b = (int) (id % P.kv.seqs);
-        tile = P.tiles - 1 - (int) (id / P.kv.seqs);                      // the longest rows first
-        kv_rows_of(P.kv, b, r0, n);
+    template <int RT> __device__ __forceinline__ void take(const KvAttnArgs& P) {
+        uint32_t id = blockIdx.x;
+        h = (int) (id % (uint32_t) P.kv.heads);
+        id /= (uint32_t) P.kv.heads;
+        split = (int) (id % (uint32_t) P.nsplit);
+        rows<RT>(P, (int) (id / (uint32_t) P.nsplit));
+    }
+    // (a place that is no sequence's: a tile past every row)
+    template <int RT> __device__ __forceinline__ void rows(const KvAttnArgs& P, int at) {
+        place = at;
+        if (P.tiles) {
+            b = (int) ((uint32_t) at % (uint32_t) P.kv.seqs);
+            tile = P.tiles - 1 - (int) ((uint32_t) at / (uint32_t) P.kv.seqs);    // the longest rows first
+            kv_rows_of(P.kv, b, r0, n);
+        } else {
+            tile = kv_find(P.kv, P.places - 1 - at, P.group, RT, 1, b, r0, n);
+        }
         R = (uint32_t) n * P.group;                                       // (rows * group is below 2^31)
         len = min(max(P.lengths[b], 0), P.kv.width * kKvB);
     }
@@ -306,7 +316,7 @@ struct KvItem {
     }
     // the item's place among the parts' sums
     __device__ __forceinline__ int64_t part(const KvAttnArgs& P) const {
-        return (((int64_t) tile * P.kv.seqs + b) * P.kv.heads + h) * P.nsplit + split;
+        return ((int64_t) place * P.kv.heads + h) * P.nsplit + split;
     }
 };
 
@@ -344,7 +354,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
     KvItem it;
-    it.take(P);
+    it.take<RT>(P);
     const int h = it.h, b = it.b;
     const uint32_t R = it.R, rw = (uint32_t) it.tile * RT, group = P.group;
     if (rw >= R) return;
@@ -487,7 +497,7 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
     KvItem it;
-    it.take(P);
+    it.take<RT>(P);
     const int h = it.h, b = it.b;
     const uint32_t R = it.R, rt0 = (uint32_t) it.tile * RT, rw = rt0 + wave * 16 * NQ, group = P.group;
     if (rt0 >= R) return;
@@ -636,11 +646,7 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
     const int r = (int) (blockIdx.x % RT);
     KvItem it;
     it.h = (int) (item % P.kv.heads);
-    it.b = (int) (item / P.kv.heads % P.kv.seqs);
-    it.tile = (int) (item / P.kv.heads / P.kv.seqs);
-    kv_rows_of(P.kv, it.b, it.r0, it.n);
-    it.R = (uint32_t) it.n * P.group;
-    it.len = min(max(P.lengths[it.b], 0), P.kv.width * kKvB);
+    it.rows<RT>(P, (int) (item / P.kv.heads));
     const uint32_t rr = (uint32_t) it.tile * RT + r, group = P.group;
     if (rr >= it.R) return;
     int kb0, count;
@@ -681,7 +687,7 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
 struct KvPlan {
     bool rows;            // kv_attn_rows_kernel (else kv_attn_kernel)
     int nq, rt;           // its tiles of 16 rows a wavefront, and the rows a block of threads takes
-    int64_t tiles;
+    int64_t tiles, places;
     int nsplit, per;      // parts, and the cache blocks of each
     int64_t blocks;       // of threads, without the parts
 };

@@ -3,12 +3,12 @@ import numpy as np
 import pytest
 
 import lm_reference as ref
-from helpers import up
-from test_gpu_lm import attn_case, compare_cache, i32, run_attn, tables, upload
+from helpers import new, up
+from test_gpu_lm import attn_case, check_attn, compare_cache, i32, run_attn, tables, upload
 
 pytestmark = pytest.mark.gpu
 
-from sycl_minimax_h3_amd import ops  # noqa: E402
+from sycl_minimax_h3_amd import Error, ops  # noqa: E402
 
 BLOCK = ref.BLOCK
 
@@ -95,3 +95,58 @@ def test_write_and_read_of_one_long_sequence_among_many(dev, heads, dim, seqs, l
             v, _ = cache.values(i, table[b], pasts[b] + np.arange(news[b]))
             want[starts[b]:starts[b + 1], i * heads * dim:(i + 1) * heads * dim] = v.transpose(1, 0, 2).reshape(-1, heads * dim)
     assert np.array_equal(y.to_numpy(), want)
+
+
+def parts_of(table, starts, lengths, picks):
+    """The rows [j, j + n) of sequence b, for each (b, j, n), as sequences of their own: their tables, the rows and their lengths."""
+    at = np.concatenate([np.arange(starts[b] + j, starts[b] + j + n) for b, j, n in picks])
+    lens = [lengths[b] - (starts[b + 1] - starts[b]) + j + n for b, j, n in picks]
+    return table[[b for b, _, _ in picks]], at, np.concatenate([[0], np.cumsum([n for _, _, n in picks])]), np.array(lens)
+
+
+@pytest.mark.parametrize("heads,group,dim,seqs,long,dt", [
+    (32, 8, 8, 1024, 8192, "BF16"),        # more tiles than a launch takes, were every sequence as long
+    (2, 8, 64, 3, 500, "BF16"),
+    (2, 8, 128, 70, 300, "F32"),           # more sequences than a wavefront has lanes
+    (1, 4, 80, 130, 200, "F16"),
+    (1, 12, 192, 5, 90, "BF16"),
+    (1, 1, 64, 4200, 100, "BF16"),         # more than 64 times as many
+])
+def test_attention_of_one_long_sequence_among_many(dev, heads, group, dim, seqs, long, dt):
+    """Prompts beside sequences that answer with a token, some of them over long caches, and sequences without a row."""
+    news, pasts = np.ones(seqs, int), np.arange(seqs) * 29 % 190
+    at = seqs // 2
+    news[at], pasts[at] = long, 40
+    news[0], pasts[0] = 1, 1900
+    news[seqs - 1], pasts[seqs - 1] = 0, 100
+    if seqs > 8:
+        news[1], news[2] = 33, 5
+        pasts[3] = 2500
+    g, table, blocks, starts = ragged(news, pasts, 84)
+    cache = ref.Cache(blocks, heads, dim, 84)
+    starts = starts + 40                                                          # (rows before the first sequence)
+    rows, stride = int(starts[-1]) + 3, heads * group * dim + 24
+    bits = ref.to_bits(g.standard_normal((rows, stride)), dt)
+    q = ref.from_bits(bits, dt)[:, 8:8 + heads * group * dim].reshape(rows, heads * group, dim)
+    lengths = pasts + news
+    got, lse = run_attn(dev, cache, table, starts, lengths, bits, q, rows, stride, None, group, dt, "F32", {"lse": True})
+    picks = [(0, 0, 1), (at, 0, 2), (at, long // 2, 2), (at, long - 2, 2)] + [(b, 0, 1) for b in {1, 2, 3, seqs // 3, seqs - 2} if 0 < b < seqs - 1 and b != at]
+    if heads * group > 64:
+        picks = picks[:1] + [(at, 10, 1), (at, 400, 1), (seqs - 2, 0, 1)]        # (a row of the reference takes its time)
+    tb, rw, st, ln = parts_of(table, starts, lengths, picks)
+    want = ref.attention(cache, tb, st, ln, q[rw], group, dt, "F32")
+    check_attn(got[rw], lse[rw], want, len(rw), str(picks))
+    own = slice(int(starts[0]), int(starts[-1]))
+    none = np.r_[0:own.start, own.stop:rows]
+    assert (got[none] == 55.0).all() and (lse[none] == 44.0).all()
+    assert np.isfinite(got[own]).all() and not (got[own] == 55.0).all(-1).any() and not (lse[own] == 44.0).any()
+
+
+def test_attention_past_a_launch_is_refused(dev):
+    """More blocks of threads than a launch takes are an error, not a part of the work."""
+    seqs, heads, dim = 1 << 22, 8, 1
+    c = ops.KvCache.new(dev, 1, heads, dim)
+    table, starts, lengths = (new(dev, "I32", s) for s in ([seqs, 1], [seqs + 1], [seqs]))
+    q, out = new(dev, "F32", [8, heads]), new(dev, "F32", [8, heads])
+    with pytest.raises(Error, match="too many blocks of work"):
+        ops.kv_attention(c, table, ops.Rows(q, 0, heads, 8, heads, dim), starts, lengths, 1, out)

@@ -79,7 +79,8 @@ typedef struct {
      * Products, softmax and sums are float32 (q to 11 bits of each value for 16-bit types, which is all they have, 22 for float32;
      * probabilities likewise), rounded once to out_dt.
      * Lengths count as at least 0 and at most the table's 64 * width tokens. out may not overlap q.
-     * max_len: about the longest of the lengths (0: the table's width); it only decides how the work is split.
+     * max_len: about the longest of the lengths (0: the table's width); it only decides how the work is split. Sequences with many
+     * rows and with few may be mixed: each takes the kernel for its number of rows.
      * work: a device workspace of at least kv_attention_work(...) bytes, 16-byte aligned, in use until the call's work is done;
      * NULL: the context's own scratch. A call recorded into a graph has to bring its own (two graphs, or a graph and eager calls,
      * would share the context's): -1 otherwise, unless it needs none. */

@@ -39,6 +39,20 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, int64_t group, in
     plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
     return plan;
 }
+// The launches of a call, one or two. Where some sequences can have many rows and others few (prompts beside answered tokens), those with up
+// to 16 (or 32: larger groups) are a launch of the shared-rows kernel if that splits their caches further: a prompt of 2048 tokens
+// beside a token over 131072, 64 heads over 8 of 128, 3469 us in one launch, 191 in two (129 and 49 by themselves); four prompts of 241 to 600
+// tokens behind up to 900, for which the second finds nothing to do, 70 and 69.
+static int kv_plans(const KvArgs& P, bool two, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus, KvPlan (&plan)[2]) {
+    plan[0] = kv_plan(P, two, most, group, max_len, window, cus);
+    const int64_t few = (group <= 16 ? 16 : 32) / group;                         // tokens
+    if (!plan[0].rows || few == 0 || (group > 16 && P.dim > 128) || std::min<int64_t>(most, P.rows) * P.seqs <= P.rows) return 1;
+    plan[1] = kv_plan(P, two, few, group, max_len, window, cus);
+    if (plan[1].nsplit <= plan[0].nsplit) return 1;
+    plan[1].greatest = (uint32_t) (few * group);
+    plan[0].least = plan[1].greatest + 1;
+    return 2;
+}
 static int64_t kv_part_floats(const KvPlan& plan, int64_t W) { return plan.nsplit > 1 ? plan.blocks * plan.nsplit * plan.rt * (W + 2) : 0; }
 
 static int attn_checks(const char* fn, const KvArgs& P, int64_t max_len, int64_t q_heads, int64_t window) {
@@ -57,8 +71,12 @@ int64_t kv_attention_work(void* ctx, const h3_kv_cache* cache, const h3_kv_batch
     if (P.seqs == 0 || P.rows == 0 || batch->most == 0) return 0;
     // (the more of what 16-bit and float32 queries take)
     int64_t floats = 0;
-    for (bool two : {false, true})
-        floats = std::max(floats, kv_part_floats(kv_plan(P, two, batch->most, q_heads / P.heads, max_len, window, c->cus), kv_width(P.dim)));
+    for (bool two : {false, true}) {
+        KvPlan plan[2];
+        int64_t sum = 0;
+        for (int n = kv_plans(P, two, batch->most, q_heads / P.heads, max_len, window, c->cus, plan); n-- > 0;) sum += kv_part_floats(plan[n], kv_width(P.dim));
+        floats = std::max(floats, sum);
+    }
     return 4 * floats;
 } catch (const std::exception& e) { return fail(e.what()); }
 
@@ -81,41 +99,51 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     if (!c) return -1;
     if (A.kv.rows * group > INT32_MAX) return fail(std::string(fn) + ": too many rows");
     const bool two = dt == H3S_F32;
-    const KvPlan plan = kv_plan(A.kv, two, batch->most, group, max_len, window, c->cus);
+    KvPlan plans[2];
+    const int launches = kv_plans(A.kv, two, batch->most, group, max_len, window, c->cus, plans);
     const int64_t W = kv_width(dim);
-    // (the merge has a block of threads a row)
-    if (plan.blocks > kKvMostBlocks || plan.blocks * (plan.nsplit > 1 ? std::max(plan.nsplit, plan.rt) : 1) > kKvMostBlocks)
-        return fail(std::string(fn) + ": too many blocks of work");
-    const int64_t floats = kv_part_floats(plan, W);
-    A.po = nullptr;
+    int64_t floats = 0;
+    for (int i = 0; i < launches; ++i) {
+        // (the merge has a block of threads a row)
+        if (plans[i].blocks > kKvMostBlocks || plans[i].blocks * (plans[i].nsplit > 1 ? std::max(plans[i].nsplit, plans[i].rt) : 1) > kKvMostBlocks)
+            return fail(std::string(fn) + ": too many blocks of work");
+        floats += kv_part_floats(plans[i], W);
+    }
+    float* parts = nullptr;
     if (floats) {
         if (work) {
             if (work_bytes < (uint64_t) (4 * floats)) return fail(std::string(fn) + ": the workspace is smaller than kv_attention_work() says");
-            A.po = (float*) work;
+            parts = (float*) work;
         } else {
             hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
             if (hipStreamIsCapturing(c->stream, &st) != hipSuccess) (void) hipGetLastError();
             if (st != hipStreamCaptureStatusNone) return fail(std::string(fn) + ": a call recorded into a graph needs a workspace of its own");
-            A.po = c->scratch<float>(Ctx::KV_PART, (size_t) floats);
-            if (!A.po) return -1;
+            parts = c->scratch<float>(Ctx::KV_PART, (size_t) floats);
+            if (!parts) return -1;
         }
     }
-    A.pml = A.po ? A.po + plan.blocks * plan.nsplit * plan.rt * W : nullptr;
     A.lengths = lengths;
     A.q = q; A.q_stride = q_stride; A.q_dt = dt; A.group = (int) group; A.q_heads = (int) q_heads;
     A.scale = (float) ((scale > 0.0f ? (double) scale : 1.0 / std::sqrt((double) dim)) * 1.4426950408889634);
     A.window = (int) std::min<int64_t>(window, INT32_MAX / 2);
     A.mask = mask; A.mask_stride = mask_stride;
     A.out = out; A.out_dt = out_dt; A.lse = lse;
-    A.tiles = (int) plan.tiles; A.places = (int) plan.places; A.nsplit = plan.nsplit; A.per = plan.per;
     A.q_vec = aligned16(q) && dim % 8 == 0 && (q_stride * elem_size(dt)) % 16 == 0;
     A.out_vec = aligned16(out) && dim % 4 == 0;
     A.mask_vec = mask && aligned16(mask) && mask_stride % 16 == 0;
-    switch (W / 64) {
-        case 1: kv_attn_64(c, A, plan, two); break;
-        case 2: kv_attn_128(c, A, plan, two); break;
-        case 3: kv_attn_192(c, A, plan, two); break;
-        default: kv_attn_256(c, A, plan, two); break;
+    for (int i = 0; i < launches; ++i) {
+        const KvPlan& plan = plans[i];
+        A.tiles = (int) plan.tiles; A.places = (int) plan.places; A.nsplit = plan.nsplit; A.per = plan.per;
+        A.least = plan.least; A.greatest = plan.greatest;
+        A.po = parts;
+        A.pml = parts ? parts + plan.blocks * plan.nsplit * plan.rt * W : nullptr;
+        if (parts) parts += kv_part_floats(plan, W);
+        switch (W / 64) {
+            case 1: kv_attn_64(c, A, plan, two); break;
+            case 2: kv_attn_128(c, A, plan, two); break;
+            case 3: kv_attn_192(c, A, plan, two); break;
+            default: kv_attn_256(c, A, plan, two); break;
+        }
     }
     return launched(fn);
 } catch (const std::exception& e) { return fail(e.what()); }

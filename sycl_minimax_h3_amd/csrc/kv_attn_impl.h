@@ -51,6 +51,7 @@ struct KvAttnArgs {
     int out_dt;
     float* lse;
     int tiles, places;                              // row tiles a sequence (0: laid out by the rows, see KvItem); row tiles of all sequences
+    uint32_t least, greatest;                       // the sequences of fewer or more rows (tokens x heads of a group) are another launch's
     int nsplit, per;                                // parts, of `per` cache blocks each (the last: the rest)
     float *po, *pml;                                // the parts' sums [place, head, part, rows, W] and (m, l) [place, head, part, rows, 2]
     bool q_vec, out_vec, mask_vec;
@@ -302,6 +303,7 @@ struct KvItem {
             tile = kv_find(P.kv, P.places - 1 - at, P.group, RT, 1, b, r0, n);
         }
         R = (uint32_t) n * P.group;                                       // (rows * group is below 2^31)
+        if (R < P.least || R > P.greatest) R = 0;
         len = min(max(P.lengths[b], 0), P.kv.width * kKvB);
     }
     // the cache blocks kb0 .. kb0 + count that any of the rows rt0 .. rt0 + rt can see
@@ -690,6 +692,7 @@ struct KvPlan {
     int64_t tiles, places;
     int nsplit, per;      // parts, and the cache blocks of each
     int64_t blocks;       // of threads, without the parts
+    uint32_t least = 0, greatest = UINT32_MAX;
 };
 
 template <int WC, int NQ, bool ROWS>

@@ -3,12 +3,12 @@ import numpy as np
 import pytest
 
 import lm_reference as ref
-from helpers import new, up
-from test_gpu_lm import attn_case, check_attn, compare_cache, i32, run_attn, tables, upload
+from helpers import launches, new, up
+from test_gpu_lm import Recorded, attn_case, check_attn, compare_cache, i32, run_attn, tables, upload
 
 pytestmark = pytest.mark.gpu
 
-from sycl_minimax_h3_amd import Error, ops  # noqa: E402
+from sycl_minimax_h3_amd import Error, Tensor, ops  # noqa: E402
 
 BLOCK = ref.BLOCK
 
@@ -150,3 +150,47 @@ def test_attention_past_a_launch_is_refused(dev):
     q, out = new(dev, "F32", [8, heads]), new(dev, "F32", [8, heads])
     with pytest.raises(Error, match="too many blocks of work"):
         ops.kv_attention(c, table, ops.Rows(q, 0, heads, 8, heads, dim), starts, lengths, 1, out)
+
+def test_attention_of_prompts_beside_answers_recorded(dev):
+    """A prompt beside sequences that answer with one token over long caches: two launches, the answers' caches split among more blocks of
+    threads. Recorded with a workspace of the size that is asked for, and replayed when other sequences have the rows."""
+    heads, group, dim, dt, seqs = 2, 8, 64, "BF16", 4
+    g = np.random.default_rng(85)
+    table, blocks = tables([60] * seqs, seed=85)
+    cache = ref.Cache(blocks, heads, dim, 85)
+    rows, width = 503, heads * group * dim
+    bits = ref.to_bits(g.standard_normal((rows, width + 24)), dt)
+    q = ref.from_bits(bits, dt)[:, 8:8 + width].reshape(rows, heads * group, dim)
+    c, t, x = upload(dev, cache), i32(dev, table), up(dev, bits, dt, [rows, width + 24])
+    starts, lengths = i32(dev, [0, 500, 501, 502, 503]), i32(dev, [500, 3800, 100, 1])
+    rq, out = ops.Rows(x, 8, width + 24, rows, heads * group, dim), up(dev, np.zeros((rows, width), np.float32), "F32", [rows, width])
+    size = ops.kv_attention_work(c, t, rq, starts, 500)
+    whole = up(dev, np.full(size + 64, 0xA5, np.uint8), "U8", [size + 64])
+    work = Tensor(whole.dtype, [size], whole.ptr(), whole, dev)
+
+    def call():
+        ops.kv_attention(c, t, rq, starts, lengths, 500, out, work=work)
+
+    ran = [name.split("<")[0] for name, _, _ in launches(dev, call)]
+    assert ran == ["kv_attn_rows_kernel", "kv_merge_kernel", "kv_attn_kernel", "kv_merge_kernel"], ran
+    graph = Recorded(dev, call)
+    for st, ln in (([0, 500, 501, 502, 503], [500, 3800, 100, 1]), ([0, 1, 2, 502, 503], [3800, 90, 3000, 2000]), ([0, 2, 5, 5, 405], [3000, 3, 64, 3700])):
+        starts._owner.write(np.array(st, np.int32))
+        lengths._owner.write(np.array(ln, np.int32))
+        out._owner.write(np.full((rows, width), 55.0, np.float32))
+        graph.replay()
+        got = out.to_numpy().reshape(rows, heads * group, dim)
+        call()                                                                    # (eager work of the context between the replays)
+        assert np.array_equal(out.to_numpy().reshape(got.shape), got)
+        long = int(np.argmax(np.diff(st)))
+        picks = [(b, 0, st[b + 1] - st[b]) for b in range(seqs) if b != long and st[b + 1] > st[b]] + [(long, j, 1) for j in (0, 60, 399)]
+        tb, rw, s2, l2 = parts_of(table, st, np.array(ln), picks)
+        check_attn(got[rw], None, ref.attention(cache, tb, s2, l2, q[rw], group, dt, "F32"), len(rw), str(st))
+        assert (got[st[-1]:] == 55.0).all()
+        assert (whole.to_numpy()[size:] == 0xA5).all()
+    graph.close()
+    # (four sequences of 100 rows cannot have one of few)
+    r400 = ops.Rows(x, 8, width + 24, 400, heads * group, dim)
+    out, work = new(dev, "F32", [400, width]), new(dev, "U8", [ops.kv_attention_work(c, t, r400, starts, 100)])
+    even = launches(dev, lambda: ops.kv_attention(c, t, r400, starts, lengths, 100, out, work=work))
+    assert [name.split("<")[0] for name, _, _ in even] == ["kv_attn_rows_kernel", "kv_merge_kernel"], even

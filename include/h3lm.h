@@ -97,8 +97,10 @@ typedef struct {
      *     W[n, k] = scale[n, g] * code - mins[n, g]     mins [N, K / group] of type scale_dt
      * group: a multiple of 32 that divides K, and K at most 2^20. Float32 sums; bias float32 [N] or NULL, added before the one rounding. codes and x
      * 16-byte aligned, rows whole 16-byte pieces (K a multiple of 32 makes them so). out may not overlap x. No workspace.
-     * The sums run over x * (16 + code), with 16 times x's sum taken off again: an infinity or NaN in a row of x makes that row of out
-     * NaN (of no other row), and so may values whose sums times 31 leave float32. */
+     * 16-bit x: the sums run over x * (16 + code), with 24 times x's sum (16 times, and the minima) taken off again. float32's rounding then counts
+     * against those: up to 2e-5 of the result where x has one sign and the codes lie within one of 8, 3e-7 for uniform codes. float32 x: the sums run
+     * over x * (code - 8) in all of x's digits (values below 2^-110 have fewer). Either way an infinity or NaN in a row of x makes that row of
+     * out infinite or NaN (and no other row), and so may values whose sums times 31 leave float32. */
     int (*linear4)(void* ctx, const void* x, int dt, int64_t M, int64_t K, const uint8_t* codes, int64_t N, const void* scale,
                    const void* mins, int scale_dt, int64_t group, const float* bias, void* out, int out_dt);
 } h3_lm_api;

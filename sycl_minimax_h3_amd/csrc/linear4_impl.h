@@ -7,8 +7,15 @@
 // instruction (16 x 16 x 32, float32 sums) with x as it stands (bfloat16, half; float32 as three bfloat16 parts). A run's sum of x is one
 // more, with a first operand of ones in one row, shared by all columns of the wavefront; it leaves the sums of four runs as the
 // first operand of a float32 instruction (16 x 16 x 4) whose second is the four 16 s + z: their products are one instruction for 128
-// inputs. What is left for the vector units is one multiply-add by s a group and output. (16 against c of 0 .. 15: the two terms are
-// at most some five times their difference, so float32 sums lose little over two bits.)
+// inputs. What is left for the vector units is one multiply-add by s a group and output.
+//
+// What that costs in digits: the two terms are roundings of numbers up to 24 / |c - 8| times their difference, more where x has one
+// sign. Against float32 sums of x (c - 8) (5376 inputs, 16 rows, float32 out): uniform codes 1.3 times their error (3e-7 of the result), codes in a bell
+// of deviation 2.5 around 8 2.2 times, those with x of mean 3 and deviation 1 20 times (5e-6), codes within one of 8 as well 66 times (1.7e-5).
+// A 16-bit x is itself off by 2^-9 or 2^-12 of each value, so it keeps this form. float32 x takes sixteen times c - 8 as operands
+// (whole numbers, exact in bfloat16; two instructions a code instead of one, for three products each) with z - 8 s against x's sums,
+// and no sums without minima: half the error of float32 sums one by one in all four (before: 1.3 to 66 times). 300 rows 14336 -> 5376 286 to 308 us with minima, 243 to 228
+// without; 8 rows 5376 -> 28672 70 to 82 and 56 to 55; one row 5376 -> 131072 101 to 117.
 //
 // Layout: a lane loads 16 bytes of a weight row, 32 codes; the four lanes of a row (16 apart) hold 128 consecutive inputs. A 4 x 4
 // exchange between them (four lane swaps) leaves each with eight codes of each of four runs of 32 inputs, so that an instruction's 32
@@ -64,9 +71,24 @@ template <int OP> __device__ __forceinline__ void l4_constants(uint32_t& m, uint
     asm volatile("" : "+s"(m));
     asm volatile("" : "+v"(e));
 }
-template <int OP> __device__ __forceinline__ uint4 l4_codes(uint32_t w, uint32_t m, uint32_t e) {
-    if constexpr (OP == H3S_F16) return make_uint4(((w << 6) & m) | e, ((w << 2) & m) | e, ((w >> 2) & m) | e, ((w >> 6) & m) | e);
+// float32 x (three PARTS): sixteen times code - 8, in the same order, exactly: a code less 8 is its four bits as a signed number once the
+// highest is flipped, and those are the high half of a signed byte
+template <int OP, int PARTS> __device__ __forceinline__ uint4 l4_codes(uint32_t w, uint32_t m, uint32_t e) {
+    if constexpr (PARTS > 1) {
+        const uint32_t even = ((w << 4) & 0xf0f0f0f0u) ^ 0x80808080u, odd = (w & 0xf0f0f0f0u) ^ 0x80808080u;
+        auto pair = [](uint32_t u, int i) {
+            const float a = (float) (int8_t) (u >> (8 * i)), b = (float) (int8_t) (u >> (8 * i + 16));
+            return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+        };
+        return make_uint4(pair(even, 0), pair(odd, 0), pair(even, 1), pair(odd, 1));
+    } else if constexpr (OP == H3S_F16) return make_uint4(((w << 6) & m) | e, ((w << 2) & m) | e, ((w >> 2) & m) | e, ((w >> 6) & m) | e);
     else return make_uint4(((w << 3) & m) | e, ((w >> 1) & m) | e, ((w >> 5) & m) | e, ((w >> 9) & m) | e);
+}
+// what x's sum is taken off with: the weights' distance from s times the operands
+template <int PARTS> __device__ __forceinline__ float l4_off(float s, float least, bool mins) {
+    if constexpr (PARTS > 1) return mins ? __builtin_fmaf(-8.0f, s, least) : 0.0f;
+    const float x = __builtin_fmaf(16.0f, s, least), y = 24.0f * s;
+    return mins ? x : y;
 }
 // eight 16-bit values in that order
 __device__ __forceinline__ uint4 l4_order(const uint4& u) {
@@ -121,7 +143,7 @@ __device__ __forceinline__ void l4_exchange(const uint4& w, uint32_t (&c)[4]) {
 // 16 a .. and the run j (zeros past the row's end); AHEAD: a run's operands are asked for before the products of the one
 // before (from LDS: 300 rows 5376 -> 28672 247 to 211 us, 14336 -> 5376 127 to 120). Rows: place l of an operand is row 4 (l % 4) + l / 4,
 // so that register i of lane group g sums row 4 i + g and up to four rows take one multiply-add (NI of them).
-template <bool AHEAD, int OP, int PARTS, int MT, int NT, int NI, int J, typename F>
+template <bool AHEAD, bool SUMS, int OP, int PARTS, int MT, int NT, int NI, int J, typename F>
 __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, uint32_t e, const uint32_t (&c)[NT][4], const float (&sc)[NT][4 / J], const float (&off)[NT],
                                             F frag, v4f_l4 (&acc)[MT][NT]) {
     v4f_l4 sx[MT];
@@ -142,7 +164,7 @@ __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, u
         for (int j = q * J; j < (q + 1) * J; ++j) {
             uint4 f[NT];
 #pragma unroll
-            for (int b = 0; b < NT; ++b) f[b] = l4_codes<OP>(c[b][j], m, e);
+            for (int b = 0; b < NT; ++b) f[b] = l4_codes<OP, PARTS>(c[b][j], m, e);
             if (AHEAD && j < 3) {
 #pragma unroll
                 for (int a = 0; a < MT; ++a) frag(a, j + 1, x[(j & 1) ^ 1][a]);
@@ -153,7 +175,7 @@ __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, u
                 if (!AHEAD) frag(a, j, xf);
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) {
-                    sx[a] = l4_mma<OP>(sel[j], xf[p], sx[a]);
+                    if constexpr (SUMS) sx[a] = l4_mma<OP>(sel[j], xf[p], sx[a]);
 #pragma unroll
                     for (int b = 0; b < NT; ++b) y[a][b] = l4_mma<OP>(xf[p], f[b], y[a][b]);
                 }
@@ -167,6 +189,7 @@ __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, u
 #pragma unroll
                 for (int i = 0; i < NI; ++i) acc[a][b][i] = __builtin_fmaf(sc[b][q], y[a][b][i], acc[a][b][i]);
     }
+    if constexpr (!SUMS) return;
 #pragma unroll
     for (int a = 0; a < MT; ++a)
 #pragma unroll
@@ -306,7 +329,7 @@ __global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P)
                 float y = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint4 f = l4_codes<OP>(c[e], cm, ce);
+                    const uint4 f = l4_codes<OP, PARTS>(c[e], cm, ce);
 #pragma unroll
                     for (int p = 0; p < PARTS; ++p) {
                         y = l4_dot<OP>(x[u][p][4 * e], f.x, y);
@@ -315,8 +338,9 @@ __global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P)
                         y = l4_dot<OP>(x[u][p][4 * e + 3], f.w, y);
                     }
                 }
-                const float s = number(sr[d][u]), off = MINS ? __builtin_fmaf(16.0f, s, number(zr[d][u])) : 24.0f * s;
-                acc = __builtin_fmaf(-off, sx[u], __builtin_fmaf(s, y, acc));
+                const float s = number(sr[d][u]);
+                acc = __builtin_fmaf(PARTS > 1 ? 0.0625f * s : s, y, acc);
+                if constexpr (MINS || PARTS == 1) acc = __builtin_fmaf(-l4_off<PARTS>(s, MINS ? number(zr[d][u]) : 0.0f, MINS), sx[u], acc);
             }
             load(d);
             acc = wave_sum<16>(acc);
@@ -342,7 +366,7 @@ __global__ __launch_bounds__(64 * kL4DotWaves) void linear4_dot_kernel(L4Args P)
 
 // The scales and minima of four steps of one column: lane group g loads those of step first + g (one gather for four steps: a gather
 // from 16 rows of weights costs about as much as 16 x 64 bytes of codes), and a step's are passed on from its group.
-template <int J, int SM> struct L4Q {
+template <int J, int SM, int PARTS> struct L4Q {
     static constexpr int CNT = 4 / J, RAW = SM == L4_S16 ? (CNT + 1) / 2 : CNT;
     uint32_t s[RAW], z[RAW];
     // scale, mins: the tile's first column's; off: the bytes from there to the lane's column; r: the first run of the lane's step
@@ -384,8 +408,11 @@ template <int J, int SM> struct L4Q {
         float own = sc[0], least = zc[0];
         if constexpr (CNT == 2) { own = g < 2 ? sc[0] : sc[1]; least = g < 2 ? zc[0] : zc[1]; }
         else if constexpr (CNT == 4) { own = g < 2 ? (g ? sc[1] : sc[0]) : (g == 2 ? sc[2] : sc[3]); least = g < 2 ? (g ? zc[1] : zc[0]) : (g == 2 ? zc[2] : zc[3]); }
-        const float x = __builtin_fmaf(16.0f, own, least), y = 24.0f * own;
-        off = P.has_mins ? x : y;
+        off = l4_off<PARTS>(own, least, P.has_mins != 0);
+        if constexpr (PARTS > 1) {
+#pragma unroll
+            for (int c = 0; c < CNT; ++c) sc[c] *= 0.0625f;
+        }
     }
     __device__ __forceinline__ float number(const L4Args& P, const uint32_t* u, int c) const {
         const uint32_t v = SM == L4_S16 && CNT > 1 ? (c & 1 ? u[c >> 1] >> 16 : u[c >> 1] & 0xffffu) : u[c];
@@ -403,7 +430,7 @@ constexpr int kL4FewWaves = 12;       // wavefronts of a block, at most
 // memory in a weight row, and are joined through LDS at the end of a tile; the loads go on across tiles.
 // XR (one quad: up to 12 x 512 inputs): a wavefront's operands of x stay in registers. Otherwise they are loaded in the step that uses
 // them (from the L2).
-template <int DT, int NT, int J, int SM, bool XR>
+template <int DT, int NT, int J, int SM, bool SUMS, bool XR>
 __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P, int quads) {
     constexpr int OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS, XES = DT == H3S_F32 ? 4 : 2, DP = XR ? 4 : 2;
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, KW = (int) (blockDim.x >> 6);
@@ -419,7 +446,7 @@ __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P,
         if (SM == L4_SANY && k >= P.K) x.zero();
     };
     uint4 w[DP][NT];                                                              // DP steps in flight
-    L4Q<J, SM> now[NT], next[NT];
+    L4Q<J, SM, PARTS> now[NT], next[NT];
     // where the loads of the codes are (the scales': one quad ahead of the step in hand): a tile's first column, the lane's bytes from there
     struct At {
         const uint8_t* codes;
@@ -507,7 +534,7 @@ __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P,
             if (r + DP < 4) load_w(here, step + DP, w[r % DP]);
             else load_w(then, nfirst + r + DP - 4, w[r % DP]);
             if (step < steps) {
-                l4_products<false, OP, PARTS, 1, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
+                l4_products<false, SUMS, OP, PARTS, 1, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
                     if constexpr (XR && DT != H3S_F32) f[0] = xr[r][j].u;
                     else xr[XR ? r : 0][j].parts(f);
                 }, acc);
@@ -541,7 +568,7 @@ __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P,
 }
 
 // CG: wavefronts side by side, of 32 columns each; the block's 8 / CG groups of them take every (8 / CG)th step of 128 inputs
-template <int DT, int MT, int CG, int J, int SM>
+template <int DT, int MT, int CG, int J, int SM, bool SUMS>
 __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
     constexpr int NT = 2, OP = DT == H3S_F16 ? H3S_F16 : H3S_BF16, PARTS = L4X<DT>::PARTS;
     constexpr int KG = 8 / CG, COLS = 16 * NT * CG;
@@ -581,7 +608,7 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) xoff[p] = (uint32_t) ((int) min<int64_t>((t + 64 * CG * p) / 16, P.M - 1 - m0) * P.K + t % 16 * 8) * XES;
     uint4 w[NT];
-    L4Q<J, SM> now[NT], next[NT];                                                 // the scales of four of the K group's steps
+    L4Q<J, SM, PARTS> now[NT], next[NT];                                          // the scales of four of the K group's steps
     auto load_x = [&](int step) {
         const char* xp = xbase + (int64_t) step * 128 * XES;
         const bool out = SM == L4_SANY && step * 128 + t % 16 * 8 >= P.K;
@@ -644,7 +671,7 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
                     }
                 }
                 load_w(min(step + KG, steps - 1));
-                l4_products<PARTS == 1, OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
+                l4_products<PARTS == 1, SUMS, OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][r & 1][a][j][q][lane ^ g];
                 }, acc);
@@ -680,54 +707,54 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
     }
 }
 
-template <int DT, int NT, int J, int SM, bool XR>
+template <int DT, int NT, int J, int SM, bool SUMS, bool XR>
 static void l4_few_run(Ctx* c, const L4Args& P, int quads, int kw) {
     // a block walks as many tiles as any other, or one less
     const int64_t tiles = (P.N + 16 * NT - 1) / (16 * NT), turns = (tiles + c->cus - 1) / c->cus;
-    linear4_few_kernel<DT, NT, J, SM, XR><<<(unsigned) ((tiles + turns - 1) / turns), 64 * kw, 0, c->stream>>>(P, quads);
+    linear4_few_kernel<DT, NT, J, SM, SUMS, XR><<<(unsigned) ((tiles + turns - 1) / turns), 64 * kw, 0, c->stream>>>(P, quads);
 }
-template <int DT, int J, int SM>
+template <int DT, int J, int SM, bool SUMS>
 static void l4_few(Ctx* c, const L4Args& P) {
     // the fewest quads of steps a wavefront that 12 wavefronts can share the inputs in
     const int steps = (P.K + 127) / 128, quads = (steps + 4 * kL4FewWaves - 1) / (4 * kL4FewWaves), kw = (steps + 4 * quads - 1) / (4 * quads);
     if constexpr (DT != H3S_F32) {
-        if (quads == 1) return l4_few_run<DT, 1, J, SM, true>(c, P, quads, kw);
+        if (quads == 1) return l4_few_run<DT, 1, J, SM, SUMS, true>(c, P, quads, kw);
     }
-    l4_few_run<DT, 2, J, SM, false>(c, P, quads, kw);
+    l4_few_run<DT, 2, J, SM, SUMS, false>(c, P, quads, kw);
 }
 // the blocks of tiles of `rows` rows and 32 cg columns; those of a column tile go to one XCD of eight, so an eighth of them is a whole number
 static int64_t l4_blocks(const L4Args& P, int rows, int cg) {
     return (P.M + rows - 1) / rows * (((P.N + 32 * cg - 1) / (32 * cg) + 7) / 8 * 8);
 }
-template <int DT, int MT, int CG, int J, int SM>
+template <int DT, int MT, int CG, int J, int SM, bool SUMS>
 static void l4_many_run(Ctx* c, const L4Args& P) {
-    linear4_many_kernel<DT, MT, CG, J, SM><<<(unsigned) l4_blocks(P, 16 * MT, CG), 512, 0, c->stream>>>(P);
+    linear4_many_kernel<DT, MT, CG, J, SM, SUMS><<<(unsigned) l4_blocks(P, 16 * MT, CG), 512, 0, c->stream>>>(P);
 }
 // Half as many columns a block, and twice the groups along the inputs, while the blocks still run at once (as far as x's stages fit LDS):
 // 5376 -> 5376, 32 rows 38 to 18 us, 128 rows 52 to 34; 14336 -> 5376, 32 rows 92 to 33 us, 128 rows 126 to 72.
-template <int DT, int MT, int J, int SM>
+template <int DT, int MT, int J, int SM, bool SUMS>
 static void l4_many(Ctx* c, const L4Args& P) {
     if constexpr (MT == 2) {
-        if (l4_blocks(P, 32, 1) <= c->cus) return l4_many_run<DT, MT, 1, J, SM>(c, P);
+        if (l4_blocks(P, 32, 1) <= c->cus) return l4_many_run<DT, MT, 1, J, SM, SUMS>(c, P);
     }
-    if (l4_blocks(P, 16 * MT, 2) <= c->cus) l4_many_run<DT, MT, 2, J, SM>(c, P);
-    else l4_many_run<DT, MT, 4, J, SM>(c, P);
+    if (l4_blocks(P, 16 * MT, 2) <= c->cus) l4_many_run<DT, MT, 2, J, SM, SUMS>(c, P);
+    else l4_many_run<DT, MT, 4, J, SM, SUMS>(c, P);
 }
-template <int DT, int J, int SM>
+template <int DT, int J, int SM, bool SUMS>
 static void l4_run(Ctx* c, const L4Args& P) {
     if constexpr (DT == H3S_F32) {
         // (three parts: x's stages of 32 rows and more than two groups do not fit LDS, those of 16 rows do: 32 rows 5376 -> 5376 56 to
         // 26 us, 14336 -> 5376 140 to 58)
-        if (P.M <= 16) l4_few<DT, J, SM>(c, P);
-        else if (l4_blocks(P, 16, 2) <= c->cus) l4_many_run<DT, 1, 2, J, SM>(c, P);
-        else l4_many_run<DT, 2, 4, J, SM>(c, P);
+        if (P.M <= 16) l4_few<DT, J, SM, SUMS>(c, P);
+        else if (l4_blocks(P, 16, 2) <= c->cus) l4_many_run<DT, 1, 2, J, SM, SUMS>(c, P);
+        else l4_many_run<DT, 2, 4, J, SM, SUMS>(c, P);
     } else {
         // Up to 16 rows as one operand, unless x's operands do not fit the wavefronts' registers there and few columns leave the inputs to
         // split (14336 -> 5376: 16 rows 41 us, in tiles of 32 rows 32). Tiles of 32 rows up to 32 rows, and beyond while the device runs
         // all blocks of 64 columns of them at once (64 rows: 5376 -> 5376 34 to 22 us, 14336 -> 5376 75 to 47).
-        if (P.M <= 4 || (P.M <= 16 && (P.K <= 512 * kL4FewWaves || l4_blocks(P, 32, 1) > c->cus))) l4_few<DT, J, SM>(c, P);
-        else if (P.M <= 32 || l4_blocks(P, 32, 2) <= c->cus) l4_many<DT, 2, J, SM>(c, P);
-        else l4_many<DT, 4, J, SM>(c, P);
+        if (P.M <= 4 || (P.M <= 16 && (P.K <= 512 * kL4FewWaves || l4_blocks(P, 32, 1) > c->cus))) l4_few<DT, J, SM, SUMS>(c, P);
+        else if (P.M <= 32 || l4_blocks(P, 32, 2) <= c->cus) l4_many<DT, 2, J, SM, SUMS>(c, P);
+        else l4_many<DT, 4, J, SM, SUMS>(c, P);
     }
 }
 template <int DT, int U>
@@ -748,21 +775,29 @@ template <int DT> static bool l4_dot_takes(Ctx* c, const L4Args& P) {
     else return false;
     return true;
 }
+// x's sums are needed but for float32 x without minima, whose operands are the weights less their scale
+template <int DT, int J, int SM>
+static void l4_sums(Ctx* c, const L4Args& P) {
+    if constexpr (DT == H3S_F32) {
+        if (!P.has_mins) return l4_run<DT, J, SM, false>(c, P);
+    }
+    l4_run<DT, J, SM, true>(c, P);
+}
 template <int DT>
 static void l4_type(Ctx* c, const L4Args& P) {
     if (l4_dot_takes<DT>(c, P)) return;
     // a step of 128 inputs has 4, 2 or 1 scales: one load where every column's lie on a boundary of their size
     const int64_t cnt = P.group % 128 == 0 ? 1 : P.group == 64 ? 2 : P.group == 32 ? 4 : 0;
     const bool vec = cnt && P.groups % cnt == 0 && ((uintptr_t) P.scale | (uintptr_t) P.mins) % (uintptr_t) (cnt * elem_size(P.scale_dt)) == 0;
-    if (!vec) l4_run<DT, 1, L4_SANY>(c, P);
+    if (!vec) l4_sums<DT, 1, L4_SANY>(c, P);
     else if (P.scale_dt == H3S_F32) {
-        if (cnt == 1) l4_run<DT, 4, L4_S32>(c, P);
-        else if (cnt == 2) l4_run<DT, 2, L4_S32>(c, P);
-        else l4_run<DT, 1, L4_S32>(c, P);
+        if (cnt == 1) l4_sums<DT, 4, L4_S32>(c, P);
+        else if (cnt == 2) l4_sums<DT, 2, L4_S32>(c, P);
+        else l4_sums<DT, 1, L4_S32>(c, P);
     } else {
-        if (cnt == 1) l4_run<DT, 4, L4_S16>(c, P);
-        else if (cnt == 2) l4_run<DT, 2, L4_S16>(c, P);
-        else l4_run<DT, 1, L4_S16>(c, P);
+        if (cnt == 1) l4_sums<DT, 4, L4_S16>(c, P);
+        else if (cnt == 2) l4_sums<DT, 2, L4_S16>(c, P);
+        else l4_sums<DT, 1, L4_S16>(c, P);
     }
 }
 void l4_bf16(Ctx* c, const L4Args& P);

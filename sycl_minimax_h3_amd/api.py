@@ -133,6 +133,13 @@ def candidates() -> list[str]:
     return out
 
 
+def _missing(what: str):
+    def call(*_):
+        raise OSError(what)
+
+    return call
+
+
 class Api:
     """The functions of include/h3hip.h, resolved once (engine/h3-sys/src/lib.rs:198-211)."""
 
@@ -147,14 +154,16 @@ class Api:
             fn.restype = res
             fn.argtypes = args
             setattr(self, name[len("h3s_"):], fn)
+        # h3lm's functions: a library without the table, or with an older and shorter one, serves everything else
         try:
             self.lm = LmApi.in_dll(self.lib, "h3lm")
+            size = self.lm.size
         except ValueError:
-            raise OSError(f"h3lm is missing from the library ({path})") from None
-        if self.lm.size < C.sizeof(LmApi):
-            raise OSError(f"h3lm is an older library's ({path})")
+            self.lm, size = None, 0
         for name, _ in LmApi._fields_[1:]:   # (a field read makes a function object: once here, not at every call)
-            setattr(self, "lm_" + name, getattr(self.lm, name))
+            field = getattr(LmApi, name)
+            there = field.offset + field.size <= size
+            setattr(self, "lm_" + name, getattr(self.lm, name) if there else _missing(f"h3lm's {name} is missing from the library ({path})"))
 
     def error(self) -> str:
         """The library's last error on this thread."""

@@ -84,9 +84,9 @@ template <int OP, int PARTS> __device__ __forceinline__ uint4 l4_codes(uint32_t 
     } else if constexpr (OP == H3S_F16) return make_uint4(((w << 6) & m) | e, ((w << 2) & m) | e, ((w >> 2) & m) | e, ((w >> 6) & m) | e);
     else return make_uint4(((w << 3) & m) | e, ((w >> 1) & m) | e, ((w >> 5) & m) | e, ((w >> 9) & m) | e);
 }
-// what x's sum is taken off with: the weights' distance from s times the operands
+// what x's sum is taken off with: the weights' distance from s times the operands (float32 x without minima has none)
 template <int PARTS> __device__ __forceinline__ float l4_off(float s, float least, bool mins) {
-    if constexpr (PARTS > 1) return mins ? __builtin_fmaf(-8.0f, s, least) : 0.0f;
+    if constexpr (PARTS > 1) return __builtin_fmaf(-8.0f, s, least);
     const float x = __builtin_fmaf(16.0f, s, least), y = 24.0f * s;
     return mins ? x : y;
 }
@@ -142,8 +142,8 @@ __device__ __forceinline__ void l4_exchange(const uint4& w, uint32_t (&c)[4]) {
 // The products of one step of 128 inputs: NT columns' codes and scales against MT x 16 rows. frag(a, j, f): the operand of the rows
 // 16 a .. and the run j (zeros past the row's end); AHEAD: a run's operands are asked for before the products of the one
 // before (from LDS: 300 rows 5376 -> 28672 247 to 211 us, 14336 -> 5376 127 to 120). Rows: place l of an operand is row 4 (l % 4) + l / 4,
-// so that register i of lane group g sums row 4 i + g and up to four rows take one multiply-add (NI of them).
-template <bool AHEAD, bool SUMS, int OP, int PARTS, int MT, int NT, int NI, int J, typename F>
+// so that register i of lane group g sums row 4 i + g.
+template <bool AHEAD, bool SUMS, int OP, int PARTS, int MT, int NT, int J, typename F>
 __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, uint32_t e, const uint32_t (&c)[NT][4], const float (&sc)[NT][4 / J], const float (&off)[NT],
                                             F frag, v4f_l4 (&acc)[MT][NT]) {
     v4f_l4 sx[MT];
@@ -187,7 +187,7 @@ __device__ __forceinline__ void l4_products(const uint4 (&sel)[4], uint32_t m, u
 #pragma unroll
             for (int b = 0; b < NT; ++b)
 #pragma unroll
-                for (int i = 0; i < NI; ++i) acc[a][b][i] = __builtin_fmaf(sc[b][q], y[a][b][i], acc[a][b][i]);
+                for (int i = 0; i < 4; ++i) acc[a][b][i] = __builtin_fmaf(sc[b][q], y[a][b][i], acc[a][b][i]);
     }
     if constexpr (!SUMS) return;
 #pragma unroll
@@ -211,11 +211,11 @@ __device__ __forceinline__ float l4_bias(const L4Args& P, int64_t n) {
     const float* p = P.bias ? P.bias + min(n, P.N - 1) : (const float*) P.codes;
     return *p;
 }
-template <int NI> __device__ __forceinline__ void l4_store(const L4Args& P, int64_t m0, int64_t n, int g, const v4f_l4& y, float read) {
+__device__ __forceinline__ void l4_store(const L4Args& P, int64_t m0, int64_t n, int g, const v4f_l4& y, float read) {
     const float bias = P.bias ? read : 0.0f;
     if (n >= P.N) return;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const int64_t m = m0 + 4 * i + g;
         if (m < P.M) store_any(P.out, P.out_dt, m * P.N + n, y[i] + bias);
     }
@@ -428,7 +428,7 @@ constexpr int kL4FewWaves = 12;       // wavefronts of a block, at most
 // J: runs of 32 inputs to one scale (4: groups are multiples of 128 inputs, 2: of 64, 1: of 32).
 // A block walks the tiles of 16 NT columns that are its own. Its KW wavefronts have 4 quads x 4 steps of 128 inputs each, one run of
 // memory in a weight row, and are joined through LDS at the end of a tile; the loads go on across tiles.
-// XR (one quad: up to 12 x 512 inputs): a wavefront's operands of x stay in registers. Otherwise they are loaded in the step that uses
+// XR (16-bit x, one quad: up to 12 x 512 inputs): a wavefront's operands of x stay in registers. Otherwise they are loaded in the step that uses
 // them (from the L2).
 template <int DT, int NT, int J, int SM, bool SUMS, bool XR>
 __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P, int quads) {
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P,
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 load_x(min(first + r, steps - 1), j, xr[r][j]);
-                if constexpr (DT != H3S_F32) xr[r][j].u = l4_order(xr[r][j].u);
+                xr[r][j].u = l4_order(xr[r][j].u);
             }
     }
     uint4 sel[4];
@@ -534,9 +534,9 @@ __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P,
             if (r + DP < 4) load_w(here, step + DP, w[r % DP]);
             else load_w(then, nfirst + r + DP - 4, w[r % DP]);
             if (step < steps) {
-                l4_products<false, SUMS, OP, PARTS, 1, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
-                    if constexpr (XR && DT != H3S_F32) f[0] = xr[r][j].u;
-                    else xr[XR ? r : 0][j].parts(f);
+                l4_products<false, SUMS, OP, PARTS, 1, NT, J>(sel, cm, ce, c, sc, off, [&](int, int j, uint4(&f)[PARTS]) {
+                    if constexpr (XR) f[0] = xr[r][j].u;
+                    else xr[0][j].parts(f);
                 }, acc);
             }
         }
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(64 * kL4FewWaves) void linear4_few_kernel(L4Args P,
                     const int64_t n = (int64_t) tile * (16 * NT) + 16 * b + l15;
                     v4f_l4 y = part[turn & 1][b][0][lane];
                     for (int v = 1; v < KW; ++v) y += part[turn & 1][b][v][lane];
-                    l4_store<4>(P, 0, n, g, y, l4_bias(P, n));
+                    l4_store(P, 0, n, g, y, l4_bias(P, n));
                 }
             }
             ++turn;
@@ -671,7 +671,7 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
                     }
                 }
                 load_w(min(step + KG, steps - 1));
-                l4_products<PARTS == 1, SUMS, OP, PARTS, MT, NT, 4, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
+                l4_products<PARTS == 1, SUMS, OP, PARTS, MT, NT, J>(sel, cm, ce, c, sc, off, [&](int a, int j, uint4(&f)[PARTS]) {
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) f[q] = xs[kg][r & 1][a][j][q][lane ^ g];
                 }, acc);
@@ -702,7 +702,7 @@ __global__ __launch_bounds__(512, 2) void linear4_many_kernel(L4Args P) {
                 v4f_l4 y = acc[a][b];
 #pragma unroll
                 for (int k = 0; k + 1 < KG; ++k) y += part[(((k * CG + wave) * MT + a) * NT + b) * 64 + lane];
-                l4_store<4>(P, m0 + 16 * a, n0 + 16 * b + l15, g, y, bias[b]);
+                l4_store(P, m0 + 16 * a, n0 + 16 * b + l15, g, y, bias[b]);
             }
     }
 }

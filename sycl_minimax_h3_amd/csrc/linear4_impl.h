@@ -231,7 +231,11 @@ template <int OP> __device__ __forceinline__ float l4_dot(uint32_t a, uint32_t b
     else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, a), __builtin_bit_cast(bf2, b), c, false);
 }
 
-constexpr int kL4DotWaves = 11;       // wavefronts of a block, at most
+// Wavefronts of a block, at most: three on a SIMD, as many as there are with 168 registers each. (Eleven: 6144 inputs in two chunks a wavefront
+// instead of one, 28672 columns 27 to 31 us where twelve take 21 to 25; 24576 inputs past the kernel, 8192 columns 34 to 67 instead of 29 to
+// 41; 5376 inputs the same. Against: float32, 12288 inputs -> 8192 columns 38 to 51 us here, 29 to 44 in linear4_few_kernel; with 28672 columns
+// 74 to 102 and 99 to 151.)
+constexpr int kL4DotWaves = 12;
 
 // A row of weights is cut into chunks of 512 inputs; a wavefront has U of them (every KW-th), with x's values for them in registers, and
 // walks down the rows: 16 lanes take a row's chunk, 32 codes each, four rows at a time. So its loads are runs of 256 bytes, the scale of a

@@ -34,6 +34,11 @@ LONG = [
     (1, 20000 * 32, 5, 32, True, "BF16", "F16"),
     (1, 1 << 20, 17, 64, False, "F16", "F16"),
     (1, 25600, 40, 128, False, "BF16", "F16"),
+    (1, 6144, 40, 64, True, "BF16", "F16"),             # twelve wavefronts with one, two and four chunks of 512 each, and one input run more
+    (1, 6176, 40, 32, False, "F32", "F16"),
+    (1, 12288, 40, 128, True, "F32", "F32"),
+    (1, 24576, 40, 32, True, "F16", "F16"),
+    (1, 24608, 40, 32, False, "BF16", "F16"),
     (1, 22528, 40, 64, True, "F16", "F16"),
     (1, 14336, 40, 32, True, "F32", "F32"),
     (1, 96 * 9999, 3, 96, True, "BF16", "BF16"),
@@ -123,3 +128,21 @@ def test_linear4_digits_of_float32(dev, M, K, mins, width, mean):
     err, other = (np.linalg.norm(y.astype(np.float64) - want) for y in (out.to_numpy(), plain))
     # both are sums of the same terms with a rounding each, in other orders: within two bits of each other
     assert err <= 4 * other, f"{err / other:.1f} times the error of float32 sums ({err / np.linalg.norm(want):.2e} of the result)"
+
+
+def test_linear4_more_blocks_than_a_launch_takes(dev):
+    """2^35 outputs (64 GiB): more blocks of threads than one launch has."""
+    M, K, N = (1 << 17) + 70, 32, 1 << 18
+    if dev.api.mem_free(dev.ctx) < 80 << 30:
+        pytest.skip("needs 80 GiB of the GPU's memory")
+    g = np.random.default_rng(93)
+    x = g.integers(-8, 9, (M, K)).astype(np.float32)
+    codes = g.integers(0, 256, (N, K // 2), dtype=np.uint8)
+    s = (2.0 ** g.integers(-2, 3, (N, 1))).astype(np.float32)
+    out = new(dev, "BF16", [M, N])
+    ops.Int4Linear(up(dev, codes, "U8", [N, K // 2]), up(dev, s, "F32", [N, 1])).forward(up(dev, x, "F32", [M, K]), out)
+    W, _, _ = weights(codes, s, None)
+    for m in (0, 31, 32, 65535, 65536, 100000, (1 << 17) - 1, 1 << 17, M - 1):
+        got = ref.from_bits(out._owner.read(2 * N, 2 * N * m).view(np.uint16), "BF16")
+        assert np.array_equal(got, ref.from_bits(ref.to_bits((x[m] @ W.T).astype(np.float32), "BF16"), "BF16")), m
+    out._owner.free()

@@ -38,3 +38,9 @@ def test_rows_of_the_cache_by_threads(lm, heads, b, fits):
     for fn in (lm.kv_write, lm.kv_read):
         rc = fn(None, cache(heads=heads, dim=8), batch(**b), P, P, 8 * heads, P, 8 * heads, A.F32)
         refused(rc, "no context" if fits else "too many blocks of work")
+
+
+@pytest.mark.parametrize("m,n,fits", [(1 << 31, 5376, True), ((1 << 31) + 1, 32, False), (7, 1 << 30, False), (1 << 20, 1 << 29, True)])
+def test_linear4_by_threads(lm, m, n, fits):
+    rc = lm.linear4(None, P, A.BF16, m, 32, P, n, P, None, A.F16, 32, None, P, A.BF16)
+    refused(rc, "no context" if fits else "too many rows or columns")

@@ -118,3 +118,20 @@ def test_read_where_nothing_is(dev, dt):
             assert not there.all()
             want[i * rows + starts[b]:i * rows + starts[b + 1], :heads * dim] = ref.to_bits(val.transpose(1, 0, 2).reshape(-1, heads * dim), dt)
     assert np.array_equal(y.to_numpy(), want)
+
+
+def test_a_table_of_no_blocks(dev):
+    """No cache block anywhere: writes do nothing, reads and attention give zeros."""
+    heads, dim = 2, 64
+    cache = ref.Cache(2, heads, dim, 106)
+    c = upload(dev, cache)
+    table, starts, past = new(dev, "I32", [2, 0]), i32(dev, [0, 1, 4]), i32(dev, [0, 90])
+    x = up(dev, np.ones((4, 2 * heads * dim), np.float32), "F32", [4, 2 * heads * dim])
+    r = [ops.Rows(x, i * heads * dim, 2 * heads * dim, 4, heads, dim) for i in (0, 1)]
+    ops.kv_write(c, table, r[0], r[1], starts, past, 3)
+    compare_cache(c, cache)
+    out, lse = up(dev, np.ones((4, heads * dim), np.float32), "F32", [4, heads * dim]), new(dev, "F32", [4, heads])
+    ops.kv_attention(c, table, r[0], starts, past, 3, out, lse=lse)
+    assert (out.to_numpy() == 0).all() and np.isneginf(lse.to_numpy()).all()
+    ops.kv_read(c, table, starts, past, 3, r[0], r[1])
+    assert (x.to_numpy() == 0).all()

@@ -492,7 +492,7 @@ template <int WC> __device__ __forceinline__ int kv_mix(int g, int c) { return (
 // Many rows: each of a block's four wavefronts has 16 NQ rows of its own, and all go through the same cache blocks. A block's codes
 // are turned to half once, by all four, into LDS in the order of the products' operands (two stages, one barrier a cache block), where
 // doing it in every wavefront took more vector instructions than the softmax. Bound by vector instructions beside the products (4096 tokens
-// over 8192, 64 heads over 8 of 128: 940-1060 us by the card, 0.78-0.87 PFLOP/s, the matrix cores 35 % busy). Operands are read from LDS a
+// over 8192, 64 heads over 8 of 128: 947-1060 us by the card, 0.78-0.87 PFLOP/s, the matrix cores 34 % busy). Operands are read from LDS a
 // step ahead of their products (960 us without, 16 sequences of 100 tokens of 256 features 203 to 181).
 template <int WC, int NQ, bool TWO>
 __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs P) {

@@ -77,7 +77,8 @@ typedef struct {
      * [rows, q_heads * dim] of type out_dt; lse NULL or float32 [rows, q_heads], the logarithm of the row's sum of exponentials. A row
      * that sees nothing gets zeros (lse -infinity). Hidden tokens have no effect, whatever their codes, scales and mask say.
      * Products, softmax and sums are float32 (q to 11 bits of each value for 16-bit types, which is all they have, 22 for float32;
-     * probabilities likewise), rounded once to out_dt.
+     * probabilities to 22, and to 11 for 16-bit q where a sequence has more than 32 rows times heads of a group, or 16 with dim above
+     * 128), rounded once to out_dt.
      * Lengths count as at least 0 and at most the table's 64 * width tokens. out may not overlap q.
      * max_len: about the longest of the lengths (0: the table's width); it only decides how the work is split. Sequences with many
      * rows and with few may be mixed: each takes the kernel for its number of rows.

@@ -8,9 +8,11 @@
 // Products on the matrix cores (16 x 16 x 32, half operands, float32 sums). The codes are whole numbers below 2^8, exact as
 // half. Query rows are scaled by a power of two that takes their largest value to 2^14 .. 2^15, so half holds 16-bit types
 // without loss down to 2^-29 of it; float32 rows are two halves (high and rest: 22 bits). Probabilities are 2^15 p, so that half keeps
-// them down to p = 2^-29 at full precision; for float32 queries they are two halves as well. (One half a probability is what 16-bit results
-// show little of: float16 queries over 500 tokens, the error against 64 bits 2.6e-4 of the result, 2.1e-4 with two halves; bfloat16 results 1.69e-3 and 1.68e-3. It
-// shows in float32 results of 16-bit queries: 1.5e-4 over 500 tokens, 0.8e-4 over 20000. Two would double the values' products.)
+// them down to p = 2^-29 at full precision. They are two halves too, but for many rows of 16-bit queries. (One half shows little in 16-bit
+// results: 500 tokens, the error against 64 bits in float16 2.6e-4 of the result, 2.1e-4 with two; in bfloat16 1.69e-3 and 1.68e-3. It shows in
+// float32 ones, 1.5e-4 and 2.5e-7. Two are 1-1.5 % of an answered token's time, whose bound is the cache's bytes - 64 sequences of up to 8192
+// tokens 131.0 and 132.2 us, one of 300 8.4 and 8.8 - but double the values' products of prompts, and two wavefronts a SIMD have no registers
+// for them.)
 //
 // Layout: S^T = K Q^T, with the keys as the first operand, leaves one query row a lane (lane % 16) and four keys a register
 // group; the row statistics are the lane's own but for two exchanges (lanes 16 and 32 apart). The rows of K are taken in the order
@@ -110,8 +112,8 @@ __device__ __forceinline__ float kv_lse(float m, float l) {
 }
 
 // What a wavefront holds of its 16 NQ query rows: row lane % 16 of each tile
-template <int WC, int NQ, bool TWO> struct KvRows {
-    static constexpr int W = 64 * WC, DT = 4 * WC, PARTS = TWO ? 2 : 1;
+template <int WC, int NQ, bool TWO, bool PTWO> struct KvRows {
+    static constexpr int W = 64 * WC, DT = 4 * WC, PARTS = TWO ? 2 : 1, PP = PTWO ? 2 : 1;   // halves of a query, of a probability
     int pos[NQ], head[NQ];                          // the row's token (-1: no row), its query head
     int64_t tok[NQ];                                // its row of q and out (-1: none)
     float rowf[NQ], m[NQ], l[NQ];
@@ -183,7 +185,7 @@ template <int WC, int NQ, bool TWO> struct KvRows {
     // One cache block's scores to probabilities: s (register t, i of lane group g: the key 16 g + 4 t + i of the block) to the operands
     // pf, times 2^15, and vsl, the factor of the block's values for each row. whole: every row sees every key.
     __device__ __forceinline__ void softmax(const KvAttnArgs& P, int b, int g, int key0, bool whole, float ks, float vs, v4f_kv (&s)[NQ][4],
-                                            v8h_kv (&pf)[NQ][2][PARTS], float (&vsl)[NQ]) {
+                                            v8h_kv (&pf)[NQ][2][PP], float (&vsl)[NQ]) {
         uint32_t hidden = 0;                        // by the mask: bit 4 t + i
         if (!whole && P.mask) {
             const int k0 = key0 + g * 16;
@@ -257,16 +259,16 @@ template <int WC, int NQ, bool TWO> struct KvRows {
                     const int at = 4 * (t & 1) + i;
                     const _Float16 hi = (_Float16) p;
                     pf[e][t >> 1][0][at] = hi;
-                    if constexpr (TWO) pf[e][t >> 1][1][at] = (_Float16) (p - (float) hi);
+                    if constexpr (PTWO) pf[e][t >> 1][1][at] = (_Float16) (p - (float) hi);
                 }
             l[e] += sum;
         }
     }
 
     // V^T P^T of a feature tile, whose codes of the keys 8 .. of each 16 are a1
-    __device__ __forceinline__ void products(const v8h_kv& a0, const v8h_kv& a1, const v8h_kv (&pf)[NQ][2][PARTS], v4f_kv (&y)[NQ]) const {
+    __device__ __forceinline__ void products(const v8h_kv& a0, const v8h_kv& a1, const v8h_kv (&pf)[NQ][2][PP], v4f_kv (&y)[NQ]) const {
 #pragma unroll
-        for (int w = 0; w < PARTS; ++w) {
+        for (int w = 0; w < PP; ++w) {
 #pragma unroll
             for (int e = 0; e < NQ; ++e) y[e] = kv_mma(a0, pf[e][0][w], w ? y[e] : v4f_kv{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
@@ -351,7 +353,7 @@ struct KvPages {
 
 // Few rows (up to 32 of a sequence and head): the four wavefronts of a block share 16 NQ rows and take every fourth cache block.
 // Bound by the cache's bytes: the next block's codes are on their way while one is worked on (64 sequences of up to 8192 tokens, 8 heads of
-// 128, 64 queries: 131 us, 4.9 TB/s; one of 131072 tokens 52.5 us, 5.1 TB/s, and the merge 4.8).
+// 128, 64 queries: 132 us, 4.9 TB/s; one of 131072 tokens 52.5 us, 5.1 TB/s, and the merge 4.8).
 template <int WC, int NQ, bool TWO>
 __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC, DT = 4 * WC, RT = 16 * NQ, KS = 4, PARTS = TWO ? 2 : 1;
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
         ks = P.kv.ks[(int64_t) page * P.kv.heads + h];
         vs = P.kv.vs[(int64_t) page * P.kv.heads + h];
     }
-    KvRows<WC, NQ, TWO> q;                          // (behind the first loads of the cache, which take longer)
+    KvRows<WC, NQ, TWO, true> q;                    // (behind the first loads of the cache, which take longer)
     q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
     while (kb < last) {
         int nkb = kb + KS, npage = 0;
@@ -424,7 +426,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
         }
         const int key0 = kb * kKvB;
         const bool whole = key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window) && !P.mask;
-        v8h_kv pf[NQ][2][PARTS];
+        v8h_kv pf[NQ][2][2];
         float vsl[NQ];
         q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
 #pragma unroll
@@ -549,7 +551,7 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
     bool more = false;
     float ks_now = 0.0f, vs_now = 0.0f;
     if (any) load(page);
-    KvRows<WC, NQ, TWO> q;
+    KvRows<WC, NQ, TWO, TWO> q;
     q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
     if (any) {
         stage(0);

@@ -194,3 +194,22 @@ def test_attention_of_prompts_beside_answers_recorded(dev):
     out, work = new(dev, "F32", [400, width]), new(dev, "U8", [ops.kv_attention_work(c, t, r400, starts, 100)])
     even = launches(dev, lambda: ops.kv_attention(c, t, r400, starts, lengths, 100, out, work=work))
     assert [name.split("<")[0] for name, _, _ in even] == ["kv_attn_rows_kernel", "kv_merge_kernel"], even
+
+
+# ---- digits of answered tokens -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dt", ["BF16", "F16"])
+@pytest.mark.parametrize("seqs,heads,group,dim,opts", [
+    ([(1, 500), (1, 64), (2, 3)], 2, 4, 128, {}),
+    ([(1, 5000)], 1, 8, 64, {}),
+    ([(4, 900), (3, 200)], 2, 8, 128, {"mask": 0.7}),
+    ([(1, 700)], 1, 3, 200, {"window": 300}),
+    ([(1, 300), (1, 1300)], 1, 8, 160, {}),
+])
+def test_attention_probabilities_of_answered_tokens_in_full(dev, seqs, heads, group, dim, dt, opts):
+    """16-bit queries of few rows: probabilities have float32's bits but two, as those of float32 queries."""
+    case = attn_case(dev, seqs, heads, group, dim, dt, opts, seed=86)
+    cache, table, starts, lengths, bits, q, rows, stride, mask = case
+    got, lse = run_attn(dev, *case, group, dt, "F32", {**opts, "lse": True})
+    want = ref.attention(cache, table, starts, lengths, q, group, "F32", "F32", None, opts.get("window", 0), mask)
+    check_attn(got, lse, want, int(starts[-1]), str(seqs))

@@ -59,6 +59,7 @@ static int attn_checks(const char* fn, const KvArgs& P, int64_t max_len, int64_t
     if (q_heads <= 0 || q_heads % P.heads != 0) return fail(std::string(fn) + ": the query heads must be a multiple of the key/value heads");
     if (q_heads > 65535) return fail(std::string(fn) + ": too many heads");
     if (max_len < 0 || window < 0) return fail(std::string(fn) + ": a negative length or window");
+    if ((int64_t) P.rows * (q_heads / P.heads) > INT32_MAX) return fail(std::string(fn) + ": too many rows");
     return 0;
 }
 
@@ -97,7 +98,6 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     const int64_t group = q_heads / A.kv.heads;
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
-    if (A.kv.rows * group > INT32_MAX) return fail(std::string(fn) + ": too many rows");
     const bool two = dt == H3S_F32;
     KvPlan plans[2];
     const int launches = kv_plans(A.kv, two, batch->most, group, max_len, window, c->cus, plans);

@@ -44,3 +44,11 @@ def test_rows_of_the_cache_by_threads(lm, heads, b, fits):
 def test_linear4_by_threads(lm, m, n, fits):
     rc = lm.linear4(None, P, A.BF16, m, 32, P, n, P, None, A.F16, 32, None, P, A.BF16)
     refused(rc, "no context" if fits else "too many rows or columns")
+
+
+def test_attention_rows_past_32_bits(lm):
+    """Rows times heads of a group are counted in 32 bits, by the call and by the size of its workspace alike."""
+    for b, heads, fits in ((dict(rows=1 << 30, most=4), 2, False), (dict(rows=1 << 30, most=4), 1, True), (dict(rows=(1 << 31) - 1, most=1 << 40, seqs=1 << 30), 65535, False)):
+        refused(lm.kv_attention_work(None, cache(heads=1, dim=8), batch(**b), 0, heads, 0), "no context" if fits else "too many rows")
+        refused(lm.kv_attention(None, cache(heads=1, dim=8), batch(**b), P, 0, P, 8 * heads, A.F32, heads, 0.0, 0, None, 0, P, A.F32, None, None, 0),
+                "no context" if fits else "too many rows")

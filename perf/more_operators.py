@@ -258,6 +258,7 @@ def _handles(s):
         h["q"] = ops.Rows(h["rows"], 0, wide, rows, heads, dk)
         h["k"] = ops.Rows(h["rows"], heads * dk, wide, rows, kv, dk)
         h["v"] = ops.Rows(h["rows"], (heads + kv) * dk, wide, rows, kv, dv)
+        h["states"] = ops.LinState(h["state"])
     else:
         heads, dim = case["kv"] * case["group"], case["dim"]
         h["cache"] = ops.KvCache(h["k"], h["v"], h["k_scale"], h["v_scale"], dim)
@@ -270,7 +271,7 @@ def _handles(s):
 def _run_own(s):
     h, t, case = s.get("handles") or _handles(s), s["t"], s["case"]
     if case["kind"] == "linear":
-        h["ops"].lin_attention(h["state"], h["decay"], h["q"], h["k"], h["v"], h["starts"], h["source"], h["target"], max(s["new"]), h["out"])
+        h["ops"].lin_attention(h["states"], h["decay"], h["q"], h["k"], h["v"], h["starts"], h["source"], h["target"], max(s["new"]), h["out"])
         return t["out"], t["state"]
     h["ops"].kv_attention(h["cache"], h["table"], h["queries"], h["starts"], h["lengths"], max(s["new"]), h["out"], max_len=max(s["lengths"]),
                           window=case["window"], sinks=case["sinks"], shared=h["groups"], mask=h.get("mask"), lse=h.get("lse"))

@@ -1,7 +1,7 @@
 /* h3lm.h - the operators of libh3hip.so that run a language model token by token: an 8-bit key/value cache, the attention
- * that reads it, and linear layers with 4-bit weights. They stand beside h3hip.h's causal attention and linear layers (the
- * text encoder's whole-sequence forms) and follow its conventions: device pointers of the context's GPU, asynchronous on the
- * context's stream in call order, 0 or -1 with the reason in h3s_last_error(), arguments checked before any work is queued,
+ * that reads it, linear attention, whose state stands in the cache's place, and linear layers with 4-bit weights. They stand
+ * beside h3hip.h's causal attention and linear layers (the text encoder's whole-sequence forms) and follow its conventions:
+ * device pointers of the context's GPU, asynchronous on the context's stream in call order, 0 or -1 with the reason in h3s_last_error(), arguments checked before any work is queued,
  * empty shapes do nothing. No counterpart in the reference.
  *
  * The library's function names are the reference's header and its additions (h3hip.h) and stay that set; these operators are
@@ -48,6 +48,22 @@ typedef struct {
     const int32_t* starts;   /* [seqs + 1] */
     int64_t seqs, width, rows, most;
 } h3_kv_batch;
+
+/* One linear attention layer's states: a pool of `slots` of them, each float32 [dk, dv] for `heads` heads; dk and dv 1 to 256. */
+typedef struct {
+    float* s;                /* [slots, heads, dk, dv] */
+    int64_t slots, heads, dk, dv;
+} h3_lin_state;
+
+/* The sequences of one lin_attention call: sequence b's tokens are the rows starts[b] .. starts[b + 1] - 1 of the row operands (as in
+ * h3_kv_batch, rows behind starts[seqs] neither read nor written). It goes on from the state in slot source[b] and leaves its own in slot
+ * target[b] (they may be one); an entry outside 0 .. slots - 1 is no state: it begins with zeros, or its state is dropped. A sequence without
+ * rows leaves its target as it is. No slot may be the target of two sequences, or the target of one and the source of another. `most`: at
+ * least the most rows of any sequence (one that has more gets results for its first `most` rows or more, and a state of some of its rows). */
+typedef struct {
+    const int32_t *starts, *source, *target;   /* [seqs + 1], [seqs], [seqs] */
+    int64_t seqs, rows, most;
+} h3_lin_batch;
 
 typedef struct {
     int64_t size;            /* bytes of this table: a later library's is longer */
@@ -104,6 +120,20 @@ typedef struct {
      * out infinite or NaN (and no other row), and so may values whose sums times 31 leave float32. */
     int (*linear4)(void* ctx, const void* x, int dt, int64_t M, int64_t K, const uint8_t* codes, int64_t N, const void* scale,
                    const void* mins, int scale_dt, int64_t group, const float* bias, void* out, int out_dt);
+
+    /* Linear attention with a decay for each head. A sequence's tokens, in order, for each head h of the states:
+     *     S = exp(-decay[h]) S + k v^T,   out = scale * q S
+     * q and k rows of q_heads and k_heads times dk features, v rows of v_heads times dv, all of type dt at their element strides; each
+     * number of heads divides the states' and head h reads head h / (heads / theirs). out [rows, heads * dv] of type out_dt. decay float32
+     * [heads], 0 or more (infinity: only the token itself). scale 0: 1 / sqrt(dk), else above 0. States, sums and decays are
+     * float32. An infinity or NaN in a token's values of a head leaves the sequence's earlier tokens as they are, and may make any of that
+     * head's results from that token on, and its state, infinite or NaN. out may not overlap q, k or v.
+     * work: as kv_attention's, of at least lin_attention_work(...) bytes. */
+    int (*lin_attention)(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, const float* decay, const void* q, int64_t q_stride,
+                         int64_t q_heads, const void* k, int64_t k_stride, int64_t k_heads, const void* v, int64_t v_stride, int64_t v_heads,
+                         int dt, float scale, void* out, int out_dt, void* work, uint64_t work_bytes);
+    /* The bytes that lin_attention needs for these arguments (0: none), or -1. */
+    int64_t (*lin_attention_work)(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, int dt);
 } h3_lm_api;
 
 extern const h3_lm_api h3lm;

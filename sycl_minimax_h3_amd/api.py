@@ -104,11 +104,26 @@ class KvBatch(C.Structure):
     _fields_ = [("table", vp), ("starts", vp), ("seqs", i64), ("width", i64), ("rows", i64), ("most", i64)]
 
 
+class LinState(C.Structure):
+    """include/h3lm.h's h3_lin_state."""
+
+    _fields_ = [("s", vp), ("slots", i64), ("heads", i64), ("dk", i64), ("dv", i64)]
+
+
+class LinBatch(C.Structure):
+    """include/h3lm.h's h3_lin_batch."""
+
+    _fields_ = [("starts", vp), ("source", vp), ("target", vp), ("seqs", i64), ("rows", i64), ("most", i64)]
+
+
 KV_BLOCK = 64
 # h3_kv_batch's fields as bytes, which go through a pointer argument faster than a structure is made
 _batch_fields = struct.Struct("PPqqqq")
 kv_batch = _batch_fields.pack   # (table, starts, seqs, width, rows, most)
 assert _batch_fields.size == C.sizeof(KvBatch)
+_lin_batch_fields = struct.Struct("PPPqqq")
+lin_batch = _lin_batch_fields.pack   # (starts, source, target, seqs, rows, most)
+assert _lin_batch_fields.size == C.sizeof(LinBatch)
 
 
 class LmApi(C.Structure):
@@ -121,6 +136,8 @@ class LmApi(C.Structure):
         ("kv_attention", C.CFUNCTYPE(i32, vp, vp, vp, vp, i64, vp, i64, i32, i64, f32, i64, vp, i64, vp, i32, vp, vp, u64)),
         ("kv_attention_work", C.CFUNCTYPE(i64, vp, vp, vp, i64, i64, i64)),
         ("linear4", C.CFUNCTYPE(i32, vp, vp, i32, i64, i64, vp, i64, vp, vp, i32, i64, vp, vp, i32)),
+        ("lin_attention", C.CFUNCTYPE(i32, vp, vp, vp, vp, vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, f32, vp, i32, vp, u64)),
+        ("lin_attention_work", C.CFUNCTYPE(i64, vp, vp, vp, i32)),
     ]
 
 

@@ -1,0 +1,186 @@
+// lin_attn.hip - lin_attention and lin_attention_work (h3lm.h): the checks, the choice of the kernel, and the form for few tokens.
+//
+// Mathematics, for one head of one sequence: S = exp(-decay) S + k v^T and out = scale q S, token by token. A column of S meets only its
+// own feature of v, so the features of v are split over blocks of threads without an exchange between them.
+#include <algorithm>
+#include <cmath>
+
+#include "lin.h"
+
+namespace h3 {
+
+constexpr int kLinCols = 32;                        // columns of S that a block of threads takes: 128 bytes of each row
+constexpr int kLinToks = 8;                         // tokens whose rows lie in LDS at once
+
+// Few tokens: a block of 256 threads holds 32 columns of a head's state in registers, rows r + 32 i and four columns a thread, over all
+// tokens of the sequence. A token's sum over the rows of S is left as 32 parts in LDS and added up once for up to eight tokens. exp(-decay) is
+// applied as S - (1 - exp(-decay)) S: a decay near 1 is held to 32 bits of its distance from 1, which is what far tokens' weights
+// depend on. Bound by the state's bytes, read and written once.
+template <int DKR, bool VEC>
+__global__ __launch_bounds__(256) void lin_step_kernel(LinArgs P) {
+    constexpr int K = 32 * DKR;
+    __shared__ float sq[kLinToks][K], sk[kLinToks][K], sv[kLinToks][kLinCols];
+    __shared__ float4 part[kLinToks][4][8];
+    uint32_t id = blockIdx.x;
+    const uint32_t slices = (uint32_t) (P.dv + kLinCols - 1) / kLinCols;
+    const int c0 = (int) (id % slices) * kLinCols;
+    id /= slices;
+    const int h = (int) (id % (uint32_t) P.heads), b = (int) (id / (uint32_t) P.heads);
+    int r0, n;
+    kv_rows_of(P.kv, b, r0, n);
+    if (n == 0 || (uint32_t) n < P.least || (uint32_t) n > P.most) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = c0 + 4 * (threadIdx.x & 7), r = threadIdx.x >> 3;
+    const int64_t from = P.source[b], to = P.target[b];
+    const int64_t head = (int64_t) P.dk * P.dv;
+    float s[DKR][4];
+    const bool begun = from >= 0 && from < P.slots;
+    const float* sp = P.s + ((begun ? from : 0) * P.heads + h) * head;
+#pragma unroll
+    for (int i = 0; i < DKR; ++i) {
+        const int row = r + 32 * i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+        if (!begun || row >= P.dk) continue;
+        if constexpr (VEC) {
+            if (c < P.dv) load_f32x(sp + (int64_t) row * P.dv + c, s[i], 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < P.dv) s[i][j] = sp[(int64_t) row * P.dv + c + j];
+        }
+    }
+    const float less = expm1f(-P.decay[h]);          // exp(-decay) - 1
+    const int64_t qo = (int64_t) (h / P.q_each) * P.dk, ko = (int64_t) (h / P.k_each) * P.dk, vo = (int64_t) (h / P.v_each) * P.dv + c0;
+    for (int t0 = 0; t0 < n; t0 += kLinToks) {
+        const int toks = min(n - t0, kLinToks);
+        if (t0) __syncthreads();
+        for (int i = threadIdx.x; i < toks * K; i += 256) {
+            const int t = i / K, d = i % K;
+            const int64_t row = (int64_t) r0 + t0 + t;
+            sq[t][d] = d < P.dk ? load_any(P.q, P.dt, row * P.q_stride + qo + d) : 0.0f;
+            sk[t][d] = d < P.dk ? load_any(P.k, P.dt, row * P.k_stride + ko + d) : 0.0f;
+        }
+        if ((int) threadIdx.x < toks * kLinCols) {
+            const int t = threadIdx.x / kLinCols, d = threadIdx.x % kLinCols;
+            sv[t][d] = c0 + d < P.dv ? load_any(P.v, P.dt, ((int64_t) r0 + t0 + t) * P.v_stride + vo + d) : 0.0f;
+        }
+        __syncthreads();
+        for (int t = 0; t < toks; ++t) {
+            const float4 v = *reinterpret_cast<const float4*>(&sv[t][4 * (threadIdx.x & 7)]);
+            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const float vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < DKR; ++i) {
+                const float kd = sk[t][r + 32 * i], qd = sq[t][r + 32 * i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[i][j] = __builtin_fmaf(kd, vv[j], __builtin_fmaf(s[i][j], less, s[i][j]));
+                    y[j] = __builtin_fmaf(qd, s[i][j], y[j]);
+                }
+            }
+            // over the wavefront's eight rows
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                y[j] += xor_lane<8>(y[j]);
+                y[j] += xor_lane<16>(y[j]);
+                y[j] += xor_lane<32>(y[j]);
+            }
+            if (lane < 8) part[t][wave][lane] = make_float4(y[0], y[1], y[2], y[3]);
+        }
+        __syncthreads();
+        if ((int) threadIdx.x < toks * kLinCols) {
+            const int t = threadIdx.x / kLinCols, d = threadIdx.x % kLinCols;
+            const float* p = reinterpret_cast<const float*>(&part[t][0][0]) + d;
+            const float y = (p[0] + p[32]) + (p[64] + p[96]);
+            if (c0 + d < P.dv) store_any(P.out, P.out_dt, (((int64_t) r0 + t0 + t) * P.heads + h) * P.dv + c0 + d, y * P.scale);
+        }
+    }
+    if (to < 0 || to >= P.slots) return;
+    float* tp = P.s + (to * P.heads + h) * head;
+#pragma unroll
+    for (int i = 0; i < DKR; ++i) {
+        const int row = r + 32 * i;
+        if (row >= P.dk) continue;
+        if constexpr (VEC) {
+            if (c < P.dv) *reinterpret_cast<float4*>(tp + (int64_t) row * P.dv + c) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < P.dv) tp[(int64_t) row * P.dv + c + j] = s[i][j];
+        }
+    }
+}
+
+template <int DKR> static void lin_step(Ctx* c, const LinArgs& P, int64_t blocks) {
+    if (P.s_vec) lin_step_kernel<DKR, true><<<(unsigned) blocks, 256, 0, c->stream>>>(P);
+    else lin_step_kernel<DKR, false><<<(unsigned) blocks, 256, 0, c->stream>>>(P);
+}
+
+static int lin_checks(const std::string& fn, const h3_lin_state* state, const h3_lin_batch* batch, int dt) {
+    if (!state || !batch) return fail(fn + ": the states and the batch are required");
+    if (state->slots <= 0 || state->heads <= 0 || state->dk <= 0 || state->dv <= 0 || state->dk > 256 || state->dv > 256)
+        return fail(fn + ": states have slots, heads and 1 to 256 features of keys and of values");
+    if (state->slots > INT32_MAX || state->heads > 65535) return fail(fn + ": too many slots or heads");
+    if (!state->s) return fail(fn + ": the states are required");
+    if ((uintptr_t) state->s & 3) return fail(fn + ": the states must be 4-byte aligned");
+    if (batch->seqs < 0 || batch->rows < 0 || batch->most < 0) return fail(fn + ": a negative size");
+    if (batch->rows > INT32_MAX || batch->seqs >= INT32_MAX) return fail(fn + ": sizes past 32 bits");
+    if (!dt_ok(dt)) return fail(fn + ": unknown element type");
+    return 0;
+}
+
+int64_t lin_attention_work(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, int dt) try {
+    const char* fn = "lin_attention_work";
+    if (lin_checks(fn, state, batch, dt)) return -1;
+    Ctx* c = ctx_of(ctx, fn);
+    if (!c) return -1;
+    return 0;
+} catch (const std::exception& e) { return fail(e.what()); }
+
+int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, const float* decay, const void* q, int64_t q_stride,
+                  int64_t q_heads, const void* k, int64_t k_stride, int64_t k_heads, const void* v, int64_t v_stride, int64_t v_heads,
+                  int dt, float scale, void* out, int out_dt, void* work, uint64_t work_bytes) try {
+    const std::string fn = "lin_attention";
+    if (lin_checks(fn, state, batch, dt)) return -1;
+    if (!dt_ok(out_dt)) return fail(fn + ": unknown element type");
+    const int64_t heads = state->heads, dk = state->dk, dv = state->dv;
+    if (q_heads <= 0 || k_heads <= 0 || v_heads <= 0 || heads % q_heads || heads % k_heads || heads % v_heads)
+        return fail(fn + ": the states' heads must be a multiple of q's, k's and v's");
+    if (!(scale >= 0.0f) || std::isinf(scale)) return fail(fn + ": the scale must be a number above 0 (or 0: 1 / sqrt(dk))");
+    if (batch->seqs == 0 || batch->rows == 0 || batch->most == 0) return 0;
+    if (!batch->starts || !batch->source || !batch->target) return fail(fn + ": starts, source and target are required");
+    if (q_stride < q_heads * dk || k_stride < k_heads * dk || v_stride < v_heads * dv) return fail(fn + ": a row stride is shorter than a row");
+    if (!decay || !q || !k || !v || !out) return fail(fn + ": decay, q, k, v and out are required");
+    if (work && !aligned16(work)) return fail(fn + ": the workspace must be 16-byte aligned");
+    const int es = elem_size(dt);
+    auto vec = [&](const void* p, int64_t stride, int64_t dim) { return aligned16(p) && stride * es % 16 == 0 && dim * es % 16 == 0; };
+    LinArgs P{};
+    P.s = state->s;
+    P.slots = state->slots;
+    P.heads = (int) heads; P.dk = (int) dk; P.dv = (int) dv;
+    P.kv.starts = batch->starts; P.kv.seqs = (int) batch->seqs; P.kv.rows = (int) batch->rows;
+    P.source = batch->source; P.target = batch->target; P.decay = decay;
+    P.q = q; P.k = k; P.v = v;
+    P.q_stride = q_stride; P.k_stride = k_stride; P.v_stride = v_stride;
+    P.q_each = (int) (heads / q_heads); P.k_each = (int) (heads / k_heads); P.v_each = (int) (heads / v_heads);
+    P.dt = dt; P.out = out; P.out_dt = out_dt;
+    P.scale = scale > 0.0f ? scale : (float) (1.0 / std::sqrt((double) dk));
+    P.least = 0; P.most = UINT32_MAX;
+    P.q_vec = vec(q, q_stride, dk); P.k_vec = vec(k, k_stride, dk); P.v_vec = vec(v, v_stride, dv);
+    P.s_vec = aligned16(P.s) && dv % 4 == 0;
+    P.out_vec = aligned16(out) && dv % 4 == 0;
+    const int64_t blocks = batch->seqs * heads * ((dv + kLinCols - 1) / kLinCols);
+    if (blocks > kKvMostBlocks) return fail(fn + ": too many blocks of work");
+    Ctx* c = ctx_of(ctx, fn.c_str());
+    if (!c) return -1;
+    switch ((dk + 63) / 64) {
+        case 1: lin_step<2>(c, P, blocks); break;
+        case 2: lin_step<4>(c, P, blocks); break;
+        case 3: lin_step<6>(c, P, blocks); break;
+        default: lin_step<8>(c, P, blocks); break;
+    }
+    return launched(fn.c_str());
+} catch (const std::exception& e) { return fail(e.what()); }
+
+}  // namespace h3

@@ -404,7 +404,7 @@ def int8_quantize(x: Tensor, q: Tensor, s: Tensor, group: int = 0) -> None:
     dev.check(dev.api.int8_quantize(dev.ctx, x.ptr(), x.dtype.kernel_code(), m, k, group, q.ptr(), s.ptr()))
 
 
-# ---- the operators of include/h3lm.h: an 8-bit key/value cache, the attention over it, linear layers with 4-bit weights ----
+# ---- the operators of include/h3lm.h: an 8-bit key/value cache, the attention over it, linear attention, linear layers with 4-bit weights ----
 
 KV_BLOCK = _api.KV_BLOCK   # tokens in a block of the cache
 
@@ -523,6 +523,63 @@ def kv_attention(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, lengths
             mask_n, out.ptr(), out.dtype.kernel_code(), _p(lse), _p(work), work.nbytes() if work is not None else 0)
     dev = _dev(cache.k)
     dev.check(dev.api.lm_kv_attention(dev.ctx, cache._p, batch, *args))
+
+
+class LinState:
+    """One linear attention layer's states (h3_lin_state): float32 [slots, heads, dk, dv], a slot for each sequence that is carried on."""
+
+    def __init__(self, s: Tensor):
+        if s.dtype is not DType.F32 or len(s.shape) != 4:
+            raise Error(f"lin state: the states must be float32 [slots, heads, dk, dv], got {s.dtype} {s.shape}")
+        self.s = s
+        self.slots, self.heads, self.dk, self.dv = (int(n) for n in s.shape)
+        if not (1 <= self.dk <= 256 and 1 <= self.dv <= 256) or self.slots < 1 or self.heads < 1:
+            raise Error(f"lin state: slots, heads and 1 to 256 features of keys and of values, got {s.shape}")
+        self._c = _api.LinState(s.ptr(), self.slots, self.heads, self.dk, self.dv)
+        self._p = _C.addressof(self._c)
+
+    @staticmethod
+    def new(dev, slots: int, heads: int, dk: int, dv: int) -> "LinState":
+        """States of their own memory; a slot's contents are undefined until a sequence leaves its state there."""
+        return LinState(Tensor.new(dev, DType.F32, [slots, heads, dk, dv]))
+
+
+def _lin_batch(starts: Tensor, source: Tensor, target: Tensor, rows: int, most: int):
+    n = starts.elements() - 1
+    if n < 0 or source.elements() != n or target.elements() != n:
+        raise Error(f"lin_attention: starts {starts.shape}, source {source.shape} and target {target.shape} are not of the same sequences")
+    if most < 0:
+        raise Error(f"the most rows of a sequence: {most}")
+    return _api.lin_batch(_i32(starts, "starts", n + 1), _i32(source, "source", n), _i32(target, "target", n), n, rows, most)
+
+
+def lin_attention_work(state: LinState, q: Rows, starts: Tensor, source: Tensor, target: Tensor, most: int) -> int:
+    """The bytes of workspace that lin_attention takes for these arguments (0: none)."""
+    dev = _dev(state.s)
+    n = dev.api.lm_lin_attention_work(dev.ctx, state._p, _lin_batch(starts, source, target, q.tokens, most), q.t.dtype.kernel_code())
+    if n < 0:
+        raise Error(dev.api.error())
+    return n
+
+
+def lin_attention(state: LinState, decay: Tensor, q: Rows, k: Rows, v: Rows, starts: Tensor, source: Tensor, target: Tensor, most: int,
+                  out: Tensor, *, scale: float = 0.0, work: Tensor | None = None) -> None:
+    """Linear attention with a decay for each head, token by token: S = exp(-decay) S + k v^T, out = scale * q S. Sequence b's tokens are
+    the rows starts[b] .. of q, k, v and out [rows, heads * dv]; it goes on from the state in slot source[b] (-1: from zeros) and leaves its
+    own in slot target[b] (-1: nowhere). q, k and v may each have fewer heads than the states, shared by neighbours. decay float32 [heads];
+    scale 0: 1 / sqrt(dk); most: at least the most rows of any sequence. work: a workspace of lin_attention_work() bytes, which a call
+    recorded into a graph has to bring if that is not 0."""
+    if q.dim != state.dk or k.dim != state.dk or v.dim != state.dv:
+        raise Error(f"lin_attention: heads of {q.dim}, {k.dim} and {v.dim} for states of {state.dk} x {state.dv}")
+    if q.tokens != k.tokens or q.tokens != v.tokens or q.t.dtype is not k.t.dtype or q.t.dtype is not v.t.dtype:
+        raise Error("lin_attention: q, k and v must share their rows and their type")
+    if out.elements() != q.tokens * state.heads * state.dv:
+        raise Error(f"lin_attention: out {out.shape} for {q.tokens} rows of {state.heads} x {state.dv}")
+    batch = _lin_batch(starts, source, target, q.tokens, most)
+    args = (_floats(decay, "the decay", state.heads), q.ptr(), q.stride, q.heads, k.ptr(), k.stride, k.heads, v.ptr(), v.stride, v.heads,
+            q.t.dtype.kernel_code(), scale, out.ptr(), out.dtype.kernel_code(), _p(work), work.nbytes() if work is not None else 0)
+    dev = _dev(state.s)
+    dev.check(dev.api.lm_lin_attention(dev.ctx, state._p, batch, *args))
 
 
 @dataclass

@@ -67,6 +67,7 @@ struct Ctx {
         LIN_F32,     // h3s_linear / h3s_linear_acc: the float32 product of a row chunk
         GEMM_PART,   // the matrix-core GEMMs: the accumulators of the split last tiles' parts
         KV_PART,     // kv_attention: the parts' sums (O, m, l)
+        LIN_STATE,   // lin_attention: the segments' sums and first states
         N_REGIONS
     };
     struct Area { void* p = nullptr; size_t bytes = 0; };

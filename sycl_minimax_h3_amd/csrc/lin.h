@@ -20,6 +20,8 @@ struct LinArgs {
     void* out;
     int out_dt;
     uint32_t least, most;                           // sequences of fewer or more rows are another launch's
+    int slices, seg;                                // in pieces: ranges of v's features, tokens of a segment
+    float* ws;                                      // the segments' sums, then their first states, one for each block of threads
     bool q_vec, k_vec, v_vec, s_vec, out_vec;       // rows that can be read (written) 16 bytes at a time
 };
 

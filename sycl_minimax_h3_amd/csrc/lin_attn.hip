@@ -5,7 +5,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "lin.h"
+#include "lin_chunk_impl.h"
 
 namespace h3 {
 
@@ -112,6 +112,49 @@ __global__ __launch_bounds__(256) void lin_step_kernel(LinArgs P) {
     }
 }
 
+// The states at the segments' beginnings, where their own sums were: a thread has 16 bytes of a state through all segments of a sequence.
+// (Blocks: 256 threads a 4 KiB piece of a state in the kernel's own layout, of a head, slice and sequence.)
+template <int KC, int NV>
+__global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs P) {
+    constexpr int FR = 2 * KC * NV;
+    uint32_t id = blockIdx.x;
+    const int fr = (int) (id % FR);
+    id /= FR;
+    const int h = (int) (id % (uint32_t) P.heads);
+    id /= (uint32_t) P.heads;
+    const int slice = (int) (id % (uint32_t) P.slices), b = (int) (id / (uint32_t) P.slices);
+    int r0, n;
+    kv_rows_of(P.kv, b, r0, n);
+    const int segs = (n + P.seg - 1) / P.seg;
+    if (segs < 2 || (uint32_t) n < P.least || (uint32_t) n > P.most) return;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int t = fr / NV, x = fr % NV;
+    const int c = slice * 64 * NV + wave * 16 * NV + (NV == 2 ? 8 * (l15 >> 2) + 4 * x + (l15 & 3) : l15);
+    const int64_t from = P.source[b];
+    v4f_lin s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (from >= 0 && from < P.slots && c < P.dv) {
+        const float* sp0 = P.s + (from * P.heads + h) * ((int64_t) P.dk * P.dv);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 16 * (t & ~1) + 8 * g + 4 * (t & 1) + i;
+            if (d < P.dk) s[i] = sp0[(int64_t) d * P.dv + c];
+        }
+    }
+    const float less = expm1f(-P.decay[h] * (float) P.seg);
+    const int64_t place = r0 / P.seg + b, step = (int64_t) P.slices * P.heads * (FR * 1024);
+    float* ws = P.ws + ((place * P.slices + slice) * P.heads + h) * (FR * 1024) + fr * 1024 + threadIdx.x * 4;
+    for (int j = 0; j < segs; ++j, ws += step) {
+        const v4f_lin own = j + 1 < segs ? *reinterpret_cast<const v4f_lin*>(ws) : v4f_lin{0.0f, 0.0f, 0.0f, 0.0f};
+        *reinterpret_cast<v4f_lin*>(ws) = s;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(s[i], less, s[i]) + own[i];
+    }
+}
+
+template <int KC, int NV> static void lin_scan_run(Ctx* c, const LinArgs& P) {
+    lin_scan_kernel<KC, NV><<<(unsigned) ((int64_t) P.kv.seqs * P.slices * P.heads * 2 * KC * NV), 256, 0, c->stream>>>(P);
+}
+
 template <int DKR> static void lin_step(Ctx* c, const LinArgs& P, int64_t blocks) {
     if (P.s_vec) lin_step_kernel<DKR, true><<<(unsigned) blocks, 256, 0, c->stream>>>(P);
     else lin_step_kernel<DKR, false><<<(unsigned) blocks, 256, 0, c->stream>>>(P);
@@ -130,12 +173,39 @@ static int lin_checks(const std::string& fn, const h3_lin_state* state, const h3
     return 0;
 }
 
+// Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces.
+// Segments: as many as give each CU two blocks of threads, of at least kLinLeast tokens.
+constexpr int kLinFew = 16, kLinLeast = 256;
+struct LinPlan {
+    bool step, chunk, split;
+    int kc, nv, slices;
+    int64_t seg, places, blocks, floats;
+};
+static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, int cus) {
+    LinPlan p{};
+    const int64_t most = std::min(batch.most, batch.rows), chains = batch.seqs * state.heads;
+    p.chunk = most > kLinFew;
+    p.step = !p.chunk || (batch.seqs > 1 && most * batch.seqs > batch.rows);
+    p.kc = (int) (state.dk + 63) / 64 * 2;
+    p.nv = state.dv > 64 && p.kc <= 4 ? 2 : 1;
+    p.slices = (int) (state.dv + 64 * p.nv - 1) / (64 * p.nv);
+    const int64_t want = std::max<int64_t>(1, 2 * (int64_t) cus / (chains * p.slices));
+    p.seg = std::max<int64_t>(kLinLeast, ((most + want - 1) / want + 63) / 64 * 64);
+    p.split = p.seg < most;
+    if (!p.split) p.seg = most;
+    p.places = p.split ? batch.rows / p.seg + batch.seqs : batch.seqs;
+    p.blocks = p.places * p.slices * state.heads;
+    p.floats = p.chunk && p.split ? p.blocks * (2 * p.kc * p.nv * 1024) : 0;
+    return p;
+}
+
 int64_t lin_attention_work(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, int dt) try {
     const char* fn = "lin_attention_work";
     if (lin_checks(fn, state, batch, dt)) return -1;
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
-    return 0;
+    if (batch->seqs == 0 || batch->rows == 0 || batch->most == 0) return 0;
+    return 4 * lin_plan(*state, *batch, c->cus).floats;
 } catch (const std::exception& e) { return fail(e.what()); }
 
 int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, const float* decay, const void* q, int64_t q_stride,
@@ -170,15 +240,53 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
     P.q_vec = vec(q, q_stride, dk); P.k_vec = vec(k, k_stride, dk); P.v_vec = vec(v, v_stride, dv);
     P.s_vec = aligned16(P.s) && dv % 4 == 0;
     P.out_vec = aligned16(out) && dv % 4 == 0;
-    const int64_t blocks = batch->seqs * heads * ((dv + kLinCols - 1) / kLinCols);
-    if (blocks > kKvMostBlocks) return fail(fn + ": too many blocks of work");
     Ctx* c = ctx_of(ctx, fn.c_str());
     if (!c) return -1;
-    switch ((dk + 63) / 64) {
-        case 1: lin_step<2>(c, P, blocks); break;
-        case 2: lin_step<4>(c, P, blocks); break;
-        case 3: lin_step<6>(c, P, blocks); break;
-        default: lin_step<8>(c, P, blocks); break;
+    const LinPlan plan = lin_plan(*state, *batch, c->cus);
+    const int64_t steps = batch->seqs * heads * ((dv + kLinCols - 1) / kLinCols), scans = batch->seqs * heads * plan.slices * 2 * plan.kc * plan.nv;
+    if ((plan.step && steps > kKvMostBlocks) || (plan.chunk && (plan.blocks > kKvMostBlocks || (plan.split && scans > kKvMostBlocks))))
+        return fail(fn + ": too many blocks of work");
+    if (plan.floats) {
+        if (work) {
+            if (work_bytes < (uint64_t) (4 * plan.floats)) return fail(fn + ": the workspace is smaller than lin_attention_work() says");
+            P.ws = (float*) work;
+        } else {
+            hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+            if (hipStreamIsCapturing(c->stream, &st) != hipSuccess) (void) hipGetLastError();
+            if (st != hipStreamCaptureStatusNone) return fail(fn + ": a call recorded into a graph needs a workspace of its own");
+            P.ws = c->scratch<float>(Ctx::LIN_STATE, (size_t) plan.floats);
+            if (!P.ws) return -1;
+        }
+    }
+    if (plan.step) {
+        P.most = plan.chunk ? kLinFew : UINT32_MAX;
+        switch (plan.kc) {
+            case 2: lin_step<2>(c, P, steps); break;
+            case 4: lin_step<4>(c, P, steps); break;
+            case 6: lin_step<6>(c, P, steps); break;
+            default: lin_step<8>(c, P, steps); break;
+        }
+    }
+    if (plan.chunk) {
+        P.least = plan.step ? kLinFew + 1 : 0;
+        P.most = UINT32_MAX;
+        P.slices = plan.slices;
+        P.seg = (int) plan.seg;
+        auto run = [&](bool outputs) {
+            if (dt == H3S_BF16) lin_chunk_bf16(c, P, plan.kc, plan.nv, plan.blocks, outputs);
+            else if (dt == H3S_F16) lin_chunk_f16(c, P, plan.kc, plan.nv, plan.blocks, outputs);
+            else lin_chunk_f32(c, P, plan.kc, plan.nv, plan.blocks, outputs);
+        };
+        if (plan.split) {
+            run(false);
+            if (plan.kc == 2 && plan.nv == 1) lin_scan_run<2, 1>(c, P);
+            else if (plan.kc == 2) lin_scan_run<2, 2>(c, P);
+            else if (plan.kc == 4 && plan.nv == 1) lin_scan_run<4, 1>(c, P);
+            else if (plan.kc == 4) lin_scan_run<4, 2>(c, P);
+            else if (plan.kc == 6) lin_scan_run<6, 1>(c, P);
+            else lin_scan_run<8, 1>(c, P);
+        }
+        run(true);
     }
     return launched(fn.c_str());
 } catch (const std::exception& e) { return fail(e.what()); }

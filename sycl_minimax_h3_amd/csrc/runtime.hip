@@ -110,6 +110,7 @@ static const char* region_name(Ctx::Region r) {
         case Ctx::ATT_AUX: return "attention scratch (scales and k's mean)";
         case Ctx::ATT_PART: return "attention scratch (partial sums)";
         case Ctx::KV_PART: return "cached attention scratch (partial sums)";
+        case Ctx::LIN_STATE: return "linear attention scratch (segments' states)";
         case Ctx::LIN_F32: return "linear scratch (float32 product)";
         default: return "scratch";
     }

@@ -49,6 +49,14 @@ typedef struct {
     int64_t seqs, width, rows, most;
 } h3_kv_batch;
 
+/* Groups of sequences whose caches begin with the same tokens: group g is the sequences first[g] .. first[g + 1] - 1 (ascending; sequences
+ * outside all groups share nothing), and the first tokens[g] / 64 entries of their rows of the table name the same blocks (those of its first
+ * sequence's row are read; a last block that is not whole belongs to each sequence alone). */
+typedef struct {
+    const int32_t *first, *tokens;   /* [groups + 1], [groups] */
+    int64_t groups, most;            /* most: about the most of tokens (0: the table's width); it only decides how the work is split */
+} h3_kv_shared;
+
 /* One linear attention layer's states: a pool of `slots` of them, each float32 [dk, dv] for `heads` heads; dk and dv 1 to 256. */
 typedef struct {
     float* s;                /* [slots, heads, dk, dv] */
@@ -120,6 +128,20 @@ typedef struct {
      * out infinite or NaN (and no other row), and so may values whose sums times 31 leave float32. */
     int (*linear4)(void* ctx, const void* x, int dt, int64_t M, int64_t K, const uint8_t* codes, int64_t N, const void* scale,
                    const void* mins, int scale_dt, int64_t group, const float* bias, void* out, int out_dt);
+
+    /* kv_attention where a row sees more than its window, or sequences share tokens: the tokens 0 .. p, of them, if window is above 0, the
+     * last `window` and the first `sinks`, of them those that the mask leaves. With shared not NULL (and groups not 0), the tokens that a group's
+     * sequences share are gone through once for all rows of the group, which changes the order of sums, not what a row sees. Blocks
+     * that no row sees any more need not be there (an entry of -1). Arguments, results and workspace as kv_attention's; probabilities
+     * of shared tokens are held to 11 bits for 16-bit q where the call's rows times heads of a group, by group of sequences, are more than 32
+     * (or 16 with dim above 128), to 22 otherwise. */
+    int (*kv_attention_spans)(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, const int32_t* lengths,
+                              int64_t max_len, const void* q, int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window,
+                              int64_t sinks, const uint8_t* mask, int64_t mask_stride, void* out, int out_dt, float* lse, void* work,
+                              uint64_t work_bytes);
+    /* The bytes that kv_attention_spans needs for these arguments (0: none), or -1. */
+    int64_t (*kv_attention_spans_work)(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared,
+                                       int64_t max_len, int64_t q_heads, int64_t window, int64_t sinks);
 
     /* Linear attention with a decay for each head. A sequence's tokens, in order, for each head h of the states:
      *     S = exp(-decay[h]) S + k v^T,   out = scale * q S

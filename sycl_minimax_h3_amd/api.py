@@ -104,6 +104,12 @@ class KvBatch(C.Structure):
     _fields_ = [("table", vp), ("starts", vp), ("seqs", i64), ("width", i64), ("rows", i64), ("most", i64)]
 
 
+class KvShared(C.Structure):
+    """include/h3lm.h's h3_kv_shared."""
+
+    _fields_ = [("first", vp), ("tokens", vp), ("groups", i64), ("most", i64)]
+
+
 class LinState(C.Structure):
     """include/h3lm.h's h3_lin_state."""
 
@@ -136,6 +142,8 @@ class LmApi(C.Structure):
         ("kv_attention", C.CFUNCTYPE(i32, vp, vp, vp, vp, i64, vp, i64, i32, i64, f32, i64, vp, i64, vp, i32, vp, vp, u64)),
         ("kv_attention_work", C.CFUNCTYPE(i64, vp, vp, vp, i64, i64, i64)),
         ("linear4", C.CFUNCTYPE(i32, vp, vp, i32, i64, i64, vp, i64, vp, vp, i32, i64, vp, vp, i32)),
+        ("kv_attention_spans", C.CFUNCTYPE(i32, vp, vp, vp, vp, vp, i64, vp, i64, i32, i64, f32, i64, i64, vp, i64, vp, i32, vp, vp, u64)),
+        ("kv_attention_spans_work", C.CFUNCTYPE(i64, vp, vp, vp, vp, i64, i64, i64, i64)),
         ("lin_attention", C.CFUNCTYPE(i32, vp, vp, vp, vp, vp, i64, i64, vp, i64, i64, vp, i64, i64, i32, f32, vp, i32, vp, u64)),
         ("lin_attention_work", C.CFUNCTYPE(i64, vp, vp, vp, i32)),
     ]

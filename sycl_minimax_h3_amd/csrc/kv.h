@@ -62,6 +62,11 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
                  int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window, const uint8_t* mask, int64_t mask_stride,
                  void* out, int out_dt, float* lse, void* work, uint64_t work_bytes);
 int64_t kv_attention_work(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, int64_t max_len, int64_t q_heads, int64_t window);
+int kv_attention_spans(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, const int32_t* lengths,
+                       int64_t max_len, const void* q, int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window, int64_t sinks,
+                       const uint8_t* mask, int64_t mask_stride, void* out, int out_dt, float* lse, void* work, uint64_t work_bytes);
+int64_t kv_attention_spans_work(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, int64_t max_len,
+                                int64_t q_heads, int64_t window, int64_t sinks);
 int linear4(void* ctx, const void* x, int dt, int64_t M, int64_t K, const uint8_t* codes, int64_t N, const void* scale, const void* mins,
             int scale_dt, int64_t group, const float* bias, void* out, int out_dt);
 

@@ -1,5 +1,5 @@
-// kv_attn.hip - kv_attention and kv_attention_work (h3lm.h) on the kernels of kv_attn_impl.h: the checks, the choice of the
-// kernel and of the parts that the cache is split into, and the workspace.
+// kv_attn.hip - kv_attention and kv_attention_spans with the sizes of their workspaces (h3lm.h) on the kernels of kv_attn_impl.h: the checks,
+// the choice of the kernel and of the parts that the cache is split into, and the workspace.
 #include <algorithm>
 #include <cmath>
 
@@ -20,7 +20,12 @@ namespace h3 {
 // blocks of threads that it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up
 // to 8192 tokens, 64 heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and
 // their merge 4, 7 and 11 us more. Longer parts: one sequence of 2000 tokens in parts of 8, 16 and 32 blocks 12.6, 15.5 and 18.5 us.)
-static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus) {
+// What decides the plans beside the batch: the heads of a group, about the longest length, the window, and (kv_attention_spans) the first tokens
+// that stay visible, the groups of sequences and about the longest of their shared tokens.
+struct KvSight { int64_t group, max_len, window, sinks, groups, shared; };
+
+static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus) {
+    const int64_t group = sight.group, max_len = sight.max_len, window = sight.window;
     KvPlan plan;
     const int64_t rows = std::min<int64_t>(most, P.rows) * group;
     auto even = [&](int64_t rt) { return (rows + rt - 1) / rt * P.seqs; };
@@ -32,7 +37,8 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, int64_t group, in
     plan.places = std::min(even(plan.rt), ragged(plan.rt));
     plan.blocks = plan.places * P.heads;
     int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
-    if (window > 0) keys = std::min(keys, std::min<int64_t>(window, INT32_MAX) + std::min<int64_t>(most, P.rows) + 2 * kKvB);
+    if (sight.groups) keys = std::max<int64_t>(keys - sight.shared, std::min<int64_t>(most, P.rows));
+    if (window > 0) keys = std::min(keys, std::min<int64_t>(window, INT32_MAX) + std::min<int64_t>(most, P.rows) + 2 * kKvB + std::min<int64_t>(sight.sinks, INT32_MAX));
     const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
     plan.per = (int) std::max(least, (blocks + want - 1) / want);
@@ -43,17 +49,37 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, int64_t group, in
 // to 16 (or 32: larger groups) are a launch of the shared-rows kernel if that splits their caches further: a prompt of 2048 tokens
 // beside a token over 131072, 64 heads over 8 of 128, 3469 us in one launch, 191 in two (129 and 49 by themselves); four prompts of 241 to 600
 // tokens behind up to 900, for which the second finds nothing to do, 70 and 69.
-static int kv_plans(const KvArgs& P, bool two, int64_t most, int64_t group, int64_t max_len, int64_t window, int cus, KvPlan (&plan)[2]) {
-    plan[0] = kv_plan(P, two, most, group, max_len, window, cus);
+static int kv_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[2]) {
+    const int64_t group = sight.group;
+    plan[0] = kv_plan(P, two, most, sight, cus);
     const int64_t few = (group <= 16 ? 16 : 32) / group;                         // tokens
     if (!plan[0].rows || few == 0 || (group > 16 && P.dim > 128) || std::min<int64_t>(most, P.rows) * P.seqs <= P.rows) return 1;
-    plan[1] = kv_plan(P, two, few, group, max_len, window, cus);
+    plan[1] = kv_plan(P, two, few, sight, cus);
     if (plan[1].nsplit <= plan[0].nsplit) return 1;
     plan[1].greatest = (uint32_t) (few * group);
     plan[0].least = plan[1].greatest + 1;
     return 2;
 }
-static int64_t kv_part_floats(const KvPlan& plan, int64_t W) { return plan.nsplit > 1 ? plan.blocks * plan.nsplit * plan.rt * (W + 2) : 0; }
+// The launch of the shared tokens: all rows of a group are as one sequence's, and how many groups' rows there are is known, not each one's.
+static KvPlan kv_shared_plan(const KvArgs& P, bool two, const KvSight& sight, int cus) {
+    KvPlan plan;
+    const int64_t rows = P.rows * sight.group, each = (rows + sight.groups - 1) / sight.groups;
+    auto places = [&](int64_t rt) { return rows / rt + sight.groups; };
+    plan.rows = each > (P.dim <= 128 ? 32 : 16);
+    plan.nq = plan.rows ? (two || each <= 96 || places(128) * P.heads < cus ? 1 : 2) : each <= 16 ? 1 : 2;
+    plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
+    plan.tiles = 0;
+    plan.places = places(plan.rt);
+    plan.blocks = plan.places * P.heads;
+    const int64_t blocks = std::max<int64_t>((sight.shared + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
+    plan.per = (int) std::max(least, (blocks + want - 1) / want);
+    plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
+    return plan;
+}
+static int64_t kv_part_floats(const KvPlan& plan, int64_t W, bool always) {
+    return plan.nsplit > 1 || always ? plan.blocks * plan.nsplit * plan.rt * (W + 2) : 0;
+}
 
 static int attn_checks(const char* fn, const KvArgs& P, int64_t max_len, int64_t q_heads, int64_t window) {
     if (q_heads <= 0 || q_heads % P.heads != 0) return fail(std::string(fn) + ": the query heads must be a multiple of the key/value heads");
@@ -63,30 +89,54 @@ static int attn_checks(const char* fn, const KvArgs& P, int64_t max_len, int64_t
     return 0;
 }
 
-int64_t kv_attention_work(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, int64_t max_len, int64_t q_heads, int64_t window) try {
-    const char* fn = "kv_attention_work";
+// The sizes that a call with or without groups has; -1 with the reason
+static int sight_of(const std::string& fn, const KvArgs& P, const h3_kv_shared* shared, int64_t max_len, int64_t q_heads, int64_t window, int64_t sinks,
+                    KvSight& sight) {
+    if (attn_checks(fn.c_str(), P, max_len, q_heads, window)) return -1;
+    if (sinks < 0) return fail(fn + ": a negative number of first tokens");
+    sight = KvSight{q_heads / P.heads, max_len, window, window > 0 ? sinks : 0, 0, 0};
+    if (!shared || shared->groups == 0) return 0;
+    if (shared->groups < 0 || shared->most < 0) return fail(fn + ": a negative number of groups or shared tokens");
+    if (shared->groups >= INT32_MAX) return fail(fn + ": too many groups");
+    if (!shared->first || !shared->tokens) return fail(fn + ": the groups' first sequences and shared tokens are required");
+    sight.groups = shared->groups;
+    sight.shared = shared->most > 0 ? std::min<int64_t>(shared->most, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
+    return 0;
+}
+// all launches' plans: of the shared tokens first, where there are any
+static int kv_all_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[3]) {
+    KvPlan own[2];
+    const int n = kv_plans(P, two, most, sight, cus, own), at = sight.groups ? 1 : 0;
+    if (at) plan[0] = kv_shared_plan(P, two, sight, cus);
+    for (int i = 0; i < n; ++i) plan[at + i] = own[i];
+    return at + n;
+}
+
+static int64_t attend_work(const char* fn, void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, int64_t max_len,
+                           int64_t q_heads, int64_t window, int64_t sinks) {
     KvArgs P;
-    if (kv_args(fn, cache, batch, P) || attn_checks(fn, P, max_len, q_heads, window)) return -1;
+    KvSight sight;
+    if (kv_args(fn, cache, batch, P) || sight_of(fn, P, shared, max_len, q_heads, window, sinks, sight)) return -1;
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
     if (P.seqs == 0 || P.rows == 0 || batch->most == 0) return 0;
     // (the more of what 16-bit and float32 queries take)
     int64_t floats = 0;
     for (bool two : {false, true}) {
-        KvPlan plan[2];
+        KvPlan plan[3];
         int64_t sum = 0;
-        for (int n = kv_plans(P, two, batch->most, q_heads / P.heads, max_len, window, c->cus, plan); n-- > 0;) sum += kv_part_floats(plan[n], kv_width(P.dim));
+        for (int n = kv_all_plans(P, two, batch->most, sight, c->cus, plan); n-- > 0;) sum += kv_part_floats(plan[n], kv_width(P.dim), sight.groups > 0);
         floats = std::max(floats, sum);
     }
     return 4 * floats;
-} catch (const std::exception& e) { return fail(e.what()); }
+}
 
-int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* lengths, int64_t max_len, const void* q,
-                 int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window, const uint8_t* mask, int64_t mask_stride,
-                 void* out, int out_dt, float* lse, void* work, uint64_t work_bytes) try {
-    const char* fn = "kv_attention";
-    KvAttnArgs A;
-    if (kv_args(fn, cache, batch, A.kv) || attn_checks(fn, A.kv, max_len, q_heads, window)) return -1;
+static int attend(const char* fn, void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, const int32_t* lengths,
+                  int64_t max_len, const void* q, int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window, int64_t sinks,
+                  const uint8_t* mask, int64_t mask_stride, void* out, int out_dt, float* lse, void* work, uint64_t work_bytes) {
+    KvAttnArgs A{};
+    KvSight sight;
+    if (kv_args(fn, cache, batch, A.kv) || sight_of(fn, A.kv, shared, max_len, q_heads, window, sinks, sight)) return -1;
     if (!dt_ok(dt) || !dt_ok(out_dt)) return fail(std::string(fn) + ": unknown element type");
     if (!(scale >= 0.0f) || std::isinf(scale)) return fail(std::string(fn) + ": the scale must be a number above 0 (or 0: 1 / sqrt(dim))");
     if (mask && mask_stride < 0) return fail(std::string(fn) + ": a negative mask stride");
@@ -95,24 +145,23 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     if (q_stride < q_heads * dim) return fail(std::string(fn) + ": the row stride is shorter than a row");
     if (!lengths || !q || !out) return fail(std::string(fn) + ": lengths, q and out are required");
     if (work && !aligned16(work)) return fail(std::string(fn) + ": the workspace must be 16-byte aligned");
-    const int64_t group = q_heads / A.kv.heads;
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
-    const bool two = dt == H3S_F32;
-    KvPlan plans[2];
-    const int launches = kv_plans(A.kv, two, batch->most, group, max_len, window, c->cus, plans);
+    const bool two = dt == H3S_F32, groups = sight.groups > 0;
+    KvPlan plans[3];
+    const int launches = kv_all_plans(A.kv, two, batch->most, sight, c->cus, plans);
     const int64_t W = kv_width(dim);
     int64_t floats = 0;
     for (int i = 0; i < launches; ++i) {
         // (the merge has a block of threads a row)
-        if (plans[i].blocks > kKvMostBlocks || plans[i].blocks * (plans[i].nsplit > 1 ? std::max(plans[i].nsplit, plans[i].rt) : 1) > kKvMostBlocks)
-            return fail(std::string(fn) + ": too many blocks of work");
-        floats += kv_part_floats(plans[i], W);
+        const int64_t each = std::max<int64_t>(plans[i].nsplit, plans[i].nsplit > 1 || groups ? plans[i].rt : 1);
+        if (plans[i].blocks > kKvMostBlocks || plans[i].blocks * each > kKvMostBlocks) return fail(std::string(fn) + ": too many blocks of work");
+        floats += kv_part_floats(plans[i], W, groups);
     }
     float* parts = nullptr;
     if (floats) {
         if (work) {
-            if (work_bytes < (uint64_t) (4 * floats)) return fail(std::string(fn) + ": the workspace is smaller than kv_attention_work() says");
+            if (work_bytes < (uint64_t) (4 * floats)) return fail(std::string(fn) + ": the workspace is smaller than " + fn + "_work() says");
             parts = (float*) work;
         } else {
             hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
@@ -123,7 +172,7 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
         }
     }
     A.lengths = lengths;
-    A.q = q; A.q_stride = q_stride; A.q_dt = dt; A.group = (int) group; A.q_heads = (int) q_heads;
+    A.q = q; A.q_stride = q_stride; A.q_dt = dt; A.group = (int) sight.group; A.q_heads = (int) q_heads;
     A.scale = (float) ((scale > 0.0f ? (double) scale : 1.0 / std::sqrt((double) dim)) * 1.4426950408889634);
     A.window = (int) std::min<int64_t>(window, INT32_MAX / 2);
     A.mask = mask; A.mask_stride = mask_stride;
@@ -131,21 +180,57 @@ int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, 
     A.q_vec = aligned16(q) && dim % 8 == 0 && (q_stride * elem_size(dt)) % 16 == 0;
     A.out_vec = aligned16(out) && dim % 4 == 0;
     A.mask_vec = mask && aligned16(mask) && mask_stride % 16 == 0;
+    A.sinks = (int) std::min<int64_t>(sight.sinks, INT32_MAX / 2);
+    if (groups) { A.first = shared->first; A.shared = shared->tokens; A.groups = (int) sight.groups; }
     for (int i = 0; i < launches; ++i) {
         const KvPlan& plan = plans[i];
         A.tiles = (int) plan.tiles; A.places = (int) plan.places; A.nsplit = plan.nsplit; A.per = plan.per;
         A.least = plan.least; A.greatest = plan.greatest;
         A.po = parts;
         A.pml = parts ? parts + plan.blocks * plan.nsplit * plan.rt * W : nullptr;
-        if (parts) parts += kv_part_floats(plan, W);
-        switch (W / 64) {
-            case 1: kv_attn_64(c, A, plan, two); break;
-            case 2: kv_attn_128(c, A, plan, two); break;
-            case 3: kv_attn_192(c, A, plan, two); break;
-            default: kv_attn_256(c, A, plan, two); break;
+        if (parts) parts += kv_part_floats(plan, W, groups);
+        const bool first = groups && i == 0;
+        if (groups || A.sinks > 0) {
+            switch (W / 64) {
+                case 1: kv_spans_64(c, A, plan, two, first); break;
+                case 2: kv_spans_128(c, A, plan, two, first); break;
+                case 3: kv_spans_192(c, A, plan, two, first); break;
+                default: kv_spans_256(c, A, plan, two, first); break;
+            }
+        } else {
+            switch (W / 64) {
+                case 1: kv_attn_64(c, A, plan, two); break;
+                case 2: kv_attn_128(c, A, plan, two); break;
+                case 3: kv_attn_192(c, A, plan, two); break;
+                default: kv_attn_256(c, A, plan, two); break;
+            }
         }
+        if (first) { A.rt2 = plan.rt; A.nsplit2 = plan.nsplit; A.po2 = A.po; A.pml2 = A.pml; }
     }
     return launched(fn);
+}
+
+int64_t kv_attention_work(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, int64_t max_len, int64_t q_heads, int64_t window) try {
+    return attend_work("kv_attention_work", ctx, cache, batch, nullptr, max_len, q_heads, window, 0);
+} catch (const std::exception& e) { return fail(e.what()); }
+
+int kv_attention(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const int32_t* lengths, int64_t max_len, const void* q,
+                 int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window, const uint8_t* mask, int64_t mask_stride,
+                 void* out, int out_dt, float* lse, void* work, uint64_t work_bytes) try {
+    return attend("kv_attention", ctx, cache, batch, nullptr, lengths, max_len, q, q_stride, dt, q_heads, scale, window, 0, mask, mask_stride, out, out_dt,
+                  lse, work, work_bytes);
+} catch (const std::exception& e) { return fail(e.what()); }
+
+int64_t kv_attention_spans_work(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, int64_t max_len,
+                                int64_t q_heads, int64_t window, int64_t sinks) try {
+    return attend_work("kv_attention_spans_work", ctx, cache, batch, shared, max_len, q_heads, window, sinks);
+} catch (const std::exception& e) { return fail(e.what()); }
+
+int kv_attention_spans(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, const int32_t* lengths,
+                       int64_t max_len, const void* q, int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window, int64_t sinks,
+                       const uint8_t* mask, int64_t mask_stride, void* out, int out_dt, float* lse, void* work, uint64_t work_bytes) try {
+    return attend("kv_attention_spans", ctx, cache, batch, shared, lengths, max_len, q, q_stride, dt, q_heads, scale, window, sinks, mask, mask_stride, out,
+                  out_dt, lse, work, work_bytes);
 } catch (const std::exception& e) { return fail(e.what()); }
 
 }  // namespace h3

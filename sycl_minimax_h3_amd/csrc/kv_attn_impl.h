@@ -59,7 +59,17 @@ struct KvAttnArgs {
     int nsplit, per;                                // parts, of `per` cache blocks each (the last: the rest)
     float *po, *pml;                                // the parts' sums [place, head, part, rows, W] and (m, l) [place, head, part, rows, 2]
     bool q_vec, out_vec, mask_vec;
+    // of kv_attention_spans:
+    int sinks;                                      // the first tokens that stay visible behind a window
+    const int32_t *first, *shared;                  // [groups + 1]: a group's first sequence; [groups]: the tokens that it shares
+    int groups;
+    int rt2, nsplit2;                               // the rows of a block, and the parts, of the shared tokens' launch
+    const float *po2, *pml2;                        // its parts
 };
+
+// What a launch goes through. kKvAll: all of a sequence's cache up to the row, or a window of it. kKvOwn: of that the first tokens too, and only
+// what lies behind the tokens that a sequence shares. kKvShared: the shared tokens, for all rows of a group of sequences as if they were one's.
+enum { kKvAll, kKvOwn, kKvShared };
 
 // four codes as half: 2^10 + (code + 128) in the low bits of a half, less 2^10 + 128 (exact)
 __device__ __forceinline__ void kv_half4(uint32_t u, v2h_kv& a, v2h_kv& b) {
@@ -112,16 +122,19 @@ __device__ __forceinline__ float kv_lse(float m, float l) {
 }
 
 // What a wavefront holds of its 16 NQ query rows: row lane % 16 of each tile
-template <int WC, int NQ, bool TWO, bool PTWO> struct KvRows {
+template <int WC, int NQ, bool TWO, bool PTWO, int MODE> struct KvRows {
     static constexpr int W = 64 * WC, DT = 4 * WC, PARTS = TWO ? 2 : 1, PP = PTWO ? 2 : 1;   // halves of a query, of a probability
     int pos[NQ], head[NQ];                          // the row's token (-1: no row), its query head
+    int seq[MODE == kKvShared ? NQ : 1];            // its sequence
     int64_t tok[NQ];                                // its row of q and out (-1: none)
     float rowf[NQ], m[NQ], l[NQ];
     v8h_kv qf[NQ][WC][2][PARTS];
     v4f_kv o[NQ][DT];
 
     // rows rw .. of the R of a sequence with n rows from r0 on and len tokens, for key/value head h
-    __device__ __forceinline__ void load(const KvAttnArgs& P, int h, int r0, int n, int len, uint32_t R, uint32_t rw, int l15, int g) {
+    // (kKvShared: with the rows' tokens and sequences in `who`, from rw on)
+    __device__ __forceinline__ void load(const KvAttnArgs& P, int h, int r0, int n, int len, uint32_t R, uint32_t rw, int l15, int g,
+                                         const int2* who = nullptr) {
         const uint32_t group = P.group;
 #pragma unroll
         for (int e = 0; e < NQ; ++e) {
@@ -130,7 +143,12 @@ template <int WC, int NQ, bool TWO, bool PTWO> struct KvRows {
             const int j = (int) (r / group);
             head[e] = (int) (h * group + r % group);
             tok[e] = valid ? (int64_t) r0 + j : -1;
-            pos[e] = valid ? len - n + j : -1;
+            if constexpr (MODE == kKvShared) {
+                pos[e] = who[16 * e + l15].x;
+                seq[e] = max(who[16 * e + l15].y, 0);
+            } else {
+                pos[e] = valid ? len - n + j : -1;
+            }
             const int64_t row = ((int64_t) r0 + j) * P.q_stride + (int64_t) head[e] * P.kv.dim;
             float f[WC * 2][8];
             float top = 0.0f;
@@ -182,33 +200,44 @@ template <int WC, int NQ, bool TWO, bool PTWO> struct KvRows {
         }
     }
 
+    // the lane's keys of a cache block that the mask hides
+    static __device__ __forceinline__ uint32_t masked(const KvAttnArgs& P, int b, int g, int key0) {
+        uint32_t hidden = 0;
+        const int k0 = key0 + g * 16;
+        const uint8_t* mp = P.mask + (int64_t) b * P.mask_stride + k0;
+        if (P.mask_vec && k0 + 16 <= P.mask_stride) {
+            const uint4 u = *reinterpret_cast<const uint4*>(mp);
+            const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 16; ++i) hidden |= ((w4[i >> 2] >> (8 * (i & 3))) & 0xffu) == 0 ? 1u << i : 0u;
+        } else {
+            for (int i = 0; i < 16; ++i)
+                if (k0 + i >= P.mask_stride || mp[i] == 0) hidden |= 1u << i;
+        }
+        return hidden;
+    }
+
     // One cache block's scores to probabilities: s (register t, i of lane group g: the key 16 g + 4 t + i of the block) to the operands
     // pf, times 2^15, and vsl, the factor of the block's values for each row. whole: every row sees every key.
     __device__ __forceinline__ void softmax(const KvAttnArgs& P, int b, int g, int key0, bool whole, float ks, float vs, v4f_kv (&s)[NQ][4],
                                             v8h_kv (&pf)[NQ][2][PP], float (&vsl)[NQ]) {
         uint32_t hidden = 0;                        // by the mask: bit 4 t + i
-        if (!whole && P.mask) {
-            const int k0 = key0 + g * 16;
-            const uint8_t* mp = P.mask + (int64_t) b * P.mask_stride + k0;
-            if (P.mask_vec && k0 + 16 <= P.mask_stride) {
-                const uint4 u = *reinterpret_cast<const uint4*>(mp);
-                const uint32_t w4[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int i = 0; i < 16; ++i) hidden |= ((w4[i >> 2] >> (8 * (i & 3))) & 0xffu) == 0 ? 1u << i : 0u;
-            } else {
-                for (int i = 0; i < 16; ++i)
-                    if (k0 + i >= P.mask_stride || mp[i] == 0) hidden |= 1u << i;
-            }
-        }
+        if (MODE != kKvShared && !whole && P.mask) hidden = masked(P, b, g, key0);
 #pragma unroll
         for (int e = 0; e < NQ; ++e) {
             uint32_t off = hidden;
             if (!whole) {
+                if (MODE == kKvShared && P.mask) off = masked(P, seq[e], g, key0);
                 const int hi = pos[e] - key0 - g * 16;                  // the lane's keys 0 .. hi of 16 are not ahead of the row
                 off |= hi >= 15 ? 0u : hi < 0 ? 0xffffu : 0xffffu & (0xfffeu << hi);
                 if (P.window > 0) {
                     const int lo = hi - P.window + 1;                    // and lo .. are inside the window
-                    off |= lo <= 0 ? 0u : lo > 15 ? 0xffffu : (1u << lo) - 1;
+                    uint32_t behind = lo <= 0 ? 0u : lo > 15 ? 0xffffu : (1u << lo) - 1;
+                    if constexpr (MODE != kKvAll) {
+                        const int first = P.sinks - key0 - g * 16;       // of them the first ones stay
+                        behind &= first <= 0 ? 0xffffu : first > 15 ? 0u : 0xffffu << first;
+                    }
+                    off |= behind;
                 }
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
@@ -284,11 +313,48 @@ template <int WC, int NQ, bool TWO, bool PTWO> struct KvRows {
     }
 };
 
+// The group that sequence b shares tokens in, or -1; found by the whole wavefront, 64 groups at a time (as kv_find).
+__device__ __forceinline__ int kv_group_of(const KvAttnArgs& P, int b) {
+    const int lane = threadIdx.x & 63;
+    int step = 1;
+    while (step * 64 < P.groups + 1) step *= 64;
+    for (int g = 0;; step /= 64) {
+        const int c = g + lane * step, f = P.first[min(c, P.groups)];
+        const int k = (int) __popcll(__ballot(c <= P.groups && f <= b) & ~1ull);
+        g += k * step;
+        if (step > 1) continue;
+        const int from = __builtin_amdgcn_readlane(f, k), to = k < 63 ? __builtin_amdgcn_readlane(f, k + 1) : P.first[min(g + 1, P.groups)];
+        return from <= b && g < P.groups && b < to ? g : -1;
+    }
+}
+// the first row of group c's sequences (of `groups`: behind the last), whatever `first` and `starts` say
+__device__ __forceinline__ int kv_group_row(const KvAttnArgs& P, int c) {
+    return min(max(P.kv.starts[min(max(P.first[min(c, P.groups)], 0), P.kv.seqs)], 0), P.kv.rows);
+}
+// kv_find of groups in place of sequences: each is as one sequence of all its rows
+__device__ __forceinline__ int kv_find_group(const KvAttnArgs& P, int at, uint32_t den, int& grp, int& r0, int& n) {
+    const int lane = threadIdx.x & 63;
+    int step = 1;
+    while (step * 64 < P.groups) step *= 64;
+    for (grp = 0;; step /= 64) {
+        const int c = grp + lane * step, s = kv_group_row(P, c);
+        const int begin = (int) ((uint32_t) s * (uint32_t) P.group / den) + min(c, P.groups);
+        const int k = (int) __popcll(__ballot(c < P.groups && begin <= at) & ~1ull);
+        grp += k * step;
+        if (step > 1) continue;
+        r0 = __builtin_amdgcn_readlane(s, k);
+        n = max(k < 63 ? __builtin_amdgcn_readlane(s, k + 1) : kv_group_row(P, grp + 1), r0) - r0;
+        return at - __builtin_amdgcn_readlane(begin, k);
+    }
+}
+
 // Which rows, head, sequence and part of the cache a block of threads has. Sequences with about as many rows each have P.tiles tiles of RT
 // rows; else each has its share: R of all sequences' rows lie in at most floor(R / RT) + 1 of the places from floor(its first / RT) + its number on.
-struct KvItem {
+template <int MODE> struct KvItem {
     int h, split, place, b, tile, r0, n, len;
     uint32_t R;
+    int b1 = 0;                                                           // kKvShared: behind the group's last sequence
+    int lo = 0, hi = 0, sink = 0, win = 0;                                // cache blocks: see range()
     template <int RT> __device__ __forceinline__ void take(const KvAttnArgs& P) {
         uint32_t id = blockIdx.x;
         h = (int) (id % (uint32_t) P.kv.heads);
@@ -299,6 +365,18 @@ struct KvItem {
     // (a place that is no sequence's: a tile past every row)
     template <int RT> __device__ __forceinline__ void rows(const KvAttnArgs& P, int at) {
         place = at;
+        if constexpr (MODE == kKvShared) {
+            int grp;
+            tile = kv_find_group(P, P.places - 1 - at, RT, grp, r0, n);
+            place = P.places - 1 - at;                                    // (kv_join_kernel counts from the groups' rows)
+            b = min(max(P.first[grp], 0), P.kv.seqs);
+            b1 = min(max(P.first[grp + 1], b), P.kv.seqs);
+            hi = min(max(P.shared[grp], 0) / kKvB, P.kv.width);
+            R = tile < 0 || b1 <= b ? 0 : (uint32_t) n * P.group;
+            b = min(b, P.kv.seqs - 1);
+            len = 0;
+            return;
+        }
         if (P.tiles) {
             b = (int) ((uint32_t) at % (uint32_t) P.kv.seqs);
             tile = P.tiles - 1 - (int) ((uint32_t) at / (uint32_t) P.kv.seqs);    // the longest rows first
@@ -309,13 +387,31 @@ struct KvItem {
         R = (uint32_t) n * P.group;                                       // (rows * group is below 2^31)
         if (R < P.least || R > P.greatest) R = 0;
         len = min(max(P.lengths[b], 0), P.kv.width * kKvB);
+        if constexpr (MODE == kKvOwn)
+            if (P.groups) {
+                const int grp = kv_group_of(P, b);
+                lo = grp < 0 ? 0 : min(max(P.shared[grp], 0) / kKvB, P.kv.width);
+            }
     }
     // the cache blocks kb0 .. kb0 + count that any of the rows rt0 .. rt0 + rt can see
-    __device__ __forceinline__ void range(const KvAttnArgs& P, uint32_t rt0, int rt, int& kb0, int& count) const {
+    __device__ __forceinline__ void range(const KvAttnArgs& P, uint32_t rt0, int rt, int& kb0, int& count) {
         const int base = len - n, bmin = base + (int) (rt0 / P.group), bmax = base + (int) ((min(R, rt0 + rt) - 1) / P.group);
+        if constexpr (MODE != kKvAll) return spans(P, bmin, bmax, kb0, count);
         kb0 = P.window > 0 ? max(bmin - P.window + 1, 0) / kKvB : 0;
         count = bmax >= 0 ? max(bmax / kKvB + 1 - kb0, 0) : 0;
     }
+    // The same of rows that are the tokens bmin .. bmax, as a count from 0: first the blocks of the first tokens, lo .. lo + sink, then those from
+    // win on. (Shared tokens end at block hi, a sequence's own begin at block lo.)
+    __device__ __forceinline__ void spans(const KvAttnArgs& P, int bmin, int bmax, int& kb0, int& count) {
+        int end = bmax >= 0 ? bmax / kKvB + 1 : 0;
+        if constexpr (MODE == kKvShared) end = min(end, hi);
+        win = max(P.window > 0 ? max(bmin - P.window + 1, 0) / kKvB : 0, lo);
+        sink = P.window > 0 ? max(min(min((P.sinks + kKvB - 1) / kKvB, end), win) - lo, 0) : 0;
+        kb0 = 0;
+        count = sink + max(end - win, 0);
+    }
+    // the block that the walk's step i is
+    __device__ __forceinline__ int block(int i) const { return MODE == kKvAll ? i : i < sink ? lo + i : win + (i - sink); }
     // the end of this part's blocks (from kb0 + split * per on); parts past the first that have none leave nothing
     __device__ __forceinline__ int end(const KvAttnArgs& P, int kb0, int count) const {
         return split + 1 == P.nsplit ? kb0 + count : kb0 + min(count, (split + 1) * P.per);
@@ -326,10 +422,72 @@ struct KvItem {
     }
 };
 
+// kKvShared: the tokens and sequences (-1: no row) of the tile's rows from rt0 on. A sequence's place is guessed as if all of the group had as many
+// rows, and searched for where that is wrong.
+template <int RT> __device__ __forceinline__ void kv_who(const KvAttnArgs& P, const KvItem<kKvShared>& it, uint32_t rt0, int2* who) {
+    const uint32_t rr = rt0 + threadIdx.x;
+    if (threadIdx.x >= RT) return;
+    int2 w = make_int2(-1, -1);
+    if (rr < it.R) {
+        const int j = (int) (rr / (uint32_t) P.group), row = it.r0 + j;
+        int b = it.b + (int) ((uint64_t) (uint32_t) j * (uint32_t) (it.b1 - it.b) / (uint32_t) it.n);
+        int from = P.kv.starts[b], to = P.kv.starts[b + 1];
+        if (row < from || row >= to) {
+            int a = it.b, e = it.b1;                            // the last that begins at or before the row
+            while (e - a > 1) {
+                const int m = (a + e) >> 1;
+                if (P.kv.starts[m] <= row) a = m;
+                else e = m;
+            }
+            b = a;
+            from = P.kv.starts[b];
+            to = P.kv.starts[b + 1];
+        }
+        from = min(max(from, 0), P.kv.rows);
+        to = min(max(to, from), P.kv.rows);
+        if (row >= from && row < to) w = make_int2(min(max(P.lengths[b], 0), P.kv.width * kKvB) - (to - row), b);
+    }
+    who[threadIdx.x] = w;
+}
+// the least and greatest token of N rows
+template <int N> __device__ __forceinline__ void kv_reach(const int2* who, int& posmin, int& posmax) {
+    posmin = INT32_MAX;
+    posmax = -1;
+#pragma unroll
+    for (int i = 0; i < (N + 63) / 64; ++i) {
+        const int at = (threadIdx.x & 63) + 64 * i;
+        const int2 w = who[N < 64 ? at % N : at];
+        if (w.y >= 0) {
+            posmin = min(posmin, w.x);
+            posmax = max(posmax, w.x);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        posmin = min(posmin, __shfl_xor(posmin, o));
+        posmax = max(posmax, __shfl_xor(posmax, o));
+    }
+    posmin = __builtin_amdgcn_readfirstlane(posmin);
+    posmax = __builtin_amdgcn_readfirstlane(posmax);
+}
+// a part that has no blocks
+template <int RT> __device__ __forceinline__ void kv_nothing(const KvAttnArgs& P, const KvItem<kKvShared>& it) {
+    if (threadIdx.x < RT) *reinterpret_cast<float2*>(P.pml + (it.part(P) * RT + threadIdx.x) * 2) = make_float2(kKvUnset, 0.0f);
+}
+// Whether a launch's sums are the results, or parts of them
+template <int MODE> __device__ __forceinline__ bool kv_direct(const KvAttnArgs& P) {
+    return MODE != kKvShared && P.nsplit == 1 && (MODE == kKvAll || P.groups == 0);
+}
+
+// Whether a key block is seen whole by rows that are the tokens posmin .. posmax
+template <int MODE> __device__ __forceinline__ bool kv_whole(const KvAttnArgs& P, int key0, int posmin, int posmax) {
+    return key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window || (MODE != kKvAll && key0 + kKvB <= P.sinks)) && !P.mask;
+}
+
 // The walk over a sequence's blocks that are there. The wavefront holds 64 entries of the table, one a lane, so that a block's number is
 // known without a wait for memory: read entry by entry, its latency stood before every block's loads (64 sequences of up to 8192 tokens
 // 133.4 us, 130.7 so; 601 float32 tokens 33.8 and 33.1).
-struct KvPages {
+template <int MODE> struct KvPages {
     const int32_t* table;
     int width, base, entry;
     __device__ __forceinline__ void take(const KvAttnArgs& P, int b) {
@@ -337,12 +495,12 @@ struct KvPages {
         width = P.kv.width;
         base = -64;
     }
-    // the first block from kb on, in steps of BY, that is there (its page), or `last`
-    template <int BY> __device__ __forceinline__ bool next(const KvAttnArgs& P, int& kb, int& page, int last, int lane) {
+    // the first block (of the walk) from kb on, in steps of BY, that is there (its page), or `last`
+    template <int BY> __device__ __forceinline__ bool next(const KvAttnArgs& P, const KvItem<MODE>& it, int& kb, int& page, int last, int lane) {
         for (; kb < last; kb += BY) {
             if (kb - base >= 64) {
                 base = kb;
-                entry = table[min(kb + lane, width - 1)];
+                entry = table[min(it.block(kb + lane), width - 1)];
             }
             page = __builtin_amdgcn_readlane(entry, kb - base);
             if (page >= 0 && page < P.kv.blocks) return true;
@@ -354,24 +512,33 @@ struct KvPages {
 // Few rows (up to 32 of a sequence and head): the four wavefronts of a block share 16 NQ rows and take every fourth cache block.
 // Bound by the cache's bytes: the next block's codes are on their way while one is worked on (64 sequences of up to 8192 tokens, 8 heads of
 // 128, 64 queries: 132 us, 4.9 TB/s; one of 131072 tokens 52.5 us, 5.1 TB/s, and the merge 4.8).
-template <int WC, int NQ, bool TWO>
+template <int WC, int NQ, bool TWO, int MODE = kKvAll>
 __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC, DT = 4 * WC, RT = 16 * NQ, KS = 4, PARTS = TWO ? 2 : 1;
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
-    KvItem it;
-    it.take<RT>(P);
+    KvItem<MODE> it;
+    it.template take<RT>(P);
     const int h = it.h, b = it.b;
     const uint32_t R = it.R, rw = (uint32_t) it.tile * RT, group = P.group;
     if (rw >= R) return;
 
     // the cache blocks that any of the rows can see, a part of them, every KS-th
-    const int posmin = it.len - it.n + (int) (rw / group), posmax = it.len - it.n + (int) ((min(R, rw + RT) - 1) / group);
+    int posmin = it.len - it.n + (int) (rw / group), posmax = it.len - it.n + (int) ((min(R, rw + RT) - 1) / group);
     int kb0, count;
-    it.range(P, rw, RT, kb0, count);
-    if (it.split && it.split * P.per >= count) return;
+    __shared__ int2 who[MODE == kKvShared ? RT : 1];
+    if constexpr (MODE == kKvShared) {
+        kv_who<RT>(P, it, rw, who);
+        __syncthreads();
+        kv_reach<RT>(who, posmin, posmax);
+        it.spans(P, posmin, posmax, kb0, count);
+        if (it.split && it.split * P.per >= count) return kv_nothing<RT>(P, it);
+    } else {
+        it.range(P, rw, RT, kb0, count);
+        if (it.split && it.split * P.per >= count) return;
+    }
     const int last = it.end(P, kb0, count);
-    KvPages pages;
+    KvPages<MODE> pages;
     pages.take(P, b);
     uint4 kr[4][WC], vr[DT];
     const int koff = ((l15 >> 2) * 16 + (l15 & 3)) * W + g * 16, voff = l15 * 64 + g * 16;
@@ -389,17 +556,17 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     };
     int kb = kb0 + it.split * P.per + wave, page = 0;
     float ks = 0.0f, vs = 0.0f;
-    if (pages.next<KS>(P, kb, page, last, lane)) {
+    if (pages.template next<KS>(P, it, kb, page, last, lane)) {
         load_k(page);
         load_v(page);
         ks = P.kv.ks[(int64_t) page * P.kv.heads + h];
         vs = P.kv.vs[(int64_t) page * P.kv.heads + h];
     }
-    KvRows<WC, NQ, TWO, true> q;                    // (behind the first loads of the cache, which take longer)
-    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
+    KvRows<WC, NQ, TWO, true, MODE> q;              // (behind the first loads of the cache, which take longer)
+    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g, who);
     while (kb < last) {
         int nkb = kb + KS, npage = 0;
-        const bool more = pages.next<KS>(P, nkb, npage, last, lane);
+        const bool more = pages.template next<KS>(P, it, nkb, npage, last, lane);
         v4f_kv s[NQ][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -424,8 +591,8 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
             ks = P.kv.ks[(int64_t) npage * P.kv.heads + h];
             vs = P.kv.vs[(int64_t) npage * P.kv.heads + h];
         }
-        const int key0 = kb * kKvB;
-        const bool whole = key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window) && !P.mask;
+        const int key0 = it.block(kb) * kKvB;
+        const bool whole = kv_whole<MODE>(P, key0, posmin, posmax);
         v8h_kv pf[NQ][2][2];
         float vsl[NQ];
         q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
@@ -476,11 +643,11 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
                     y[2] = __builtin_fmaf(v.z, wt[w], y[2]);
                     y[3] = __builtin_fmaf(v.w, wt[w], y[3]);
                 }
-                if (P.nsplit == 1) kv_store4(P, at * P.kv.dim, d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+                if (kv_direct<MODE>(P)) kv_store4(P, at * P.kv.dim, d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
                 else *reinterpret_cast<float4*>(P.po + row * W + d) = make_float4(y[0], y[1], y[2], y[3]);
             }
             if (c == 0) {
-                if (P.nsplit > 1) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(mx, lt);
+                if (!kv_direct<MODE>(P)) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(mx, lt);
                 else if (P.lse) P.lse[at] = kv_lse(mx, lt);
             }
         }
@@ -496,25 +663,35 @@ template <int WC> __device__ __forceinline__ int kv_mix(int g, int c) { return (
 // doing it in every wavefront took more vector instructions than the softmax. Bound by vector instructions beside the products (4096 tokens
 // over 8192, 64 heads over 8 of 128: 947-1060 us by the card, 0.78-0.87 PFLOP/s, the matrix cores 34 % busy). Operands are read from LDS a
 // step ahead of their products (960 us without, 16 sequences of 100 tokens of 256 features 203 to 181).
-template <int WC, int NQ, bool TWO>
+template <int WC, int NQ, bool TWO, int MODE = kKvAll>
 __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC, DT = 4 * WC, RT = 64 * NQ, PARTS = TWO ? 2 : 1;
     __shared__ v8h_kv sk[2][4][WC][2][64], sv[2][DT][2][64];              // [stage][key tile or feature tile][...][half][lane]
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int) (threadIdx.x >> 6));
-    KvItem it;
-    it.take<RT>(P);
+    KvItem<MODE> it;
+    it.template take<RT>(P);
     const int h = it.h, b = it.b;
     const uint32_t R = it.R, rt0 = (uint32_t) it.tile * RT, rw = rt0 + wave * 16 * NQ, group = P.group;
     if (rt0 >= R) return;
     // the cache blocks that any of the block's rows can see, a part of them; the wavefront's own rows see posmin .. posmax
     const int base = it.len - it.n;
-    const int posmin = base + (int) (rw / group), posmax = rw < R ? base + (int) ((min(R, rw + 16 * NQ) - 1) / group) : -1;
+    int posmin = base + (int) (rw / group), posmax = rw < R ? base + (int) ((min(R, rw + 16 * NQ) - 1) / group) : -1;
     int kb0, count;
-    it.range(P, rt0, RT, kb0, count);
-    if (it.split && it.split * P.per >= count) return;
+    __shared__ int2 who[MODE == kKvShared ? RT : 1];
+    if constexpr (MODE == kKvShared) {
+        kv_who<RT>(P, it, rt0, who);
+        __syncthreads();
+        kv_reach<RT>(who, posmin, posmax);
+        it.spans(P, posmin, posmax, kb0, count);
+        if (it.split && it.split * P.per >= count) return kv_nothing<RT>(P, it);
+        kv_reach<16 * NQ>(who + wave * 16 * NQ, posmin, posmax);
+    } else {
+        it.range(P, rt0, RT, kb0, count);
+        if (it.split && it.split * P.per >= count) return;
+    }
     const int last = it.end(P, kb0, count);
-    KvPages pages;
+    KvPages<MODE> pages;
     pages.take(P, b);
     // the thread's 16-byte pieces of a block's codes: piece t + 256 i
     uint4 kr[WC], vr[WC];
@@ -546,24 +723,24 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
         }
     };
     int kb = kb0 + it.split * P.per, page = 0, st = 0;
-    const bool any = pages.next<1>(P, kb, page, last, lane);
+    const bool any = pages.template next<1>(P, it, kb, page, last, lane);
     int nkb = kb, npage = 0;
     bool more = false;
     float ks_now = 0.0f, vs_now = 0.0f;
     if (any) load(page);
-    KvRows<WC, NQ, TWO, TWO> q;
-    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g);
+    KvRows<WC, NQ, TWO, TWO, MODE> q;
+    q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g, who + (MODE == kKvShared ? wave * 16 * NQ : 0));
     if (any) {
         stage(0);
         ks_now = ks;
         vs_now = vs;
         nkb = kb + 1;
-        more = pages.next<1>(P, nkb, npage, last, lane);
+        more = pages.template next<1>(P, it, nkb, npage, last, lane);
         if (more) load(npage);
     }
     lds_barrier();
     while (kb < last) {
-        const int key0 = kb * kKvB;
+        const int key0 = it.block(kb) * kKvB;
         if (key0 <= posmax) {
             // a feature chunk's operands of all four key tiles are read while the one before is multiplied: four tiles' sums in turn
             // leave no product waiting for the last
@@ -586,7 +763,7 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
                             s[e][t] = kv_mma(a[i & 1][t], q.qf[e][i / 2][i % 2][w], i + w ? s[e][t] : v4f_kv{0.0f, 0.0f, 0.0f, 0.0f});
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const bool whole = key0 + kKvB - 1 <= posmin && (P.window == 0 || key0 > posmax - P.window) && !P.mask;
+            const bool whole = kv_whole<MODE>(P, key0, posmin, posmax);
             v8h_kv pf[NQ][2][PARTS];
             float vsl[NQ];
             q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
@@ -616,7 +793,7 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
         kb = nkb;
         if (more) {
             nkb = kb + 1;
-            more = pages.next<1>(P, nkb, npage, last, lane);
+            more = pages.template next<1>(P, it, nkb, npage, last, lane);
             if (more) load(npage);
         }
         lds_barrier();
@@ -626,7 +803,7 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
     for (int e = 0; e < NQ; ++e) {
         const float l = kv_sum4(q.l[e]);
         if (q.tok[e] < 0) continue;
-        if (P.nsplit == 1) {
+        if (kv_direct<MODE>(P)) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t at = q.tok[e] * P.q_heads + q.head[e];
 #pragma unroll
@@ -644,15 +821,15 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
 }
 
 // joins the parts of one row: one block of 256 threads a row, its wavefronts taking every fourth part, in that order
-template <int WC, int RT>
+template <int WC, int RT, int MODE = kKvAll>
 __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t item = blockIdx.x / RT;
     const int r = (int) (blockIdx.x % RT);
-    KvItem it;
+    KvItem<MODE> it;
     it.h = (int) (item % P.kv.heads);
-    it.rows<RT>(P, (int) (item / P.kv.heads));
+    it.template rows<RT>(P, (int) (item / P.kv.heads));
     const uint32_t rr = (uint32_t) it.tile * RT + r, group = P.group;
     if (rr >= it.R) return;
     int kb0, count;
@@ -689,6 +866,71 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
     if (P.lse && threadIdx.x == 0) P.lse[at] = kv_lse(mx, lt);
 }
 
+// Joins the parts of one row over its sequence's own blocks and, where its sequence shares tokens, over those: one block of 256 threads a row.
+template <int WC, int RT>
+__global__ __launch_bounds__(256) void kv_join_kernel(KvAttnArgs P) {
+    constexpr int W = 64 * WC;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t item = blockIdx.x / RT;
+    const int r = (int) (blockIdx.x % RT);
+    KvItem<kKvOwn> it;
+    it.h = (int) (item % P.kv.heads);
+    it.template rows<RT>(P, (int) (item / P.kv.heads));
+    const uint32_t rr = (uint32_t) it.tile * RT + r, group = P.group;
+    if (rr >= it.R) return;
+    int kb0, count;
+    it.range(P, (uint32_t) it.tile * RT, RT, kb0, count);
+    const int own = min(max((count + P.per - 1) / P.per, 1), P.nsplit);
+    const int64_t row0 = item * P.nsplit * RT + r;
+    int parts = own;
+    int64_t row2 = 0;
+    const int grp = kv_group_of(P, it.b);
+    if (grp >= 0) {
+        const int from = kv_group_row(P, grp), to = kv_group_row(P, grp + 1);
+        const int row = it.r0 + (int) (rr / group);
+        if (row >= from && row < to) {
+            const uint32_t r2 = (uint32_t) (row - from) * group + rr % group, rt2 = (uint32_t) P.rt2;
+            const int64_t place = (int) ((uint32_t) from * group / rt2) + grp + (int) (r2 / rt2);
+            row2 = (place * P.kv.heads + it.h) * P.nsplit2 * rt2 + r2 % rt2;
+            parts += P.nsplit2;
+        }
+    }
+    auto ml_of = [&](int s) {
+        return s < own ? *reinterpret_cast<const float2*>(P.pml + (row0 + (int64_t) s * RT) * 2)
+                       : *reinterpret_cast<const float2*>(P.pml2 + (row2 + (int64_t) (s - own) * P.rt2) * 2);
+    };
+    float mx = kKvUnset;
+    for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, ml_of(s).x);
+    mx = wave_max<64>(mx);
+    float lt = 0.0f;
+    for (int s = lane; s < parts; s += 64) {
+        const float2 ml = ml_of(s);
+        lt += ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
+    }
+    lt = wave_sum<64>(lt);
+    float y[WC];
+#pragma unroll
+    for (int t = 0; t < WC; ++t) y[t] = 0.0f;
+#pragma unroll 4
+    for (int s = wave; s < parts; s += 4) {
+        const float2 ml = ml_of(s);
+        if (ml.y == 0.0f) continue;                                       // (nothing seen: there are no sums)
+        const float w = __builtin_amdgcn_exp2f(ml.x - mx);
+        const float* o = s < own ? P.po + (row0 + (int64_t) s * RT) * W : P.po2 + (row2 + (int64_t) (s - own) * P.rt2) * W;
+#pragma unroll
+        for (int t = 0; t < WC; ++t) y[t] = __builtin_fmaf(o[64 * t + lane], w, y[t]);
+    }
+    __shared__ float sy[4][W];
+#pragma unroll
+    for (int t = 0; t < WC; ++t) sy[wave][64 * t + lane] = y[t];
+    __syncthreads();
+    const int64_t at = ((int64_t) it.r0 + rr / group) * P.q_heads + it.h * group + rr % group;
+    const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+    for (int d = threadIdx.x; d < P.kv.dim; d += 256)
+        store_any(P.out, P.out_dt, at * P.kv.dim + d, ((sy[0][d] + sy[1][d]) + (sy[2][d] + sy[3][d])) * inv);
+    if (P.lse && threadIdx.x == 0) P.lse[at] = kv_lse(mx, lt);
+}
+
 // which kernel takes the call, and in how many parts
 struct KvPlan {
     bool rows;            // kv_attn_rows_kernel (else kv_attn_kernel)
@@ -699,32 +941,42 @@ struct KvPlan {
     uint32_t least = 0, greatest = UINT32_MAX;
 };
 
-template <int WC, int NQ, bool ROWS>
+template <int WC, int NQ, bool ROWS, int MODE>
 static void kv_attn_run(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two) {
     const unsigned grid = (unsigned) (plan.blocks * plan.nsplit);
     constexpr int RT = (ROWS ? 64 : 16) * NQ;
     if constexpr (ROWS) {
-        if (!two) kv_attn_rows_kernel<WC, NQ, false><<<grid, 256, 0, c->stream>>>(P);
-        else if constexpr (NQ == 1) kv_attn_rows_kernel<WC, 1, true><<<grid, 256, 0, c->stream>>>(P);
+        if (!two) kv_attn_rows_kernel<WC, NQ, false, MODE><<<grid, 256, 0, c->stream>>>(P);
+        else if constexpr (NQ == 1) kv_attn_rows_kernel<WC, 1, true, MODE><<<grid, 256, 0, c->stream>>>(P);
     } else {
-        if (two) kv_attn_kernel<WC, NQ, true><<<grid, 256, 0, c->stream>>>(P);
-        else kv_attn_kernel<WC, NQ, false><<<grid, 256, 0, c->stream>>>(P);
+        if (two) kv_attn_kernel<WC, NQ, true, MODE><<<grid, 256, 0, c->stream>>>(P);
+        else kv_attn_kernel<WC, NQ, false, MODE><<<grid, 256, 0, c->stream>>>(P);
     }
-    if (plan.nsplit > 1) kv_merge_kernel<WC, RT><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
+    if constexpr (MODE == kKvOwn)
+        if (P.groups) {
+            kv_join_kernel<WC, RT><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
+            return;
+        }
+    if constexpr (MODE != kKvShared)
+        if (plan.nsplit > 1) kv_merge_kernel<WC, RT, MODE><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
 }
 
-// heads of up to 64 WC features (kv_attn_64.hip .. kv_attn_256.hip)
+// heads of up to 64 WC features (kv_attn_64.hip .. kv_attn_256.hip), the same of kv_attention_spans (kv_spans_64.hip .. kv_spans_256.hip)
 void kv_attn_64(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
 void kv_attn_128(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
 void kv_attn_192(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
 void kv_attn_256(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two);
+void kv_spans_64(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two, bool shared);
+void kv_spans_128(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two, bool shared);
+void kv_spans_192(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two, bool shared);
+void kv_spans_256(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two, bool shared);
 
-template <int WC>
+template <int WC, int MODE = kKvAll>
 static void kv_attn_width(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool two) {
-    if (plan.rows && plan.nq == 1) kv_attn_run<WC, 1, true>(c, P, plan, two);
-    else if (plan.rows) kv_attn_run<WC, 2, true>(c, P, plan, two);
-    else if (plan.nq == 1) kv_attn_run<WC, 1, false>(c, P, plan, two);
-    else if constexpr (WC <= 2) kv_attn_run<WC, 2, false>(c, P, plan, two);
+    if (plan.rows && plan.nq == 1) kv_attn_run<WC, 1, true, MODE>(c, P, plan, two);
+    else if (plan.rows) kv_attn_run<WC, 2, true, MODE>(c, P, plan, two);
+    else if (plan.nq == 1) kv_attn_run<WC, 1, false, MODE>(c, P, plan, two);
+    else if constexpr (WC <= 2) kv_attn_run<WC, 2, false, MODE>(c, P, plan, two);
 }
 
 }  // namespace h3

@@ -366,6 +366,6 @@ int kv_read(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const
 #ifndef __HIP_DEVICE_COMPILE__
 extern "C" __attribute__((visibility("default"))) const h3_lm_api h3lm = {
     (int64_t) sizeof(h3_lm_api), h3::kv_write, h3::kv_read, h3::kv_attention, h3::kv_attention_work, h3::linear4,
-    h3::lin_attention, h3::lin_attention_work,
+    h3::kv_attention_spans, h3::kv_attention_spans_work, h3::lin_attention, h3::lin_attention_work,
 };
 #endif

@@ -488,25 +488,46 @@ def kv_read(cache: KvCache, table: Tensor, starts: Tensor, first: Tensor, most: 
     dev.check(dev.api.lm_kv_read(dev.ctx, cache._p, batch, *args))
 
 
-def kv_attention_work(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, most: int, *, max_len: int = 0, window: int = 0) -> int:
+class KvShared:
+    """Groups of sequences whose caches begin with the same tokens (h3_kv_shared): group g is the sequences first[g] .. first[g + 1] - 1, and
+    the first tokens[g] // KV_BLOCK entries of their rows of the block table are the same. first int32 [groups + 1], tokens int32 [groups];
+    most: about the most of tokens (0: the table's width)."""
+
+    def __init__(self, first: Tensor, tokens: Tensor, most: int = 0):
+        self.groups = first.elements() - 1
+        if self.groups < 0 or tokens.elements() != self.groups:
+            raise Error(f"kv shared: first {first.shape} and tokens {tokens.shape} are not of the same groups")
+        if most < 0:
+            raise Error(f"kv shared: the most shared tokens: {most}")
+        self.first, self.tokens, self.most = first, tokens, int(most)
+        self._c = _api.KvShared(_i32(first, "first", self.groups + 1), _i32(tokens, "tokens", self.groups), self.groups, most)
+        self._p = _C.addressof(self._c)
+
+
+def kv_attention_work(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, most: int, *, max_len: int = 0, window: int = 0,
+                      sinks: int = 0, shared: KvShared | None = None) -> int:
     """The bytes of workspace that kv_attention takes for these arguments (0: none)."""
     batch, _ = _kv_batch(table, starts, q.tokens, most)
     dev = _dev(cache.k)
-    n = dev.api.lm_kv_attention_work(dev.ctx, cache._p, batch, max_len, q.heads, window)
+    if sinks or shared is not None:
+        n = dev.api.lm_kv_attention_spans_work(dev.ctx, cache._p, batch, shared._p if shared is not None else None, max_len, q.heads, window, sinks)
+    else:
+        n = dev.api.lm_kv_attention_work(dev.ctx, cache._p, batch, max_len, q.heads, window)
     if n < 0:
         raise Error(dev.api.error())
     return n
 
 
 def kv_attention(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, lengths: Tensor, most: int, out: Tensor, *, max_len: int = 0,
-                 window: int = 0, mask: Tensor | None = None, scale: float = 0.0, lse: Tensor | None = None,
-                 work: Tensor | None = None) -> None:
+                 window: int = 0, sinks: int = 0, shared: KvShared | None = None, mask: Tensor | None = None, scale: float = 0.0,
+                 lse: Tensor | None = None, work: Tensor | None = None) -> None:
     """Causal attention of each sequence's newest tokens (rows starts[b] .. of q) over its lengths[b] tokens in the cache, those
     newest ones among them: softmax(q k^T scale) v per head, query head h reading head h // (q.heads // cache.heads). out
-    [rows, q.heads * dim]. scale 0: 1 / sqrt(dim). window: only the last so many tokens; mask uint8 [sequences, n]: only tokens
-    whose byte is not 0 (tokens from n on are hidden); a row that sees nothing gets zeros. lse float32 [rows, q.heads]: the
-    logarithm of each row's sum of exponentials. max_len: about the longest length (0: the table's width). work: a workspace of
-    kv_attention_work() bytes, which a call recorded into a graph has to bring if that is not 0."""
+    [rows, q.heads * dim]. scale 0: 1 / sqrt(dim). window: only the last so many tokens, and the first `sinks`; mask uint8 [sequences, n]:
+    only tokens whose byte is not 0 (tokens from n on are hidden); a row that sees nothing gets zeros. shared: tokens that groups of
+    sequences have in common, gone through once for all of a group's rows. lse float32 [rows, q.heads]: the logarithm of each row's sum of
+    exponentials. max_len: about the longest length (0: the table's width). work: a workspace of kv_attention_work() bytes, which a call
+    recorded into a graph has to bring if that is not 0."""
     if q.dim != cache.dim:
         raise Error(f"kv_attention: q heads of {q.dim} for a cache of {cache.dim}")
     if out.elements() != q.tokens * q.heads * q.dim:
@@ -519,10 +540,14 @@ def kv_attention(cache: KvCache, table: Tensor, q: Rows, starts: Tensor, lengths
         mask_p, mask_n = mask.ptr(), int(mask.shape[1])
     if lse is not None and (lse.dtype != DType.F32 or lse.elements() != q.tokens * q.heads):
         raise Error(f"kv_attention: lse must be float32 [{q.tokens}, {q.heads}], got {lse.dtype} {lse.shape}")
-    args = (_i32(lengths, "lengths", seqs), max_len, q.ptr(), q.stride, q.t.dtype.kernel_code(), q.heads, scale, window, mask_p,
-            mask_n, out.ptr(), out.dtype.kernel_code(), _p(lse), _p(work), work.nbytes() if work is not None else 0)
     dev = _dev(cache.k)
-    dev.check(dev.api.lm_kv_attention(dev.ctx, cache._p, batch, *args))
+    lens, rows = _i32(lengths, "lengths", seqs), (max_len, q.ptr(), q.stride, q.t.dtype.kernel_code(), q.heads, scale, window)
+    rest = (mask_p, mask_n, out.ptr(), out.dtype.kernel_code(), _p(lse), _p(work), work.nbytes() if work is not None else 0)
+    if sinks or shared is not None:
+        groups = shared._p if shared is not None else None
+        dev.check(dev.api.lm_kv_attention_spans(dev.ctx, cache._p, batch, groups, lens, *rows, sinks, *rest))
+    else:
+        dev.check(dev.api.lm_kv_attention(dev.ctx, cache._p, batch, lens, *rows, *rest))
 
 
 class LinState:

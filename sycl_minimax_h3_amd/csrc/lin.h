@@ -22,7 +22,7 @@ struct LinArgs {
     uint32_t least, most;                           // sequences of fewer or more rows are another launch's
     int slices, seg;                                // in pieces: ranges of v's features, tokens of a segment
     float* ws;                                      // the segments' sums, then their first states, one for each block of threads
-    bool q_vec, k_vec, v_vec, s_vec, out_vec;       // rows that can be read (written) 16 bytes at a time
+    bool vec, s_vec;                                // rows of q, k, v and out, and states, that can be read and written 16 bytes at a time
 };
 
 int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, const float* decay, const void* q, int64_t q_stride,

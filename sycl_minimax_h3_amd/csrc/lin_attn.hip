@@ -113,12 +113,12 @@ __global__ __launch_bounds__(256) void lin_step_kernel(LinArgs P) {
 }
 
 // The states at the segments' beginnings, where their own sums were: a thread has 16 bytes of a state through all segments of a sequence.
-// (Blocks: 256 threads a 4 KiB piece of a state in the kernel's own layout, of a head, slice and sequence.)
-template <int KC, int NV>
-__global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs P) {
-    constexpr int FR = 2 * KC * NV;
+// (Blocks: a sixteen-row piece of a state in the chunk kernel's own layout, of a head, slice and sequence.)
+template <int KC, int NW, int NV>
+__global__ __launch_bounds__(64 * NW) void lin_scan_kernel(LinArgs P) {
+    constexpr int FR = 2 * KC * NV, T = 64 * NW;
     uint32_t id = blockIdx.x;
-    const int fr = (int) (id % FR);
+    const int fr = (int) (id % FR), t = fr / NV, x = fr % NV;
     id /= FR;
     const int h = (int) (id % (uint32_t) P.heads);
     id /= (uint32_t) P.heads;
@@ -128,8 +128,7 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs P) {
     const int segs = (n + P.seg - 1) / P.seg;
     if (segs < 2 || (uint32_t) n < P.least || (uint32_t) n > P.most) return;
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-    const int t = fr / NV, x = fr % NV;
-    const int c = slice * 64 * NV + wave * 16 * NV + (NV == 2 ? 8 * (l15 >> 2) + 4 * x + (l15 & 3) : l15);
+    const int c = slice * 16 * NW * NV + (wave * NV + x) * 16 + l15;
     const int64_t from = P.source[b];
     v4f_lin s = {0.0f, 0.0f, 0.0f, 0.0f};
     if (from >= 0 && from < P.slots && c < P.dv) {
@@ -141,8 +140,8 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs P) {
         }
     }
     const float less = expm1f(-P.decay[h] * (float) P.seg);
-    const int64_t place = r0 / P.seg + b, step = (int64_t) P.slices * P.heads * (FR * 1024);
-    float* ws = P.ws + ((place * P.slices + slice) * P.heads + h) * (FR * 1024) + fr * 1024 + threadIdx.x * 4;
+    const int64_t place = r0 / P.seg + b, step = (int64_t) P.slices * P.heads * (FR * T * 4);
+    float* ws = P.ws + ((place * P.slices + slice) * P.heads + h) * (FR * T * 4) + fr * (T * 4) + threadIdx.x * 4;
     for (int j = 0; j < segs; ++j, ws += step) {
         const v4f_lin own = j + 1 < segs ? *reinterpret_cast<const v4f_lin*>(ws) : v4f_lin{0.0f, 0.0f, 0.0f, 0.0f};
         *reinterpret_cast<v4f_lin*>(ws) = s;
@@ -151,8 +150,13 @@ __global__ __launch_bounds__(256) void lin_scan_kernel(LinArgs P) {
     }
 }
 
-template <int KC, int NV> static void lin_scan_run(Ctx* c, const LinArgs& P) {
-    lin_scan_kernel<KC, NV><<<(unsigned) ((int64_t) P.kv.seqs * P.slices * P.heads * 2 * KC * NV), 256, 0, c->stream>>>(P);
+template <int KC, bool WIDE> static void lin_scan_run(Ctx* c, const LinArgs& P) {
+    constexpr int NW = LinWaves<KC, WIDE>::NW, NV = LinWaves<KC, WIDE>::NV;
+    lin_scan_kernel<KC, NW, NV><<<(unsigned) ((int64_t) P.kv.seqs * P.slices * P.heads * 2 * KC * NV), 64 * NW, 0, c->stream>>>(P);
+}
+template <int KC> static void lin_scan(Ctx* c, const LinArgs& P, bool wide) {
+    if (wide) lin_scan_run<KC, true>(c, P);
+    else lin_scan_run<KC, false>(c, P);
 }
 
 template <int DKR> static void lin_step(Ctx* c, const LinArgs& P, int64_t blocks) {
@@ -178,7 +182,8 @@ static int lin_checks(const std::string& fn, const h3_lin_state* state, const h3
 constexpr int kLinFew = 16, kLinLeast = 256;
 struct LinPlan {
     bool step, chunk, split;
-    int kc, nv, slices;
+    int kc, slices;
+    bool wide;
     int64_t seg, places, blocks, floats;
 };
 static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, int cus) {
@@ -187,15 +192,15 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
     p.chunk = most > kLinFew;
     p.step = !p.chunk || (batch.seqs > 1 && most * batch.seqs > batch.rows);
     p.kc = (int) (state.dk + 63) / 64 * 2;
-    p.nv = state.dv > 64 && p.kc <= 4 ? 2 : 1;
-    p.slices = (int) (state.dv + 64 * p.nv - 1) / (64 * p.nv);
+    p.wide = state.dv > 64;
+    p.slices = p.wide ? (int) (state.dv + 127) / 128 : 1;
     const int64_t want = std::max<int64_t>(1, 2 * (int64_t) cus / (chains * p.slices));
     p.seg = std::max<int64_t>(kLinLeast, ((most + want - 1) / want + 63) / 64 * 64);
     p.split = p.seg < most;
     if (!p.split) p.seg = most;
     p.places = p.split ? batch.rows / p.seg + batch.seqs : batch.seqs;
     p.blocks = p.places * p.slices * state.heads;
-    p.floats = p.chunk && p.split ? p.blocks * (2 * p.kc * p.nv * 1024) : 0;
+    p.floats = p.chunk && p.split ? p.blocks * (32 * p.kc) * (p.wide ? 128 : 64) : 0;
     return p;
 }
 
@@ -224,7 +229,10 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
     if (!decay || !q || !k || !v || !out) return fail(fn + ": decay, q, k, v and out are required");
     if (work && !aligned16(work)) return fail(fn + ": the workspace must be 16-byte aligned");
     const int es = elem_size(dt);
-    auto vec = [&](const void* p, int64_t stride, int64_t dim) { return aligned16(p) && stride * es % 16 == 0 && dim * es % 16 == 0; };
+    // (in pieces the rows of 64 tokens are reached by 32 bits of distance)
+    auto vec = [&](const void* p, int64_t stride, int64_t dim) {
+        return aligned16(p) && stride < (1 << 22) && stride * es % 16 == 0 && dim * es % 16 == 0;
+    };
     LinArgs P{};
     P.s = state->s;
     P.slots = state->slots;
@@ -237,14 +245,13 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
     P.dt = dt; P.out = out; P.out_dt = out_dt;
     P.scale = scale > 0.0f ? scale : (float) (1.0 / std::sqrt((double) dk));
     P.least = 0; P.most = UINT32_MAX;
-    P.q_vec = vec(q, q_stride, dk); P.k_vec = vec(k, k_stride, dk); P.v_vec = vec(v, v_stride, dv);
     P.s_vec = aligned16(P.s) && dv % 4 == 0;
-    P.out_vec = aligned16(out) && dv % 4 == 0;
+    P.vec = vec(q, q_stride, dk) && vec(k, k_stride, dk) && vec(v, v_stride, dv) && aligned16(out) && heads * dv < (1 << 22);
     Ctx* c = ctx_of(ctx, fn.c_str());
     if (!c) return -1;
     const LinPlan plan = lin_plan(*state, *batch, c->cus);
-    const int64_t steps = batch->seqs * heads * ((dv + kLinCols - 1) / kLinCols), scans = batch->seqs * heads * plan.slices * 2 * plan.kc * plan.nv;
-    if ((plan.step && steps > kKvMostBlocks) || (plan.chunk && (plan.blocks > kKvMostBlocks || (plan.split && scans > kKvMostBlocks))))
+    const int64_t steps = batch->seqs * heads * ((dv + kLinCols - 1) / kLinCols), scans = batch->seqs * heads * plan.slices * 4 * plan.kc;
+    if ((plan.step && steps > kKvMostBlocks) || (plan.chunk && (plan.blocks > kKvMostBlocks / 2 || (plan.split && scans > kKvMostBlocks / 2))))
         return fail(fn + ": too many blocks of work");
     if (plan.floats) {
         if (work) {
@@ -273,18 +280,18 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
         P.slices = plan.slices;
         P.seg = (int) plan.seg;
         auto run = [&](bool outputs) {
-            if (dt == H3S_BF16) lin_chunk_bf16(c, P, plan.kc, plan.nv, plan.blocks, outputs);
-            else if (dt == H3S_F16) lin_chunk_f16(c, P, plan.kc, plan.nv, plan.blocks, outputs);
-            else lin_chunk_f32(c, P, plan.kc, plan.nv, plan.blocks, outputs);
+            if (dt == H3S_BF16) lin_chunk_bf16(c, P, plan.kc, plan.wide, plan.blocks, outputs);
+            else if (dt == H3S_F16) lin_chunk_f16(c, P, plan.kc, plan.wide, plan.blocks, outputs);
+            else lin_chunk_f32(c, P, plan.kc, plan.wide, plan.blocks, outputs);
         };
         if (plan.split) {
             run(false);
-            if (plan.kc == 2 && plan.nv == 1) lin_scan_run<2, 1>(c, P);
-            else if (plan.kc == 2) lin_scan_run<2, 2>(c, P);
-            else if (plan.kc == 4 && plan.nv == 1) lin_scan_run<4, 1>(c, P);
-            else if (plan.kc == 4) lin_scan_run<4, 2>(c, P);
-            else if (plan.kc == 6) lin_scan_run<6, 1>(c, P);
-            else lin_scan_run<8, 1>(c, P);
+            switch (plan.kc) {
+                case 2: lin_scan<2>(c, P, plan.wide); break;
+                case 4: lin_scan<4>(c, P, plan.wide); break;
+                case 6: lin_scan<6>(c, P, plan.wide); break;
+                default: lin_scan<8>(c, P, plan.wide); break;
+            }
         }
         run(true);
     }

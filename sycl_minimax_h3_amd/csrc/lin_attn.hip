@@ -177,7 +177,8 @@ static int lin_checks(const std::string& fn, const h3_lin_state* state, const h3
     return 0;
 }
 
-// Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces.
+// Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces. Where the sequences beside the longest
+// have more than 2 kLinFew tokens on average, all go in pieces: a launch that finds nothing to do takes 3 to 5 us.
 // Segments: as many as give each CU two blocks of threads, of at least kLinLeast tokens.
 constexpr int kLinFew = 16, kLinLeast = 256;
 struct LinPlan {
@@ -190,8 +191,8 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
     LinPlan p{};
     const int64_t most = std::min(batch.most, batch.rows), chains = batch.seqs * state.heads;
     p.chunk = most > kLinFew;
-    p.step = !p.chunk || (batch.seqs > 1 && most * batch.seqs > batch.rows);
-    p.kc = (int) (state.dk + 63) / 64 * 2;
+    p.step = !p.chunk || (batch.seqs > 1 && batch.rows - most <= 2 * kLinFew * (batch.seqs - 1) && most * batch.seqs > batch.rows);
+    p.kc = state.dk > 64 && state.dk <= 96 ? 3 : (int) (state.dk + 63) / 64 * 2;
     p.wide = state.dv > 64;
     p.slices = p.wide ? (int) (state.dv + 127) / 128 : 1;
     const int64_t want = std::max<int64_t>(1, 2 * (int64_t) cus / (chains * p.slices));
@@ -269,6 +270,7 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
         P.most = plan.chunk ? kLinFew : UINT32_MAX;
         switch (plan.kc) {
             case 2: lin_step<2>(c, P, steps); break;
+            case 3:
             case 4: lin_step<4>(c, P, steps); break;
             case 6: lin_step<6>(c, P, steps); break;
             default: lin_step<8>(c, P, steps); break;
@@ -288,6 +290,7 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
             run(false);
             switch (plan.kc) {
                 case 2: lin_scan<2>(c, P, plan.wide); break;
+                case 3: lin_scan<3>(c, P, plan.wide); break;
                 case 4: lin_scan<4>(c, P, plan.wide); break;
                 case 6: lin_scan<6>(c, P, plan.wide); break;
                 default: lin_scan<8>(c, P, plan.wide); break;

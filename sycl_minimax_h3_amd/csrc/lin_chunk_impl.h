@@ -86,7 +86,8 @@ template <int DT, int KC, int NW, int NV> struct LinShape {
     static constexpr int NP = DT == H3S_BF16 ? 1 : DT == H3S_F16 ? 2 : 3;   // parts of an input
     static constexpr int NS = NP == 3 ? 3 : 2;                              // of the state and of a piece's products
     static constexpr int CT = NP == 1 && KC <= 4 ? 4 : 2, C = 16 * CT, U = CT / 2;
-    static constexpr int T = 64 * NW, DKP = 32 * KC, DVB = 16 * NW * NV;
+    // (in LDS a row is an even number of steps)
+    static constexpr int T = 64 * NW, DKP = 64 * ((KC + 1) / 2), DVB = 16 * NW * NV;
 };
 
 template <int DT, int KC, int NW, int NV, bool OUT, bool VEC>
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(64 * NW, 2) void lin_chunk_kernel(LinArgs P) {
     for (int t = 0; t < 2 * KC; ++t)
 #pragma unroll
         for (int x = 0; x < NV; ++x) s[t][x] = v4f_lin{0.0f, 0.0f, 0.0f, 0.0f};
-    float* ws = P.ws + (int64_t) blockIdx.x * (DKP * DVB) + threadIdx.x * 4;
+    float* ws = P.ws + (int64_t) blockIdx.x * (32 * KC * DVB) + threadIdx.x * 4;
     const int64_t head = (int64_t) P.dk * P.dv;
     if (OUT && it.segs > 1) {
 #pragma unroll
@@ -643,7 +644,7 @@ __global__ __launch_bounds__(64 * NW, 2) void lin_chunk_kernel(LinArgs P) {
     }
 }
 
-// How features of keys (32 KC) and a block's of values (16 NW NV) go to wavefronts: two tiles of values a wavefront read an operand of q and k for
+// How features of keys (32 KC, in steps of 32) and a block's of values (16 NW NV) go to wavefronts: two tiles of values a wavefront read an operand of q and k for
 // twice the products, as long as the state leaves room for them (keys' features up to 128).
 template <int KC, bool WIDE> struct LinWaves { static constexpr int NV = WIDE && KC <= 4 ? 2 : 1, NW = WIDE && KC > 4 ? 8 : 4; };
 
@@ -661,6 +662,7 @@ template <int DT, int KC, bool WIDE> static void lin_chunk_run(Ctx* c, const Lin
 template <int DT, bool WIDE> static void lin_chunk_width(Ctx* c, const LinArgs& P, int kc, int64_t blocks, bool out) {
     switch (kc) {
         case 2: lin_chunk_run<DT, 2, WIDE>(c, P, blocks, out); break;
+        case 3: lin_chunk_run<DT, 3, WIDE>(c, P, blocks, out); break;
         case 4: lin_chunk_run<DT, 4, WIDE>(c, P, blocks, out); break;
         case 6: lin_chunk_run<DT, 6, WIDE>(c, P, blocks, out); break;
         default: lin_chunk_run<DT, 8, WIDE>(c, P, blocks, out); break;

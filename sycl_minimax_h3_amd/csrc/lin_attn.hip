@@ -180,7 +180,7 @@ static int lin_checks(const std::string& fn, const h3_lin_state* state, const h3
 // Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces. Where the sequences beside the longest
 // have more than 2 kLinFew tokens on average, all go in pieces: a launch that finds nothing to do takes 3 to 5 us.
 // Segments: as many as give each CU two blocks of threads, of at least kLinLeast tokens.
-constexpr int kLinFew = 16, kLinLeast = 256;
+constexpr int kLinFew = 16, kLinLeast = 128;
 struct LinPlan {
     bool step, chunk, split;
     int kc, slices;

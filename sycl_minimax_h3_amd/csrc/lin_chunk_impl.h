@@ -346,7 +346,7 @@ __global__ __launch_bounds__(64 * NW, 2) void lin_chunk_kernel(LinArgs P) {
     auto same = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
     const float less_whole = same(expm1f(-decay * (float) C));              // l^C - 1
     const float lp[4] = {1.0f, same(fade(1)), same(fade(2)), same(fade(3))}, lt[4] = {1.0f, same(fade(16)), same(fade(32)), same(fade(48))};
-    const float row_fade = fade(l15 + 1) * P.scale, back_fade = fade(12 - 4 * g);
+    const float row_fade = fade(l15 + 1) * P.scale, back_fade = fade(12 - 4 * g), left_fade = fade(13 + l15 - 4 * g) * P.scale;
     if constexpr (OUT) {
         // the tiles right of the diagonal that share an operand with one on it
         for (int i = threadIdx.x; i < CT * U * NS * 64; i += T) (&sp[0][0][0])[i] = make_uint4(0, 0, 0, 0);
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(64 * NW, 2) void lin_chunk_kernel(LinArgs P) {
             // P^T = K Q^T . D of every NW-th tile, as an operand
             for (int e = wave; e < CT * (CT + 1) / 2; e += NW) {
                 const int ti = e >= 6 ? 3 : e >= 3 ? 2 : e >= 1 ? 1 : 0, tj = e - ti * (ti + 1) / 2;
-                v4f_lin x = {0.0f, 0.0f, 0.0f, 0.0f};
+                v4f_lin z2[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
                 for (int u = 0; u < KC; ++u) {
                     uint4 a[NP], b[NP];
@@ -379,13 +379,20 @@ __global__ __launch_bounds__(64 * NW, 2) void lin_chunk_kernel(LinArgs P) {
                     for (int y = 0; y < NP; ++y)
 #pragma unroll
                         for (int z = 0; z < NP; ++z)
-                            if (NP < 3 || y + z < NP) x = lin_mma(a[y], b[z], x);
+                            if (NP < 3 || y + z < NP) z2[u & 1] = lin_mma(a[y], b[z], z2[u & 1]);
                 }
+                const v4f_lin x = z2[0] + z2[1];
                 float f[4];
+                if (ti == tj) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int steps = 16 * (ti - tj) + l15 - 4 * g - i;
-                    f[i] = steps < 0 ? 0.0f : x[i] * (fade(steps) * P.scale);
+                    for (int i = 0; i < 4; ++i) {
+                        const int steps = l15 - 4 * g - i;
+                        f[i] = steps < 0 ? 0.0f : x[i] * (fade(steps) * P.scale);
+                    }
+                } else {                                                    // 16 (ti - tj) + l15 - 4 g - i steps, all above 0
+                    const float w = left_fade * (ti - tj == 1 ? 1.0f : ti - tj == 2 ? lt[1] : lt[2]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[i] = x[i] * (w * lp[3 - i]);
                 }
                 uint32_t w[2][NS];
                 lin_split<NS>(f[0], f[1], w[0]);

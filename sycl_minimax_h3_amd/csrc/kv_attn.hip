@@ -63,10 +63,11 @@ static int kv_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sigh
 // The launch of the shared tokens: all rows of a group are as one sequence's, and how many groups' rows there are is known, not each one's.
 static KvPlan kv_shared_plan(const KvArgs& P, bool two, const KvSight& sight, int cus) {
     KvPlan plan;
+    plan.shared = true;
     const int64_t rows = P.rows * sight.group, each = (rows + sight.groups - 1) / sight.groups;
     auto places = [&](int64_t rt) { return rows / rt + sight.groups; };
     plan.rows = each > (P.dim <= 128 ? 32 : 16);
-    plan.nq = plan.rows ? (two || each <= 96 || places(128) * P.heads < cus ? 1 : 2) : each <= 16 ? 1 : 2;
+    plan.nq = plan.rows ? (two || each <= 96 ? 1 : 2) : each <= 16 ? 1 : 2;
     plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
     plan.tiles = 0;
     plan.places = places(plan.rt);
@@ -77,8 +78,8 @@ static KvPlan kv_shared_plan(const KvArgs& P, bool two, const KvSight& sight, in
     plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
     return plan;
 }
-static int64_t kv_part_floats(const KvPlan& plan, int64_t W, bool always) {
-    return plan.nsplit > 1 || always ? plan.blocks * plan.nsplit * plan.rt * (W + 2) : 0;
+static int64_t kv_part_floats(const KvPlan& plan, int64_t W) {
+    return plan.nsplit > 1 || plan.shared ? plan.blocks * plan.nsplit * plan.rt * (W + 2) : 0;
 }
 
 static int attn_checks(const char* fn, const KvArgs& P, int64_t max_len, int64_t q_heads, int64_t window) {
@@ -103,10 +104,20 @@ static int sight_of(const std::string& fn, const KvArgs& P, const h3_kv_shared* 
     sight.shared = shared->most > 0 ? std::min<int64_t>(shared->most, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     return 0;
 }
-// all launches' plans: of the shared tokens first, where there are any
+// Whether shared tokens are a launch of their own. A launch and the reading of its sums cost 8 us or more; below so many bytes of all sequences'
+// caches a CU it takes less to go through the shared ones again for each (they come from the caches of the device).
+constexpr int64_t kKvApart = 192 << 10;
+static bool kv_apart(const KvArgs& P, const KvSight& sight, int cus) {
+    const int64_t tokens = sight.max_len > 0 ? std::min<int64_t>(sight.max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
+    return sight.groups > 0 && std::max(tokens, sight.shared) * P.seqs > cus * kKvApart / (2 * P.heads * kv_width(P.dim));
+}
+// all launches' plans: of the shared tokens first, where they have one
 static int kv_all_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[3]) {
     KvPlan own[2];
-    const int n = kv_plans(P, two, most, sight, cus, own), at = sight.groups ? 1 : 0;
+    const int at = kv_apart(P, sight, cus) ? 1 : 0;
+    KvSight behind = sight;
+    if (!at) behind.shared = 0;
+    const int n = kv_plans(P, two, most, behind, cus, own);
     if (at) plan[0] = kv_shared_plan(P, two, sight, cus);
     for (int i = 0; i < n; ++i) plan[at + i] = own[i];
     return at + n;
@@ -125,7 +136,7 @@ static int64_t attend_work(const char* fn, void* ctx, const h3_kv_cache* cache, 
     for (bool two : {false, true}) {
         KvPlan plan[3];
         int64_t sum = 0;
-        for (int n = kv_all_plans(P, two, batch->most, sight, c->cus, plan); n-- > 0;) sum += kv_part_floats(plan[n], kv_width(P.dim), sight.groups > 0);
+        for (int n = kv_all_plans(P, two, batch->most, sight, c->cus, plan); n-- > 0;) sum += kv_part_floats(plan[n], kv_width(P.dim));
         floats = std::max(floats, sum);
     }
     return 4 * floats;
@@ -154,9 +165,9 @@ static int attend(const char* fn, void* ctx, const h3_kv_cache* cache, const h3_
     int64_t floats = 0;
     for (int i = 0; i < launches; ++i) {
         // (the merge has a block of threads a row)
-        const int64_t each = std::max<int64_t>(plans[i].nsplit, plans[i].nsplit > 1 || groups ? plans[i].rt : 1);
+        const int64_t each = std::max<int64_t>(plans[i].nsplit, plans[i].nsplit > 1 ? plans[i].rt : 1);
         if (plans[i].blocks > kKvMostBlocks || plans[i].blocks * each > kKvMostBlocks) return fail(std::string(fn) + ": too many blocks of work");
-        floats += kv_part_floats(plans[i], W, groups);
+        floats += kv_part_floats(plans[i], W);
     }
     float* parts = nullptr;
     if (floats) {
@@ -188,8 +199,8 @@ static int attend(const char* fn, void* ctx, const h3_kv_cache* cache, const h3_
         A.least = plan.least; A.greatest = plan.greatest;
         A.po = parts;
         A.pml = parts ? parts + plan.blocks * plan.nsplit * plan.rt * W : nullptr;
-        if (parts) parts += kv_part_floats(plan, W, groups);
-        const bool first = groups && i == 0;
+        if (parts) parts += kv_part_floats(plan, W);
+        const bool first = plan.shared;
         if (groups || A.sinks > 0) {
             switch (W / 64) {
                 case 1: kv_spans_64(c, A, plan, two, first); break;

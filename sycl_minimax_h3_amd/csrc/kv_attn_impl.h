@@ -63,7 +63,7 @@ struct KvAttnArgs {
     int sinks;                                      // the first tokens that stay visible behind a window
     const int32_t *first, *shared;                  // [groups + 1]: a group's first sequence; [groups]: the tokens that it shares
     int groups;
-    int rt2, nsplit2;                               // the rows of a block, and the parts, of the shared tokens' launch
+    int rt2, nsplit2;                               // the rows of a block, and the parts, of the shared tokens' launch (0 parts: there is none)
     const float *po2, *pml2;                        // its parts
 };
 
@@ -313,37 +313,48 @@ template <int WC, int NQ, bool TWO, bool PTWO, int MODE> struct KvRows {
     }
 };
 
-// The group that sequence b shares tokens in, or -1; found by the whole wavefront, 64 groups at a time (as kv_find).
-__device__ __forceinline__ int kv_group_of(const KvAttnArgs& P, int b) {
+// the first row of group c's sequences (of `groups`: behind the last), whatever `first` and `starts` say
+__device__ __forceinline__ int kv_first_row(const KvAttnArgs& P, int first) {
+    return min(max(P.kv.starts[min(max(first, 0), P.kv.seqs)], 0), P.kv.rows);
+}
+// The group that sequence b shares tokens in, or -1, its first sequence, the cache blocks that it shares and its rows [row, end); found by the
+// whole wavefront, 64 groups at a time (as kv_find).
+__device__ __forceinline__ int kv_group_of(const KvAttnArgs& P, int b, int& first, int& blocks, int& row, int& end) {
     const int lane = threadIdx.x & 63;
     int step = 1;
     while (step * 64 < P.groups + 1) step *= 64;
     for (int g = 0;; step /= 64) {
-        const int c = g + lane * step, f = P.first[min(c, P.groups)];
+        const int c = g + lane * step, f = P.first[min(c, P.groups)], n = P.shared[min(c, P.groups - 1)];
         const int k = (int) __popcll(__ballot(c <= P.groups && f <= b) & ~1ull);
         g += k * step;
         if (step > 1) continue;
-        const int from = __builtin_amdgcn_readlane(f, k), to = k < 63 ? __builtin_amdgcn_readlane(f, k + 1) : P.first[min(g + 1, P.groups)];
-        return from <= b && g < P.groups && b < to ? g : -1;
+        first = __builtin_amdgcn_readlane(f, k);
+        const int to = k < 63 ? __builtin_amdgcn_readlane(f, k + 1) : P.first[min(g + 1, P.groups)];
+        blocks = min(max(__builtin_amdgcn_readlane(n, k), 0) / kKvB, P.kv.width);
+        if (first > b || g >= P.groups || b >= to) return -1;
+        first = max(first, 0);
+        row = kv_first_row(P, first);
+        end = kv_first_row(P, to);
+        return g;
     }
 }
-// the first row of group c's sequences (of `groups`: behind the last), whatever `first` and `starts` say
-__device__ __forceinline__ int kv_group_row(const KvAttnArgs& P, int c) {
-    return min(max(P.kv.starts[min(max(P.first[min(c, P.groups)], 0), P.kv.seqs)], 0), P.kv.rows);
-}
-// kv_find of groups in place of sequences: each is as one sequence of all its rows
-__device__ __forceinline__ int kv_find_group(const KvAttnArgs& P, int at, uint32_t den, int& grp, int& r0, int& n) {
+// kv_find of groups in place of sequences: each is as one sequence of all its rows. Also its sequences [b, b1) and shared cache blocks.
+__device__ __forceinline__ int kv_find_group(const KvAttnArgs& P, int at, uint32_t den, int& r0, int& n, int& b, int& b1, int& blocks) {
     const int lane = threadIdx.x & 63;
     int step = 1;
     while (step * 64 < P.groups) step *= 64;
-    for (grp = 0;; step /= 64) {
-        const int c = grp + lane * step, s = kv_group_row(P, c);
+    for (int g = 0;; step /= 64) {
+        const int c = g + lane * step, f = P.first[min(c, P.groups)], t = P.shared[min(c, P.groups - 1)], s = kv_first_row(P, f);
         const int begin = (int) ((uint32_t) s * (uint32_t) P.group / den) + min(c, P.groups);
         const int k = (int) __popcll(__ballot(c < P.groups && begin <= at) & ~1ull);
-        grp += k * step;
+        g += k * step;
         if (step > 1) continue;
         r0 = __builtin_amdgcn_readlane(s, k);
-        n = max(k < 63 ? __builtin_amdgcn_readlane(s, k + 1) : kv_group_row(P, grp + 1), r0) - r0;
+        b = min(max(__builtin_amdgcn_readlane(f, k), 0), P.kv.seqs);
+        blocks = min(max(__builtin_amdgcn_readlane(t, k), 0) / kKvB, P.kv.width);
+        const int next = k < 63 ? __builtin_amdgcn_readlane(f, k + 1) : P.first[min(g + 1, P.groups)];
+        b1 = min(max(next, b), P.kv.seqs);
+        n = max(k < 63 ? __builtin_amdgcn_readlane(s, k + 1) : kv_first_row(P, next), r0) - r0;
         return at - __builtin_amdgcn_readlane(begin, k);
     }
 }
@@ -354,7 +365,8 @@ template <int MODE> struct KvItem {
     int h, split, place, b, tile, r0, n, len;
     uint32_t R;
     int b1 = 0;                                                           // kKvShared: behind the group's last sequence
-    int lo = 0, hi = 0, sink = 0, win = 0;                                // cache blocks: see range()
+    int lo = 0, hi = 0, sink = 0, win = 0;                                // cache blocks: see spans()
+    int first = 0, group = -1, row = 0, end_row = 0;                      // kKvOwn: the first sequence of its group, its group and that one's rows
     template <int RT> __device__ __forceinline__ void take(const KvAttnArgs& P) {
         uint32_t id = blockIdx.x;
         h = (int) (id % (uint32_t) P.kv.heads);
@@ -366,12 +378,8 @@ template <int MODE> struct KvItem {
     template <int RT> __device__ __forceinline__ void rows(const KvAttnArgs& P, int at) {
         place = at;
         if constexpr (MODE == kKvShared) {
-            int grp;
-            tile = kv_find_group(P, P.places - 1 - at, RT, grp, r0, n);
-            place = P.places - 1 - at;                                    // (kv_join_kernel counts from the groups' rows)
-            b = min(max(P.first[grp], 0), P.kv.seqs);
-            b1 = min(max(P.first[grp + 1], b), P.kv.seqs);
-            hi = min(max(P.shared[grp], 0) / kKvB, P.kv.width);
+            place = P.places - 1 - at;                                    // (the longest rows first; kv_shared_row counts from the groups' rows)
+            tile = kv_find_group(P, place, RT, r0, n, b, b1, hi);
             R = tile < 0 || b1 <= b ? 0 : (uint32_t) n * P.group;
             b = min(b, P.kv.seqs - 1);
             len = 0;
@@ -389,8 +397,9 @@ template <int MODE> struct KvItem {
         len = min(max(P.lengths[b], 0), P.kv.width * kKvB);
         if constexpr (MODE == kKvOwn)
             if (P.groups) {
-                const int grp = kv_group_of(P, b);
-                lo = grp < 0 ? 0 : min(max(P.shared[grp], 0) / kKvB, P.kv.width);
+                group = kv_group_of(P, b, first, hi, row, end_row);
+                if (group < 0) { first = b; hi = 0; }
+                lo = P.nsplit2 ? hi : 0;
             }
     }
     // the cache blocks kb0 .. kb0 + count that any of the rows rt0 .. rt0 + rt can see
@@ -401,7 +410,7 @@ template <int MODE> struct KvItem {
         count = bmax >= 0 ? max(bmax / kKvB + 1 - kb0, 0) : 0;
     }
     // The same of rows that are the tokens bmin .. bmax, as a count from 0: first the blocks of the first tokens, lo .. lo + sink, then those from
-    // win on. (Shared tokens end at block hi, a sequence's own begin at block lo.)
+    // win on. (Shared tokens end at block hi, a sequence's own begin at block lo: hi too, or 0 where there is no launch of the shared ones.)
     __device__ __forceinline__ void spans(const KvAttnArgs& P, int bmin, int bmax, int& kb0, int& count) {
         int end = bmax >= 0 ? bmax / kKvB + 1 : 0;
         if constexpr (MODE == kKvShared) end = min(end, hi);
@@ -474,9 +483,30 @@ template <int N> __device__ __forceinline__ void kv_reach(const int2* who, int& 
 template <int RT> __device__ __forceinline__ void kv_nothing(const KvAttnArgs& P, const KvItem<kKvShared>& it) {
     if (threadIdx.x < RT) *reinterpret_cast<float2*>(P.pml + (it.part(P) * RT + threadIdx.x) * 2) = make_float2(kKvUnset, 0.0f);
 }
-// Whether a launch's sums are the results, or parts of them
-template <int MODE> __device__ __forceinline__ bool kv_direct(const KvAttnArgs& P) {
-    return MODE != kKvShared && P.nsplit == 1 && (MODE == kKvAll || P.groups == 0);
+// Whether a launch's sums are the results (with the shared tokens' parts), or parts of them
+template <int MODE> __device__ __forceinline__ bool kv_direct(const KvAttnArgs& P) { return MODE != kKvShared && P.nsplit == 1; }
+
+// kKvOwn: the first of the parts over shared tokens of row rr of the item's sequence, rt2 rows apart, or -1
+__device__ __forceinline__ int64_t kv_shared_row(const KvAttnArgs& P, const KvItem<kKvOwn>& it, uint32_t rr) {
+    if (it.group < 0 || P.nsplit2 == 0) return -1;
+    const int row = it.r0 + (int) (rr / (uint32_t) P.group);
+    if (row < it.row || row >= it.end_row) return -1;
+    const uint32_t r2 = (uint32_t) (row - it.row) * (uint32_t) P.group + rr % (uint32_t) P.group, rt2 = (uint32_t) P.rt2;
+    const int64_t place = (int) ((uint32_t) it.row * (uint32_t) P.group / rt2) + it.group + (int) (r2 / rt2);
+    return (place * P.kv.heads + it.h) * P.nsplit2 * rt2 + r2 % rt2;
+}
+// The row's maximum and sum with the parts over shared tokens, and the factor for its own sums
+__device__ __forceinline__ float kv_shared_top(const KvAttnArgs& P, int64_t row2, float& mx, float& lt) {
+    float m = mx, l = 0.0f;
+    for (int s = 0; s < P.nsplit2; ++s) m = fmaxf(m, P.pml2[(row2 + (int64_t) s * P.rt2) * 2]);
+    const float own = __builtin_amdgcn_exp2f(mx - m);
+    for (int s = 0; s < P.nsplit2; ++s) {
+        const float2 ml = *reinterpret_cast<const float2*>(P.pml2 + (row2 + (int64_t) s * P.rt2) * 2);
+        l = __builtin_fmaf(ml.y, __builtin_amdgcn_exp2f(ml.x - m), l);
+    }
+    mx = m;
+    lt = __builtin_fmaf(lt, own, l);
+    return own;
 }
 
 // Whether a key block is seen whole by rows that are the tokens posmin .. posmax
@@ -488,10 +518,11 @@ template <int MODE> __device__ __forceinline__ bool kv_whole(const KvAttnArgs& P
 // known without a wait for memory: read entry by entry, its latency stood before every block's loads (64 sequences of up to 8192 tokens
 // 133.4 us, 130.7 so; 601 float32 tokens 33.8 and 33.1).
 template <int MODE> struct KvPages {
-    const int32_t* table;
+    const int32_t *table, *shared;                  // kKvOwn: the sequence's row, and that of its group's first sequence for the blocks before hi
     int width, base, entry;
-    __device__ __forceinline__ void take(const KvAttnArgs& P, int b) {
-        table = P.kv.table + (int64_t) b * P.kv.width;
+    __device__ __forceinline__ void take(const KvAttnArgs& P, const KvItem<MODE>& it) {
+        table = P.kv.table + (int64_t) it.b * P.kv.width;
+        if constexpr (MODE == kKvOwn) shared = P.kv.table + (int64_t) it.first * P.kv.width;
         width = P.kv.width;
         base = -64;
     }
@@ -500,7 +531,9 @@ template <int MODE> struct KvPages {
         for (; kb < last; kb += BY) {
             if (kb - base >= 64) {
                 base = kb;
-                entry = table[min(it.block(kb + lane), width - 1)];
+                const int at = min(it.block(kb + lane), width - 1);
+                if constexpr (MODE == kKvOwn) entry = (at < it.hi ? shared : table)[at];
+                else entry = table[at];
             }
             page = __builtin_amdgcn_readlane(entry, kb - base);
             if (page >= 0 && page < P.kv.blocks) return true;
@@ -528,9 +561,14 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     int kb0, count;
     __shared__ int2 who[MODE == kKvShared ? RT : 1];
     if constexpr (MODE == kKvShared) {
-        kv_who<RT>(P, it, rw, who);
-        __syncthreads();
-        kv_reach<RT>(who, posmin, posmax);
+        // (without a window the rows' places decide nothing before the first scores: they are found behind the first loads)
+        if (P.window > 0) {
+            kv_who<RT>(P, it, rw, who);
+            __syncthreads();
+            kv_reach<RT>(who, posmin, posmax);
+        } else {
+            posmin = posmax = INT32_MAX;
+        }
         it.spans(P, posmin, posmax, kb0, count);
         if (it.split && it.split * P.per >= count) return kv_nothing<RT>(P, it);
     } else {
@@ -539,7 +577,7 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     }
     const int last = it.end(P, kb0, count);
     KvPages<MODE> pages;
-    pages.take(P, b);
+    pages.take(P, it);
     uint4 kr[4][WC], vr[DT];
     const int koff = ((l15 >> 2) * 16 + (l15 & 3)) * W + g * 16, voff = l15 * 64 + g * 16;
     auto load_k = [&](int page) {
@@ -562,6 +600,12 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
         ks = P.kv.ks[(int64_t) page * P.kv.heads + h];
         vs = P.kv.vs[(int64_t) page * P.kv.heads + h];
     }
+    if constexpr (MODE == kKvShared)
+        if (P.window == 0) {
+            kv_who<RT>(P, it, rw, who);
+            __syncthreads();
+            kv_reach<RT>(who, posmin, posmax);
+        }
     KvRows<WC, NQ, TWO, true, MODE> q;              // (behind the first loads of the cache, which take longer)
     q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g, who);
     while (kb < last) {
@@ -630,6 +674,16 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
             }
             const int64_t at = ((int64_t) it.r0 + rr / group) * P.q_heads + h * group + rr % group;
             const int64_t row = it.part(P) * RT + 16 * e + r;
+            float top = mx;
+            int64_t row2 = -1;
+            if constexpr (MODE == kKvOwn) {
+                row2 = kv_direct<MODE>(P) ? kv_shared_row(P, it, rr) : -1;
+                if (row2 >= 0) {
+                    const float own = kv_shared_top(P, row2, top, lt);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) wt[w] *= own;
+                }
+            }
             const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
 #pragma unroll
             for (int t = 0; t < WC; ++t) {
@@ -643,12 +697,27 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
                     y[2] = __builtin_fmaf(v.z, wt[w], y[2]);
                     y[3] = __builtin_fmaf(v.w, wt[w], y[3]);
                 }
+                if constexpr (MODE == kKvOwn)
+                    if (row2 >= 0) {
+#pragma unroll 4
+                        for (int s = 0; s < P.nsplit2; ++s) {
+                            const int64_t from = row2 + (int64_t) s * P.rt2;
+                            const float2 ml = *reinterpret_cast<const float2*>(P.pml2 + from * 2);
+                            const float4 v = *reinterpret_cast<const float4*>(P.po2 + from * W + d);
+                            if (ml.y == 0.0f) continue;                   // (nothing seen: there are no sums)
+                            const float w = __builtin_amdgcn_exp2f(ml.x - top);
+                            y[0] = __builtin_fmaf(v.x, w, y[0]);
+                            y[1] = __builtin_fmaf(v.y, w, y[1]);
+                            y[2] = __builtin_fmaf(v.z, w, y[2]);
+                            y[3] = __builtin_fmaf(v.w, w, y[3]);
+                        }
+                    }
                 if (kv_direct<MODE>(P)) kv_store4(P, at * P.kv.dim, d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
                 else *reinterpret_cast<float4*>(P.po + row * W + d) = make_float4(y[0], y[1], y[2], y[3]);
             }
             if (c == 0) {
                 if (!kv_direct<MODE>(P)) *reinterpret_cast<float2*>(P.pml + row * 2) = make_float2(mx, lt);
-                else if (P.lse) P.lse[at] = kv_lse(mx, lt);
+                else if (P.lse) P.lse[at] = kv_lse(top, lt);
             }
         }
     }
@@ -680,19 +749,22 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
     int kb0, count;
     __shared__ int2 who[MODE == kKvShared ? RT : 1];
     if constexpr (MODE == kKvShared) {
-        kv_who<RT>(P, it, rt0, who);
-        __syncthreads();
-        kv_reach<RT>(who, posmin, posmax);
+        if (P.window > 0) {                         // (as above)
+            kv_who<RT>(P, it, rt0, who);
+            __syncthreads();
+            kv_reach<RT>(who, posmin, posmax);
+        } else {
+            posmin = posmax = INT32_MAX;
+        }
         it.spans(P, posmin, posmax, kb0, count);
         if (it.split && it.split * P.per >= count) return kv_nothing<RT>(P, it);
-        kv_reach<16 * NQ>(who + wave * 16 * NQ, posmin, posmax);
     } else {
         it.range(P, rt0, RT, kb0, count);
         if (it.split && it.split * P.per >= count) return;
     }
     const int last = it.end(P, kb0, count);
     KvPages<MODE> pages;
-    pages.take(P, b);
+    pages.take(P, it);
     // the thread's 16-byte pieces of a block's codes: piece t + 256 i
     uint4 kr[WC], vr[WC];
     float ks = 0.0f, vs = 0.0f;
@@ -728,6 +800,13 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
     bool more = false;
     float ks_now = 0.0f, vs_now = 0.0f;
     if (any) load(page);
+    if constexpr (MODE == kKvShared) {
+        if (P.window == 0) {
+            kv_who<RT>(P, it, rt0, who);
+            __syncthreads();
+        }
+        kv_reach<16 * NQ>(who + wave * 16 * NQ, posmin, posmax);
+    }
     KvRows<WC, NQ, TWO, TWO, MODE> q;
     q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g, who + (MODE == kKvShared ? wave * 16 * NQ : 0));
     if (any) {
@@ -801,8 +880,30 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
     }
 #pragma unroll
     for (int e = 0; e < NQ; ++e) {
-        const float l = kv_sum4(q.l[e]);
+        float l = kv_sum4(q.l[e]);
         if (q.tok[e] < 0) continue;
+        if constexpr (MODE == kKvOwn) {
+            const int64_t row2 = kv_direct<MODE>(P) ? kv_shared_row(P, it, rw + 16 * e + l15) : -1;
+            if (row2 >= 0) {
+                const float own = kv_shared_top(P, row2, q.m[e], l);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) q.o[e][t] *= own;
+                for (int s = 0; s < P.nsplit2; ++s) {
+                    const int64_t from = row2 + (int64_t) s * P.rt2;
+                    const float2 ml = *reinterpret_cast<const float2*>(P.pml2 + from * 2);
+                    if (ml.y == 0.0f) continue;                           // (nothing seen: there are no sums)
+                    const float w = __builtin_amdgcn_exp2f(ml.x - q.m[e]);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const float4 v = *reinterpret_cast<const float4*>(P.po2 + from * W + 16 * t + 4 * g);
+                        q.o[e][t][0] = __builtin_fmaf(v.x, w, q.o[e][t][0]);
+                        q.o[e][t][1] = __builtin_fmaf(v.y, w, q.o[e][t][1]);
+                        q.o[e][t][2] = __builtin_fmaf(v.z, w, q.o[e][t][2]);
+                        q.o[e][t][3] = __builtin_fmaf(v.w, w, q.o[e][t][3]);
+                    }
+                }
+            }
+        }
         if (kv_direct<MODE>(P)) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t at = q.tok[e] * P.q_heads + q.head[e];
@@ -882,19 +983,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttnArgs P) {
     it.range(P, (uint32_t) it.tile * RT, RT, kb0, count);
     const int own = min(max((count + P.per - 1) / P.per, 1), P.nsplit);
     const int64_t row0 = item * P.nsplit * RT + r;
-    int parts = own;
-    int64_t row2 = 0;
-    const int grp = kv_group_of(P, it.b);
-    if (grp >= 0) {
-        const int from = kv_group_row(P, grp), to = kv_group_row(P, grp + 1);
-        const int row = it.r0 + (int) (rr / group);
-        if (row >= from && row < to) {
-            const uint32_t r2 = (uint32_t) (row - from) * group + rr % group, rt2 = (uint32_t) P.rt2;
-            const int64_t place = (int) ((uint32_t) from * group / rt2) + grp + (int) (r2 / rt2);
-            row2 = (place * P.kv.heads + it.h) * P.nsplit2 * rt2 + r2 % rt2;
-            parts += P.nsplit2;
-        }
-    }
+    const int64_t row2 = kv_shared_row(P, it, rr);
+    const int parts = own + (row2 >= 0 ? P.nsplit2 : 0);
     auto ml_of = [&](int s) {
         return s < own ? *reinterpret_cast<const float2*>(P.pml + (row0 + (int64_t) s * RT) * 2)
                        : *reinterpret_cast<const float2*>(P.pml2 + (row2 + (int64_t) (s - own) * P.rt2) * 2);
@@ -939,6 +1029,7 @@ struct KvPlan {
     int nsplit, per;      // parts, and the cache blocks of each
     int64_t blocks;       // of threads, without the parts
     uint32_t least = 0, greatest = UINT32_MAX;
+    bool shared = false;  // of the shared tokens
 };
 
 template <int WC, int NQ, bool ROWS, int MODE>
@@ -953,8 +1044,8 @@ static void kv_attn_run(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool tw
         else kv_attn_kernel<WC, NQ, false, MODE><<<grid, 256, 0, c->stream>>>(P);
     }
     if constexpr (MODE == kKvOwn)
-        if (P.groups) {
-            kv_join_kernel<WC, RT><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
+        if (P.nsplit2) {
+            if (plan.nsplit > 1) kv_join_kernel<WC, RT><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
             return;
         }
     if constexpr (MODE != kKvShared)

@@ -1,5 +1,7 @@
 """Attention over the key/value cache behind a window with first tokens that stay visible, and over tokens that groups of sequences share
 (include/h3lm.h, kv_attention_spans), against its restatement in numpy (spans_reference.py)."""
+import os
+
 import numpy as np
 import pytest
 
@@ -13,6 +15,33 @@ pytestmark = pytest.mark.gpu
 from sycl_minimax_h3_amd import Device, Error, ops  # noqa: E402
 
 BLOCK = lm.BLOCK
+
+
+def context(cus):
+    """A context that sizes its grids for so many compute units: shared tokens are a launch of their own from fewer bytes on."""
+    old = os.environ.get("H3S_CUS")
+    os.environ["H3S_CUS"] = str(cus)
+    try:
+        return Device.open()
+    finally:
+        if old is None:
+            del os.environ["H3S_CUS"]
+        else:
+            os.environ["H3S_CUS"] = old
+
+
+@pytest.fixture(scope="module")
+def dev2():
+    d = context(2)
+    yield d
+    d.close()
+
+
+@pytest.fixture(scope="module")
+def dev16():
+    d = context(16)
+    yield d
+    d.close()
 
 
 class Case:
@@ -120,7 +149,10 @@ SHARED = [
 
 
 @pytest.mark.parametrize("seqs,groups,heads,group,dim,dt", SHARED)
-def test_shared_tokens(dev, seqs, groups, heads, group, dim, dt):
+@pytest.mark.parametrize("apart", [False, True])
+def test_shared_tokens(dev, dev2, seqs, groups, heads, group, dim, dt, apart):
+    """Through a launch of their own and not."""
+    dev = dev2 if apart else dev
     case = Case(dev, seqs, heads, group, dim, dt, groups)
     for out_dt in ("F32", dt if dt != "F32" else "BF16"):
         case.check(case.run(out_dt), case.want(out_dt), out_dt)
@@ -131,7 +163,25 @@ def test_shared_tokens(dev, seqs, groups, heads, group, dim, dt):
     masked.check(masked.run(window=100, sinks=3), masked.want(window=100, sinks=3), "mask, window")
 
 
-def test_shared_blocks_that_are_not_there(dev):
+@pytest.mark.parametrize("seqs,groups,dim,dt", [
+    ([(1, 2100), (1, 1900), (2, 1500)], [(0, 3, 1000)], 256, "BF16"),
+    ([(30, 1100), (1, 1900), (2, 1500)], [(0, 3, 960)], 128, "F32"),
+])
+def test_shared_tokens_in_parts(dev16, seqs, groups, dim, dt):
+    """Both the shared tokens and the sequences' own in several parts, which a launch of its own joins."""
+    case = Case(dev16, seqs, 4, 2, dim, dt, groups)
+    args, shared, _ = case.upload()
+    out = new(dev16, "F32", [case.rows, 8 * dim])
+    work = new(dev16, "U8", [ops.kv_attention_work(*args[:4], case.most, shared=shared)])
+    ran = [name.split("<")[0] for name, _, _ in launches(dev16, lambda: ops.kv_attention(*args, out, shared=shared, work=work))]
+    assert "kv_join_kernel" in ran, ran
+    case.check(case.run(), case.want())
+    case.check(case.run(window=700, sinks=100), case.want(window=700, sinks=100), "window")
+
+
+@pytest.mark.parametrize("apart", [False, True])
+def test_shared_blocks_that_are_not_there(dev, dev2, apart):
+    dev = dev2 if apart else dev
     case = Case(dev, [(1, 600), (1, 500), (40, 480)], 2, 4, 64, "BF16", [(0, 3, 448)])
     case.table[0, [1, 2, 6]] = [-1, 1 << 29, -(1 << 31)]
     case.check(case.run(), case.want())
@@ -142,8 +192,10 @@ def test_shared_blocks_that_are_not_there(dev):
     assert (got[0][:42] == 0).all() and np.isneginf(got[1][:42]).all()
 
 
-def test_infinite_scales_of_shared_blocks(dev):
+@pytest.mark.parametrize("apart", [False, True])
+def test_infinite_scales_of_shared_blocks(dev, dev2, apart):
     """A shared block whose scale is NaN, hidden by the mask or by the window, has no effect; seen, it makes its rows NaN."""
+    dev = dev2 if apart else dev
     for seqs in ([(1, 300), (1, 260)], [(50, 300), (20, 260)]):
         case = Case(dev, seqs, 1, 4, 64, "BF16", [(0, 2, 192)])
         case.cache.s[:, case.table[0, 0]] = np.nan
@@ -155,8 +207,10 @@ def test_infinite_scales_of_shared_blocks(dev):
         assert np.isnan(case.run()[0][:int(case.starts[-1])]).all()
 
 
-def test_groups_out_of_order_and_range(dev):
+@pytest.mark.parametrize("apart", [False, True])
+def test_groups_out_of_order_and_range(dev, dev2, apart):
     """Firsts that run back, below zero or past the sequences: nothing outside the buffers is touched, sequences in no group are right."""
+    dev = dev2 if apart else dev
     for first in ([-5, 2, 1, 9], [3, 1, 4, 2], [1 << 30, -(1 << 31), 5, 0], [0, 0, 0, 0]):
         case = Case(dev, [(1, 200), (2, 300), (1, 150), (1, 90)], 1, 4, 64, "F32")
         args, _, _ = case.upload()
@@ -183,10 +237,10 @@ def test_without_first_tokens_or_groups_it_is_kv_attention(dev):
 
 
 @pytest.mark.parametrize("sinks", [0, 70])
-def test_workspace_and_graph(dev, sinks):
+def test_workspace_and_graph(dev16, sinks):
     """With a workspace of its own a call can be recorded, and replayed on new lengths and shared tokens; a smaller one is refused, and so
     is none while a graph is recorded. Two graphs, each with its own, take turns with eager calls."""
-    made = []
+    dev, made = dev16, []
     for seed in (31, 32):
         case = Case(dev, [(1, 900), (1, 1200), (2, 800), (1, 1000)], 2, 4, 128, "BF16", [(0, 3, 700)] if not sinks else (), seed=seed)
         args, shared, _ = case.upload()
@@ -220,7 +274,7 @@ def test_workspace_and_graph(dev, sinks):
 
 def test_two_contexts(dev):
     """Two contexts on streams of their own, called in turn without a wait between: each its own scratch."""
-    other = Device.open()
+    other = context(2)
     case = [Case(d, [(1, 900), (1, 1200), (1, 800)], 2, 4, 128, "BF16", [(0, 3, 700)], seed=33 + i) for i, d in enumerate((dev, other))]
     held = [(c.upload(), new(c.dev, "F32", [c.rows, 1024])) for c in case]
     for _ in range(20):
@@ -234,12 +288,14 @@ def test_two_contexts(dev):
     other.close()
 
 
-def test_which_kernels_run(dev):
-    """The shared tokens' launch, the sequences' own, and what joins them."""
-    case = Case(dev, [(1, 300)] * 8, 2, 8, 128, "BF16", [(0, 8, 256)])
-    args, shared, _ = case.upload()
-    out = new(dev, "F32", [case.rows, 2 * 8 * 128])
-    work = new(dev, "U8", [ops.kv_attention_work(*args[:4], 1, shared=shared)])
-    ran = [name for name, _, _ in launches(dev, lambda: ops.kv_attention(*args, out, shared=shared, work=work))]
-    assert [n.split("<")[0] for n in ran] == ["kv_attn_rows_kernel", "kv_attn_kernel", "kv_join_kernel"], ran
-    assert ran[0].startswith("kv_attn_rows_kernel<2, 1, false, 2>") and ran[1].startswith("kv_attn_kernel<2, 1, false, 1>"), ran
+def test_which_kernels_run(dev, dev2):
+    """A small batch goes through the shared tokens for each sequence; a larger one (for the context) has a launch of them, whose sums the
+    sequences' own launch takes up."""
+    for d, want in ((dev, ["kv_attn_kernel<2, 1, false, 1>", "kv_merge_kernel<2, 16, 1>"]),
+                    (dev2, ["kv_attn_rows_kernel<2, 1, false, 2>", "kv_attn_kernel<2, 1, false, 1>"])):
+        case = Case(d, [(1, 700)] * 8, 2, 8, 128, "BF16", [(0, 8, 256)])
+        args, shared, _ = case.upload()
+        out = new(d, "F32", [case.rows, 2 * 8 * 128])
+        work = new(d, "U8", [ops.kv_attention_work(*args[:4], 1, shared=shared)])
+        ran = [name for name, _, _ in launches(d, lambda: ops.kv_attention(*args, out, shared=shared, work=work))]
+        assert len(ran) == 2 and all(r.startswith(w) for r, w in zip(ran, want)), ran

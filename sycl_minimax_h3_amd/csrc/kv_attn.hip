@@ -22,7 +22,10 @@ namespace h3 {
 // their merge 4, 7 and 11 us more. Longer parts: one sequence of 2000 tokens in parts of 8, 16 and 32 blocks 12.6, 15.5 and 18.5 us.)
 // What decides the plans beside the batch: the heads of a group, about the longest length, the window, and (kv_attention_spans) the first tokens
 // that stay visible, the groups of sequences and about the longest of their shared tokens.
-struct KvSight { int64_t group, max_len, window, sinks, groups, shared; };
+struct KvSight {
+    int64_t group, max_len, window, sinks, groups, shared;
+    bool spans() const { return sinks > 0 || groups > 0; }
+};
 
 static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus) {
     const int64_t group = sight.group, max_len = sight.max_len, window = sight.window;
@@ -42,6 +45,9 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& si
     const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
     plan.per = (int) std::max(least, (blocks + want - 1) / want);
+    // (with first or shared tokens: up to 12 blocks are one part, a third step of the wavefronts for the 4 us of a merge: four sequences of 612
+    // tokens, 64 heads over 8 of 128, 15 to 11 us)
+    if (sight.spans() && !plan.rows && blocks <= 12) plan.per = 12;
     plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
     return plan;
 }
@@ -54,6 +60,8 @@ static int kv_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sigh
     plan[0] = kv_plan(P, two, most, sight, cus);
     const int64_t few = (group <= 16 ? 16 : 32) / group;                         // tokens
     if (!plan[0].rows || few == 0 || (group > 16 && P.dim > 128) || std::min<int64_t>(most, P.rows) * P.seqs <= P.rows) return 1;
+    // (with first or shared tokens: where the sequences beside the longest have more rows on average, the rows' kernel takes those with few too)
+    if (sight.spans() && P.rows - std::min<int64_t>(most, P.rows) > 2 * few * (P.seqs - 1)) return 1;
     plan[1] = kv_plan(P, two, few, sight, cus);
     if (plan[1].nsplit <= plan[0].nsplit) return 1;
     plan[1].greatest = (uint32_t) (few * group);
@@ -72,9 +80,20 @@ static KvPlan kv_shared_plan(const KvArgs& P, bool two, const KvSight& sight, in
     plan.tiles = 0;
     plan.places = places(plan.rt);
     plan.blocks = plan.places * P.heads;
-    const int64_t blocks = std::max<int64_t>((sight.shared + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
-    plan.per = (int) std::max(least, (blocks + want - 1) / want);
+    const int64_t blocks = std::max<int64_t>((sight.shared + kKvB - 1) / kKvB, 1), slots = 2 * (int64_t) cus;
+    if (plan.rows) {
+        // As many parts as make the rounds of blocks of threads over the device shortest: a round takes a part's cache blocks, and about three more
+        // for its beginning and the sums that it leaves. (Of the places only those with rows count: about rows / rt, and one at least a group.)
+        const int64_t real = std::max((rows + plan.rt - 1) / plan.rt, sight.groups) * P.heads;
+        int64_t best = INT64_MAX;
+        for (int64_t n = 1; n <= std::min<int64_t>(blocks, 64); ++n) {
+            const int64_t per = (blocks + n - 1) / n, cost = (real * n + slots - 1) / slots * (per + 3);
+            if (cost < best) { best = cost; plan.per = (int) per; }
+        }
+    } else {
+        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(plan.blocks, 1), 512));
+        plan.per = (int) std::max<int64_t>(8, (blocks + want - 1) / want);
+    }
     plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
     return plan;
 }
@@ -105,16 +124,18 @@ static int sight_of(const std::string& fn, const KvArgs& P, const h3_kv_shared* 
     return 0;
 }
 // Whether shared tokens are a launch of their own. A launch and the reading of its sums cost 8 us or more; below so many bytes of all sequences'
-// caches a CU it takes less to go through the shared ones again for each (they come from the caches of the device).
+// caches a CU it takes less to go through the shared ones again for each (they come from the caches of the device). So it does where sequences
+// have many rows each, which are bound by their products either way (eight sequences of up to 256 tokens over 4096 shared ones, 64 heads over 8 of
+// 128: 363 us apart, 359 not).
 constexpr int64_t kKvApart = 192 << 10;
-static bool kv_apart(const KvArgs& P, const KvSight& sight, int cus) {
+static bool kv_apart(const KvArgs& P, const KvSight& sight, int64_t most, int cus) {
     const int64_t tokens = sight.max_len > 0 ? std::min<int64_t>(sight.max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
-    return sight.groups > 0 && std::max(tokens, sight.shared) * P.seqs > cus * kKvApart / (2 * P.heads * kv_width(P.dim));
+    return sight.groups > 0 && std::min<int64_t>(most, P.rows) * sight.group <= 96 && std::max(tokens, sight.shared) * P.seqs > cus * kKvApart / (2 * P.heads * kv_width(P.dim));
 }
 // all launches' plans: of the shared tokens first, where they have one
 static int kv_all_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[3]) {
     KvPlan own[2];
-    const int at = kv_apart(P, sight, cus) ? 1 : 0;
+    const int at = kv_apart(P, sight, most, cus) ? 1 : 0;
     KvSight behind = sight;
     if (!at) behind.shared = 0;
     const int n = kv_plans(P, two, most, behind, cus, own);

@@ -495,19 +495,12 @@ __device__ __forceinline__ int64_t kv_shared_row(const KvAttnArgs& P, const KvIt
     const int64_t place = (int) ((uint32_t) it.row * (uint32_t) P.group / rt2) + it.group + (int) (r2 / rt2);
     return (place * P.kv.heads + it.h) * P.nsplit2 * rt2 + r2 % rt2;
 }
-// The row's maximum and sum with the parts over shared tokens, and the factor for its own sums
-__device__ __forceinline__ float kv_shared_top(const KvAttnArgs& P, int64_t row2, float& mx, float& lt) {
-    float m = mx, l = 0.0f;
-    for (int s = 0; s < P.nsplit2; ++s) m = fmaxf(m, P.pml2[(row2 + (int64_t) s * P.rt2) * 2]);
-    const float own = __builtin_amdgcn_exp2f(mx - m);
-    for (int s = 0; s < P.nsplit2; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(P.pml2 + (row2 + (int64_t) s * P.rt2) * 2);
-        l = __builtin_fmaf(ml.y, __builtin_amdgcn_exp2f(ml.x - m), l);
-    }
-    mx = m;
-    lt = __builtin_fmaf(lt, own, l);
-    return own;
+// (m, l) of the part s over shared tokens of a row
+__device__ __forceinline__ float2 kv_shared_ml(const KvAttnArgs& P, int64_t row2, int s) {
+    return s < P.nsplit2 ? *reinterpret_cast<const float2*>(P.pml2 + (row2 + (int64_t) s * P.rt2) * 2) : make_float2(kKvUnset, 0.0f);
 }
+// The weight of a part: 0 where nothing was seen, whose sums say nothing
+__device__ __forceinline__ float kv_weight(const float2& ml, float top) { return ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top); }
 
 // Whether a key block is seen whole by rows that are the tokens posmin .. posmax
 template <int MODE> __device__ __forceinline__ bool kv_whole(const KvAttnArgs& P, int key0, int posmin, int posmax) {
@@ -678,17 +671,44 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
             int64_t row2 = -1;
             if constexpr (MODE == kKvOwn) {
                 row2 = kv_direct<MODE>(P) ? kv_shared_row(P, it, rr) : -1;
+            }
+            float4 more[WC];                                              // the parts over shared tokens: a lane has (m, l) of every 16th
+#pragma unroll
+            for (int t = 0; t < WC; ++t) more[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if constexpr (MODE == kKvOwn)
                 if (row2 >= 0) {
-                    const float own = kv_shared_top(P, row2, top, lt);
+                    float2 ml = kv_shared_ml(P, row2, c);
+                    top = fmaxf(top, wave_max<16>(ml.x));
+                    for (int s = 16; s < P.nsplit2; s += 16) top = fmaxf(top, wave_max<16>(kv_shared_ml(P, row2, s + c).x));
+                    const float own = __builtin_amdgcn_exp2f(mx - top);
+                    lt *= own;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) wt[w] *= own;
+                    for (int s0 = 0; s0 < P.nsplit2; s0 += 16) {
+                        if (s0) ml = kv_shared_ml(P, row2, s0 + c);
+                        const float wl = kv_weight(ml, top);
+                        lt += wave_sum<16>(ml.y * wl);
+#pragma unroll 8
+                        for (int s = s0; s < min(P.nsplit2, s0 + 16); ++s) {
+                            const float w = __shfl(wl, s - s0, 16);
+                            float4 v[WC];
+#pragma unroll
+                            for (int t = 0; t < WC; ++t) v[t] = *reinterpret_cast<const float4*>(P.po2 + (row2 + (int64_t) s * P.rt2) * W + 64 * t + 4 * c);
+#pragma unroll
+                            for (int t = 0; t < WC; ++t) {
+                                more[t].x = w == 0.0f ? more[t].x : __builtin_fmaf(v[t].x, w, more[t].x);
+                                more[t].y = w == 0.0f ? more[t].y : __builtin_fmaf(v[t].y, w, more[t].y);
+                                more[t].z = w == 0.0f ? more[t].z : __builtin_fmaf(v[t].z, w, more[t].z);
+                                more[t].w = w == 0.0f ? more[t].w : __builtin_fmaf(v[t].w, w, more[t].w);
+                            }
+                        }
+                    }
                 }
-            }
             const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
 #pragma unroll
             for (int t = 0; t < WC; ++t) {
                 const int d = 64 * t + 4 * c;
-                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float y[4] = {more[t].x, more[t].y, more[t].z, more[t].w};
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const float4 v = *reinterpret_cast<const float4*>(&so[w][r][d]);
@@ -697,21 +717,6 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
                     y[2] = __builtin_fmaf(v.z, wt[w], y[2]);
                     y[3] = __builtin_fmaf(v.w, wt[w], y[3]);
                 }
-                if constexpr (MODE == kKvOwn)
-                    if (row2 >= 0) {
-#pragma unroll 4
-                        for (int s = 0; s < P.nsplit2; ++s) {
-                            const int64_t from = row2 + (int64_t) s * P.rt2;
-                            const float2 ml = *reinterpret_cast<const float2*>(P.pml2 + from * 2);
-                            const float4 v = *reinterpret_cast<const float4*>(P.po2 + from * W + d);
-                            if (ml.y == 0.0f) continue;                   // (nothing seen: there are no sums)
-                            const float w = __builtin_amdgcn_exp2f(ml.x - top);
-                            y[0] = __builtin_fmaf(v.x, w, y[0]);
-                            y[1] = __builtin_fmaf(v.y, w, y[1]);
-                            y[2] = __builtin_fmaf(v.z, w, y[2]);
-                            y[3] = __builtin_fmaf(v.w, w, y[3]);
-                        }
-                    }
                 if (kv_direct<MODE>(P)) kv_store4(P, at * P.kv.dim, d, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
                 else *reinterpret_cast<float4*>(P.po + row * W + d) = make_float4(y[0], y[1], y[2], y[3]);
             }
@@ -885,17 +890,22 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
         if constexpr (MODE == kKvOwn) {
             const int64_t row2 = kv_direct<MODE>(P) ? kv_shared_row(P, it, rw + 16 * e + l15) : -1;
             if (row2 >= 0) {
-                const float own = kv_shared_top(P, row2, q.m[e], l);
+                float top = q.m[e];
+#pragma unroll 4
+                for (int s = 0; s < P.nsplit2; ++s) top = fmaxf(top, kv_shared_ml(P, row2, s).x);
+                const float own = __builtin_amdgcn_exp2f(q.m[e] - top);
+                q.m[e] = top;
+                l *= own;
 #pragma unroll
                 for (int t = 0; t < DT; ++t) q.o[e][t] *= own;
                 for (int s = 0; s < P.nsplit2; ++s) {
-                    const int64_t from = row2 + (int64_t) s * P.rt2;
-                    const float2 ml = *reinterpret_cast<const float2*>(P.pml2 + from * 2);
-                    if (ml.y == 0.0f) continue;                           // (nothing seen: there are no sums)
-                    const float w = __builtin_amdgcn_exp2f(ml.x - q.m[e]);
+                    const float2 ml = kv_shared_ml(P, row2, s);
+                    const float w = kv_weight(ml, top);
+                    if (w == 0.0f) continue;
+                    l = __builtin_fmaf(ml.y, w, l);
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
-                        const float4 v = *reinterpret_cast<const float4*>(P.po2 + from * W + 16 * t + 4 * g);
+                        const float4 v = *reinterpret_cast<const float4*>(P.po2 + (row2 + (int64_t) s * P.rt2) * W + 16 * t + 4 * g);
                         q.o[e][t][0] = __builtin_fmaf(v.x, w, q.o[e][t][0]);
                         q.o[e][t][1] = __builtin_fmaf(v.y, w, q.o[e][t][1]);
                         q.o[e][t][2] = __builtin_fmaf(v.z, w, q.o[e][t][2]);
@@ -1003,9 +1013,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttnArgs P) {
     for (int t = 0; t < WC; ++t) y[t] = 0.0f;
 #pragma unroll 4
     for (int s = wave; s < parts; s += 4) {
-        const float2 ml = ml_of(s);
-        if (ml.y == 0.0f) continue;                                       // (nothing seen: there are no sums)
-        const float w = __builtin_amdgcn_exp2f(ml.x - mx);
+        const float w = kv_weight(ml_of(s), mx);
+        if (w == 0.0f) continue;
         const float* o = s < own ? P.po + (row0 + (int64_t) s * RT) * W : P.po2 + (row2 + (int64_t) (s - own) * P.rt2) * W;
 #pragma unroll
         for (int t = 0; t < WC; ++t) y[t] = __builtin_fmaf(o[64 * t + lane], w, y[t]);

@@ -244,10 +244,10 @@ def test_workspace_and_graph(dev16, sinks):
     for seed in (31, 32):
         case = Case(dev, [(1, 900), (1, 1200), (2, 800), (1, 1000)], 2, 4, 128, "BF16", [(0, 3, 700)] if not sinks else (), seed=seed)
         args, shared, _ = case.upload()
-        n = ops.kv_attention_work(*args[:4], case.most, window=500 if sinks else 0, sinks=sinks, shared=shared)
+        n = ops.kv_attention_work(*args[:4], case.most, window=900 if sinks else 0, sinks=sinks, shared=shared)
         assert n > 0
         out, work = new(dev, "F32", [case.rows, 1024]), new(dev, "U8", [n])
-        kw = dict(window=500 if sinks else 0, sinks=sinks, shared=shared)
+        kw = dict(window=900 if sinks else 0, sinks=sinks, shared=shared)
         graph = Recorded(dev, lambda: ops.kv_attention(*args, out, work=work, **kw))
         with pytest.raises(Error, match="smaller"):
             ops.kv_attention(*args, out, work=new(dev, "U8", [n - 16]), **kw)
@@ -293,7 +293,7 @@ def test_which_kernels_run(dev, dev2):
     sequences' own launch takes up."""
     for d, want in ((dev, ["kv_attn_kernel<2, 1, false, 1>", "kv_merge_kernel<2, 16, 1>"]),
                     (dev2, ["kv_attn_rows_kernel<2, 1, false, 2>", "kv_attn_kernel<2, 1, false, 1>"])):
-        case = Case(d, [(1, 700)] * 8, 2, 8, 128, "BF16", [(0, 8, 256)])
+        case = Case(d, [(1, 1000)] * 8, 2, 8, 128, "BF16", [(0, 8, 256)])
         args, shared, _ = case.upload()
         out = new(d, "F32", [case.rows, 2 * 8 * 128])
         work = new(d, "U8", [ops.kv_attention_work(*args[:4], 1, shared=shared)])

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * NW) void lin_scan_kernel(LinArgs P) {
     const int slice = (int) (id % (uint32_t) P.slices), b = (int) (id / (uint32_t) P.slices);
     int r0, n;
     kv_rows_of(P.kv, b, r0, n);
-    const int segs = (n + P.seg - 1) / P.seg;
+    const int segs = (int) (((uint32_t) n + (uint32_t) P.seg - 1) / (uint32_t) P.seg);
     if (segs < 2 || (uint32_t) n < P.least || (uint32_t) n > P.most) return;
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
     const int c = slice * 16 * NW * NV + (wave * NV + x) * 16 + l15;
@@ -205,12 +205,22 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
     return p;
 }
 
+// Whether a launch could take 2^32 threads or more (blocks of up to 512), however the device's size splits the call
+static bool lin_too_many(const h3_lin_state& state, const h3_lin_batch& batch) {
+    const LinPlan p = lin_plan(state, batch, 1);
+    const int64_t steps = (state.dv + kLinCols - 1) / kLinCols, most = kKvMostBlocks / state.heads;
+    return (p.step && batch.seqs > most / steps) ||
+           (p.chunk && (batch.rows / kLinLeast + batch.seqs > most / 2 / p.slices || batch.seqs > most / 2 / (p.slices * 4 * p.kc)));
+}
+
 int64_t lin_attention_work(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, int dt) try {
     const char* fn = "lin_attention_work";
     if (lin_checks(fn, state, batch, dt)) return -1;
+    const bool none = batch->seqs == 0 || batch->rows == 0 || batch->most == 0;
+    if (!none && lin_too_many(*state, *batch)) return fail(std::string(fn) + ": too many blocks of work");
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
-    if (batch->seqs == 0 || batch->rows == 0 || batch->most == 0) return 0;
+    if (none) return 0;
     return 4 * lin_plan(*state, *batch, c->cus).floats;
 } catch (const std::exception& e) { return fail(e.what()); }
 
@@ -248,12 +258,11 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
     P.least = 0; P.most = UINT32_MAX;
     P.s_vec = aligned16(P.s) && dv % 4 == 0;
     P.vec = vec(q, q_stride, dk) && vec(k, k_stride, dk) && vec(v, v_stride, dv) && aligned16(out) && heads * dv < (1 << 22);
+    if (lin_too_many(*state, *batch)) return fail(fn + ": too many blocks of work");
     Ctx* c = ctx_of(ctx, fn.c_str());
     if (!c) return -1;
     const LinPlan plan = lin_plan(*state, *batch, c->cus);
-    const int64_t steps = batch->seqs * heads * ((dv + kLinCols - 1) / kLinCols), scans = batch->seqs * heads * plan.slices * 4 * plan.kc;
-    if ((plan.step && steps > kKvMostBlocks) || (plan.chunk && (plan.blocks > kKvMostBlocks / 2 || (plan.split && scans > kKvMostBlocks / 2))))
-        return fail(fn + ": too many blocks of work");
+    const int64_t steps = batch->seqs * heads * ((dv + kLinCols - 1) / kLinCols);
     if (plan.floats) {
         if (work) {
             if (work_bytes < (uint64_t) (4 * plan.floats)) return fail(fn + ": the workspace is smaller than lin_attention_work() says");

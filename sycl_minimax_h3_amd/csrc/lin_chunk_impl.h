@@ -71,7 +71,7 @@ struct LinItem {
         place = (int) (id / (uint32_t) P.slices);
         if (P.ws) {
             seg = kv_find(P.kv, place, 1, (uint32_t) P.seg, 1, b, r0, n);
-            segs = (n + P.seg - 1) / P.seg;
+            segs = (int) (((uint32_t) n + (uint32_t) P.seg - 1) / (uint32_t) P.seg);
         } else {                                                            // a segment is a sequence
             b = place;
             kv_rows_of(P.kv, b, r0, n);

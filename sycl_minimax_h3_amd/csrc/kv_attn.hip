@@ -27,6 +27,30 @@ struct KvSight {
     bool spans() const { return sinks > 0 || groups > 0; }
 };
 
+// The rows' kernel of kv_attention_spans: its tiles and parts by an estimate of the time, in microseconds. Where the device is full, a cache block
+// takes a tile of 128 rows 3.2 and one of 64 rows 2.2 (heads of 128, 16-bit queries; more features and float32 queries in proportion), a
+// part's beginning and end about two more; a last round of at most a block of threads a CU goes faster by 0.7; parts are written and read at
+// 5 TB/s, and joined by a launch (or taken up by the sequences' own: 0.6 each). (About 80 rows of each of 18 sequences over 7000 tokens, 8 heads of 96: 188 us in tiles and parts as
+// kv_attention's, 98 so.) tiles(rt): tiles of a head; join: 0 where the parts are taken up by another launch.
+template <typename F> static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int64_t dim, int64_t blocks, bool two, int cus, double join) {
+    const int wc = (int) (kv_width(dim) / 64);
+    const int64_t a_cu = wc == 1 ? 3 : wc == 2 ? 2 : 1, slots = a_cu * cus;
+    double best = 1e300;
+    for (int nq = 1; nq <= (two ? 1 : 2); ++nq) {
+        const int64_t real = tiles(64 * nq) * heads;
+        const double step = (nq == 2 ? 3.2 : 2.2) * (two ? 1.6 : 1.0) * (wc + 0.3) / 2.3 * (double) a_cu / 2;
+        for (int64_t n = 1; n <= std::min<int64_t>(blocks, 64); ++n) {
+            const int64_t per = (blocks + n - 1) / n, rest = real * n % slots;
+            const double rounds = (double) (real * n / slots) + (rest == 0 ? 0.0 : rest <= cus && a_cu > 1 ? 0.7 : 1.0);
+            const double parts = n > 1 || join == 0.0 ? (double) n * rows * heads * dim * 8.0 / 5e6 : 0.0;
+            const double cost = rounds * (per + 2) * step + parts + (join == 0.0 ? 0.6 * n : n > 1 ? join : 0.0);
+            if (cost < best) { best = cost; plan.nq = nq; plan.per = (int) per; }
+        }
+    }
+    plan.rt = 64 * plan.nq;
+    plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
+}
+
 static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus) {
     const int64_t group = sight.group, max_len = sight.max_len, window = sight.window;
     KvPlan plan;
@@ -34,14 +58,25 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& si
     auto even = [&](int64_t rt) { return (rows + rt - 1) / rt * P.seqs; };
     auto ragged = [&](int64_t rt) { return P.rows * group / rt + P.seqs; };
     plan.rows = rows > (P.dim <= 128 ? 32 : 16);
+    int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
+    if (sight.groups) keys = std::max<int64_t>(keys - sight.shared, std::min<int64_t>(most, P.rows));
+    if (window > 0) keys = std::min(keys, std::min<int64_t>(window, INT32_MAX) + std::min<int64_t>(most, P.rows) + 2 * kKvB + std::min<int64_t>(sight.sinks, INT32_MAX));
+    if (plan.rows && sight.spans()) {
+        // (sequences have as many rows on average; a tile sees its window)
+        const int64_t each = (P.rows * group + P.seqs - 1) / P.seqs;
+        if (window > 0) keys = std::min<int64_t>(keys, std::min<int64_t>(window + sight.sinks, INT32_MAX) + 128 / group + 2 * kKvB);
+        kv_rows_plan(plan, [&](int64_t rt) { return (each + rt - 1) / rt * P.seqs; }, P.rows * group, P.heads, P.dim,
+                     std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), two, cus, 6.0);
+        plan.tiles = even(plan.rt) <= ragged(plan.rt) ? (rows + plan.rt - 1) / plan.rt : 0;
+        plan.places = std::min(even(plan.rt), ragged(plan.rt));
+        plan.blocks = plan.places * P.heads;
+        return plan;
+    }
     plan.nq = plan.rows ? (two || rows <= 96 || std::min(even(128), ragged(128)) * P.heads < cus ? 1 : 2) : rows <= 16 ? 1 : 2;
     plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
     plan.tiles = even(plan.rt) <= ragged(plan.rt) ? (rows + plan.rt - 1) / plan.rt : 0;
     plan.places = std::min(even(plan.rt), ragged(plan.rt));
     plan.blocks = plan.places * P.heads;
-    int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
-    if (sight.groups) keys = std::max<int64_t>(keys - sight.shared, std::min<int64_t>(most, P.rows));
-    if (window > 0) keys = std::min(keys, std::min<int64_t>(window, INT32_MAX) + std::min<int64_t>(most, P.rows) + 2 * kKvB + std::min<int64_t>(sight.sinks, INT32_MAX));
     const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
     plan.per = (int) std::max(least, (blocks + want - 1) / want);
@@ -75,26 +110,22 @@ static KvPlan kv_shared_plan(const KvArgs& P, bool two, const KvSight& sight, in
     const int64_t rows = P.rows * sight.group, each = (rows + sight.groups - 1) / sight.groups;
     auto places = [&](int64_t rt) { return rows / rt + sight.groups; };
     plan.rows = each > (P.dim <= 128 ? 32 : 16);
-    plan.nq = plan.rows ? (two || each <= 96 ? 1 : 2) : each <= 16 ? 1 : 2;
-    plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
-    plan.tiles = 0;
-    plan.places = places(plan.rt);
-    plan.blocks = plan.places * P.heads;
-    const int64_t blocks = std::max<int64_t>((sight.shared + kKvB - 1) / kKvB, 1), slots = 2 * (int64_t) cus;
+    const int64_t blocks = std::max<int64_t>((sight.shared + kKvB - 1) / kKvB, 1);
     if (plan.rows) {
-        // As many parts as make the rounds of blocks of threads over the device shortest: a round takes a part's cache blocks, and about three more
-        // for its beginning and the sums that it leaves. (Of the places only those with rows count: about rows / rt, and one at least a group.)
-        const int64_t real = std::max((rows + plan.rt - 1) / plan.rt, sight.groups) * P.heads;
-        int64_t best = INT64_MAX;
-        for (int64_t n = 1; n <= std::min<int64_t>(blocks, 64); ++n) {
-            const int64_t per = (blocks + n - 1) / n, cost = (real * n + slots - 1) / slots * (per + 3);
-            if (cost < best) { best = cost; plan.per = (int) per; }
-        }
+        kv_rows_plan(plan, [&](int64_t rt) { return std::max((rows + rt - 1) / rt, sight.groups); }, rows, P.heads, P.dim, blocks, two, cus, 0.0);
+        plan.tiles = 0;
+        plan.places = places(plan.rt);
+        plan.blocks = plan.places * P.heads;
     } else {
-        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(plan.blocks, 1), 512));
+        plan.nq = each <= 16 ? 1 : 2;
+        plan.rt = 16 * plan.nq;
+        plan.tiles = 0;
+        plan.places = places(plan.rt);
+        plan.blocks = plan.places * P.heads;
+        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
         plan.per = (int) std::max<int64_t>(8, (blocks + want - 1) / want);
+        plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
     }
-    plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
     return plan;
 }
 static int64_t kv_part_floats(const KvPlan& plan, int64_t W) {
@@ -125,12 +156,15 @@ static int sight_of(const std::string& fn, const KvArgs& P, const h3_kv_shared* 
 }
 // Whether shared tokens are a launch of their own. A launch and the reading of its sums cost 8 us or more; below so many bytes of all sequences'
 // caches a CU it takes less to go through the shared ones again for each (they come from the caches of the device). So it does where sequences
-// have many rows each, which are bound by their products either way (eight sequences of up to 256 tokens over 4096 shared ones, 64 heads over 8 of
-// 128: 363 us apart, 359 not).
+// have many rows each, which are bound by their products either way, unless their tiles would be much emptier than the groups' (eight sequences of
+// up to 256 tokens over 4096 shared ones, 64 heads over 8 of 128: 363 us apart, 359 not).
 constexpr int64_t kKvApart = 192 << 10;
 static bool kv_apart(const KvArgs& P, const KvSight& sight, int64_t most, int cus) {
+    if (sight.groups == 0) return false;
     const int64_t tokens = sight.max_len > 0 ? std::min<int64_t>(sight.max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
-    return sight.groups > 0 && std::min<int64_t>(most, P.rows) * sight.group <= 96 && std::max(tokens, sight.shared) * P.seqs > cus * kKvApart / (2 * P.heads * kv_width(P.dim));
+    if (std::max(tokens, sight.shared) * P.seqs <= cus * kKvApart / (2 * P.heads * kv_width(P.dim))) return false;
+    const int64_t rows = P.rows * sight.group, each = (rows + P.seqs - 1) / P.seqs;
+    return std::min<int64_t>(most, P.rows) * sight.group <= 96 || 4 * ((each + 63) / 64 * 64 * P.seqs) > 5 * (rows + 32 * sight.groups);
 }
 // all launches' plans: of the shared tokens first, where they have one
 static int kv_all_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[3]) {

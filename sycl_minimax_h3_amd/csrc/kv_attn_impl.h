@@ -932,13 +932,13 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
 }
 
 // joins the parts of one row: one block of 256 threads a row, its wavefronts taking every fourth part, in that order
-template <int WC, int RT, int MODE = kKvAll>
+template <int WC, int RT>
 __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t item = blockIdx.x / RT;
     const int r = (int) (blockIdx.x % RT);
-    KvItem<MODE> it;
+    KvItem<kKvAll> it;
     it.h = (int) (item % P.kv.heads);
     it.template rows<RT>(P, (int) (item / P.kv.heads));
     const uint32_t rr = (uint32_t) it.tile * RT + r, group = P.group;
@@ -977,57 +977,59 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(KvAttnArgs P) {
     if (P.lse && threadIdx.x == 0) P.lse[at] = kv_lse(mx, lt);
 }
 
-// Joins the parts of one row over its sequence's own blocks and, where its sequence shares tokens, over those: one block of 256 threads a row.
+// Joins the parts of a row over its sequence's own blocks and, where its sequence shares tokens, over those. A block of 256 threads takes 16
+// rows, 16 lanes each: a lane has four features of every 64 and (m, l) of every 16th part. (A block a row: 20 to 27 us for 12288 rows of two
+// or three parts, most of it the blocks' beginnings; so 7.)
 template <int WC, int RT>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t item = blockIdx.x / RT;
-    const int r = (int) (blockIdx.x % RT);
+    const int c = threadIdx.x & 15, r = (int) (blockIdx.x % (RT / 16)) * 16 + (int) (threadIdx.x >> 4);
+    const int64_t item = blockIdx.x / (RT / 16);
     KvItem<kKvOwn> it;
     it.h = (int) (item % P.kv.heads);
     it.template rows<RT>(P, (int) (item / P.kv.heads));
     const uint32_t rr = (uint32_t) it.tile * RT + r, group = P.group;
-    if (rr >= it.R) return;
+    if (rr >= it.R) return;                         // (16 lanes go together)
     int kb0, count;
     it.range(P, (uint32_t) it.tile * RT, RT, kb0, count);
     const int own = min(max((count + P.per - 1) / P.per, 1), P.nsplit);
-    const int64_t row0 = item * P.nsplit * RT + r;
-    const int64_t row2 = kv_shared_row(P, it, rr);
+    const int64_t row0 = item * P.nsplit * RT + r, row2 = kv_shared_row(P, it, rr);
     const int parts = own + (row2 >= 0 ? P.nsplit2 : 0);
     auto ml_of = [&](int s) {
-        return s < own ? *reinterpret_cast<const float2*>(P.pml + (row0 + (int64_t) s * RT) * 2)
-                       : *reinterpret_cast<const float2*>(P.pml2 + (row2 + (int64_t) (s - own) * P.rt2) * 2);
+        if (s >= parts) return make_float2(kKvUnset, 0.0f);
+        return s < own ? *reinterpret_cast<const float2*>(P.pml + (row0 + (int64_t) s * RT) * 2) : kv_shared_ml(P, row2, s - own);
     };
-    float mx = kKvUnset;
-    for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, ml_of(s).x);
-    mx = wave_max<64>(mx);
-    float lt = 0.0f;
-    for (int s = lane; s < parts; s += 64) {
-        const float2 ml = ml_of(s);
-        lt += ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
-    }
-    lt = wave_sum<64>(lt);
-    float y[WC];
+    float2 ml = ml_of(c);
+    float top = wave_max<16>(ml.x), lt = 0.0f;
+    for (int s = 16; s < parts; s += 16) top = fmaxf(top, wave_max<16>(ml_of(s + c).x));
+    float4 y[WC];
 #pragma unroll
-    for (int t = 0; t < WC; ++t) y[t] = 0.0f;
+    for (int t = 0; t < WC; ++t) y[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < parts; s0 += 16) {
+        if (s0) ml = ml_of(s0 + c);
+        const float wl = kv_weight(ml, top);
+        lt += wave_sum<16>(ml.y * wl);
 #pragma unroll 4
-    for (int s = wave; s < parts; s += 4) {
-        const float w = kv_weight(ml_of(s), mx);
-        if (w == 0.0f) continue;
-        const float* o = s < own ? P.po + (row0 + (int64_t) s * RT) * W : P.po2 + (row2 + (int64_t) (s - own) * P.rt2) * W;
+        for (int s = s0; s < min(parts, s0 + 16); ++s) {
+            const float w = __shfl(wl, s - s0, 16);
+            const float* o = s < own ? P.po + (row0 + (int64_t) s * RT) * W : P.po2 + (row2 + (int64_t) (s - own) * P.rt2) * W;
+            float4 v[WC];
 #pragma unroll
-        for (int t = 0; t < WC; ++t) y[t] = __builtin_fmaf(o[64 * t + lane], w, y[t]);
+            for (int t = 0; t < WC; ++t) v[t] = *reinterpret_cast<const float4*>(o + 64 * t + 4 * c);
+#pragma unroll
+            for (int t = 0; t < WC; ++t) {          // (no weight: nothing seen, and there are no sums)
+                y[t].x = w == 0.0f ? y[t].x : __builtin_fmaf(v[t].x, w, y[t].x);
+                y[t].y = w == 0.0f ? y[t].y : __builtin_fmaf(v[t].y, w, y[t].y);
+                y[t].z = w == 0.0f ? y[t].z : __builtin_fmaf(v[t].z, w, y[t].z);
+                y[t].w = w == 0.0f ? y[t].w : __builtin_fmaf(v[t].w, w, y[t].w);
+            }
+        }
     }
-    __shared__ float sy[4][W];
-#pragma unroll
-    for (int t = 0; t < WC; ++t) sy[wave][64 * t + lane] = y[t];
-    __syncthreads();
     const int64_t at = ((int64_t) it.r0 + rr / group) * P.q_heads + it.h * group + rr % group;
     const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-    for (int d = threadIdx.x; d < P.kv.dim; d += 256)
-        store_any(P.out, P.out_dt, at * P.kv.dim + d, ((sy[0][d] + sy[1][d]) + (sy[2][d] + sy[3][d])) * inv);
-    if (P.lse && threadIdx.x == 0) P.lse[at] = kv_lse(mx, lt);
+#pragma unroll
+    for (int t = 0; t < WC; ++t) kv_store4(P, at * P.kv.dim, 64 * t + 4 * c, y[t].x * inv, y[t].y * inv, y[t].z * inv, y[t].w * inv);
+    if (P.lse && c == 0) P.lse[at] = kv_lse(top, lt);
 }
 
 // which kernel takes the call, and in how many parts
@@ -1052,13 +1054,10 @@ static void kv_attn_run(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool tw
         if (two) kv_attn_kernel<WC, NQ, true, MODE><<<grid, 256, 0, c->stream>>>(P);
         else kv_attn_kernel<WC, NQ, false, MODE><<<grid, 256, 0, c->stream>>>(P);
     }
-    if constexpr (MODE == kKvOwn)
-        if (P.nsplit2) {
-            if (plan.nsplit > 1) kv_join_kernel<WC, RT><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
-            return;
-        }
-    if constexpr (MODE != kKvShared)
-        if (plan.nsplit > 1) kv_merge_kernel<WC, RT, MODE><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
+    if (plan.nsplit > 1) {
+        if constexpr (MODE == kKvOwn) kv_join_kernel<WC, RT><<<(unsigned) (plan.blocks * (RT / 16)), 256, 0, c->stream>>>(P);
+        if constexpr (MODE == kKvAll) kv_merge_kernel<WC, RT><<<(unsigned) (plan.blocks * RT), 256, 0, c->stream>>>(P);
+    }
 }
 
 // heads of up to 64 WC features (kv_attn_64.hip .. kv_attn_256.hip), the same of kv_attention_spans (kv_spans_64.hip .. kv_spans_256.hip)

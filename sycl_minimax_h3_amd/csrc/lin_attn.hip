@@ -142,11 +142,19 @@ __global__ __launch_bounds__(64 * NW) void lin_scan_kernel(LinArgs P) {
     const float less = expm1f(-P.decay[h] * (float) P.seg);
     const int64_t place = r0 / P.seg + b, step = (int64_t) P.slices * P.heads * (FR * T * 4);
     float* ws = P.ws + ((place * P.slices + slice) * P.heads + h) * (FR * T * 4) + fr * (T * 4) + threadIdx.x * 4;
-    for (int j = 0; j < segs; ++j, ws += step) {
-        const v4f_lin own = j + 1 < segs ? *reinterpret_cast<const v4f_lin*>(ws) : v4f_lin{0.0f, 0.0f, 0.0f, 0.0f};
-        *reinterpret_cast<v4f_lin*>(ws) = s;
+    // (eight segments' sums are on their way at once: one after another their latency is all there is)
+    constexpr int A = 8;
+    v4f_lin own[A];
+    for (int j0 = 0; j0 < segs; j0 += A, ws += A * step) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(s[i], less, s[i]) + own[i];
+        for (int j = 0; j < A; ++j) own[j] = j0 + j + 1 < segs ? *reinterpret_cast<const v4f_lin*>(ws + j * step) : v4f_lin{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < A; ++j) {
+            if (j0 + j >= segs) break;
+            *reinterpret_cast<v4f_lin*>(ws + j * step) = s;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(s[i], less, s[i]) + own[j][i];
+        }
     }
 }
 
@@ -179,24 +187,42 @@ static int lin_checks(const std::string& fn, const h3_lin_state* state, const h3
 
 // Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces. Where the sequences beside the longest
 // have more than 2 kLinFew tokens on average, all go in pieces: a launch that finds nothing to do takes 3 to 5 us.
-// Segments: as many as give each CU two blocks of threads, of at least kLinLeast tokens.
-constexpr int kLinFew = 16, kLinLeast = 128;
+constexpr int kLinFew = 16;
+constexpr int64_t kLinLeast = 32, kLinSegs = 256;   // the least tokens of a segment, the most segments of an average sequence
 struct LinPlan {
     bool step, chunk, split;
     int kc, slices;
     bool wide;
     int64_t seg, places, blocks, floats;
 };
-static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, int cus) {
+static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, int dt, int cus) {
     LinPlan p{};
-    const int64_t most = std::min(batch.most, batch.rows), chains = batch.seqs * state.heads;
+    const int64_t most = std::min(batch.most, batch.rows);
     p.chunk = most > kLinFew;
     p.step = !p.chunk || (batch.seqs > 1 && batch.rows - most <= 2 * kLinFew * (batch.seqs - 1) && most * batch.seqs > batch.rows);
-    p.kc = state.dk > 64 && state.dk <= 96 ? 3 : (int) (state.dk + 63) / 64 * 2;
+    p.kc = state.dk <= 32 ? 1 : state.dk > 64 && state.dk <= 96 ? 3 : (int) (state.dk + 63) / 64 * 2;
     p.wide = state.dv > 64;
     p.slices = p.wide ? (int) (state.dv + 127) / 128 : 1;
-    const int64_t want = std::max<int64_t>(1, 2 * (int64_t) cus / (chains * p.slices));
-    p.seg = std::max<int64_t>(kLinLeast, ((most + want - 1) / want + 63) / 64 * 64);
+    // Segments by an estimate of the time in microseconds, of the average sequence (with a launch for few tokens: of as many of the longest's length
+    // as there are rows for): a piece takes 6 (64 tokens; 32 of the shapes that have such pieces
+    // 4.5) where a CU has one block of threads and 0.8 of that for each where it has more; a split one's own sums half as much again, and
+    // launches, the states (written and read twice) at 4.5 TB/s and 0.3 a segment of the walk over them. (8192 tokens, 64 heads of 128: 1, 4, 8 and
+    // 12 segments a head 770, 270, 220 and 240 us; four float32 prompts of up to 1500 tokens, 16 heads of 80 x 96, in segments of 256 and
+    // 192 94 and 79.)
+    const int64_t piece = dt == H3S_BF16 && p.kc <= 4 ? 64 : 32, seqs = p.step ? std::max<int64_t>(batch.rows / most, 1) : batch.seqs;
+    const int64_t length = std::max<int64_t>(std::min(most, batch.rows / seqs), 1), chains = seqs * state.heads;
+    const int64_t pieces = (length + piece - 1) / piece;
+    double best = 1e300;
+    p.seg = most;
+    for (int64_t n = 1; n <= std::min(pieces, kLinSegs); ++n) {
+        const int64_t per = (pieces + n - 1) / n, segs = (pieces + per - 1) / per, load = (chains * p.slices * segs + cus - 1) / cus;
+        const double states = (double) chains * segs * state.dk * state.dv * 16.0 / 4.5e6;
+        const double cost = per * (piece == 64 ? 6.0 : 4.5) * (load > 1 ? 0.8 * load : 1.0) * (segs > 1 ? 1.5 : 1.0) + (segs > 1 ? 11.0 + 0.3 * segs + states : 0.0);
+        if (cost < best) {
+            best = cost;
+            p.seg = segs > 1 ? std::max(per * piece, kLinLeast) : most;
+        }
+    }
     p.split = p.seg < most;
     if (!p.split) p.seg = most;
     p.places = p.split ? batch.rows / p.seg + batch.seqs : batch.seqs;
@@ -207,10 +233,11 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
 
 // Whether a launch could take 2^32 threads or more (blocks of up to 512), however the device's size splits the call
 static bool lin_too_many(const h3_lin_state& state, const h3_lin_batch& batch) {
-    const LinPlan p = lin_plan(state, batch, 1);
+    const LinPlan p = lin_plan(state, batch, H3S_BF16, 1);
     const int64_t steps = (state.dv + kLinCols - 1) / kLinCols, most = kKvMostBlocks / state.heads;
+    const int64_t seg = std::max(kLinLeast, std::min({batch.most, batch.rows, batch.rows / batch.seqs}) / kLinSegs);   // the shortest
     return (p.step && batch.seqs > most / steps) ||
-           (p.chunk && (batch.rows / kLinLeast + batch.seqs > most / 2 / p.slices || batch.seqs > most / 2 / (p.slices * 4 * p.kc)));
+           (p.chunk && (batch.rows / seg + batch.seqs > most / 2 / p.slices || batch.seqs > most / 2 / (p.slices * 4 * p.kc)));
 }
 
 int64_t lin_attention_work(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, int dt) try {
@@ -221,7 +248,7 @@ int64_t lin_attention_work(void* ctx, const h3_lin_state* state, const h3_lin_ba
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
     if (none) return 0;
-    return 4 * lin_plan(*state, *batch, c->cus).floats;
+    return 4 * lin_plan(*state, *batch, dt, c->cus).floats;
 } catch (const std::exception& e) { return fail(e.what()); }
 
 int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, const float* decay, const void* q, int64_t q_stride,
@@ -261,7 +288,7 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
     if (lin_too_many(*state, *batch)) return fail(fn + ": too many blocks of work");
     Ctx* c = ctx_of(ctx, fn.c_str());
     if (!c) return -1;
-    const LinPlan plan = lin_plan(*state, *batch, c->cus);
+    const LinPlan plan = lin_plan(*state, *batch, dt, c->cus);
     const int64_t steps = batch->seqs * heads * ((dv + kLinCols - 1) / kLinCols);
     if (plan.floats) {
         if (work) {
@@ -278,6 +305,7 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
     if (plan.step) {
         P.most = plan.chunk ? kLinFew : UINT32_MAX;
         switch (plan.kc) {
+            case 1:
             case 2: lin_step<2>(c, P, steps); break;
             case 3:
             case 4: lin_step<4>(c, P, steps); break;
@@ -298,6 +326,7 @@ int lin_attention(void* ctx, const h3_lin_state* state, const h3_lin_batch* batc
         if (plan.split) {
             run(false);
             switch (plan.kc) {
+                case 1: lin_scan<1>(c, P, plan.wide); break;
                 case 2: lin_scan<2>(c, P, plan.wide); break;
                 case 3: lin_scan<3>(c, P, plan.wide); break;
                 case 4: lin_scan<4>(c, P, plan.wide); break;

@@ -668,6 +668,7 @@ template <int DT, int KC, bool WIDE> static void lin_chunk_run(Ctx* c, const Lin
 }
 template <int DT, bool WIDE> static void lin_chunk_width(Ctx* c, const LinArgs& P, int kc, int64_t blocks, bool out) {
     switch (kc) {
+        case 1: lin_chunk_run<DT, 1, WIDE>(c, P, blocks, out); break;
         case 2: lin_chunk_run<DT, 2, WIDE>(c, P, blocks, out); break;
         case 3: lin_chunk_run<DT, 3, WIDE>(c, P, blocks, out); break;
         case 4: lin_chunk_run<DT, 4, WIDE>(c, P, blocks, out); break;

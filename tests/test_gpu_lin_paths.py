@@ -93,11 +93,11 @@ def test_workspace_and_graph(dev):
     """With a workspace of its own a call can be recorded and replayed: the state goes on from replay to replay as in eager calls, bit for bit.
     A smaller workspace is refused, and so is none while a graph is recorded. Two graphs take turns."""
     made = []
-    for seed, counts in ((61, [300, 40]), (62, [1, 2])):
+    for seed, counts in ((61, [900, 40]), (62, [1, 2])):
         case = Case(dev, counts, 2, (1, 1, 1), 64, 64, "BF16", seed)
         eager, held = case.operands(), case.operands()
         n = ops.lin_attention_work(held[0], *held[2:3], *held[5:])
-        assert (n > 0) == (counts[0] == 300)
+        assert (n > 0) == (counts[0] == 900)
         out, want = new(dev, "F32", [case.rows, 128]), new(dev, "F32", [case.rows, 128])
         work = new(dev, "U8", [n]) if n else None
         graph = Recorded(dev, lambda: ops.lin_attention(*held, out, work=work))
@@ -122,7 +122,7 @@ def test_workspace_and_graph(dev):
 def test_two_contexts(dev):
     """Two contexts on streams of their own, called in turn without a wait between: each its own scratch."""
     other = Device.open()
-    case = [Case(d, [400, 70], 2, (1, 1, 1), 64, 64, "BF16", 63 + i) for i, d in enumerate((dev, other))]
+    case = [Case(d, [1000, 70], 2, (1, 1, 1), 64, 64, "BF16", 63 + i) for i, d in enumerate((dev, other))]
     held = [(c.operands(), new(c.dev, "F32", [c.rows, 128])) for c in case]
     for args, out in held:
         args[6]._owner.write(np.array([-1, -1], np.int32))                           # (every call begins anew)

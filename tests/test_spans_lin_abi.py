@@ -112,7 +112,8 @@ def test_lin_arguments(lm):
 @pytest.mark.parametrize("heads,b,fits", [
     (64, dict(seqs=1 << 16, rows=1 << 16, most=1), True),
     (64, dict(seqs=1 << 17, rows=1 << 17, most=1), False),                      # 3 blocks of 256 threads a head: past 2^24
-    (1, dict(seqs=1, rows=(1 << 31) - 1, most=1 << 31), False),                 # 2^24 segments of 128
+    (1, dict(seqs=1, rows=(1 << 31) - 1, most=1 << 31), True),                  # (in at most 256 segments)
+    (1, dict(seqs=1 << 22, rows=1 << 27, most=40), False),                      # 2^22 segments of a sequence each, and as many more
     (1, dict(seqs=1, rows=1 << 29, most=1 << 29), True),
     (1, dict(seqs=1 << 21, rows=1 << 28, most=300), False),
     (1, dict(seqs=1 << 18, rows=1 << 25, most=300), True),

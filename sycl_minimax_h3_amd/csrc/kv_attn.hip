@@ -7,31 +7,20 @@
 
 namespace h3 {
 
-// Rows: `most` tokens of a sequence times the heads that share a key/value head. Up to 32 (heads of up to 128 features) or 16 the four
-// wavefronts of a block share 16 or 32 of them and the cache is read by all four (an answered token is bound by the cache's bytes);
-// beyond, each has 16 or 32 rows of its own. With more rows shared, or wider heads, a wavefront holds so much that one runs on a SIMD: 16
-// sequences of 4096 tokens, 8 heads, 64 rows: 65 us shared, 50 not; 32 rows 44 and 45; 32 rows of 256 features, 2048 tokens, 72 and 66.
-// 32 rows of its own: where blocks of 128 rows still give each CU one and less than a quarter of their rows is none, and never for float32
-// queries, whose two halves leave room for one wavefront a SIMD only (2048 tokens over 4096, 64 heads over 8 of 128: 16-bit 265 us
-// with 32 rows, 356 with 16; float32 588 and 460; 64 sequences of 72 rows over 2048 tokens: 86 and 75).
-// Places: a tile of rows each; as many as the rows of all sequences can lie in, where that is fewer than `most` rows of each take (one
-// prompt of 8192 tokens among 1024 sequences of a token, 8 heads a key/value head: 1599 instead of 524288).
-// Parts: of the same number of cache blocks for every sequence (at least eight, or four of a prompt's), as many as give each CU the two
-// blocks of threads that it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up
-// to 8192 tokens, 64 heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and
-// their merge 4, 7 and 11 us more. Longer parts: one sequence of 2000 tokens in parts of 8, 16 and 32 blocks 12.6, 15.5 and 18.5 us.)
 // What decides the plans beside the batch: the heads of a group, about the longest length, the window, and (kv_attention_spans) the first tokens
 // that stay visible, the groups of sequences and about the longest of their shared tokens.
 struct KvSight {
     int64_t group, max_len, window, sinks, groups, shared;
     bool spans() const { return sinks > 0 || groups > 0; }
+    int64_t seen() const { return window > 0 ? window + sinks : INT64_MAX / 2; }   // tokens, by a row at most
 };
 
 // The rows' kernel of kv_attention_spans: its tiles and parts by an estimate of the time, in microseconds. Where the device is full, a cache block
 // takes a tile of 128 rows 3.2 and one of 64 rows 2.2 (heads of 128, 16-bit queries; more features and float32 queries in proportion), a
 // part's beginning and end about two more; a last round of at most a block of threads a CU goes faster by 0.7; parts are written and read at
-// 5 TB/s, and joined by a launch (or taken up by the sequences' own: 0.6 each). (About 80 rows of each of 18 sequences over 7000 tokens, 8 heads of 96: 188 us in tiles and parts as
-// kv_attention's, 98 so.) tiles(rt): tiles of a head; join: 0 where the parts are taken up by another launch.
+// 5 TB/s, and joined by a launch (or taken up by the sequences' own: 0.6 each). About 80 rows of each of 18 sequences over 7000 tokens, 8
+// heads of 96: 188 us in tiles and parts as kv_attention's, 98 so.
+// tiles(rt): tiles of a head; join: 0 where the parts are taken up by another launch.
 template <typename F> static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int64_t dim, int64_t blocks, bool two, int cus, double join) {
     const int wc = (int) (kv_width(dim) / 64);
     const int64_t a_cu = wc == 1 ? 3 : wc == 2 ? 2 : 1, slots = a_cu * cus;
@@ -51,6 +40,19 @@ template <typename F> static void kv_rows_plan(KvPlan& plan, F tiles, int64_t ro
     plan.nsplit = (int) ((blocks + plan.per - 1) / plan.per);
 }
 
+// Rows: `most` tokens of a sequence times the heads that share a key/value head. Up to 32 (heads of up to 128 features) or 16 the four
+// wavefronts of a block share 16 or 32 of them and the cache is read by all four (an answered token is bound by the cache's bytes);
+// beyond, each has 16 or 32 rows of its own. With more rows shared, or wider heads, a wavefront holds so much that one runs on a SIMD: 16
+// sequences of 4096 tokens, 8 heads, 64 rows: 65 us shared, 50 not; 32 rows 44 and 45; 32 rows of 256 features, 2048 tokens, 72 and 66.
+// 32 rows of its own: where blocks of 128 rows still give each CU one and less than a quarter of their rows is none, and never for float32
+// queries, whose two halves leave room for one wavefront a SIMD only (2048 tokens over 4096, 64 heads over 8 of 128: 16-bit 265 us
+// with 32 rows, 356 with 16; float32 588 and 460; 64 sequences of 72 rows over 2048 tokens: 86 and 75).
+// Places: a tile of rows each; as many as the rows of all sequences can lie in, where that is fewer than `most` rows of each take (one
+// prompt of 8192 tokens among 1024 sequences of a token, 8 heads a key/value head: 1599 instead of 524288).
+// Parts: of the same number of cache blocks for every sequence (at least eight, or four of a prompt's), as many as give each CU the two
+// blocks of threads that it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up
+// to 8192 tokens, 64 heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and
+// their merge 4, 7 and 11 us more. Longer parts: one sequence of 2000 tokens in parts of 8, 16 and 32 blocks 12.6, 15.5 and 18.5 us.)
 static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus) {
     const int64_t group = sight.group, max_len = sight.max_len, window = sight.window;
     KvPlan plan;
@@ -60,11 +62,11 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& si
     plan.rows = rows > (P.dim <= 128 ? 32 : 16);
     int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     if (sight.groups) keys = std::max<int64_t>(keys - sight.shared, std::min<int64_t>(most, P.rows));
-    if (window > 0) keys = std::min(keys, std::min<int64_t>(window, INT32_MAX) + std::min<int64_t>(most, P.rows) + 2 * kKvB + std::min<int64_t>(sight.sinks, INT32_MAX));
+    if (window > 0) keys = std::min(keys, sight.seen() + std::min<int64_t>(most, P.rows) + 2 * kKvB);
     if (plan.rows && sight.spans()) {
         // (sequences have as many rows on average; a tile sees its window)
         const int64_t each = (P.rows * group + P.seqs - 1) / P.seqs;
-        if (window > 0) keys = std::min<int64_t>(keys, std::min<int64_t>(window + sight.sinks, INT32_MAX) + 128 / group + 2 * kKvB);
+        if (window > 0) keys = std::min<int64_t>(keys, sight.seen() + 128 / group + 2 * kKvB);
         kv_rows_plan(plan, [&](int64_t rt) { return (each + rt - 1) / rt * P.seqs; }, P.rows * group, P.heads, P.dim,
                      std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), two, cus, 6.0);
         plan.tiles = even(plan.rt) <= ragged(plan.rt) ? (rows + plan.rt - 1) / plan.rt : 0;
@@ -104,13 +106,15 @@ static int kv_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sigh
     return 2;
 }
 // The launch of the shared tokens: all rows of a group are as one sequence's, and how many groups' rows there are is known, not each one's.
+// Behind a window its parts are as long as what the rows can see (64 sequences over 8192 shared tokens, window 1024: 52 us in parts of all
+// the shared blocks, 28 so).
 static KvPlan kv_shared_plan(const KvArgs& P, bool two, const KvSight& sight, int cus) {
     KvPlan plan;
     plan.shared = true;
     const int64_t rows = P.rows * sight.group, each = (rows + sight.groups - 1) / sight.groups;
     auto places = [&](int64_t rt) { return rows / rt + sight.groups; };
     plan.rows = each > (P.dim <= 128 ? 32 : 16);
-    const int64_t blocks = std::max<int64_t>((sight.shared + kKvB - 1) / kKvB, 1);
+    const int64_t blocks = std::max<int64_t>((std::min(sight.shared, sight.seen() + 2 * kKvB) + kKvB - 1) / kKvB, 1);
     if (plan.rows) {
         kv_rows_plan(plan, [&](int64_t rt) { return std::max((rows + rt - 1) / rt, sight.groups); }, rows, P.heads, P.dim, blocks, two, cus, 0.0);
         plan.tiles = 0;
@@ -145,7 +149,7 @@ static int sight_of(const std::string& fn, const KvArgs& P, const h3_kv_shared* 
                     KvSight& sight) {
     if (attn_checks(fn.c_str(), P, max_len, q_heads, window)) return -1;
     if (sinks < 0) return fail(fn + ": a negative number of first tokens");
-    sight = KvSight{q_heads / P.heads, max_len, window, window > 0 ? sinks : 0, 0, 0};
+    sight = KvSight{q_heads / P.heads, max_len, std::min<int64_t>(window, INT32_MAX), window > 0 ? std::min<int64_t>(sinks, INT32_MAX) : 0, 0, 0};
     if (!shared || shared->groups == 0) return 0;
     if (shared->groups < 0 || shared->most < 0) return fail(fn + ": a negative number of groups or shared tokens");
     if (shared->groups >= INT32_MAX) return fail(fn + ": too many groups");
@@ -162,7 +166,7 @@ constexpr int64_t kKvApart = 192 << 10;
 static bool kv_apart(const KvArgs& P, const KvSight& sight, int64_t most, int cus) {
     if (sight.groups == 0) return false;
     const int64_t tokens = sight.max_len > 0 ? std::min<int64_t>(sight.max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
-    if (std::max(tokens, sight.shared) * P.seqs <= cus * kKvApart / (2 * P.heads * kv_width(P.dim))) return false;
+    if (std::min(std::max(tokens, sight.shared), sight.seen()) * P.seqs <= cus * kKvApart / (2 * P.heads * kv_width(P.dim))) return false;
     const int64_t rows = P.rows * sight.group, each = (rows + P.seqs - 1) / P.seqs;
     return std::min<int64_t>(most, P.rows) * sight.group <= 96 || 4 * ((each + 63) / 64 * 64 * P.seqs) > 5 * (rows + 32 * sight.groups);
 }

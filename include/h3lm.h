@@ -1,8 +1,8 @@
 /* h3lm.h - the operators of libh3hip.so that run a language model token by token: an 8-bit key/value cache, the attention
  * that reads it, linear attention, whose state stands in the cache's place, and linear layers with 4-bit weights. They stand
  * beside h3hip.h's causal attention and linear layers (the text encoder's whole-sequence forms) and follow its conventions:
- * device pointers of the context's GPU, asynchronous on the context's stream in call order, 0 or -1 with the reason in h3s_last_error(), arguments checked before any work is queued,
- * empty shapes do nothing. No counterpart in the reference.
+ * device pointers of the context's GPU, asynchronous on the context's stream in call order, 0 or -1 with the reason in
+ * h3s_last_error(), arguments checked before any work is queued, empty shapes do nothing. No counterpart in the reference.
  *
  * The library's function names are the reference's header and its additions (h3hip.h) and stay that set; these operators are
  * reached through one exported table of function pointers, `h3lm`:
@@ -133,8 +133,8 @@ typedef struct {
      * last `window` and the first `sinks`, of them those that the mask leaves. With shared not NULL (and groups not 0), the tokens that a group's
      * sequences share are gone through once for all rows of the group, which changes the order of sums, not what a row sees. Blocks
      * that no row sees any more need not be there (an entry of -1). Arguments, results and workspace as kv_attention's; probabilities
-     * of shared tokens are held to 11 bits for 16-bit q where the call's rows times heads of a group, by group of sequences, are more than 32
-     * (or 16 with dim above 128), to 22 otherwise. */
+     * are to 11 bits for 16-bit q also where most of a call's sequences have more rows than that, and those of shared tokens where out is
+     * bfloat16. */
     int (*kv_attention_spans)(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, const int32_t* lengths,
                               int64_t max_len, const void* q, int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window,
                               int64_t sinks, const uint8_t* mask, int64_t mask_stride, void* out, int out_dt, float* lse, void* work,

@@ -21,13 +21,13 @@ struct KvSight {
 // 5 TB/s, and joined by a launch (or taken up by the sequences' own: 0.6 each). About 80 rows of each of 18 sequences over 7000 tokens, 8
 // heads of 96: 188 us in tiles and parts as kv_attention's, 98 so.
 // tiles(rt): tiles of a head; join: 0 where the parts are taken up by another launch.
-template <typename F> static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int64_t dim, int64_t blocks, bool two, int cus, double join) {
+template <typename F> static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int64_t dim, int64_t blocks, bool two, int cus, double join, bool fine = false) {
     const int wc = (int) (kv_width(dim) / 64);
     const int64_t a_cu = wc == 1 ? 3 : wc == 2 ? 2 : 1, slots = a_cu * cus;
     double best = 1e300;
-    for (int nq = 1; nq <= (two ? 1 : 2); ++nq) {
+    for (int nq = 1; nq <= (two || fine ? 1 : 2); ++nq) {
         const int64_t real = tiles(64 * nq) * heads;
-        const double step = (nq == 2 ? 3.2 : 2.2) * (two ? 1.6 : 1.0) * (wc + 0.3) / 2.3 * (double) a_cu / 2;
+        const double step = (nq == 2 ? 3.2 : 2.2) * (two ? 1.6 : fine ? 1.3 : 1.0) * (wc + 0.3) / 2.3 * (double) a_cu / 2;
         for (int64_t n = 1; n <= std::min<int64_t>(blocks, 64); ++n) {
             const int64_t per = (blocks + n - 1) / n, rest = real * n % slots;
             const double rounds = (double) (real * n / slots) + (rest == 0 ? 0.0 : rest <= cus && a_cu > 1 ? 0.7 : 1.0);
@@ -106,17 +106,20 @@ static int kv_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sigh
     return 2;
 }
 // The launch of the shared tokens: all rows of a group are as one sequence's, and how many groups' rows there are is known, not each one's.
+// fine: probabilities as two halves, as the few rows' kernel holds them for 16-bit queries; results of bfloat16 do not show it (48 tokens over 4096
+// shared ones in six groups, 4 heads of 64: 16.8 us with one half, 17.1 so; 18 sequences of 30 tokens over 7000, 8 heads of 96, 78 and 104).
 // Behind a window its parts are as long as what the rows can see (64 sequences over 8192 shared tokens, window 1024: 52 us in parts of all
 // the shared blocks, 28 so).
-static KvPlan kv_shared_plan(const KvArgs& P, bool two, const KvSight& sight, int cus) {
+static KvPlan kv_shared_plan(const KvArgs& P, bool two, bool fine, const KvSight& sight, int cus) {
     KvPlan plan;
     plan.shared = true;
+    plan.fine = fine;
     const int64_t rows = P.rows * sight.group, each = (rows + sight.groups - 1) / sight.groups;
     auto places = [&](int64_t rt) { return rows / rt + sight.groups; };
     plan.rows = each > (P.dim <= 128 ? 32 : 16);
     const int64_t blocks = std::max<int64_t>((std::min(sight.shared, sight.seen() + 2 * kKvB) + kKvB - 1) / kKvB, 1);
     if (plan.rows) {
-        kv_rows_plan(plan, [&](int64_t rt) { return std::max((rows + rt - 1) / rt, sight.groups); }, rows, P.heads, P.dim, blocks, two, cus, 0.0);
+        kv_rows_plan(plan, [&](int64_t rt) { return std::max((rows + rt - 1) / rt, sight.groups); }, rows, P.heads, P.dim, blocks, two, cus, 0.0, fine);
         plan.tiles = 0;
         plan.places = places(plan.rt);
         plan.blocks = plan.places * P.heads;
@@ -171,13 +174,14 @@ static bool kv_apart(const KvArgs& P, const KvSight& sight, int64_t most, int cu
     return std::min<int64_t>(most, P.rows) * sight.group <= 96 || 4 * ((each + 63) / 64 * 64 * P.seqs) > 5 * (rows + 32 * sight.groups);
 }
 // all launches' plans: of the shared tokens first, where they have one
-static int kv_all_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[3]) {
+static int kv_all_plans(const KvArgs& P, bool two, bool fine, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[3]) {
     KvPlan own[2];
     const int at = kv_apart(P, sight, most, cus) ? 1 : 0;
     KvSight behind = sight;
     if (!at) behind.shared = 0;
     const int n = kv_plans(P, two, most, behind, cus, own);
-    if (at) plan[0] = kv_shared_plan(P, two, sight, cus);
+    // (probabilities as two halves where the sequences' own are: some have few rows)
+    if (at) plan[0] = kv_shared_plan(P, two, fine && (!own[0].rows || n == 2), sight, cus);
     for (int i = 0; i < n; ++i) plan[at + i] = own[i];
     return at + n;
 }
@@ -190,12 +194,12 @@ static int64_t attend_work(const char* fn, void* ctx, const h3_kv_cache* cache, 
     Ctx* c = ctx_of(ctx, fn);
     if (!c) return -1;
     if (P.seqs == 0 || P.rows == 0 || batch->most == 0) return 0;
-    // (the more of what 16-bit and float32 queries take)
+    // (the most of what float32 queries take, and 16-bit ones for 16-bit and float32 results)
     int64_t floats = 0;
-    for (bool two : {false, true}) {
+    for (int type = 0; type < (sight.groups ? 3 : 2); ++type) {
         KvPlan plan[3];
         int64_t sum = 0;
-        for (int n = kv_all_plans(P, two, batch->most, sight, c->cus, plan); n-- > 0;) sum += kv_part_floats(plan[n], kv_width(P.dim));
+        for (int n = kv_all_plans(P, type == 1, type == 2, batch->most, sight, c->cus, plan); n-- > 0;) sum += kv_part_floats(plan[n], kv_width(P.dim));
         floats = std::max(floats, sum);
     }
     return 4 * floats;
@@ -219,7 +223,7 @@ static int attend(const char* fn, void* ctx, const h3_kv_cache* cache, const h3_
     if (!c) return -1;
     const bool two = dt == H3S_F32, groups = sight.groups > 0;
     KvPlan plans[3];
-    const int launches = kv_all_plans(A.kv, two, batch->most, sight, c->cus, plans);
+    const int launches = kv_all_plans(A.kv, two, !two && out_dt != H3S_BF16, batch->most, sight, c->cus, plans);
     const int64_t W = kv_width(dim);
     int64_t floats = 0;
     for (int i = 0; i < launches; ++i) {

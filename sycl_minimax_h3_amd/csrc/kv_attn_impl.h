@@ -501,6 +501,26 @@ __device__ __forceinline__ float2 kv_shared_ml(const KvAttnArgs& P, int64_t row2
 }
 // The weight of a part: 0 where nothing was seen, whose sums say nothing
 __device__ __forceinline__ float kv_weight(const float2& ml, float top) { return ml.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top); }
+// y += the sums of four parts times their weights, which the lanes first .. of 16 have in w; sums(i): a lane's in part i. Loaded together: one by
+// one each waits for memory. (No weight: nothing seen, and there may be no sums.)
+template <int WC, typename F> __device__ __forceinline__ void kv_take(float4 (&y)[WC], float w, int first, F sums) {
+    float4 v[4][WC];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int t = 0; t < WC; ++t) v[i][t] = *reinterpret_cast<const float4*>(sums(i) + 64 * t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float wi = __shfl(w, first + i, 16);
+#pragma unroll
+        for (int t = 0; t < WC; ++t) {
+            y[t].x = wi == 0.0f ? y[t].x : __builtin_fmaf(v[i][t].x, wi, y[t].x);
+            y[t].y = wi == 0.0f ? y[t].y : __builtin_fmaf(v[i][t].y, wi, y[t].y);
+            y[t].z = wi == 0.0f ? y[t].z : __builtin_fmaf(v[i][t].z, wi, y[t].z);
+            y[t].w = wi == 0.0f ? y[t].w : __builtin_fmaf(v[i][t].w, wi, y[t].w);
+        }
+    }
+}
 
 // Whether a key block is seen whole by rows that are the tokens posmin .. posmax
 template <int MODE> __device__ __forceinline__ bool kv_whole(const KvAttnArgs& P, int key0, int posmin, int posmax) {
@@ -688,20 +708,8 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
                         if (s0) ml = kv_shared_ml(P, row2, s0 + c);
                         const float wl = kv_weight(ml, top);
                         lt += wave_sum<16>(ml.y * wl);
-#pragma unroll 8
-                        for (int s = s0; s < min(P.nsplit2, s0 + 16); ++s) {
-                            const float w = __shfl(wl, s - s0, 16);
-                            float4 v[WC];
-#pragma unroll
-                            for (int t = 0; t < WC; ++t) v[t] = *reinterpret_cast<const float4*>(P.po2 + (row2 + (int64_t) s * P.rt2) * W + 64 * t + 4 * c);
-#pragma unroll
-                            for (int t = 0; t < WC; ++t) {
-                                more[t].x = w == 0.0f ? more[t].x : __builtin_fmaf(v[t].x, w, more[t].x);
-                                more[t].y = w == 0.0f ? more[t].y : __builtin_fmaf(v[t].y, w, more[t].y);
-                                more[t].z = w == 0.0f ? more[t].z : __builtin_fmaf(v[t].z, w, more[t].z);
-                                more[t].w = w == 0.0f ? more[t].w : __builtin_fmaf(v[t].w, w, more[t].w);
-                            }
-                        }
+                        for (int s = s0; s < min(P.nsplit2, s0 + 16); s += 4)
+                            kv_take<WC>(more, wl, s - s0, [&](int i) { return P.po2 + (row2 + (int64_t) min(s + i, P.nsplit2 - 1) * P.rt2) * W + 4 * c; });
                     }
                 }
             const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
@@ -737,7 +745,7 @@ template <int WC> __device__ __forceinline__ int kv_mix(int g, int c) { return (
 // doing it in every wavefront took more vector instructions than the softmax. Bound by vector instructions beside the products (4096 tokens
 // over 8192, 64 heads over 8 of 128: 947-1060 us by the card, 0.78-0.87 PFLOP/s, the matrix cores 34 % busy). Operands are read from LDS a
 // step ahead of their products (960 us without, 16 sequences of 100 tokens of 256 features 203 to 181).
-template <int WC, int NQ, bool TWO, int MODE = kKvAll>
+template <int WC, int NQ, bool TWO, int MODE = kKvAll, bool PTWO = TWO>
 __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC, DT = 4 * WC, RT = 64 * NQ, PARTS = TWO ? 2 : 1;
     __shared__ v8h_kv sk[2][4][WC][2][64], sv[2][DT][2][64];              // [stage][key tile or feature tile][...][half][lane]
@@ -812,7 +820,7 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
         }
         kv_reach<16 * NQ>(who + wave * 16 * NQ, posmin, posmax);
     }
-    KvRows<WC, NQ, TWO, TWO, MODE> q;
+    KvRows<WC, NQ, TWO, PTWO, MODE> q;
     q.load(P, h, it.r0, it.n, it.len, R, rw, l15, g, who + (MODE == kKvShared ? wave * 16 * NQ : 0));
     if (any) {
         stage(0);
@@ -848,7 +856,7 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
                 __builtin_amdgcn_sched_barrier(0);
             }
             const bool whole = kv_whole<MODE>(P, key0, posmin, posmax);
-            v8h_kv pf[NQ][2][PARTS];
+            v8h_kv pf[NQ][2][PTWO ? 2 : 1];
             float vsl[NQ];
             q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
             // likewise a feature tile's operands, and the sums of the tile before are added to o meanwhile
@@ -1009,21 +1017,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttnArgs P) {
         if (s0) ml = ml_of(s0 + c);
         const float wl = kv_weight(ml, top);
         lt += wave_sum<16>(ml.y * wl);
-#pragma unroll 4
-        for (int s = s0; s < min(parts, s0 + 16); ++s) {
-            const float w = __shfl(wl, s - s0, 16);
-            const float* o = s < own ? P.po + (row0 + (int64_t) s * RT) * W : P.po2 + (row2 + (int64_t) (s - own) * P.rt2) * W;
-            float4 v[WC];
-#pragma unroll
-            for (int t = 0; t < WC; ++t) v[t] = *reinterpret_cast<const float4*>(o + 64 * t + 4 * c);
-#pragma unroll
-            for (int t = 0; t < WC; ++t) {          // (no weight: nothing seen, and there are no sums)
-                y[t].x = w == 0.0f ? y[t].x : __builtin_fmaf(v[t].x, w, y[t].x);
-                y[t].y = w == 0.0f ? y[t].y : __builtin_fmaf(v[t].y, w, y[t].y);
-                y[t].z = w == 0.0f ? y[t].z : __builtin_fmaf(v[t].z, w, y[t].z);
-                y[t].w = w == 0.0f ? y[t].w : __builtin_fmaf(v[t].w, w, y[t].w);
-            }
-        }
+        for (int s = s0; s < min(parts, s0 + 16); s += 4)
+            kv_take<WC>(y, wl, s - s0, [&](int i) {
+                const int at = min(s + i, parts - 1);
+                return (at < own ? P.po + (row0 + (int64_t) at * RT) * W : P.po2 + (row2 + (int64_t) (at - own) * P.rt2) * W) + 4 * c;
+            });
     }
     const int64_t at = ((int64_t) it.r0 + rr / group) * P.q_heads + it.h * group + rr % group;
     const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
@@ -1041,6 +1039,7 @@ struct KvPlan {
     int64_t blocks;       // of threads, without the parts
     uint32_t least = 0, greatest = UINT32_MAX;
     bool shared = false;  // of the shared tokens
+    bool fine = false;    // kv_attn_rows_kernel with probabilities as two halves (float32 queries' are anyway)
 };
 
 template <int WC, int NQ, bool ROWS, int MODE>
@@ -1048,6 +1047,8 @@ static void kv_attn_run(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool tw
     const unsigned grid = (unsigned) (plan.blocks * plan.nsplit);
     constexpr int RT = (ROWS ? 64 : 16) * NQ;
     if constexpr (ROWS) {
+        if constexpr (MODE == kKvShared && NQ == 1)
+            if (!two && plan.fine) return kv_attn_rows_kernel<WC, 1, false, MODE, true><<<grid, 256, 0, c->stream>>>(P);
         if (!two) kv_attn_rows_kernel<WC, NQ, false, MODE><<<grid, 256, 0, c->stream>>>(P);
         else if constexpr (NQ == 1) kv_attn_rows_kernel<WC, 1, true, MODE><<<grid, 256, 0, c->stream>>>(P);
     } else {

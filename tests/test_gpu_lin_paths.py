@@ -9,19 +9,34 @@ import spans_reference as spans
 from helpers import launches, new, up
 from test_gpu_lin import Case, i32, run
 from test_gpu_lm import Recorded
+from test_gpu_spans import context
 
 pytestmark = pytest.mark.gpu
 
 from sycl_minimax_h3_amd import Device, Error, Tensor, ops  # noqa: E402
 
 
+@pytest.fixture(scope="module")
+def dev1():
+    d = context(1)
+    yield d
+    d.close()
+
+
+@pytest.fixture(scope="module")
+def dev8():
+    d = context(8)
+    yield d
+    d.close()
+
+
 def test_which_kernels_run(dev):
     """Few tokens: one launch; many: pieces, split into segments where heads are few; both where a batch has both."""
     for counts, heads, each, want in (
         ([1, 1, 3], 2, (1, 1, 1), ["lin_step_kernel"]),
-        ([200], 2, (1, 1, 1), ["lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"]),
+        ([600], 2, (1, 1, 1), ["lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"]),
         ([100, 90], 2, (1, 1, 1), ["lin_chunk_kernel"]),
-        ([1, 300, 1, 1], 2, (1, 1, 1), ["lin_step_kernel", "lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"]),
+        ([1, 600, 1, 1], 2, (1, 1, 1), ["lin_step_kernel", "lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"]),
     ):
         case = Case(dev, counts, heads, each, 64, 64, "BF16", 51)
         args = case.operands()
@@ -34,13 +49,36 @@ def test_which_kernels_run(dev):
 
 
 @pytest.mark.parametrize("dt", ["BF16", "F16", "F32"])
-@pytest.mark.parametrize("dk,dv", [(32, 64), (64, 128), (96, 100), (128, 64), (128, 200), (160, 48), (192, 128), (256, 256)])
-def test_every_width(dev, dk, dv, dt):
-    """Each number of steps over the keys' features and of values a block has, whole pieces and rests, several segments."""
+@pytest.mark.parametrize("dk,dv", [(32, 64), (32, 128), (64, 128), (96, 100), (128, 64), (128, 200), (160, 48), (192, 128), (256, 256)])
+@pytest.mark.parametrize("full", [False, True])
+def test_every_width(dev, dev1, dk, dv, dt, full):
+    """Each number of steps over the keys' features and of values a block has, whole pieces and rests. (A device that is full takes 128 features
+    of values a block, where there are more than 64.)"""
+    dev = dev1 if full else dev
     case = Case(dev, [259, 64, 17, 1], 2, (1, 2, 1), dk, dv, dt, 52 + dk + dv, begin=[1])
     case.check(*run(case), "F32")
     case = Case(dev, [70, 31], 1, (1, 1, 1), dk, dv, dt, 53 + dk + dv, begin=[1], offset=3, pad=2)
     case.check(*run(case, dt), dt, what="rows off 16 bytes")
+
+
+def kernels(case):
+    args = case.operands()
+    out = new(case.dev, "F32", [case.rows, case.state.shape[1] * case.dv])
+    work = new(case.dev, "U8", [max(ops.lin_attention_work(args[0], *args[2:3], *args[5:]), 16)])
+    return [k for k, _, _ in launches(case.dev, lambda: ops.lin_attention(*args, out, work=work))]
+
+
+@pytest.mark.parametrize("dt", ["BF16", "F16", "F32"])
+@pytest.mark.parametrize("dk,dv", [(32, 128), (64, 100), (96, 128), (128, 100), (192, 128)])
+def test_segments_of_every_width(dev, dev8, dk, dv, dt):
+    """Several segments, in blocks of 64 and of 128 features of values."""
+    for d, counts, wide in ((dev, [1100, 40], False), (dev8, [1100], True)):
+        case = Case(d, counts, 2, (1, 1, 1), dk, dv, dt, 59 + dk, begin=[0])
+        ran = kernels(case)
+        assert [k.split("<")[0] for k in ran] == ["lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"], ran
+        waves, tiles = (int(x) for x in ran[0].split("<")[1].split(",")[2:4])
+        assert 16 * waves * tiles == (128 if wide else 64), ran
+        case.check(*run(case), "F32", what=str(wide))
 
 
 def test_states_off_16_bytes_and_wide_rows(dev):

@@ -25,7 +25,7 @@ template <typename F>
 static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int64_t dim, int64_t blocks, bool two, int cus, double join, bool fine = false) {
     const int wc = (int) (kv_width(dim) / 64);
     const int64_t a_cu = wc == 1 ? 3 : wc == 2 ? 2 : 1, slots = a_cu * cus;
-    double best = 1e300;
+    plan.cost = 1e300;
     for (int nq = 1; nq <= (two || fine ? 1 : 2); ++nq) {
         const int64_t real = tiles(64 * nq) * heads;
         const double step = (nq == 2 ? 3.2 : 2.2) * (two ? 1.6 : fine ? 1.3 : 1.0) * (wc + 0.3) / 2.3 * (double) a_cu / 2;
@@ -34,7 +34,7 @@ static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int
             const double rounds = (double) (real * n / slots) + (rest == 0 ? 0.0 : rest <= cus && a_cu > 1 ? 0.7 : 1.0);
             const double parts = n > 1 || join == 0.0 ? (double) n * rows * heads * dim * 8.0 / 5e6 : 0.0;
             const double cost = rounds * (per + 2) * step + parts + (join == 0.0 ? 0.6 * n : n > 1 ? join : 0.0);
-            if (cost < best) { best = cost; plan.nq = nq; plan.per = (int) per; }
+            if (cost < plan.cost) { plan.cost = cost; plan.nq = nq; plan.per = (int) per; }
         }
     }
     plan.rt = 64 * plan.nq;
@@ -162,29 +162,33 @@ static int sight_of(const std::string& fn, const KvArgs& P, const h3_kv_shared* 
     sight.shared = shared->most > 0 ? std::min<int64_t>(shared->most, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     return 0;
 }
-// Whether shared tokens are a launch of their own. A launch and the reading of its sums cost 8 us or more; below so many bytes of all sequences'
-// caches a CU it takes less to go through the shared ones again for each (they come from the caches of the device). So it does where sequences
-// have many rows each, which are bound by their products either way, unless their tiles would be much emptier than the groups' (eight sequences of
-// up to 256 tokens over 4096 shared ones, 64 heads over 8 of 128: 364 us apart, 355 not).
+// All launches' plans: of the shared tokens first, where they have one. A launch and the reading of its sums cost 8 us or more; below so many bytes
+// of all sequences' caches a CU it takes less to go through the shared ones again for each (they come from the caches of the device). Where
+// sequences have many rows each, whose products bound them either way, the estimates decide: tiles of a group's rows are fuller (53
+// sequences of up to 31 tokens over 5376 shared ones in 13 groups, 8 heads over one of 80: 67 us apart, 77 not; eight of up to 256 over 4096, 64
+// heads over 8 of 128: 364 us apart, 355 not).
 constexpr int64_t kKvApart = 192 << 10;
-static bool kv_apart(const KvArgs& P, const KvSight& sight, int64_t most, int cus) {
-    if (sight.groups == 0) return false;
-    const int64_t tokens = sight.max_len > 0 ? std::min<int64_t>(sight.max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
-    if (std::min(std::max(tokens, sight.shared), sight.seen()) * P.seqs <= cus * kKvApart / (2 * P.heads * kv_width(P.dim))) return false;
-    const int64_t rows = P.rows * sight.group, each = (rows + P.seqs - 1) / P.seqs;
-    return std::min<int64_t>(most, P.rows) * sight.group <= 96 || 4 * ((each + 63) / 64 * 64 * P.seqs) > 5 * (rows + 32 * sight.groups);
-}
-// all launches' plans: of the shared tokens first, where they have one
 static int kv_all_plans(const KvArgs& P, bool two, bool fine, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[3]) {
-    KvPlan own[2];
-    const int at = kv_apart(P, sight, most, cus) ? 1 : 0;
-    KvSight behind = sight;
-    if (!at) behind.shared = 0;
-    const int n = kv_plans(P, two, most, behind, cus, own);
-    // (probabilities as two halves where the sequences' own are: some have few rows)
-    if (at) plan[0] = kv_shared_plan(P, two, fine && (!own[0].rows || n == 2), sight, cus);
-    for (int i = 0; i < n; ++i) plan[at + i] = own[i];
-    return at + n;
+    KvPlan own[2], behind[2], shared;
+    KvSight all = sight;
+    all.shared = 0;
+    int n = kv_plans(P, two, most, all, cus, own);
+    const int64_t tokens = sight.max_len > 0 ? std::min<int64_t>(sight.max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
+    bool apart = sight.groups > 0 &&
+                 std::min(std::max(tokens, sight.shared), sight.seen()) * P.seqs > cus * kKvApart / (2 * P.heads * kv_width(P.dim));
+    if (apart) {
+        const int m = kv_plans(P, two, most, sight, cus, behind);
+        // (probabilities as two halves where the sequences' own are: some have few rows)
+        shared = kv_shared_plan(P, two, fine && (!behind[0].rows || m == 2), sight, cus);
+        apart = !own[0].rows || shared.cost + behind[0].cost + 6.0 < own[0].cost;
+        if (apart) {
+            n = m;
+            std::copy(behind, behind + m, own);
+            plan[0] = shared;
+        }
+    }
+    std::copy(own, own + n, plan + apart);
+    return n + apart;
 }
 
 static int64_t attend_work(const char* fn, void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, int64_t max_len,

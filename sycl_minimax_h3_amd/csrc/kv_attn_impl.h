@@ -224,17 +224,47 @@ template <int WC, int NQ, bool TWO, bool PTWO, int MODE> struct KvRows {
         return hidden;
     }
 
+    // kKvOwn, kKvShared: the mask's bytes of the lane's keys of a cache block (0: hidden), for the item's sequence or each row's. They are loaded before
+    // the block's products and looked at behind them: where the scores want them, each block waits for them (53 sequences of up to 31 tokens
+    // over 5376 shared ones in 13 groups, 8 heads over one of 80: 85 to 79 us).
+    static constexpr int MASKS = MODE == kKvShared ? NQ : 1;
+    __device__ __forceinline__ void mask_bytes(const KvAttnArgs& P, int b, int g, int key0, uint4 (&m)[MASKS]) const {
+        if (MODE == kKvAll || !P.mask) return;
+#pragma unroll
+        for (int e = 0; e < MASKS; ++e) {
+            const int k0 = key0 + g * 16;
+            const uint8_t* mp = P.mask + (int64_t) (MODE == kKvShared ? seq[e] : b) * P.mask_stride + k0;
+            if (P.mask_vec && k0 + 16 <= P.mask_stride) {
+                m[e] = *reinterpret_cast<const uint4*>(mp);
+            } else {
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (k0 + i < P.mask_stride) w[i >> 2] |= (uint32_t) mp[i] << (8 * (i & 3));
+                m[e] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+    static __device__ __forceinline__ uint32_t none_of(const uint4& m) {
+        // (a byte that is not 0 carries into its highest bit; the four bits' weights are summed by a dot product of bytes)
+        auto some = [](uint32_t w) { return ((((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) >> 7) & 0x01010101u; };
+        const uint32_t lo = __builtin_amdgcn_udot4(some(m.y), 0x80402010u, __builtin_amdgcn_udot4(some(m.x), 0x08040201u, 0, false), false);
+        const uint32_t hi = __builtin_amdgcn_udot4(some(m.w), 0x80402010u, __builtin_amdgcn_udot4(some(m.z), 0x08040201u, 0, false), false);
+        return (lo | hi << 8) ^ 0xffffu;
+    }
+
     // One cache block's scores to probabilities: s (register t, i of lane group g: the key 16 g + 4 t + i of the block) to the operands
     // pf, times 2^15, and vsl, the factor of the block's values for each row. whole: every row sees every key.
     __device__ __forceinline__ void softmax(const KvAttnArgs& P, int b, int g, int key0, bool whole, float ks, float vs, v4f_kv (&s)[NQ][4],
-                                            v8h_kv (&pf)[NQ][2][PP], float (&vsl)[NQ]) {
+                                            v8h_kv (&pf)[NQ][2][PP], float (&vsl)[NQ], const uint4 (&mask)[MASKS]) {
         uint32_t hidden = 0;                        // by the mask: bit 4 t + i
-        if (MODE != kKvShared && !whole && P.mask) hidden = masked(P, b, g, key0);
+        if (MODE == kKvAll && !whole && P.mask) hidden = masked(P, b, g, key0);
+        if (MODE == kKvOwn && !whole && P.mask) hidden = none_of(mask[0]);
 #pragma unroll
         for (int e = 0; e < NQ; ++e) {
             uint32_t off = hidden;
             if (!whole) {
-                if (MODE == kKvShared && P.mask) off = masked(P, seq[e], g, key0);
+                if (MODE == kKvShared && P.mask) off = none_of(mask[MODE == kKvShared ? e : 0]);
                 const int hi = pos[e] - key0 - g * 16;                  // the lane's keys 0 .. hi of 16 are not ahead of the row
                 off |= hi >= 15 ? 0u : hi < 0 ? 0xffffu : 0xffffu & (0xfffeu << hi);
                 if (P.window > 0) {
@@ -631,6 +661,9 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
     while (kb < last) {
         int nkb = kb + KS, npage = 0;
         const bool more = pages.template next<KS>(P, it, nkb, npage, last, lane);
+        const int key0 = it.block(kb) * kKvB;
+        uint4 mask[MODE == kKvShared ? NQ : 1];
+        q.mask_bytes(P, b, g, key0, mask);
         v4f_kv s[NQ][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -655,11 +688,10 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(KvAttnArgs P) {
             ks = P.kv.ks[(int64_t) npage * P.kv.heads + h];
             vs = P.kv.vs[(int64_t) npage * P.kv.heads + h];
         }
-        const int key0 = it.block(kb) * kKvB;
         const bool whole = kv_whole<MODE>(P, key0, posmin, posmax);
         v8h_kv pf[NQ][2][2];
         float vsl[NQ];
-        q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
+        q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl, mask);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
             v4f_kv y[NQ];
@@ -841,6 +873,8 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
     while (kb < last) {
         const int key0 = it.block(kb) * kKvB;
         if (key0 <= posmax) {
+            uint4 mask[MODE == kKvShared ? NQ : 1];
+            q.mask_bytes(P, b, g, key0, mask);
             // a feature chunk's operands of all four key tiles are read while the one before is multiplied: four tiles' sums in turn
             // leave no product waiting for the last
             v4f_kv s[NQ][4];
@@ -865,7 +899,7 @@ __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv
             const bool whole = kv_whole<MODE>(P, key0, posmin, posmax);
             v8h_kv pf[NQ][2][PTWO ? 2 : 1];
             float vsl[NQ];
-            q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl);
+            q.softmax(P, b, g, key0, whole, ks_now, vs_now, s, pf, vsl, mask);
             // likewise a feature tile's operands, and the sums of the tile before are added to o meanwhile
             v8h_kv x[2][2];
             auto feats = [&](int t) {
@@ -1046,6 +1080,7 @@ struct KvPlan {
     int64_t blocks;       // of threads, without the parts
     uint32_t least = 0, greatest = UINT32_MAX;
     bool shared = false;  // of the shared tokens
+    double cost = 0.0;    // kv_attention_spans' rows: the estimate, in microseconds
     bool fine = false;    // kv_attn_rows_kernel with probabilities as two halves (float32 queries' are anyway)
 };
 

@@ -98,6 +98,25 @@ def test_states_off_16_bytes_and_wide_rows(dev):
     case.check(*run(case), "F32", what="wide rows")
 
 
+def test_states_past_32_bits(dev):
+    """The last slots of a pool of more than 2^31 numbers (and its one before the last of the first 2^31), few tokens and many, as in a small pool."""
+    heads, d, rows = 64, 128, 73
+    x = lm.to_bits(np.random.default_rng(64).standard_normal((rows, 3 * heads * d)), "BF16")
+    decay = up(dev, np.linspace(0, 0.3, heads).astype(np.float32), "F32", [heads])
+    x = up(dev, x, "BF16", [rows, 3 * heads * d])
+    r = [ops.Rows(x, i * heads * d, 3 * heads * d, rows, heads, d) for i in range(3)]
+    got = []
+    for slots, a, b in ((3, 0, 2), ((1 << 31) // (heads * d * d) + 6, (1 << 31) // (heads * d * d) - 1, (1 << 31) // (heads * d * d) + 5)):
+        state = ops.LinState.new(dev, slots, heads, d, d)
+        out = new(dev, "F32", [rows, heads * d])
+        ops.lin_attention(state, decay, *r, i32(dev, [0, 3]), i32(dev, [-1]), i32(dev, [a]), 3, out)
+        ops.lin_attention(state, decay, *r, i32(dev, [3, rows]), i32(dev, [a]), i32(dev, [b]), rows - 3, out)
+        ops.lin_attention(state, decay, *r, i32(dev, [0, 2]), i32(dev, [b]), i32(dev, [b]), 2, out)
+        got.append(out.to_numpy())
+        del state
+    assert np.isfinite(got[0]).all() and np.array_equal(*got)
+
+
 def test_a_batch_past_one_segment_each(dev):
     """Ragged prompts whose segments begin anywhere among the rows, against one prompt at a time: within the bounds, states and all."""
     counts = [513, 128, 0, 129, 127, 1, 700, 64]

@@ -106,6 +106,7 @@ SINKS = [
     ([(33, 200)], 2, 4, 192, "BF16", 20, 200),
     ([(60, 250)], 1, 4, 256, "F32", 90, 5),
     ([(2, 260)], 3, 3, 33, "BF16", 10, 1 << 40),
+    ([(2, 260), (1, 70)], 1, 40, 64, "F16", 50, 7),
 ]
 
 
@@ -145,6 +146,8 @@ SHARED = [
     ([(1, 200), (1, 200)], [(0, 2, 1 << 30)], 1, 4, 64, "F32"),
     ([(1, 200), (1, 200)], [(0, 2, -5)], 1, 4, 64, "F32"),
     ([(1, 64), (1, 100), (3, 20)], [(0, 3, 128)], 1, 4, 64, "BF16"),
+    ([(1, 300), (3, 200), (1, 256)], [(0, 3, 128)], 1, 48, 64, "BF16"),
+    ([(1, 300), (2, 200)], [(0, 2, 128)], 1, 17, 200, "F16"),
 ]
 
 

@@ -575,7 +575,9 @@ def _lin_batch(starts: Tensor, source: Tensor, target: Tensor, rows: int, most: 
         raise Error(f"lin_attention: starts {starts.shape}, source {source.shape} and target {target.shape} are not of the same sequences")
     if most < 0:
         raise Error(f"the most rows of a sequence: {most}")
-    return _api.lin_batch(_i32(starts, "starts", n + 1), _i32(source, "source", n), _i32(target, "target", n), n, rows, most)
+    if not (starts.dtype is source.dtype is target.dtype is DType.I32):
+        raise Error(f"starts, source and target must be int32, got {starts.dtype}, {source.dtype} and {target.dtype}")
+    return _api.lin_batch(starts.ptr(), source.ptr(), target.ptr(), n, rows, most)
 
 
 def lin_attention_work(state: LinState, q: Rows, starts: Tensor, source: Tensor, target: Tensor, most: int) -> int:

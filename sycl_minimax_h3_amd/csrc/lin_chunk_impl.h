@@ -197,13 +197,19 @@ __global__ __launch_bounds__(64 * NW, 2) void lin_chunk_kernel(LinArgs P) {
             for (int x = 0; x < NP; ++x) p[x] = make_uint4(w[0][x], w[1][x], w[2][x], w[3][x]);
         }
     };
-    // The 16-byte place of a token's slot (8 features). 16 tokens' same slot, 16 slots of a token, and the eight tokens by four or two slots of a
-    // transposing read lie on as many banks as they can (64 of 4 bytes): the slot's low bits are mixed with the token's.
-    auto mix = [](uint32_t rows, uint32_t token) {                          // rows: slots a token
+    // The 16-byte place of a token's slot (8 features): the slot's low bits are mixed with the token's, so that the lanes of an access that are
+    // served together lie on as many of the 64 banks as they can. Those of a 16-byte read are 0-3, 12-15 and 20-27, and 4-11, 16-19 and
+    // 28-31 (counted): rows of q and k, a token a lane and two neighbouring slots, so the slots' last bit goes with one of a token's last
+    // two (8192 tokens of 64 heads: 7.5 to 2.8 million cycles of conflicts, 149.7 to 147.7 us). A transposing read of k meets eight tokens by
+    // four slots, of v by two: other bits of the token's for v.
+    auto mix_k = [](uint32_t rows, uint32_t token) {                        // rows: slots a token
+        return rows % 16 == 0 ? ((token & 2) << 2) | (token & 4) | ((token >> 2) & 2) | (token & 1) : (token & 4) | ((token >> 2) & 2) | ((token >> 1) & 1);
+    };
+    auto mix_v = [](uint32_t rows, uint32_t token) {
         return rows % 16 == 0 ? ((token & 3) << 2) | ((token >> 1) & 2) | ((token >> 3) & 1) : ((token & 2) << 1) | ((token >> 1) & 2) | ((token >> 3) & 1);
     };
-    auto at_k = [&](uint32_t token, uint32_t slot) { return token * (DKP / 8) + (slot ^ mix(DKP / 8, token)); };
-    auto at_v = [&](uint32_t token, uint32_t slot) { return token * (DVB / 8) + (slot ^ mix(DVB / 8, token)); };
+    auto at_k = [&](uint32_t token, uint32_t slot) { return token * (DKP / 8) + (slot ^ mix_k(DKP / 8, token)); };
+    auto at_v = [&](uint32_t token, uint32_t slot) { return token * (DVB / 8) + (slot ^ mix_v(DVB / 8, token)); };
 
     // a thread's pieces of 8 elements are the same features of every KS-th (VS-th) token, where a row's pieces divide the threads: their places in
     // LDS then differ by constants, if those tokens are 16 or more apart (the mix goes by a token's lowest four bits)

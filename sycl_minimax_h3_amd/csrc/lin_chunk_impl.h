@@ -97,7 +97,7 @@ template <int DT, int KC, int NW, int NV> struct LinShape {
 };
 
 template <int DT, int KC, int NW, int NV, bool OUT, bool VEC>
-__global__ __launch_bounds__(64 * NW, 2) void lin_chunk_kernel(LinArgs P) {
+__global__ __launch_bounds__(64 * NW, (DT == H3S_F32 && KC > 4 && NW == 4 && OUT ? 1 : 2)) void lin_chunk_kernel(LinArgs P) {   // (1: LDS for one block)
     using Sh = LinShape<DT, KC, NW, NV>;
     constexpr int NP = Sh::NP, NS = Sh::NS, CT = Sh::CT, C = Sh::C, U = Sh::U, DKP = Sh::DKP, DVB = Sh::DVB, T = Sh::T;
     constexpr int ES = DT == H3S_F32 ? 4 : 2, RAW = ES / 2;                 // 16-byte loads for 8 elements

@@ -186,9 +186,12 @@ static int lin_checks(const std::string& fn, const h3_lin_state* state, const h3
     return 0;
 }
 
-// Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces. Where the sequences beside the longest
-// have more than 2 kLinFew tokens on average, all go in pieces: a launch that finds nothing to do takes 3 to 5 us.
-constexpr int kLinFew = 16;
+// Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces (64 sequences of 64 heads of 128 x 128,
+// of up to 1, 4, 8 and 16 tokens, two thirds of that on average: 49, 61, 87 and 139 us, in pieces 85, 87, 90 and 97; 16 of 16 heads of 256 x
+// 256 17, 20, 26 and 41, in pieces 22). A launch for few tokens beside the others' takes 5 us and more: where the sequences beside the
+// longest have more than kLinBeside tokens on average, or are up to four blocks of pieces a CU, all go in pieces (64 sequences of up to 8
+// tokens in two launches 96 us; eight of up to 39 37, in pieces 21).
+constexpr int kLinFew = 6, kLinBeside = 4;
 constexpr int64_t kLinLeast = 32, kLinSegs = 256;   // the least tokens of a segment, the most segments of an average sequence
 struct LinPlan {
     bool step, chunk, split;
@@ -214,7 +217,8 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
     LinPlan p{};
     const int64_t most = std::min(batch.most, batch.rows);
     p.chunk = most > kLinFew;
-    p.step = !p.chunk || (batch.seqs > 1 && batch.rows - most <= 2 * kLinFew * (batch.seqs - 1) && most * batch.seqs > batch.rows);
+    p.step = !p.chunk || ((batch.seqs - 1) * state.heads * ((state.dv + 63) / 64) > 4 * (int64_t) cus &&
+                          batch.rows - most <= kLinBeside * (batch.seqs - 1) && most * batch.seqs > batch.rows);
     p.kc = state.dk <= 32 ? 1 : state.dk > 64 && state.dk <= 96 ? 3 : (int) (state.dk + 63) / 64 * 2;
     // Segments, and a block's features of values, by an estimate of the time, of the average sequence (with a launch for few tokens: of as many
     // of the longest's length as there are rows for): the pieces one after another; a split one's own sums half as much again, and launches,

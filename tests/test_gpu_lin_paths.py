@@ -30,13 +30,14 @@ def dev8():
     d.close()
 
 
-def test_which_kernels_run(dev):
-    """Few tokens: one launch; many: pieces, split into segments where heads are few; both where a batch has both."""
-    for counts, heads, each, want in (
-        ([1, 1, 3], 2, (1, 1, 1), ["lin_step_kernel"]),
-        ([600], 2, (1, 1, 1), ["lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"]),
-        ([100, 90], 2, (1, 1, 1), ["lin_chunk_kernel"]),
-        ([1, 600, 1, 1], 2, (1, 1, 1), ["lin_step_kernel", "lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"]),
+def test_which_kernels_run(dev, dev1):
+    """Few tokens: one launch; many: pieces, split into segments where heads are few; both where a batch has both and fills the device."""
+    for dev, counts, heads, each, want in (
+        (dev, [1, 1, 3], 2, (1, 1, 1), ["lin_step_kernel"]),
+        (dev, [600], 2, (1, 1, 1), ["lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"]),
+        (dev, [100, 90], 2, (1, 1, 1), ["lin_chunk_kernel"]),
+        (dev, [1, 600, 1, 1], 2, (1, 1, 1), ["lin_chunk_kernel", "lin_scan_kernel", "lin_chunk_kernel"]),
+        (dev1, [1, 600, 6, 1, 7, 1], 2, (1, 1, 1), ["lin_step_kernel", "lin_chunk_kernel"]),
     ):
         case = Case(dev, counts, heads, each, 64, 64, "BF16", 51)
         args = case.operands()

@@ -65,11 +65,11 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& si
     if (sight.groups) keys = std::max<int64_t>(keys - sight.shared, std::min<int64_t>(most, P.rows));
     if (window > 0) keys = std::min(keys, sight.seen() + std::min<int64_t>(most, P.rows) + 2 * kKvB);
     if (plan.rows && sight.spans()) {
-        // (sequences have as many rows on average; a tile sees its window)
-        const int64_t each = (P.rows * group + P.seqs - 1) / P.seqs;
+        // (sequences have as many rows on average, and half a tile more, but none more tiles than the longest; a tile sees its window)
+        const int64_t all = P.rows * group;
+        auto tiles = [&](int64_t rt) { return std::max(std::min(all / rt + P.seqs / 2, (rows + rt - 1) / rt * P.seqs), (int64_t) P.seqs); };
         if (window > 0) keys = std::min<int64_t>(keys, sight.seen() + 128 / group + 2 * kKvB);
-        kv_rows_plan(plan, [&](int64_t rt) { return (each + rt - 1) / rt * P.seqs; }, P.rows * group, P.heads, P.dim,
-                     std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), two, cus, 6.0);
+        kv_rows_plan(plan, tiles, all, P.heads, P.dim, std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), two, cus, 6.0);
         plan.tiles = even(plan.rt) <= ragged(plan.rt) ? (rows + plan.rt - 1) / plan.rt : 0;
         plan.places = std::min(even(plan.rt), ragged(plan.rt));
         plan.blocks = plan.places * P.heads;

@@ -102,7 +102,8 @@ typedef struct {
      * that sees nothing gets zeros (lse -infinity). Hidden tokens have no effect, whatever their codes, scales and mask say.
      * Products, softmax and sums are float32 (q to 11 bits of each value for 16-bit types, which is all they have, 22 for float32;
      * probabilities to 22, and to 11 for 16-bit q where a sequence has more than 32 rows times heads of a group, or 16 with dim above
-     * 128), rounded once to out_dt.
+     * 128; such a sequence beside others makes it 11 for them too where out is bfloat16, and where rows has room for `most` rows of
+     * each), rounded once to out_dt.
      * Lengths count as at least 0 and at most the table's 64 * width tokens. out may not overlap q.
      * max_len: about the longest of the lengths (0: the table's width); it only decides how the work is split. Sequences with many
      * rows and with few may be mixed: each takes the kernel for its number of rows.
@@ -132,9 +133,8 @@ typedef struct {
     /* kv_attention where a row sees more than its window, or sequences share tokens: the tokens 0 .. p, of them, if window is above 0, the
      * last `window` and the first `sinks`, of them those that the mask leaves. With shared not NULL (and groups not 0), the tokens that a group's
      * sequences share are gone through once for all rows of the group, which changes the order of sums, not what a row sees. Blocks
-     * that no row sees any more need not be there (an entry of -1). Arguments, results and workspace as kv_attention's; probabilities
-     * are to 11 bits for 16-bit q also where most of a call's sequences have more rows than that, and those of shared tokens where out is
-     * bfloat16. */
+     * that no row sees any more need not be there (an entry of -1). Arguments, results and workspace as kv_attention's; where out is
+     * bfloat16 and q of 16 bits, probabilities of shared tokens are to 11 bits. */
     int (*kv_attention_spans)(void* ctx, const h3_kv_cache* cache, const h3_kv_batch* batch, const h3_kv_shared* shared, const int32_t* lengths,
                               int64_t max_len, const void* q, int64_t q_stride, int dt, int64_t q_heads, float scale, int64_t window,
                               int64_t sinks, const uint8_t* mask, int64_t mask_stride, void* out, int out_dt, float* lse, void* work,

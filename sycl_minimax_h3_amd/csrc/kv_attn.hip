@@ -54,7 +54,7 @@ static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int
 // blocks of threads that it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up
 // to 8192 tokens, 64 heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and
 // their merge 4, 7 and 11 us more. Longer parts: one sequence of 2000 tokens in parts of 8, 16 and 32 blocks 12.6, 15.5 and 18.5 us.)
-static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus) {
+static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, bool halves = false) {
     const int64_t group = sight.group, max_len = sight.max_len, window = sight.window;
     KvPlan plan;
     const int64_t rows = std::min<int64_t>(most, P.rows) * group;
@@ -75,13 +75,14 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& si
         plan.blocks = plan.places * P.heads;
         return plan;
     }
-    plan.nq = plan.rows ? (two || rows <= 96 || std::min(even(128), ragged(128)) * P.heads < cus ? 1 : 2) : rows <= 16 ? 1 : 2;
+    plan.nq = plan.rows ? (two || rows <= 96 || std::min(even(128), ragged(128)) * P.heads < cus ? 1 : 2) : rows <= 16 || halves ? 1 : 2;
     plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
     plan.tiles = even(plan.rt) <= ragged(plan.rt) ? (rows + plan.rt - 1) / plan.rt : 0;
     plan.places = std::min(even(plan.rt), ragged(plan.rt));
     plan.blocks = plan.places * P.heads;
     const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(plan.blocks, 1), 512));
+    const int64_t parted = halves ? (int64_t) P.seqs * P.heads : plan.blocks;   // (few have a second tile)
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(parted, 1), 512));
     plan.per = (int) std::max(least, (blocks + want - 1) / want);
     // (with first or shared tokens: up to 12 blocks are one part, a third step of the wavefronts for the 4 us of a merge: four sequences of 612
     // tokens, 64 heads over 8 of 128, 15 to 11 us)
@@ -93,15 +94,20 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& si
 // to 16 (or 32: larger groups) are a launch of the shared-rows kernel if that splits their caches further: a prompt of 2048 tokens
 // beside a token over 131072, 64 heads over 8 of 128, 3469 us in one launch, 191 in two (129 and 49 by themselves); four prompts of 241 to 600
 // tokens behind up to 900, for which the second finds nothing to do, 70 and 69.
-static int kv_plans(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[2]) {
+// fine (16-bit queries, results that are not bfloat16): sequences of few rows have probabilities as two halves whatever stands beside them, so the
+// rows' kernel never takes them. The second launch has all of up to 32 rows (16 of wide heads) then, in tiles of 16: answered tokens fill
+// one, and the wavefronts of a tile of 32 run one on a SIMD. float16 results, in one launch and in two: a prompt of 8 tokens beside seven answers
+// over 8192, 64 heads over 8 of 128, 42 and 59 us (17 and 30 behind a window of 1024); the four prompts 87 and 89; bfloat16 does not show it.
+static int kv_plans(const KvArgs& P, bool two, bool fine, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[2]) {
     const int64_t group = sight.group;
     plan[0] = kv_plan(P, two, most, sight, cus);
-    const int64_t few = (group <= 16 ? 16 : 32) / group;                         // tokens
+    const int64_t limit = fine ? (P.dim > 128 ? 16 : 32) : group <= 16 ? 16 : 32;
+    const int64_t few = limit / group;                                           // tokens
     if (!plan[0].rows || few == 0 || (group > 16 && P.dim > 128) || std::min<int64_t>(most, P.rows) * P.seqs <= P.rows) return 1;
     // (with first or shared tokens: where the sequences beside the longest have more rows on average, the rows' kernel takes those with few too)
-    if (sight.spans() && P.rows - std::min<int64_t>(most, P.rows) > 2 * few * (P.seqs - 1)) return 1;
-    plan[1] = kv_plan(P, two, few, sight, cus);
-    if (plan[1].nsplit <= plan[0].nsplit) return 1;
+    if (!fine && sight.spans() && P.rows - std::min<int64_t>(most, P.rows) > 2 * few * (P.seqs - 1)) return 1;
+    plan[1] = kv_plan(P, two, few, sight, cus, fine && group <= 16);
+    if (!fine && plan[1].nsplit <= plan[0].nsplit) return 1;
     plan[1].greatest = (uint32_t) (few * group);
     plan[0].least = plan[1].greatest + 1;
     return 2;
@@ -172,12 +178,12 @@ static int kv_all_plans(const KvArgs& P, bool two, bool fine, int64_t most, cons
     KvPlan own[2], behind[2], shared;
     KvSight all = sight;
     all.shared = 0;
-    int n = kv_plans(P, two, most, all, cus, own);
+    int n = kv_plans(P, two, fine, most, all, cus, own);
     const int64_t tokens = sight.max_len > 0 ? std::min<int64_t>(sight.max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     bool apart = sight.groups > 0 &&
                  std::min(std::max(tokens, sight.shared), sight.seen()) * P.seqs > cus * kKvApart / (2 * P.heads * kv_width(P.dim));
     if (apart) {
-        const int m = kv_plans(P, two, most, sight, cus, behind);
+        const int m = kv_plans(P, two, fine, most, sight, cus, behind);
         // (probabilities as two halves where the sequences' own are: some have few rows)
         shared = kv_shared_plan(P, two, fine && (!behind[0].rows || m == 2), sight, cus);
         apart = !own[0].rows || shared.cost + behind[0].cost + 6.0 < own[0].cost;
@@ -201,7 +207,7 @@ static int64_t attend_work(const char* fn, void* ctx, const h3_kv_cache* cache, 
     if (P.seqs == 0 || P.rows == 0 || batch->most == 0) return 0;
     // (the most of what float32 queries take, and 16-bit ones for 16-bit and float32 results)
     int64_t floats = 0;
-    for (int type = 0; type < (sight.groups ? 3 : 2); ++type) {
+    for (int type = 0; type < 3; ++type) {
         KvPlan plan[3];
         int64_t sum = 0;
         for (int n = kv_all_plans(P, type == 1, type == 2, batch->most, sight, c->cus, plan); n-- > 0;) sum += kv_part_floats(plan[n], kv_width(P.dim));

@@ -162,7 +162,7 @@ static int sight_of(const std::string& fn, const KvArgs& P, const h3_kv_shared* 
     sight = KvSight{q_heads / P.heads, max_len, std::min<int64_t>(window, INT32_MAX), window > 0 ? std::min<int64_t>(sinks, INT32_MAX) : 0, 0, 0};
     if (!shared || shared->groups == 0) return 0;
     if (shared->groups < 0 || shared->most < 0) return fail(fn + ": a negative number of groups or shared tokens");
-    if (shared->groups >= INT32_MAX) return fail(fn + ": too many groups");
+    if (shared->groups > kKvMostBlocks) return fail(fn + ": too many groups");   // (kv_group_of's steps of 64 stay within an int)
     if (!shared->first || !shared->tokens) return fail(fn + ": the groups' first sequences and shared tokens are required");
     sight.groups = shared->groups;
     sight.shared = shared->most > 0 ? std::min<int64_t>(shared->most, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;

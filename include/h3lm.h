@@ -150,7 +150,8 @@ typedef struct {
      * [heads], 0 or more (infinity: only the token itself). scale 0: 1 / sqrt(dk), else above 0. States, sums and decays are
      * float32; in a prompt's products of 16-bit types the states and the tokens' weights count to 17 bits. An infinity or NaN in a
      * token's values of a head leaves the sequence's earlier tokens as they are, and may make any of that head's results from that
-     * token on, and its state, infinite or NaN. out may not overlap q, k or v.
+     * token on, and its state, infinite or NaN. out may not overlap q, k or v. Batches whose launches could take 2^32 threads are refused:
+     * with 64 heads of 128 x 128 more than 65535 sequences, or 16383 if any may have more than 32 tokens.
      * work: as kv_attention's, of at least lin_attention_work(...) bytes. */
     int (*lin_attention)(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, const float* decay, const void* q, int64_t q_stride,
                          int64_t q_heads, const void* k, int64_t k_stride, int64_t k_heads, const void* v, int64_t v_stride, int64_t v_heads,

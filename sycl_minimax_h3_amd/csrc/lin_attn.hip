@@ -259,13 +259,17 @@ static LinPlan lin_plan(const h3_lin_state& state, const h3_lin_batch& batch, in
     return p;
 }
 
-// Whether a launch could take 2^32 threads or more (blocks of up to 512), however the device's size splits the call
+// Whether a launch could take 2^32 threads or more, however the device's size splits the call; counted in 256 threads: a block of 64 features of
+// values is one, of 128 two where keys have more than 128 features, and the walk has 2 or 4 kc of them a sequence and head.
 static bool lin_too_many(const h3_lin_state& state, const h3_lin_batch& batch) {
     const LinPlan p = lin_plan(state, batch, H3S_BF16, 1);
-    const int64_t steps = (state.dv + kLinCols - 1) / kLinCols, most = kKvMostBlocks / state.heads, slices = (state.dv + 63) / 64;
+    const int64_t steps = (state.dv + kLinCols - 1) / kLinCols, most = kKvMostBlocks / state.heads;
+    const int64_t narrow = (state.dv + 63) / 64, wide = state.dv > 64 ? (state.dv + 127) / 128 * 2 : 0;
+    const bool split = std::min(batch.most, batch.rows) > kLinLeast;
     const int64_t seg = std::max(kLinLeast, std::min({batch.most, batch.rows, batch.rows / batch.seqs}) / kLinSegs);   // the shortest
-    return (p.step && batch.seqs > most / steps) ||
-           (p.chunk && (batch.rows / seg + batch.seqs > most / 2 / slices || batch.seqs > most / 2 / (slices * 4 * p.kc)));
+    const int64_t places = split ? batch.rows / seg + batch.seqs : batch.seqs;
+    return (p.step && batch.seqs > most / steps) || (p.chunk && places > most / (p.kc > 4 ? std::max(narrow, wide) : narrow)) ||
+           (p.chunk && split && batch.seqs > most / (2 * p.kc * std::max(narrow, wide)));
 }
 
 int64_t lin_attention_work(void* ctx, const h3_lin_state* state, const h3_lin_batch* batch, int dt) try {

@@ -15,7 +15,7 @@ constexpr int kLinToks = 8;                         // tokens whose rows lie in 
 // Few tokens: a block of 256 threads holds 32 columns of a head's state in registers, rows r + 32 i and four columns a thread, over all
 // tokens of the sequence. A token's sum over the rows of S is left as 32 parts in LDS and added up once for up to eight tokens. exp(-decay) is
 // applied as S - (1 - exp(-decay)) S: a decay near 1 is held to 32 bits of its distance from 1, which is what far tokens' weights
-// depend on. Bound by the state's bytes, read and written once (64 sequences, 64 heads of 128 x 128: 106 us, 5.1 TB/s).
+// depend on. Bound by the state's bytes, read and written once (64 sequences, 64 heads of 128 x 128: 106 us, 5.1 TB/s, other states each pass).
 template <int DKR, bool VEC>
 __global__ __launch_bounds__(256) void lin_step_kernel(LinArgs P) {
     constexpr int K = 32 * DKR;
@@ -186,11 +186,13 @@ static int lin_checks(const std::string& fn, const h3_lin_state* state, const h3
     return 0;
 }
 
-// Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces (64 sequences of 64 heads of 128 x 128,
-// of up to 1, 4, 8 and 16 tokens, two thirds of that on average: 49, 61, 87 and 139 us, in pieces 85, 87, 90 and 97; 16 of 16 heads of 256 x
-// 256 17, 20, 26 and 41, in pieces 22). A launch for few tokens beside the others' takes 5 us and more: where the sequences beside the
-// longest have more than kLinBeside tokens on average, or are up to four blocks of pieces a CU, all go in pieces (64 sequences of up to 8
-// tokens in two launches 96 us; eight of up to 39 37, in pieces 21).
+// Which kernels take the call. Sequences of up to kLinFew tokens go token by token, others in pieces. 64 sequences of 64 heads of 128 x 128, of up to
+// 1, 4, 6, 8 and 16 tokens, 0.7 of that on average, in a queue of passes over the same states: carried on 91, 96, 109, 120 and 163 us, in pieces
+// 167, 172, 176, 178 and 187; begun, so that a state is only written, 48, 61, 72, 80 and 127, in pieces 86, 85, 86, 88 and 94. 16 of 16 heads
+// of 256 x 256 carried on 25, 28, 31, 33 and 46, in pieces 35; begun 16, 19, 23, 26 and 40, in pieces 22: 6 is where these lose nothing yet, carried
+// on 8 and more would pay. A launch for few tokens beside the others' takes 5 us and more: where the sequences beside the longest have more
+// than kLinBeside tokens on average, or are up to four blocks of pieces a CU, all go in pieces (64 sequences of up to 8 tokens in two
+// launches 96 us; eight of up to 39 37, in pieces 21; all begun).
 constexpr int kLinFew = 6, kLinBeside = 4;
 constexpr int64_t kLinLeast = 32, kLinSegs = 256;   // the least tokens of a segment, the most segments of an average sequence
 struct LinPlan {

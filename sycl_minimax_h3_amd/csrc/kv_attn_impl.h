@@ -784,6 +784,8 @@ template <int WC> __device__ __forceinline__ int kv_mix(int g, int c) { return (
 // doing it in every wavefront took more vector instructions than the softmax. Bound by vector instructions beside the products (4096 tokens
 // over 8192, 64 heads over 8 of 128: 947-1060 us by the card, 0.78-0.87 PFLOP/s, the matrix cores 34 % busy). Operands are read from LDS a
 // step ahead of their products (960 us without, 16 sequences of 100 tokens of 256 features 203 to 181).
+// (Heads of up to 64 features in tiles of 128 rows, three blocks a CU: where first or shared tokens are walked over too, 8 vector and 19 scalar
+// registers go to memory, 2 vector ones in the launch of shared tokens; kv_attention's form has none.)
 template <int WC, int NQ, bool TWO, int MODE = kKvAll, bool PTWO = TWO>
 __global__ __launch_bounds__(256, WC == 1 ? 3 : WC == 2 && !TWO ? 2 : 1) void kv_attn_rows_kernel(KvAttnArgs P) {
     constexpr int W = 64 * WC, DT = 4 * WC, RT = 64 * NQ, PARTS = TWO ? 2 : 1;

@@ -54,13 +54,14 @@ static void kv_rows_plan(KvPlan& plan, F tiles, int64_t rows, int64_t heads, int
 // blocks of threads that it runs at once. (Parts beyond that, to even out sequences of different lengths, gave nothing: 64 sequences of up
 // to 8192 tokens, 64 heads over 8 of 128, in 512, 1024 and 2048 blocks 133, 143 and 156 us, one of 131072 tokens 53, 57 and 62 us, and
 // their merge 4, 7 and 11 us more. Longer parts: one sequence of 2000 tokens in parts of 8, 16 and 32 blocks 12.6, 15.5 and 18.5 us.)
-static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, bool halves = false) {
+static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& sight, int cus, bool fine = false, bool tiles16 = false) {
     const int64_t group = sight.group, max_len = sight.max_len, window = sight.window;
     KvPlan plan;
     const int64_t rows = std::min<int64_t>(most, P.rows) * group;
     auto even = [&](int64_t rt) { return (rows + rt - 1) / rt * P.seqs; };
     auto ragged = [&](int64_t rt) { return P.rows * group / rt + P.seqs; };
     plan.rows = rows > (P.dim <= 128 ? 32 : 16);
+    plan.fine = plan.rows && fine;
     int64_t keys = max_len > 0 ? std::min<int64_t>(max_len, (int64_t) P.width * kKvB) : (int64_t) P.width * kKvB;
     if (sight.groups) keys = std::max<int64_t>(keys - sight.shared, std::min<int64_t>(most, P.rows));
     if (window > 0) keys = std::min(keys, sight.seen() + std::min<int64_t>(most, P.rows) + 2 * kKvB);
@@ -69,19 +70,19 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& si
         const int64_t all = P.rows * group;
         auto tiles = [&](int64_t rt) { return std::max(std::min(all / rt + P.seqs / 2, (rows + rt - 1) / rt * P.seqs), (int64_t) P.seqs); };
         if (window > 0) keys = std::min<int64_t>(keys, sight.seen() + 128 / group + 2 * kKvB);
-        kv_rows_plan(plan, tiles, all, P.heads, P.dim, std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), two, cus, 6.0);
+        kv_rows_plan(plan, tiles, all, P.heads, P.dim, std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), two, cus, 6.0, fine);
         plan.tiles = even(plan.rt) <= ragged(plan.rt) ? (rows + plan.rt - 1) / plan.rt : 0;
         plan.places = std::min(even(plan.rt), ragged(plan.rt));
         plan.blocks = plan.places * P.heads;
         return plan;
     }
-    plan.nq = plan.rows ? (two || rows <= 96 || std::min(even(128), ragged(128)) * P.heads < cus ? 1 : 2) : rows <= 16 || halves ? 1 : 2;
+    plan.nq = plan.rows ? (two || fine || rows <= 96 || std::min(even(128), ragged(128)) * P.heads < cus ? 1 : 2) : rows <= 16 || tiles16 ? 1 : 2;
     plan.rt = 16 * plan.nq * (plan.rows ? 4 : 1);
     plan.tiles = even(plan.rt) <= ragged(plan.rt) ? (rows + plan.rt - 1) / plan.rt : 0;
     plan.places = std::min(even(plan.rt), ragged(plan.rt));
     plan.blocks = plan.places * P.heads;
     const int64_t blocks = std::max<int64_t>((keys + kKvB - 1) / kKvB, 1), least = plan.rows ? 4 : 8;
-    const int64_t parted = halves ? (int64_t) P.seqs * P.heads : plan.blocks;   // (few have a second tile)
+    const int64_t parted = tiles16 ? (int64_t) P.seqs * P.heads : plan.blocks;   // (few have a second tile)
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t) cus / std::max<int64_t>(parted, 1), 512));
     plan.per = (int) std::max(least, (blocks + want - 1) / want);
     // (with first or shared tokens: up to 12 blocks are one part, a third step of the wavefronts for the 4 us of a merge: four sequences of 612
@@ -94,19 +95,26 @@ static KvPlan kv_plan(const KvArgs& P, bool two, int64_t most, const KvSight& si
 // to 16 (or 32: larger groups) are a launch of the shared-rows kernel if that splits their caches further: a prompt of 2048 tokens
 // beside a token over 131072, 64 heads over 8 of 128, 3469 us in one launch, 191 in two (129 and 49 by themselves); four prompts of 241 to 600
 // tokens behind up to 900, for which the second finds nothing to do, 70 and 69.
-// fine (16-bit queries, results that are not bfloat16): sequences of few rows have probabilities as two halves whatever stands beside them, so the
-// rows' kernel never takes them. The second launch has all of up to 32 rows (16 of wide heads) then, in tiles of 16: answered tokens fill
-// one, and the wavefronts of a tile of 32 run one on a SIMD. float16 results, in one launch and in two: a prompt of 8 tokens beside seven answers
-// over 8192, 64 heads over 8 of 128, 42 and 59 us (17 and 30 behind a window of 1024); the four prompts 87 and 89; bfloat16 does not show it.
+// fine (16-bit queries, results that are not bfloat16): sequences of few rows have probabilities as two halves whatever stands beside them. Where
+// none is longer than kKvHalves rows and the others have up to a tile (kKvBeside) on average, the rows' kernel has them so for all; else a
+// second launch has all sequences of up to 32 rows (16 of wide heads), in tiles of 16 where most have no more, as tiles of 32 leave a SIMD one
+// wavefront. float16 results, 64 heads over 8 of 128, by the rows' kernel with one half (11 bits) / with two / by two launches: 8 tokens beside seven
+// answers over 8192 42, 47 and 59 us, behind a window of 1024 17, 18 and 30; 63 sequences of 4 tokens beside one of 8, over 8192, 236, 268 and
+// 385; 15 of 4 beside one of 40, over 4096, 83, 93 and 108. Past the limits: 18 of 20 to 30 tokens over 7000 shared ones, 32 heads over 8 of 96, 101,
+// 136 and 117; 53 of 12 to 31 over 5376, 8 over one of 80, 82, 112 and 73. bfloat16's last place does not show it.
+constexpr int64_t kKvHalves = 512, kKvBeside = 64;   // rows: tokens times heads of a group
 static int kv_plans(const KvArgs& P, bool two, bool fine, int64_t most, const KvSight& sight, int cus, KvPlan (&plan)[2]) {
-    const int64_t group = sight.group;
-    plan[0] = kv_plan(P, two, most, sight, cus);
+    const int64_t group = sight.group, longest = std::min<int64_t>(most, P.rows), others = P.rows - longest;
+    const bool ragged = longest * P.seqs > P.rows;
+    const bool all = fine && ragged && longest * group <= kKvHalves && others * group <= kKvBeside * (P.seqs - 1);
+    plan[0] = kv_plan(P, two, most, sight, cus, all);
+    fine = fine && !all;                                                         // (from here on: the second launch is needed)
     const int64_t limit = fine ? (P.dim > 128 ? 16 : 32) : group <= 16 ? 16 : 32;
     const int64_t few = limit / group;                                           // tokens
-    if (!plan[0].rows || few == 0 || (group > 16 && P.dim > 128) || std::min<int64_t>(most, P.rows) * P.seqs <= P.rows) return 1;
+    if (!plan[0].rows || few == 0 || (group > 16 && P.dim > 128) || !ragged) return 1;
     // (with first or shared tokens: where the sequences beside the longest have more rows on average, the rows' kernel takes those with few too)
-    if (!fine && sight.spans() && P.rows - std::min<int64_t>(most, P.rows) > 2 * few * (P.seqs - 1)) return 1;
-    plan[1] = kv_plan(P, two, few, sight, cus, fine && group <= 16);
+    if (!fine && sight.spans() && others > 2 * few * (P.seqs - 1)) return 1;
+    plan[1] = kv_plan(P, two, few, sight, cus, false, fine && group <= 16 && others * group <= 16 * (P.seqs - 1));
     if (!fine && plan[1].nsplit <= plan[0].nsplit) return 1;
     plan[1].greatest = (uint32_t) (few * group);
     plan[0].least = plan[1].greatest + 1;
@@ -185,7 +193,7 @@ static int kv_all_plans(const KvArgs& P, bool two, bool fine, int64_t most, cons
     if (apart) {
         const int m = kv_plans(P, two, fine, most, sight, cus, behind);
         // (probabilities as two halves where the sequences' own are: some have few rows)
-        shared = kv_shared_plan(P, two, fine && (!behind[0].rows || m == 2), sight, cus);
+        shared = kv_shared_plan(P, two, fine && (!behind[0].rows || behind[0].fine || m == 2), sight, cus);
         apart = !own[0].rows || shared.cost + behind[0].cost + 6.0 < own[0].cost;
         if (apart) {
             n = m;

@@ -8,7 +8,7 @@
 // Products on the matrix cores (16 x 16 x 32, half operands, float32 sums). The codes are whole numbers below 2^8, exact as
 // half. Query rows are scaled by a power of two that takes their largest value to 2^14 .. 2^15, so half holds 16-bit types
 // without loss down to 2^-29 of it; float32 rows are two halves (high and rest: 22 bits). Probabilities are 2^15 p, so that half keeps
-// them down to p = 2^-29 at full precision. They are two halves too, but for many rows of 16-bit queries. (One half shows little in 16-bit
+// them down to p = 2^-29 at full precision. They are two halves too, but for many rows of 16-bit queries (kv_plans says which). (One half shows little in 16-bit
 // results: 500 tokens, the error against 64 bits in float16 2.6e-4 of the result, 2.1e-4 with two; in bfloat16 1.69e-3 and 1.68e-3. It shows in
 // float32 ones, 1.5e-4 and 2.5e-7. Two are 1-1.5 % of an answered token's time, whose bound is the cache's bytes - 64 sequences of up to 8192
 // tokens 131.0 and 132.2 us, one of 300 8.4 and 8.8 - but double the values' products of prompts, and two wavefronts a SIMD have no registers
@@ -1091,10 +1091,11 @@ static void kv_attn_run(Ctx* c, const KvAttnArgs& P, const KvPlan& plan, bool tw
     const unsigned grid = (unsigned) (plan.blocks * plan.nsplit);
     constexpr int RT = (ROWS ? 64 : 16) * NQ;
     if constexpr (ROWS) {
-        if constexpr (MODE == kKvShared && NQ == 1)
-            if (!two && plan.fine) return kv_attn_rows_kernel<WC, 1, false, MODE, true><<<grid, 256, 0, c->stream>>>(P);
-        if (!two) kv_attn_rows_kernel<WC, NQ, false, MODE><<<grid, 256, 0, c->stream>>>(P);
-        else if constexpr (NQ == 1) kv_attn_rows_kernel<WC, 1, true, MODE><<<grid, 256, 0, c->stream>>>(P);
+        if (!two && !(NQ == 1 && plan.fine)) kv_attn_rows_kernel<WC, NQ, false, MODE><<<grid, 256, 0, c->stream>>>(P);
+        if constexpr (NQ == 1) {
+            if (two) kv_attn_rows_kernel<WC, 1, true, MODE><<<grid, 256, 0, c->stream>>>(P);
+            else if (plan.fine) kv_attn_rows_kernel<WC, 1, false, MODE, true><<<grid, 256, 0, c->stream>>>(P);
+        }
     } else {
         if (two) kv_attn_kernel<WC, NQ, true, MODE><<<grid, 256, 0, c->stream>>>(P);
         else kv_attn_kernel<WC, NQ, false, MODE><<<grid, 256, 0, c->stream>>>(P);

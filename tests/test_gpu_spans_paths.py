@@ -69,17 +69,22 @@ def test_digits_of_few_rows_beside_many(dev, dev2, seqs, heads, group, dim, grou
 
 @pytest.mark.parametrize("dt,out_dt", [("BF16", "F32"), ("F16", "F16")])
 @pytest.mark.parametrize("units", [256, 2])
-def test_few_rows_in_two_tiles(cus, dt, out_dt, units):
-    """Sequences of up to 32 rows beside a longer one are a launch of tiles of 16, in parts where caches are long; with a window, first tokens and a
-    mask too."""
-    for seqs in ([(4, 300), (3, 200), (70, 320), (2, 250), (0, 9), (1, 200), (4, 4)], [(4, 2500), (1, 3000), (5, 700)]):
+def test_few_rows_beside_many_by_launches(cus, dt, out_dt, units):
+    """Sequences of up to 32 rows beside a long one are a launch of tiles of 16 (most have no more) or 32; where none is long all are a launch of the
+    rows' kernel with probabilities as two halves. With a window, first tokens and a mask too."""
+    for seqs, few in (([(4, 300), (1, 200), (70, 320), (2, 250), (0, 9), (1, 200), (1, 4)], 1),
+                      ([(4, 300), (3, 200), (70, 320), (4, 250), (0, 9), (1, 200), (4, 4)], 2),
+                      ([(4, 2500), (1, 3000), (5, 700)], 0), ([(40, 300), (2, 280), (0, 7), (1, 200)], 0)):
         for mask in (None, 0.6):
             case = Case(cus(units), seqs, 2, 8, 128, dt, seed=45, mask=mask)
             for window, sinks in ((0, 0), (100, 0), (100, 30)):
                 mode = 1 if sinks else 0
                 ran = kernels(case, out_dt, window=window, sinks=sinks)
-                assert any(r.startswith(f"kv_attn_kernel<2, 1, false, {mode}>") for r in ran) and "rows" in ran[0], ran
-                rows = some_rows(case, 60) if case.rows < 50 else [r for r in range(case.starts[-1]) if r < 8 or r > 74]
+                if few:
+                    assert any(r.startswith(f"kv_attn_kernel<2, {few}, false, {mode}>") for r in ran) and ", false>" in ran[0], ran
+                else:
+                    assert ran[0].startswith(f"kv_attn_rows_kernel<2, 1, false, {mode}, true>"), ran
+                rows = some_rows(case, 60) if case.rows < 50 else [r for r in range(case.starts[-1]) if r < 8 or r > 72]
                 check_rows(case, case.run(out_dt, window=window, sinks=sinks), rows, out_dt, str((seqs, window, mask)), window=window, sinks=sinks)
 
 
@@ -107,33 +112,35 @@ APART = [
     ((3, 1, 6, 448, 700, 2), 1, 16, 160, "F32", "F32", 0, 4, "rows1 rows1 join"),
     ((9, 0, 6, 448, 700, 1), 1, 2, 160, "F32", "F32", 1000, 4, "rows1 rows1 join"),
     ((9, 1, 20, 256, 700, 1), 1, 4, 256, "F32", "F32", 1000, 8, "rows1 rows1 join"),
-    ((20, 1, 4, 960, 40, 2), 1, 2, 64, "BF16", "F32", 0, 2, "rows1 rows1 few1"),
-    ((12, 1, 6, 256, 40, 2), 1, 2, 160, "F16", "F32", 300, 1, "rows1 rows1 few1"),
-    ((20, 0, 6, 640, 700, 1), 1, 1, 160, "BF16", "F32", 0, 4, "rows1 rows1 join few1"),
-    ((20, 1, 4, 1280, 700, 3), 1, 1, 160, "BF16", "F32", 0, 8, "few1 rows1 join few1"),
+    ((20, 1, 4, 960, 40, 2), 1, 2, 64, "BF16", "F32", 0, 2, "rows1h rows1h"),
+    ((12, 1, 6, 256, 40, 2), 1, 2, 160, "F16", "F32", 300, 1, "rows1h rows1h"),
+    ((20, 0, 6, 640, 700, 1), 1, 1, 160, "BF16", "F32", 0, 4, "rows1h rows1h join"),
+    ((20, 1, 4, 1280, 700, 3), 1, 1, 160, "BF16", "F32", 0, 8, "few1 rows1h join"),
+    ((12, 1, 4, 640, 3000, 4), 1, 2, 256, "F16", "F16", 0, 4, "few1 rows1h few1 join"),
+    ((9, 0, 4, 1280, 3000, 1), 1, 2, 256, "BF16", "F32", 0, 4, "rows1h rows1h few1 join"),
+    ((20, 1, 4, 1280, 3000, 1), 1, 1, 160, "F32", "F32", 0, 4, "rows1 rows1 few1 join"),
+    ((17, 0, 20, 4096, 37, 20), 1, 4, 64, "F16", "F16", 4096, 16, "rows1h rows1 few2"),
+    ((5, 0, 20, 4096, 25, 2), 1, 16, 80, "BF16", "F32", 0, 1, "rows1h rows2 few2"),
     ((20, 1, 4, 640, 300, 3), 1, 1, 160, "BF16", "BF16", 1000, 4, "few1 rows1"),
     ((20, 1, 4, 1280, 40, 3), 2, 2, 80, "F32", "F32", 0, 4, "few2 rows1"),
-    ((20, 1, 4, 640, 100, 3), 1, 2, 80, "F16", "F32", 1000, 1, "few2 rows1 few1"),
+    ((20, 1, 4, 640, 100, 3), 1, 2, 80, "F16", "F32", 1000, 1, "few2 rows1h"),
     ((20, 0, 4, 448, 100, 1), 1, 1, 80, "F32", "F32", 0, 2, "rows1 few2"),
-    ((12, 1, 4, 448, 40, 1), 1, 2, 96, "F16", "F32", 700, 2, "rows1 few2"),
+    ((12, 1, 4, 448, 40, 1), 1, 2, 96, "F16", "F32", 700, 2, "rows1h few2"),
 ]
 
 
-def named(want, dim, dt, dt_out):
-    """The kernels that a line of APART means."""
-    wide, two, seen = (dim + 63) // 64, "true" if dt == "F32" else "false", []
-    words = want.split()
-    for i, w in enumerate(words):
-        mode = 1 if seen else 2
-        if w == "join":
-            tile = 64 * int(words[i - 1][-1])
+def named(want, dim, dt):
+    """The kernels that a line of APART means (h: probabilities as two halves, as those of float32 queries are)."""
+    wide, two, seen, tile = (dim + 63) // 64, "true" if dt == "F32" else "false", [], 0
+    for word in want.split():
+        mode, tiles = 1 if seen else 2, word.strip("rowsfewjoinh")
+        if word == "join":
             seen.append(f"kv_join_kernel<{wide}, {tile}>")
-        elif w[:-1] == "few":
-            seen.append(f"kv_attn_kernel<{wide}, {w[-1]}, {two}, {mode}>")
+        elif word.startswith("few"):
+            seen.append(f"kv_attn_kernel<{wide}, {tiles}, {two}, {mode}>")
         else:
-            some_few = words[-1][:-1] == "few"
-            halves = "true" if dt == "F32" or (mode == 2 and some_few and dt_out != "BF16") else "false"
-            seen.append(f"kv_attn_rows_kernel<{wide}, {w[-1]}, {two}, {mode}, {halves}>")
+            seen.append(f"kv_attn_rows_kernel<{wide}, {tiles}, {two}, {mode}, {'true' if word[-1] == 'h' else two}>")
+        tile = (64 if word[0] == "r" else 16) * int(tiles or 0)
     return seen
 
 
@@ -160,12 +167,12 @@ def test_shared_tokens_apart_from_many_rows(cus, shape, heads, group, dim, dt, o
     for mask in (None, 0.5):
         case = Case(dev, seqs, heads, group, dim, dt, groups, seed=42, mask=mask)
         ran = kernels(case, out_dt, **kw)
-        names = named(want, dim, dt, out_dt)
+        names = named(want, dim, dt)
         assert [r[:len(n)] for r, n in zip(ran, names)] == names and len(ran) == len(names), (ran, names)
         check_rows(case, case.run(out_dt, **kw), some_rows(case), out_dt, f"mask {mask}", **kw)
 
 
-MANY = [0, 1, 4, 6, 8, 12, 14, 17]   # of APART: each kind of launch
+MANY = [0, 1, 4, 6, 8, 12, 14, 17, 18, 20]   # of APART: each kind of launch
 
 
 @pytest.mark.parametrize("i", MANY)
